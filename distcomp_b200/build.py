@@ -22,7 +22,7 @@ INCLUDE = PKG.parent / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O2", "--expt-relaxed-constexpr",
-              "-Xptxas", "-warn-spills"]
+              "-Xptxas", "-warn-spills", "--threads", "0"]
 
 
 def nvcc() -> str:

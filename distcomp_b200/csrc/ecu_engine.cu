@@ -10,6 +10,7 @@
 #include "../../include/engine_cuda.h"
 #include "ecu_attn.cuh"
 #include "ecu_gemv.cuh"
+#include "ecu_kv4.h"
 #include "ecu_mega.cuh"
 #include "ecu_misc.cuh"
 #include "ecu_model.h"
@@ -32,6 +33,8 @@
 #include <vector>
 
 static std::atomic<uint64_t> g_launches{0};
+
+void ecu_count_launches(int n) { g_launches += (uint64_t)n; }
 
 #define CK(call)                                                                        \
     do {                                                                                \

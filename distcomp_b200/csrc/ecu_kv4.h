@@ -1,0 +1,75 @@
+// ecu_kv4.h -- host side of the paged 4-bit K/V cache, shared by the
+// translation units that use it.
+#pragma once
+#include "../../include/engine_cuda.h"
+
+#include <cuda_runtime.h>
+#include <cstdint>
+#include <map>
+#include <vector>
+
+// Which sequence holds which page, and how many hold each page.  Pure host
+// bookkeeping: every operation either succeeds or leaves everything as it
+// was, and collects the page copies and device words that follow from it.
+struct KvBook {
+    int n_pages = 0, n_seq = 0, max_pages = 0;
+    struct Seq { int len = 0; std::vector<int> page; };
+    std::vector<Seq>      seq;
+    std::vector<int>      ref;
+    std::vector<uint64_t> taken;      // bit p: page p is held
+    size_t                hint = 0;   // no free page lies in a word below
+    int                   used = 0;
+
+    struct Copy { int from, to; };
+    struct Set { int at, value; };    // device words: table [n_seq][max_pages], then len [n_seq]
+    std::vector<Copy> copies;         // of the last operation
+    std::vector<Set>  sets;
+
+    void init(int pages, int seqs, int per_seq);
+    int  extend(const int *s, const int *n_new, int n);
+    int  fork(const int *src, const int *dst, int n);
+    int  truncate(const int *s, const int *len, int n);
+    int  compact();
+    int  fail();                      // takes the operation back; -1
+
+private:
+    struct Undo { int kind, a, b; };
+    std::vector<Undo> log_;
+    std::vector<std::pair<int, int>> cell_;    // table cells (sequence, index) that changed
+    std::vector<int>                 length_;  // sequences whose length changed
+    int  take();
+    void hold(int p);
+    void drop(int p);
+    void begin();
+    void finish();
+    bool slot(int s, const char *what);
+};
+
+struct ecu_kv {
+    int    n_layer = 0, n_head_kv = 0, head_dim = 0, device = -1, sms = 0;
+    size_t page_bytes = 0, device_bytes = 0;
+    uint8_t *data = nullptr;
+    bool     own_data = false;
+    int     *meta = nullptr;          // device: table, then len
+    KvBook   book;
+    std::map<void *, void *> ws;      // stream -> its attention workspace
+    int *table() const { return meta; }
+    int *len() const { return meta ? meta + (size_t)book.n_seq * book.max_pages : nullptr; }
+};
+
+// The current device for the time of a call.
+struct DeviceScope {
+    int  old = -1;
+    bool ok;
+    explicit DeviceScope(int dev)
+    {
+        ok = cudaGetDevice(&old) == cudaSuccess && (old == dev || cudaSetDevice(dev) == cudaSuccess);
+        if (old == dev) old = -1;
+    }
+    ~DeviceScope()
+    {
+        if (old >= 0) cudaSetDevice(old);
+    }
+};
+
+void ecu_count_launches(int n);       // ecu_kernel_launches()

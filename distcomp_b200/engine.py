@@ -50,6 +50,12 @@ class EcuKprof(C.Structure):
                 ("bytes_per_launch", C.c_double)]
 
 
+class EcuKvInfo(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("n_layer", "n_head_kv", "head_dim", "n_pages", "n_seq", "max_pages", "device",
+                                       "used")] + [("page_bytes", C.c_size_t), ("device_bytes", C.c_size_t),
+                                                   ("data", C.c_void_p), ("table", C.c_void_p), ("len", C.c_void_p)]
+
+
 # (name, restype, argtypes) of every symbol include/engine_cuda.h declares
 SIGNATURES = [
     ("ecu_model_open", C.c_int, [C.POINTER(C.c_void_p), C.c_void_p, C.c_size_t, C.c_char_p, C.c_size_t]),
@@ -114,6 +120,26 @@ SIGNATURES = [
     ("ecu_profile_steps", C.c_int, [C.c_void_p, C.c_int, C.POINTER(EcuKprof), C.c_int]),
     ("ecu_profile_cta_ns", C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.POINTER(C.c_int), C.c_char_p,
                                      C.c_size_t]),
+    ("ecu_kv4_page_bytes", C.c_size_t, [C.c_int, C.c_int]),
+    ("ecu_kv_open", C.c_int, [C.POINTER(C.c_void_p), C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                              C.c_void_p, C.c_char_p, C.c_size_t]),
+    ("ecu_kv_close", None, [C.c_void_p]),
+    ("ecu_kv_get_info", C.c_int, [C.c_void_p, C.POINTER(EcuKvInfo)]),
+    ("ecu_kv_len", C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int]),
+    ("ecu_kv_extend", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    ("ecu_kv_fork", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    ("ecu_kv_truncate", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    ("ecu_kv_free", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    ("ecu_kv_compact", C.c_int, [C.c_void_p, C.c_void_p]),
+    ("ecu_kv_append", C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_long, C.c_long, C.c_void_p,
+                                C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
+    ("ecu_kv_attend", C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_long, C.c_long,
+                                C.c_void_p, C.c_int, C.c_float, C.c_void_p, C.c_void_p]),
+    ("ecu_kv_ws_bytes", C.c_size_t, [C.c_void_p]),
+    ("ecu_kv_read", C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
+    ("ecu_attn_prompt", C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
+                                  C.c_long, C.c_long, C.c_long, C.c_long, C.c_void_p, C.c_void_p, C.c_int, C.c_float,
+                                  C.c_int, C.c_void_p]),
     ("ecu_last_error", C.c_char_p, []),
     ("ecu_kernel_launches", C.c_uint64, []),
     ("ecu_version", C.c_char_p, []),

@@ -299,6 +299,130 @@ int  ecu_matvec(unsigned ggml_type, const void *w_raw, int n_in, int n_out, cons
 int  ecu_matvec_argmax_noalloc(unsigned ggml_type, const void *d_w, int n_in, int n_out,
                                const float *d_x, float *d_y, int *d_token, void *stream);
 
+/* ---- a K/V cache in pages of 4-bit rows, shared by many sequences -------- */
+
+/* The contexts above keep one dense fp32 cache each (the reference keeps one
+ * llm_ctx per process, src/daemon.c:757); a server of many sequences keeps
+ * theirs in one pool of pages instead, at 4.5 bits a value (fp32 contexts:
+ * 32), and forks share the pages of their common prefix.
+ *
+ * A page holds ECU_KV4_PAGE positions of every KV head of one layer; page p
+ * of layer l lies at data + (l * n_pages + p) * ecu_kv4_page_bytes().  One
+ * page id names the same positions in every layer.  Per KV head a page has
+ * 72 * head_dim bytes: K codes of the 64 positions (head_dim / 2 bytes each),
+ * V codes, K scales, V scales (fp16, [64][head_dim / 32]).  A position's
+ * codes are 16-byte chunks, one per block of 32 dimensions, two codes a byte
+ * in order, the low nibble first; chunk b of position t lies at place
+ * b ^ ((t >> 1) & 3) for head_dim 128, b ^ ((t >> 2) & 1) for 64, b for 32
+ * and 96 (so that eight positions' chunks fall into different banks of
+ * shared memory, where pages are copied whole).  A value is
+ * (code - 8) * scale: the values of GGUF's Q4_0 blocks.  The scale is
+ * fp16(m / -8), m the block's value of largest magnitude (the first of
+ * equals; at most 65504 in magnitude), a code floor(x / scale + 8.5) clamped
+ * to 0..15, decided exactly; a block with a value that is not finite reads
+ * as NaN, one whose scale rounds to zero as zeros. */
+#define ECU_KV4_PAGE 64
+
+/* element types of the rows that the operators below read and write */
+enum { ECU_F32 = 0, ECU_F16 = 1, ECU_BF16 = 2 };
+
+typedef struct ecu_kv ecu_kv;
+
+/* Bytes of one page of one layer; 0 for a shape that is not covered
+ * (head_dim 32, 64, 96 and 128 are). */
+size_t ecu_kv4_page_bytes(int n_head_kv, int head_dim);
+
+/* A pool of n_pages pages for up to n_seq sequences (slots 0..n_seq-1, all
+ * empty) of up to max_pages pages each.  data: n_layer * n_pages pages of
+ * device memory that the caller keeps (16-byte aligned, its contents left as
+ * they are), or NULL: the pool allocates them.  The bookkeeping (which
+ * sequence holds which page, how many hold a page) is on the host, its table
+ * and lengths are mirrored in device memory at fixed addresses.  device -1:
+ * the bookkeeping alone, without a GPU (to plan capacity).  A pool is
+ * single-threaded, like a context. */
+int  ecu_kv_open(ecu_kv **out, int n_layer, int n_head_kv, int head_dim, int n_pages, int n_seq, int max_pages,
+                 int device, void *data, char *err, size_t errlen);
+void ecu_kv_close(ecu_kv *kv);
+
+typedef struct {
+    int    n_layer, n_head_kv, head_dim, n_pages, n_seq, max_pages, device;
+    int    used;              /* pages that some sequence holds */
+    size_t page_bytes, device_bytes;
+    void  *data;              /* the pages */
+    int   *table, *len;       /* device: page ids [n_seq][max_pages] (-1: none), positions [n_seq] */
+} ecu_kv_info;
+int  ecu_kv_get_info(const ecu_kv *kv, ecu_kv_info *info);
+/* Positions of a sequence (-1: no such slot); its page ids into
+ * pages[0..n) (NULL: none wanted). */
+int  ecu_kv_len(const ecu_kv *kv, int seq, int *pages, int n);
+
+/* The next four change n sequences in the list's order; each either does all
+ * of it or, with -1, nothing.  What they change on the device is enqueued on
+ * `stream` (NULL: the legacy default stream); calls on the same pool from
+ * different streams are ordered by the caller, and a stream that is being
+ * captured is refused (the bookkeeping would not be replayed).
+ *
+ * extend: sequence seq[i] grows by n_new[i] positions; pages are taken
+ * lowest free id first.  Where its last page is partly filled and other
+ * sequences hold it too, the sequence gets a copy of its own first (every
+ * layer).  New positions' rows are what ecu_kv_append writes.
+ * fork: dst[i], an empty slot, becomes a copy of src[i], sharing its pages.
+ * truncate: sequence seq[i] keeps its first len[i] positions (at most its
+ * length); pages past them are given back.  ecu_kv_free: all of them. */
+int  ecu_kv_extend(ecu_kv *kv, const int *seq, const int *n_new, int n, void *stream);
+int  ecu_kv_fork(ecu_kv *kv, const int *src, const int *dst, int n, void *stream);
+int  ecu_kv_truncate(ecu_kv *kv, const int *seq, const int *len, int n, void *stream);
+int  ecu_kv_free(ecu_kv *kv, const int *seq, int n, void *stream);
+/* Moves pages so that those in use are pages 0..used-1: the k-th lowest page
+ * at or above `used` goes to the k-th lowest hole below it (every layer), and
+ * the tables follow.  Returns the number of pages moved, or -1. */
+int  ecu_kv_compact(ecu_kv *kv, void *stream);
+
+/* The rows of n sequences' newest positions, quantised into layer `layer`'s
+ * pages: sequence seq[i] (NULL: slots 0..n-1; no slot twice) gets n_new[i]
+ * rows, its positions len - n_new[i] .. len - 1, from consecutive rows of k
+ * and v (device, `dtype`, a row's KV heads one after the other, rows k_stride
+ * / v_stride elements apart).  The positions' pages must be the sequence's
+ * own (freshly extended ones are).  k_out, v_out (or NULL): the values as the
+ * cache holds them, `out_dtype`, rows of n_head_kv * head_dim without gaps.
+ * The lengths are read on the device when the call runs, so a captured call
+ * appends to the then newest positions. */
+int  ecu_kv_append(ecu_kv *kv, int layer, int dtype, const void *k, const void *v, long k_stride, long v_stride,
+                   const int *seq, const int *n_new, int n, int out_dtype, void *k_out, void *v_out, void *stream);
+
+/* Attention of one query row per sequence over all of its positions in layer
+ * `layer`: out row i = softmax(scale * q_h K^T) V for the n_head query heads
+ * (head h reads KV head h / (n_head / n_head_kv)) of sequence seq[i] (NULL:
+ * slots 0..n-1; a slot may come twice).  q and out: device, `dtype`, a row's
+ * heads one after the other, rows q_stride / out_stride elements apart.  An
+ * empty sequence's row becomes zeros.  Sums and the softmax are fp32; fp32
+ * queries keep their 24 bits.  The lengths are read on the device when the
+ * call runs.
+ * ws: ecu_kv_ws_bytes() bytes of device memory, zeroed once before their
+ * first use, that no other call uses at the same time; NULL: the pool's own
+ * for this stream, which a stream that is being captured must not take. */
+int    ecu_kv_attend(ecu_kv *kv, int layer, int dtype, const void *q, void *out, int n_head, long q_stride,
+                     long out_stride, const int *seq, int n, float scale, void *ws, void *stream);
+size_t ecu_kv_ws_bytes(const ecu_kv *kv);
+/* Positions pos .. pos + n - 1 of a sequence as fp32 rows [n][n_head_kv *
+ * head_dim] in host memory (K and V as the cache holds them; either may be
+ * NULL): the cache's ecu_dequant_tensor.  Synchronises `stream`. */
+int    ecu_kv_read(ecu_kv *kv, int layer, int seq, int pos, int n, float *k, float *v, void *stream);
+
+/* Causal attention of packed prompts, on the tensor cores: sequence s has
+ * query rows cu_q[s] .. cu_q[s+1]-1 and key/value rows cu_k[s] .. cu_k[s+1]-1
+ * (host arrays of n_seq + 1 non-decreasing offsets from 0; cu_k NULL: the
+ * queries').  The last query sees every key of its sequence, each earlier one
+ * one key less; a row that sees none becomes zeros.  q, k, v, out: device,
+ * `dtype` (ECU_F16 or ECU_BF16), 16-byte aligned, a row's heads one after the
+ * other, rows a multiple of 8 elements apart; head_dim 64 or 128.  What lies
+ * behind the last row, or in keys that a row does not see (NaN and infinities
+ * too), has no effect.  Sums and the softmax are fp32; the weights are
+ * rounded to `dtype` before their product with V. */
+int  ecu_attn_prompt(int dtype, const void *q, const void *k, const void *v, void *out, int n_head, int n_head_kv,
+                     int head_dim, long q_stride, long k_stride, long v_stride, long out_stride, const int *cu_q,
+                     const int *cu_k, int n_seq, float scale, int device, void *stream);
+
 /* ---- failure-path testing ------------------------------------------------ */
 
 /* No counterpart in the reference, whose failure paths are host retries and
