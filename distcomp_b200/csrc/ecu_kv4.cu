@@ -421,23 +421,44 @@ extern "C" int ecu_kv_read(ecu_kv *kv, int layer, int seq, int pos, int n, float
 
 // ---------------------------------------------------------------- attend ---
 
-template <typename T, int N>
-static int attend_launch(ecu_kv *kv, const KvAttendArgs &a, int n_head, const int *seq, int first, int n, cudaStream_t s)
+// Heads of a group: one 8-column tile, two where an fp32 query has more than
+// 4 heads on its KV head (two groups would read the cache twice).
+static int attend_tiles(int dtype, int n_rep) { return dtype == ECU_F32 && n_rep > 4 ? 2 : 1; }
+
+template <typename T, int NB, int NT, int N>
+static int attend_launch(ecu_kv *kv, const KvAttendArgs &a, const int *seq, int first, int n, bool whole, cudaStream_t s)
 {
+    using S = KvShape<T, NB, NT>;
     KvSeqs<N> list;
     list.n = n;
-    for (int i = 0; i < n; i++) list.seq[i] = (uint16_t)(seq ? seq[i] : first + i);
-    k_kv4_attend_simple<T, N><<<dim3((unsigned)n, (unsigned)n_head), 128, 0, s>>>(a, list, kv->head_dim);
+    const long long rows_seq = (long long)kv->n_head_kv * ((a.n_rep + S::HG - 1) / S::HG);
+    long long       units = 0, rows = 0;
+    for (int i = 0; i < n; i++) {
+        list.seq[i] = (uint16_t)(seq ? seq[i] : first + i);
+        const long long u = (kv->book.seq[list.seq[i]].len + KV4_UNIT - 1) / KV4_UNIT;
+        units += u * rows_seq;
+        rows += u ? rows_seq : 0;
+    }
+    // one CTA per SM, fewer where the warps would find less than a unit each;
+    // a CTA per row at least, so that few short rows are merged inside a CTA.
+    // A captured call is replayed at lengths to come: every SM.
+    const long long want = std::max((units + S::W - 1) / S::W, rows);
+    const int       grid = whole ? kv->sms : (int)std::max(1ll, std::min<long long>(kv->sms, want));
+    const size_t    smem = S::smem(n);
+    auto            kern = k_kv4_attend<T, NB, NT, N>;
+    CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem(N)));
+    kern<<<grid, S::W * 32, smem, s>>>(a, list);
     return launched("ecu_kv_attend");
 }
 
-template <typename T>
-static int attend_list(ecu_kv *kv, KvAttendArgs a, int n_head, const int *seq, int n, cudaStream_t s)
+template <typename T, int NB, int NT>
+static int attend_list(ecu_kv *kv, KvAttendArgs a, const int *seq, int n, bool whole, cudaStream_t s)
 {
     for (int i = 0; i < n; i += KV4_LIST) {
         const int  m = std::min(KV4_LIST, n - i);
         const int *q = seq ? seq + i : nullptr;
-        if ((m <= 64 ? attend_launch<T, 64>(kv, a, n_head, q, i, m, s) : attend_launch<T, KV4_LIST>(kv, a, n_head, q, i, m, s)) != 0)
+        if ((m <= 64 ? attend_launch<T, NB, NT, 64>(kv, a, q, i, m, whole, s)
+                     : attend_launch<T, NB, NT, KV4_LIST>(kv, a, q, i, m, whole, s)) != 0)
             return -1;
         a.q = (const T *)a.q + (size_t)m * a.q_stride;
         a.out = (T *)a.out + (size_t)m * a.out_stride;
@@ -445,7 +466,24 @@ static int attend_list(ecu_kv *kv, KvAttendArgs a, int n_head, const int *seq, i
     return 0;
 }
 
-extern "C" size_t ecu_kv_ws_bytes(const ecu_kv *kv) { return kv ? 4096 : 0; }
+template <typename T, int NT>
+static int attend_dim(ecu_kv *kv, const KvAttendArgs &a, const int *seq, int n, bool whole, cudaStream_t s)
+{
+    switch (kv->head_dim / 32) {
+    case 1: return attend_list<T, 1, NT>(kv, a, seq, n, whole, s);
+    case 2: return attend_list<T, 2, NT>(kv, a, seq, n, whole, s);
+    case 3: return attend_list<T, 3, NT>(kv, a, seq, n, whole, s);
+    default: return attend_list<T, 4, NT>(kv, a, seq, n, whole, s);
+    }
+}
+
+// Tickets of each CTA's row, then two partials a CTA of at most 8 heads.
+static size_t count_bytes(const ecu_kv *kv) { return ((size_t)kv->sms * sizeof(unsigned) + 255) & ~(size_t)255; }
+
+extern "C" size_t ecu_kv_ws_bytes(const ecu_kv *kv)
+{
+    return kv && kv->device >= 0 ? count_bytes(kv) + (size_t)kv->sms * 2 * 8 * (kv->head_dim + 2) * sizeof(float) : 0;
+}
 
 extern "C" int ecu_kv_attend(ecu_kv *kv, int layer, int dtype, const void *q, void *out, int n_head, long q_stride,
                              long out_stride, const int *seq, int n, float scale, void *ws, void *stream)
@@ -473,9 +511,10 @@ extern "C" int ecu_kv_attend(ecu_kv *kv, int layer, int dtype, const void *q, vo
     DeviceScope d(kv->device);
     if (!d.ok) return say(what, "the pool's device cannot be used");
     const cudaStream_t s = (cudaStream_t)stream;
+    const int          cap = capturing(s, what);
+    if (cap < 0) return -1;
     if (!ws) {
-        const int c = capturing(s, what);
-        if (c) return c < 0 ? -1 : say(what, "a captured call needs a workspace of its own");
+        if (cap) return say(what, "a captured call needs a workspace of its own");
         try {
             void *&own = kv->ws[stream];
             if (!own) {
@@ -506,9 +545,10 @@ extern "C" int ecu_kv_attend(ecu_kv *kv, int layer, int dtype, const void *q, vo
     a.n_kv = kv->n_head_kv;
     a.n_rep = n_head / kv->n_head_kv;
     a.scale = scale;
+    a.wide_q = !(((uintptr_t)q | (uintptr_t)(q_stride * (long)es)) & 15);
     a.count = (unsigned *)ws;
-    a.part = (float *)ws;
-    if (dtype == ECU_F32) return attend_list<float>(kv, a, n_head, seq, n, s);
-    if (dtype == ECU_F16) return attend_list<__half>(kv, a, n_head, seq, n, s);
-    return attend_list<__nv_bfloat16>(kv, a, n_head, seq, n, s);
+    a.part = (float *)((uint8_t *)ws + count_bytes(kv));
+    if (dtype == ECU_F16) return attend_dim<__half, 1>(kv, a, seq, n, cap, s);
+    if (dtype == ECU_BF16) return attend_dim<__nv_bfloat16, 1>(kv, a, seq, n, cap, s);
+    return attend_tiles(dtype, a.n_rep) == 2 ? attend_dim<float, 2>(kv, a, seq, n, cap, s) : attend_dim<float, 1>(kv, a, seq, n, cap, s);
 }

@@ -221,50 +221,631 @@ struct KvAttendArgs {
     const int     *table, *len;
     int            max_pages, n_pages, n_kv, n_rep;
     float          scale;
+    bool           wide_q;
     float         *part;          // workspace: partials of rows that several CTAs share
     unsigned      *count;         //   and their tickets
 };
 
-// One CTA per (row, query head), a warp per position, lanes over dimensions.
-template <typename T, int N>
-__global__ void __launch_bounds__(128) k_kv4_attend_simple(const KvAttendArgs a, const KvSeqs<N> list, int hd)
+// The attention is one pass over the cached rows with a running maximum and
+// sum.  K and V are integer codes times a scale per 32 dimensions, so both
+// products run on the tensor cores (mma.sync m16n8k16, fp16 operands, fp32
+// sums) on the codes themselves, which fp16 holds exactly:
+//
+//   score[t][col] = sum_b Kscale[t][b] * (Kcode[t][b] . q[col][b])
+//   O^T[d][col]  += sum_t Vcode[t][d] * (weight[t][col] * Vscale[t][b(d)])
+//
+// The columns are the query heads that share the KV head.  An fp32 query is
+// two columns, its fp16 part and the fp16 part of the rest (22 bits), and so
+// is its weight * Vscale; the two add up in one thread.  16-bit queries are
+// one column (exact after scaling by a power of two), and so are their
+// weights (one rounding to 11 bits, which fp16 and bf16 outputs do not see).
+// To stay in fp16's range a query is scaled by the power of two that brings
+// its largest element to 2^13, and a weight is 2^(score - M + 14) with M the
+// running maximum of score + log2 of the tile's largest V scale, so that
+// weight * scale never passes 2^14 and loses nothing above 2^-38 of that.
+// Every unit's V product starts from zero and is added to the running sums
+// by one fma with the rescaling factor: no long chains inside the tensor core,
+// which cuts off instead of rounding.
+//
+// Unpacking a word of 8 codes: (w & 0xF000F) | 0x64006400 is 1024 + code in
+// each half, (w & 0xF000F0) | ... 1024 + 16 * code; one fp16x2 subtraction or
+// fma leaves code - 8.  ldmatrix gives a thread the K codes of 8 dimensions of
+// one position, and transposed the V codes of 4 dimensions of two positions:
+// both are the operand layouts of the products, in the stored order.
+//
+// Work is cut into units of 32 positions of one KV head of one sequence,
+// numbered sequence by sequence, head by head, and dealt out evenly: CTAs get
+// equal runs of units, and within a CTA the warps do, whatever the lengths.
+// Each warp streams its units through a ring of its own (bulk copies; no
+// barrier between warps) and keeps its own softmax.  A row that several warps
+// share is merged in shared memory, one that several CTAs share through the
+// workspace by whichever CTA ends last, in the order of the CTAs, so that the
+// result does not depend on timing.
+#define KV4_UNIT 32
+#define KV4_STAGES 2
+
+template <typename T> struct KvSplit { static constexpr int N = 1; };
+template <> struct KvSplit<float> { static constexpr int N = 2; };
+
+template <int NT> struct KvWarps { static constexpr int N = NT == 1 ? 16 : 8; };
+
+template <typename T, int NB, int NT> struct KvShape {
+    static constexpr int HD = NB * 32, P = KvSplit<T>::N, W = KvWarps<NT>::N;
+    static constexpr int HG = 8 * NT / P;                 // query heads of a group
+    static constexpr int STAGE = 36 * HD;                 // one unit: K codes, V codes, K scales, V scales
+    static constexpr int ENTRY = HG * (HD + 2);           // a partial: per head the sums, M and the weights' sum
+    static constexpr size_t ring = (size_t)W * KV4_STAGES * STAGE, heads = (size_t)W * ENTRY * 4;
+    static constexpr size_t smem(int n) { return ring + heads + W * KV4_STAGES * 8 + (size_t)(n + 1) * 8; }
+    static_assert(ring >= heads, "the tail partials take the ring's place");
+};
+
+__device__ __forceinline__ float kv4_ex2(float x)
 {
-    __shared__ float part[4][130];
-    const int i = blockIdx.x, head = blockIdx.y, g = head / a.n_rep, s = list.seq[i];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nb = hd / 32;
-    const int n = min(__ldg(a.len + s), a.max_pages * KV4_PAGE);
-    const T  *q = (const T *)a.q + (size_t)i * a.q_stride + (size_t)head * hd;
-    float     qv[4], o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0.0f;
-    for (int b = 0; b < nb; b++) qv[b] = kv4_float(q[b * 32 + lane]);
-    for (int p = warp; p < n; p += 4) {
-        const int page = min(max(__ldg(a.table + (size_t)s * a.max_pages + p / KV4_PAGE), 0), a.n_pages - 1), t = p % KV4_PAGE;
-        const uint8_t *c = a.layer + (size_t)page * a.page_bytes + (size_t)g * 72 * hd;
-        const __half  *sc = reinterpret_cast<const __half *>(c + 64 * hd);
-        float          dot = 0.0f, v[4];
-        for (int b = 0; b < nb; b++) {
-            const int at = t * (hd / 2) + kv4_place(t, b, nb) * 16 + lane / 2;
-            const int kc = (c[at] >> (4 * (lane & 1))) & 15, vc = (c[32 * hd + at] >> (4 * (lane & 1))) & 15;
-            dot = fmaf(qv[b], (float)(kc - 8) * __half2float(sc[t * nb + b]), dot);
-            v[b] = (float)(vc - 8) * __half2float(sc[2 * hd + t * nb + b]);
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void kv4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Four nibbles of each half of w, minus 8, as fp16 pairs (low half, high half).
+__device__ __forceinline__ void kv4_unpack(uint32_t w, uint32_t (&n)[4])
+{
+    const __half2 off = __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));     // 1032
+    const __half2 six = __halves2half2(__ushort_as_half(0x2C00), __ushort_as_half(0x2C00));     // 1 / 16
+    const __half2 low = __halves2half2(__ushort_as_half(0xD480), __ushort_as_half(0xD480));     // -72
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const uint32_t x = w >> (8 * k), a = (x & 0x000F000Fu) | 0x64006400u, b = (x & 0x00F000F0u) | 0x64006400u;
+        const __half2  p = __hsub2(*reinterpret_cast<const __half2 *>(&a), off);
+        const __half2  q = __hfma2(*reinterpret_cast<const __half2 *>(&b), six, low);
+        n[2 * k] = *reinterpret_cast<const uint32_t *>(&p);
+        n[2 * k + 1] = *reinterpret_cast<const uint32_t *>(&q);
+    }
+}
+
+__device__ __forceinline__ uint32_t kv4_pack(__half lo, __half hi)
+{
+    return (uint32_t)__half_as_ushort(lo) | ((uint32_t)__half_as_ushort(hi) << 16);
+}
+
+__device__ __forceinline__ uint32_t kv4_turn(uint32_t x)
+{
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// Codes of blocks b, b + 1 (b + 1 < NB) or b alone for 16 positions:
+// r[0], r[1] positions 0-7 and 8-15 of block b, r[2], r[3] of block b + 1.
+template <bool TRANS, bool PAIR> __device__ __forceinline__ void kv4_ldsm(uint32_t (&r)[4], uint32_t addr)
+{
+    if (PAIR) {
+        if (TRANS)
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+        else
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+    } else {
+        if (TRANS)
+            asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
+                         : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+        else
+            asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];"
+                         : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+    }
+}
+
+// A place in the numbering of units: sequence i of the list, row r of its
+// KV heads and head groups, unit j of the row's nu.
+struct KvCursor {
+    int       i, r, j;
+    long long nu;
+};
+
+template <typename T, int NB, int NT, int N>
+__global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvAttendArgs a, const KvSeqs<N> list)
+{
+    using S = KvShape<T, NB, NT>;
+    constexpr int HD = S::HD, P = S::P, W = S::W, HG = S::HG, STAGE = S::STAGE, ENTRY = S::ENTRY;
+    constexpr int HL = NT * (P == 2 ? 1 : 2);             // query heads whose columns a thread holds
+    extern __shared__ __align__(128) uint8_t smem[];
+    float     *tails = reinterpret_cast<float *>(smem);   // after the loop: tail partials, in the ring's place
+    float     *heads = reinterpret_cast<float *>(smem + S::ring);
+    uint64_t  *bars = reinterpret_cast<uint64_t *>(smem + S::ring + S::heads);
+    long long *pre = reinterpret_cast<long long *>(bars + W * KV4_STAGES);     // units of a KV head before sequence i
+    __shared__ long long rid[2 * W];                      // the row of each warp's head and tail partial, -1: none
+    __shared__ int       last_s;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+    const int n = list.n, n_grp = (a.n_rep + HG - 1) / HG, R = a.n_kv * n_grp;
+    const int cap = a.max_pages * KV4_PAGE;
+    uint8_t  *ring = smem + (size_t)warp * KV4_STAGES * STAGE;
+    uint64_t *bar = bars + warp * KV4_STAGES;
+
+    if (lane == 0)
+        for (int k = 0; k < KV4_STAGES; k++) mbar_init(bar + k, 1);
+    if (tid < 2 * W) rid[tid] = -1;
+    // units before each sequence: every warp scans 32 at a time, the last one's sums carried on
+    if (warp == 0) {
+        long long run = 0;
+        for (int i0 = 0; i0 < n; i0 += 32) {
+            const int i = i0 + lane;
+            long long u = i < n ? (min(max(__ldg(a.len + list.seq[i]), 0), cap) + KV4_UNIT - 1) / KV4_UNIT : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long v = __shfl_up_sync(0xffffffffu, u, o);
+                if (lane >= o) u += v;
+            }
+            if (i < n) pre[i + 1] = run + u;
+            run += __shfl_sync(0xffffffffu, u, 31);
         }
-        const float x = warp_sum(dot) * a.scale, mn = fmaxf(m, x), f = expf(m - mn), e = expf(x - mn);
-        m = mn;
-        l = l * f + e;
-        for (int b = 0; b < nb; b++) o[b] = o[b] * f + e * v[b];
+        if (lane == 0) pre[0] = 0;
     }
-    for (int b = 0; b < nb; b++) part[warp][b * 32 + lane] = o[b];
-    part[warp][128] = m;
-    part[warp][129] = l;
+    mbar_init_fence();
     __syncthreads();
-    float M = -INFINITY, L = 0.0f, w[4];
-    for (int k = 0; k < 4; k++) M = fmaxf(M, part[k][128]);
-    for (int k = 0; k < 4; k++) {
-        w[k] = part[k][128] > -INFINITY ? expf(part[k][128] - M) : 0.0f;
-        L += w[k] * part[k][129];
+
+    // an empty sequence's row is zeros
+    for (int i = blockIdx.x; i < n; i += gridDim.x)
+        if (pre[i + 1] == pre[i])
+            for (int x = tid; x < a.n_kv * a.n_rep * HD; x += W * 32)
+                ((T *)a.out)[(size_t)i * a.out_stride + x] = kv4_from<T>(0.0f);
+
+    const long long total = pre[n] * R;
+    // CTAs with a run: none of them empty, since a shared row waits for a ticket from each
+    const long long ctas = min((long long)gridDim.x, total);
+    const bool      busy = blockIdx.x < ctas;
+    const long long cu0 = busy ? total * blockIdx.x / ctas : 0, cu1 = busy ? total * (blockIdx.x + 1) / ctas : 0;
+    const long long u0 = cu0 + (cu1 - cu0) * warp / W, u1 = cu0 + (cu1 - cu0) * (warp + 1) / W;
+
+    auto locate = [&](long long u) {
+        KvCursor p;
+        int      lo = 0, hi = n;                          // the last sequence whose units begin at or before u
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (pre[mid] * R <= u) lo = mid;
+            else hi = mid;
+        }
+        p.i = lo;
+        p.nu = pre[lo + 1] - pre[lo];
+        const long long v = u - pre[lo] * R;
+        p.r = (int)(v / p.nu);
+        p.j = (int)(v - p.r * p.nu);
+        return p;
+    };
+    auto next = [&](KvCursor &p) {
+        if (++p.j < p.nu) return;
+        p.j = 0;
+        if (++p.r < R) return;
+        p.r = 0;
+        do p.i++;
+        while (p.i < n && pre[p.i + 1] == pre[p.i]);
+        p.nu = p.i < n ? pre[p.i + 1] - pre[p.i] : 1;
+    };
+    auto page_of = [&](const KvCursor &p) {
+        return __ldg(a.table + (size_t)list.seq[p.i] * a.max_pages + p.j / (KV4_PAGE / KV4_UNIT));
+    };
+    // the unit's four pieces of its page (held inside the pool whatever the table says)
+    auto issue = [&](const KvCursor &p, int page, int k) {
+        if (lane) return;
+        page = min(max(page, 0), a.n_pages - 1);
+        const int      half = p.j & 1;
+        const uint8_t *src = a.layer + (size_t)page * a.page_bytes + (size_t)(p.r / n_grp) * 72 * HD;
+        uint8_t       *dst = ring + (size_t)k * STAGE;
+        mbar_expect_tx(bar + k, STAGE);
+        bulk_g2s(dst, src + half * 16 * HD, 16 * HD, bar + k);
+        bulk_g2s(dst + 16 * HD, src + (32 + half * 16) * HD, 16 * HD, bar + k);
+        bulk_g2s(dst + 32 * HD, src + (64 + half * 2) * HD, 2 * HD, bar + k);
+        bulk_g2s(dst + 34 * HD, src + (68 + half * 2) * HD, 2 * HD, bar + k);
+    };
+
+    uint32_t qf[NT][NB][4];                               // the query columns, as the products' B operands
+    float    fac[HL];                                     // score * fac: in units of log2
+    float    O[NT][NB][2][4], M[HL], l[HL];
+
+    // the queries of row p.r: column col is query head HG * group + col / P, part col % P
+    auto load_q = [&](const KvCursor &p) {
+        const int kvh = p.r / n_grp, grp = p.r - kvh * n_grp;
+        float     f[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const int col = nt * 8 + g, hh = grp * HG + col / P;
+            float     x[NB][8], m = 0.0f;
+            if (hh < a.n_rep) {
+                const T *q = (const T *)a.q + (size_t)p.i * a.q_stride + (size_t)(kvh * a.n_rep + hh) * HD + 8 * c;
+#pragma unroll
+                for (int b = 0; b < NB; b++) kv4_load8(q + 32 * b, a.wide_q, x[b]);
+            } else {
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[b][e] = 0.0f;
+            }
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(x[b][e]));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            // 2^sh brings m to [2^13, 2^14); held where both it and its inverse are normal numbers
+            const int sh = min(126, max(-126, 140 - (int)((__float_as_uint(fmaxf(m, 1e-38f)) >> 23) & 255)));
+            const float up = __uint_as_float((uint32_t)(sh + 127) << 23);
+            f[nt] = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - sh) << 23);
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                __half h[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float y = x[b][e] * up;
+                    h[e] = __float2half_rn(y);
+                    if (P == 2 && (col & 1)) h[e] = __float2half_rn(y - __half2float(h[e]));
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++) qf[nt][b][k] = kv4_pack(h[k], h[k + 4]);
+            }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            if (P == 2) fac[nt] = __shfl_sync(0xffffffffu, f[nt], 8 * c);
+            else {
+                fac[2 * nt] = __shfl_sync(0xffffffffu, f[nt], 8 * c);
+                fac[2 * nt + 1] = __shfl_sync(0xffffffffu, f[nt], 8 * c + 4);
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < HL; h++) {
+            M[h] = -INFINITY;
+            l[h] = 0.0f;
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) O[nt][b][0][k] = O[nt][b][1][k] = 0.0f;
+    };
+    // NB fp16 scales of one position, as pairs; zeros for a position past the end
+    auto scales = [&](const uint8_t *base, int t, bool live, uint32_t (&w)[(NB + 1) / 2]) {
+        if (NB == 4) {
+            const uint2 v = *reinterpret_cast<const uint2 *>(base + t * 8);
+            w[0] = live ? v.x : 0u;
+            w[(NB + 1) / 2 - 1] = live ? v.y : 0u;
+        } else if (NB == 2) {
+            w[0] = live ? *reinterpret_cast<const uint32_t *>(base + t * 4) : 0u;
+        } else {
+            const uint16_t *p = reinterpret_cast<const uint16_t *>(base) + t * NB;
+#pragma unroll
+            for (int k = 0; k < (NB + 1) / 2; k++)
+                w[k] = live ? (uint32_t)p[2 * k] | (2 * k + 1 < NB ? (uint32_t)p[2 * k + 1] << 16 : 0u) : 0u;
+        }
+    };
+    auto half_of = [](uint32_t w, int k) { return __half2float(__ushort_as_half((unsigned short)(k ? w >> 16 : w & 0xFFFFu))); };
+
+    auto unit = [&](const uint8_t *st, int j, int len) {
+        const uint32_t kaddr = smem_addr(st), vaddr = kaddr + 16 * HD;
+        const int      mt_row = (lane & 7) + ((lane >> 3) & 1) * 8, mt_blk = lane >> 4;
+        float          sc[2][2][HL];
+        uint32_t       vs[2][2][(NB + 1) / 2];
+        float          top[HL], vmax = 0.0f;
+#pragma unroll
+        for (int h = 0; h < HL; h++) top[h] = -INFINITY;
+#pragma unroll
+        for (int mt = 0; mt < 2; mt++) {
+            float acc[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) acc[nt][k] = 0.0f;
+            const int  t = mt * 16 + g, t2 = mt * 16 + mt_row;
+            const bool live0 = j * KV4_UNIT + t < len, live1 = j * KV4_UNIT + t + 8 < len;
+            uint32_t   ks0[(NB + 1) / 2], ks1[(NB + 1) / 2];
+            scales(st + 32 * HD, t, true, ks0);
+            scales(st + 32 * HD, t + 8, true, ks1);
+            scales(st + 34 * HD, t, live0, vs[mt][0]);
+            scales(st + 34 * HD, t + 8, live1, vs[mt][1]);
+#pragma unroll
+            for (int b = 0; b < NB; b += 2) {
+                uint32_t r[4];
+                if (b + 1 < NB) kv4_ldsm<false, true>(r, kaddr + t2 * (HD / 2) + kv4_place(t2, b + mt_blk, NB) * 16);
+                else kv4_ldsm<false, false>(r, kaddr + t2 * (HD / 2) + kv4_place(t2, b, NB) * 16);
+#pragma unroll
+                for (int d = 0; d < 2; d++) {
+                    if (b + d >= NB) continue;
+                    uint32_t x[4], y[4];
+                    kv4_unpack(r[2 * d], x);
+                    kv4_unpack(r[2 * d + 1], y);
+                    const float s0 = half_of(ks0[(b + d) / 2], (b + d) & 1), s1 = half_of(ks1[(b + d) / 2], (b + d) & 1);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        kv4_mma(e, x[0], y[0], x[1], y[1], qf[nt][b + d][0], qf[nt][b + d][1]);
+                        kv4_mma(e, x[2], y[2], x[3], y[3], qf[nt][b + d][2], qf[nt][b + d][3]);
+                        acc[nt][0] = fmaf(s0, e[0], acc[nt][0]);
+                        acc[nt][1] = fmaf(s0, e[1], acc[nt][1]);
+                        acc[nt][2] = fmaf(s1, e[2], acc[nt][2]);
+                        acc[nt][3] = fmaf(s1, e[3], acc[nt][3]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < HL; h++) {
+                const int nt = P == 2 ? h : h >> 1, k = h & 1;
+                sc[mt][0][h] = (P == 2 ? acc[nt][0] + acc[nt][1] : acc[nt][k]) * fac[h];
+                sc[mt][1][h] = (P == 2 ? acc[nt][2] + acc[nt][3] : acc[nt][2 + k]) * fac[h];
+                if (!live0) sc[mt][0][h] = -INFINITY;
+                if (!live1) sc[mt][1][h] = -INFINITY;
+                top[h] = fmaxf(top[h], fmaxf(sc[mt][0][h], sc[mt][1][h]));
+            }
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int k = 0; k < (NB + 1) / 2; k++)
+                    vmax = fmaxf(vmax, fmaxf(fabsf(half_of(vs[mt][x][k], 0)), fabsf(half_of(vs[mt][x][k], 1))));
+        }
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+            vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+#pragma unroll
+            for (int h = 0; h < HL; h++) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], o));
+        }
+        // every V scale of the unit is below 2^ve (scales below 2^-24 are zeros)
+        const float ve = (float)max((int)(__float_as_uint(vmax) >> 23) - 126, -24);
+        float       alpha[HL];
+#pragma unroll
+        for (int h = 0; h < HL; h++) {
+            const float m = fmaxf(M[h], top[h] + ve);
+            alpha[h] = kv4_ex2(M[h] - m);
+            M[h] = m;
+            float sum = 0.0f;
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const bool live = j * KV4_UNIT + mt * 16 + g + 8 * x < len;
+                    sc[mt][x][h] = live ? kv4_ex2(sc[mt][x][h] - m + 14.0f) : 0.0f;
+                    sum += sc[mt][x][h];
+                }
+            l[h] = fmaf(l[h], alpha[h], sum);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b += 2) {
+            uint32_t r[2][4];
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++) {
+                const int t2 = mt * 16 + mt_row;
+                if (b + 1 < NB) kv4_ldsm<true, true>(r[mt], vaddr + t2 * (HD / 2) + kv4_place(t2, b + mt_blk, NB) * 16);
+                else kv4_ldsm<true, false>(r[mt], vaddr + t2 * (HD / 2) + kv4_place(t2, b, NB) * 16);
+            }
+#pragma unroll
+            for (int d = 0; d < 2; d++) {
+                if (b + d >= NB) continue;
+                float e[NT][2][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) e[nt][0][k] = e[nt][1][k] = 0.0f;
+#pragma unroll
+                for (int mt = 0; mt < 2; mt++) {
+                    uint32_t x[4], y[4];
+                    kv4_unpack(r[mt][2 * d], x);
+                    kv4_unpack(r[mt][2 * d + 1], y);
+                    const float v0 = half_of(vs[mt][0][(b + d) / 2], (b + d) & 1), v1 = half_of(vs[mt][1][(b + d) / 2], (b + d) & 1);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        uint32_t p0, p1;
+                        if (P == 2) {
+                            const float  w0 = sc[mt][0][nt] * v0, w1 = sc[mt][1][nt] * v1;
+                            const __half h0 = __float2half_rn(w0), h1 = __float2half_rn(w1);
+                            p0 = kv4_pack(h0, __float2half_rn(w0 - __half2float(h0)));
+                            p1 = kv4_pack(h1, __float2half_rn(w1 - __half2float(h1)));
+                        } else {
+                            const __half2 h0 = __floats2half2_rn(sc[mt][0][2 * nt] * v0, sc[mt][0][(2 * nt + 1) % HL] * v0);
+                            const __half2 h1 = __floats2half2_rn(sc[mt][1][2 * nt] * v1, sc[mt][1][(2 * nt + 1) % HL] * v1);
+                            p0 = *reinterpret_cast<const uint32_t *>(&h0);
+                            p1 = *reinterpret_cast<const uint32_t *>(&h1);
+                        }
+                        const uint32_t b0 = kv4_turn(p0), b1 = kv4_turn(p1);
+                        kv4_mma(e[nt][0], x[0], x[1], y[0], y[1], b0, b1);
+                        kv4_mma(e[nt][1], x[2], x[3], y[2], y[3], b0, b1);
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int s = 0; s < 2; s++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            O[nt][b + d][s][k] = fmaf(O[nt][b + d][s][k], alpha[P == 2 ? nt : 2 * nt + (k & 1)], e[nt][s][k]);
+            }
+        }
+    };
+    // f(head of the group, dimension, sum) for what this thread holds of the row
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    const float *o = O[nt][b][s];
+                    const int    d = 32 * b + 4 * g + 2 * s;
+                    if (P == 2) {
+                        f(nt * 4 + c, nt, d, o[0] + o[1]);
+                        f(nt * 4 + c, nt, d + 1, o[2] + o[3]);
+                    } else {
+                        f(nt * 8 + 2 * c, 2 * nt, d, o[0]);
+                        f(nt * 8 + 2 * c, 2 * nt, d + 1, o[2]);
+                        f(nt * 8 + 2 * c + 1, (2 * nt + 1) % HL, d, o[1]);
+                        f(nt * 8 + 2 * c + 1, (2 * nt + 1) % HL, d + 1, o[3]);
+                    }
+                }
+    };
+    auto store_part = [&](float *e) {
+        each([&](int h, int, int d, float v) { e[h * (HD + 2) + d] = v; });
+        if (g == 0)
+#pragma unroll
+            for (int h = 0; h < HL; h++) {
+                const int hh = P == 2 ? h * 4 + c : (h >> 1) * 8 + 2 * c + (h & 1);
+                e[hh * (HD + 2) + HD] = M[h];
+                e[hh * (HD + 2) + HD + 1] = l[h];
+            }
+    };
+    auto sum_l = [&] {
+#pragma unroll
+        for (int h = 0; h < HL; h++)
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], o);
+    };
+
+    bool tail = false;                                    // this warp ends inside a row that began in its run
+    if (u0 < u1) {
+        KvCursor at = locate(u0), ahead = at;
+        int      pages[KV4_STAGES + 1];
+        {
+            KvCursor p = at;
+#pragma unroll
+            for (int k = 0; k <= KV4_STAGES; k++) {       // independent loads
+                pages[k] = u0 + k < u1 ? page_of(p) : 0;
+                if (u0 + k + 1 < u1) next(p);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < KV4_STAGES; k++)
+            if (u0 + k < u1) {
+                issue(ahead, pages[k], k);
+                if (u0 + k + 1 < u1) next(ahead);
+            }
+        int page = pages[KV4_STAGES];                     // of the unit that is issued next
+        load_q(at);
+        int  j0 = at.j, k = 0;
+        unsigned phase = 0;
+        int  len = min(__ldg(a.len + list.seq[at.i]), cap);
+        for (long long u = u0; u < u1; u++) {
+            // a wait that gives up leaves NaN behind (the copies are this
+            // warp's own, so it never should)
+            const bool come = mbar_wait(bar + k, phase, nullptr);
+            unit(ring + (size_t)k * STAGE, at.j, len);
+            if (!come) l[0] = NAN;
+            __syncwarp();
+            if (u + KV4_STAGES < u1) {
+                issue(ahead, page, k);
+                if (u + KV4_STAGES + 1 < u1) {
+                    next(ahead);
+                    page = page_of(ahead);
+                }
+            }
+            if (++k == KV4_STAGES) {
+                k = 0;
+                phase ^= 1;
+            }
+            const bool row_end = at.j + 1 == at.nu, run_end = u + 1 == u1;
+            if (row_end || run_end) {
+                sum_l();
+                const long long row = (long long)at.i * R + at.r;
+                if (j0 > 0) {
+                    store_part(heads + warp * ENTRY);
+                    if (lane == 0) rid[2 * warp] = row;
+                } else if (!row_end) {
+                    tail = true;
+                    if (lane == 0) rid[2 * warp + 1] = row;
+                } else {
+                    const int kvh = at.r / n_grp, grp = at.r - kvh * n_grp;
+                    T        *o = (T *)a.out + (size_t)at.i * a.out_stride + (size_t)kvh * a.n_rep * HD;
+                    each([&](int h, int hl, int d, float v) {
+                        if (grp * HG + h < a.n_rep) o[(size_t)(grp * HG + h) * HD + d] = kv4_from<T>(v / l[hl]);
+                    });
+                }
+                if (!run_end) {
+                    next(at);
+                    j0 = 0;
+                    load_q(at);
+                    len = min(__ldg(a.len + list.seq[at.i]), cap);
+                }
+            } else {
+                at.j++;
+            }
+        }
     }
-    if ((int)threadIdx.x < hd) {
-        float v = 0.0f;
-        for (int k = 0; k < 4; k++) v += w[k] * part[k][threadIdx.x];
-        ((T *)a.out)[(size_t)i * a.out_stride + (size_t)head * hd + threadIdx.x] = kv4_from<T>(n > 0 ? v / L : 0.0f);
+    __syncthreads();                                      // every ring is idle
+    if (tail) store_part(tails + warp * ENTRY);
+    __syncthreads();
+
+    // rows that this CTA's warps share
+    auto entry = [&](int e) { return (e & 1) ? tails + (e >> 1) * ENTRY : heads + (e >> 1) * ENTRY; };
+    auto write = [&](long long row, int x, float v) {
+        const int i = (int)(row / R), r = (int)(row - (long long)i * R), kvh = r / n_grp, grp = r - kvh * n_grp, h = grp * HG + x / HD;
+        if (h < a.n_rep)
+            ((T *)a.out)[(size_t)i * a.out_stride + (size_t)(kvh * a.n_rep + h) * HD + x % HD] = kv4_from<T>(v);
+    };
+    for (int e = 0; e < 2 * W; e++) {
+        const long long row = rid[e];
+        if (row < 0) continue;
+        int end = e + 1;                                  // the row's partials: e .. end - 1 (-1 between them)
+        while (end < 2 * W && (rid[end] < 0 || rid[end] == row)) end++;
+        const int       i = (int)(row / R);
+        const long long nu = pre[i + 1] - pre[i], first = pre[i] * R + (row - (long long)i * R) * nu;
+        const bool      whole = first >= cu0 && first + nu <= cu1;
+        float          *out = a.part + ((size_t)blockIdx.x * 2 + (first >= cu0)) * ENTRY;
+        for (int x = tid; x < HG * HD; x += W * 32) {
+            const int h = x / HD, at = h * (HD + 2);
+            float     m = -INFINITY, L = 0.0f, v = 0.0f;
+            for (int k = e; k < end; k++)
+                if (rid[k] >= 0) m = fmaxf(m, entry(k)[at + HD]);
+            for (int k = e; k < end; k++)
+                if (rid[k] >= 0) {
+                    const float w = kv4_ex2(entry(k)[at + HD] - m);
+                    L = fmaf(w, entry(k)[at + HD + 1], L);
+                    v = fmaf(w, entry(k)[at + x % HD], v);
+                }
+            if (whole) write(row, x, v / L);
+            else {
+                out[at + x % HD] = v;
+                if (x % HD == 0) {
+                    out[at + HD] = m;
+                    out[at + HD + 1] = L;
+                }
+            }
+        }
+        if (!whole) {
+            // the CTAs of the row: those whose runs hold its units
+            auto cta_of = [&](long long u) {
+                long long b = u * ctas / total;
+                while (total * (b + 1) / ctas <= u) b++;
+                while (total * b / ctas > u) b--;
+                return (int)b;
+            };
+            const int c0 = cta_of(first), c1 = cta_of(first + nu - 1);
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) last_s = atomicAdd(a.count + c0, 1u) == (unsigned)(c1 - c0);
+            __syncthreads();
+            if (last_s) {
+                __threadfence();
+                for (int x = tid; x < HG * HD; x += W * 32) {
+                    const int h = x / HD, at = h * (HD + 2);
+                    auto      part = [&](int b) { return a.part + ((size_t)b * 2 + (b == c0)) * ENTRY + at; };
+                    float     m = -INFINITY, L = 0.0f, v = 0.0f;
+#pragma unroll 8
+                    for (int b = c0; b <= c1; b++) m = fmaxf(m, __ldcg(part(b) + HD));
+#pragma unroll 8
+                    for (int b = c0; b <= c1; b++) {
+                        const float w = kv4_ex2(__ldcg(part(b) + HD) - m);
+                        L = fmaf(w, __ldcg(part(b) + HD + 1), L);
+                        v = fmaf(w, __ldcg(part(b) + x % HD), v);
+                    }
+                    write(row, x, v / L);
+                }
+                if (tid == 0) a.count[c0] = 0;            // as the next call finds it
+            }
+            __syncthreads();
+        }
+        e = end - 1;
     }
 }
