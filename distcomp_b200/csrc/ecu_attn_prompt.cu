@@ -1,6 +1,6 @@
 // ecu_attn_prompt.cu -- causal attention of packed prompts behind
 // engine_cuda.h.
-#include "ecu_kv4.cuh"
+#include "ecu_attn_prompt.cuh"
 #include "ecu_kv4.h"
 #include "ecu_model.h"
 
@@ -8,65 +8,10 @@
 #include <climits>
 #include <cmath>
 #include <exception>
+#include <numeric>
+#include <vector>
 
 #define PA_LIST 1024              // sequences of one launch
-
-struct PromptArgs {
-    const void *q, *k, *v;
-    void       *out;
-    long        q_stride, k_stride, v_stride, out_stride;
-    int         n_rep, hd;
-    float       scale;
-};
-
-template <int N> struct PromptSeqs {
-    int n;
-    int q0[N + 1], k0[N + 1];
-};
-
-// One CTA per (query row, head): a warp per key, lanes over dimensions.
-template <typename T, int N>
-__global__ void __launch_bounds__(128) k_attn_prompt_simple(const PromptArgs a, const PromptSeqs<N> list)
-{
-    __shared__ float part[4][130];
-    const int r = list.q0[0] + blockIdx.x, head = blockIdx.y, g = head / a.n_rep, hd = a.hd, nb = hd / 32;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int       lo = 0, hi = list.n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (list.q0[mid] <= r) lo = mid;
-        else hi = mid;
-    }
-    const int n = list.k0[lo + 1] - list.k0[lo] - (list.q0[lo + 1] - 1 - r);    // keys that the row sees
-    const T  *q = (const T *)a.q + (size_t)r * a.q_stride + (size_t)head * hd;
-    float     qv[4], o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0.0f;
-    for (int b = 0; b < nb; b++) qv[b] = kv4_float(q[b * 32 + lane]);
-    for (int p = warp; p < n; p += 4) {
-        const T *k = (const T *)a.k + (size_t)(list.k0[lo] + p) * a.k_stride + (size_t)g * hd;
-        const T *v = (const T *)a.v + (size_t)(list.k0[lo] + p) * a.v_stride + (size_t)g * hd;
-        float    dot = 0.0f;
-        for (int b = 0; b < nb; b++) dot = fmaf(qv[b], kv4_float(k[b * 32 + lane]), dot);
-        const float x = warp_sum(dot) * a.scale, mn = fmaxf(m, x), f = expf(m - mn), e = expf(x - mn);
-        m = mn;
-        l = l * f + e;
-        for (int b = 0; b < nb; b++) o[b] = o[b] * f + e * kv4_float(v[b * 32 + lane]);
-    }
-    for (int b = 0; b < nb; b++) part[warp][b * 32 + lane] = o[b];
-    part[warp][128] = m;
-    part[warp][129] = l;
-    __syncthreads();
-    float M = -INFINITY, L = 0.0f, w[4];
-    for (int k = 0; k < 4; k++) M = fmaxf(M, part[k][128]);
-    for (int k = 0; k < 4; k++) {
-        w[k] = part[k][128] > -INFINITY ? expf(part[k][128] - M) : 0.0f;
-        L += w[k] * part[k][129];
-    }
-    if ((int)threadIdx.x < hd) {
-        float x = 0.0f;
-        for (int k = 0; k < 4; k++) x += w[k] * part[k][threadIdx.x];
-        ((T *)a.out)[(size_t)r * a.out_stride + (size_t)head * hd + threadIdx.x] = kv4_from<T>(n > 0 ? x / L : 0.0f);
-    }
-}
 
 static int say(const char *why)
 {
@@ -74,23 +19,90 @@ static int say(const char *why)
     return -1;
 }
 
-template <typename T, int N>
-static int launch(const PromptArgs &a, int n_head, const int *cu_q, const int *cu_k, int n, cudaStream_t s)
+typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiled encode_tiled()
+{
+    static const EncodeTiled f = [] {
+        void                           *p = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r) != cudaSuccess ||
+            r != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return (EncodeTiled)p;
+    }();
+    return f;
+}
+
+// Rows x heads x head_dim in boxes of 128 rows of 64 elements of one head.
+static int make_map(CUtensorMap *m, int dtype, const void *p, int head_dim, int heads, long rows, long stride)
+{
+    const EncodeTiled f = encode_tiled();
+    if (!f) return say("the driver has no cuTensorMapEncodeTiled");
+    const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)head_dim * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[3] = {64, 1, 128}, ones[3] = {1, 1, 1};
+    const CUresult   r = f(m, dtype == ECU_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                           const_cast<void *>(p), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        ecu_set_error(nullptr, 0, "ecu_attn_prompt: the rows cannot be mapped (%d)", (int)r);
+        return -1;
+    }
+    return 0;
+}
+
+template <typename T, int HD, int N>
+static int launch(const CUtensorMap (&m)[3], const PromptArgs &a, const int *cu_q, const int *cu_k, const int *order, int n,
+                  cudaStream_t s)
 {
     PromptSeqs<N> list;
     list.n = n;
-    for (int i = 0; i <= n; i++) {
-        list.q0[i] = cu_q[i];
-        list.k0[i] = cu_k[i];
+    long long ctas = 0;
+    for (int i = 0; i < n; i++) {
+        const int x = order[i];
+        list.q0[i] = cu_q[x];
+        list.nq[i] = cu_q[x + 1] - cu_q[x];
+        list.k0[i] = cu_k[x];
+        list.nk[i] = cu_k[x + 1] - cu_k[x];
+        list.cta[i] = (int)ctas;
+        ctas += (((long long)(list.nq[i] + 127) / 128 * a.n_rep + 1) / 2) * a.n_kv;
     }
-    if (cu_q[n] == cu_q[0]) return 0;
-    k_attn_prompt_simple<T, N><<<dim3((unsigned)(cu_q[n] - cu_q[0]), (unsigned)n_head), 128, 0, s>>>(a, list);
-    const cudaError_t e = cudaGetLastError();
+    if (ctas > INT_MAX) return say("too many rows and heads");
+    list.cta[n] = (int)ctas;
+    auto kern = k_attn_prompt<T, HD, N>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PaShape<HD>::smem);
+    if (e == cudaSuccess) {
+        kern<<<(unsigned)ctas, PA_THREADS, PaShape<HD>::smem, s>>>(m[0], m[1], m[2], a, list);
+        e = cudaGetLastError();
+    }
     if (e != cudaSuccess) {
         ecu_set_error(nullptr, 0, "ecu_attn_prompt: launch failed: %s", cudaGetErrorString(e));
         return -1;
     }
     ecu_count_launches(1);
+    return 0;
+}
+
+template <typename T>
+static int launch_all(const CUtensorMap (&m)[3], const PromptArgs &a, int head_dim, const int *cu_q, const int *cu_k, int n_seq,
+                      cudaStream_t s)
+{
+    // sequences with query rows, the most keys first: their last tiles are the longest walks
+    std::vector<int> order;
+    for (int i = 0; i < n_seq; i++)
+        if (cu_q[i + 1] > cu_q[i]) order.push_back(i);
+    std::stable_sort(order.begin(), order.end(),
+                     [&](int x, int y) { return cu_k[x + 1] - cu_k[x] > cu_k[y + 1] - cu_k[y]; });
+    for (int i = 0; i < (int)order.size(); i += PA_LIST) {
+        const int  c = std::min<int>(PA_LIST, (int)order.size() - i);
+        const int *o = order.data() + i;
+        const int  rc = head_dim == 128 ? (c <= 32 ? launch<T, 128, 32>(m, a, cu_q, cu_k, o, c, s) : launch<T, 128, PA_LIST>(m, a, cu_q, cu_k, o, c, s))
+                                        : (c <= 32 ? launch<T, 64, 32>(m, a, cu_q, cu_k, o, c, s) : launch<T, 64, PA_LIST>(m, a, cu_q, cu_k, o, c, s));
+        if (rc != 0) return rc;
+    }
     return 0;
 }
 
@@ -108,7 +120,7 @@ extern "C" int ecu_attn_prompt(int dtype, const void *q, const void *k, const vo
         return -1;
     }
     if (n_seq < 0 || (n_seq > 0 && !cu_q)) return say("null offsets or negative count");
-    if (!std::isfinite(scale)) return say("the scale is not finite");
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return say("the scale is not a positive finite number");
     if (n_seq == 0) return 0;
     if (!cu_k) cu_k = cu_q;
     if (cu_q[0] != 0 || cu_k[0] != 0) return say("offsets begin at 0");
@@ -117,6 +129,8 @@ extern "C" int ecu_attn_prompt(int dtype, const void *q, const void *k, const vo
     if (cu_q[n_seq] == 0) return 0;
     const long es = 2, qr = (long)n_head * head_dim, kr = (long)n_head_kv * head_dim;
     const bool keys = cu_k[n_seq] > 0;
+    if (cu_q[n_seq] == 1) q_stride = out_stride = qr;       // one row: no stride
+    if (cu_k[n_seq] <= 1) k_stride = v_stride = kr;
     if (!q || !out || (keys && (!k || !v))) return say("null rows");
     if ((cu_q[n_seq] > 1 && (q_stride < qr || out_stride < qr)) || (cu_k[n_seq] > 1 && (k_stride < kr || v_stride < kr)))
         return say("rows overlap: a stride below the row's heads");
@@ -131,15 +145,18 @@ extern "C" int ecu_attn_prompt(int dtype, const void *q, const void *k, const vo
     }
     DeviceScope d(device);
     if (!d.ok) return say("the device cannot be used");
-    PromptArgs a{q, k, v, out, q_stride, k_stride, v_stride, out_stride, n_head / n_head_kv, head_dim, scale};
-    for (int i = 0; i < n_seq; i += PA_LIST) {
-        const int m = std::min(PA_LIST, n_seq - i);
-        const int *cq = cu_q + i, *ck = cu_k + i;
-        const cudaStream_t s = (cudaStream_t)stream;
-        int rc;
-        if (dtype == ECU_F16) rc = m <= 64 ? launch<__half, 64>(a, n_head, cq, ck, m, s) : launch<__half, PA_LIST>(a, n_head, cq, ck, m, s);
-        else rc = m <= 64 ? launch<__nv_bfloat16, 64>(a, n_head, cq, ck, m, s) : launch<__nv_bfloat16, PA_LIST>(a, n_head, cq, ck, m, s);
-        if (rc != 0) return rc;
+    PromptArgs  a{v, out, v_stride, out_stride, n_head_kv, n_head / n_head_kv, scale};
+    CUtensorMap m[3];
+    // a pointer that no row is read from is not mapped: q stands in
+    if (make_map(m + 0, dtype, q, head_dim, n_head, cu_q[n_seq], q_stride) != 0 ||
+        make_map(m + 1, dtype, keys ? k : q, head_dim, keys ? n_head_kv : 1, keys ? cu_k[n_seq] : 1, keys ? k_stride : qr) != 0 ||
+        make_map(m + 2, dtype, keys ? v : q, head_dim, keys ? n_head_kv : 1, keys ? cu_k[n_seq] : 1, keys ? v_stride : qr) != 0)
+        return -1;
+    const cudaStream_t s = (cudaStream_t)stream;
+    try {
+        return dtype == ECU_F16 ? launch_all<__half>(m, a, head_dim, cu_q, cu_k, n_seq, s)
+                                : launch_all<__nv_bfloat16>(m, a, head_dim, cu_q, cu_k, n_seq, s);
+    } catch (const std::exception &e) {
+        return say(e.what());
     }
-    return 0;
 }

@@ -1,0 +1,430 @@
+// ecu_attn_prompt.cuh -- causal attention of packed prompts on tcgen05.
+//
+// A CTA works on two query tiles of 128 rows (a "pair": query heads of one KV
+// head, so that both read the same K and V) and walks their keys 128 at a
+// time:  S = Q K^T (fp32, tensor memory), P = exp2(S * scale * log2 e - m)
+// rounded to 16 bits over S's place, O += P V (fp32, tensor memory).  The two
+// tiles take turns: while one's softmax runs, the tensor core computes the
+// other's products.  Roles by warp:
+//   0-3, 4-7  softmax of tile 0 and 1, a thread per row; O's rescaling and
+//             the output at the end
+//   8         copies: Q once, K and V tiles through a ring (TMA)
+//   9         issues the products (one thread)
+//   10, 11    clean V tiles that some row sees only in part: an element that
+//             is not finite would turn 0 * element into NaN for rows that do
+//             not see it.  Such elements are zeroed in shared memory, their
+//             keys noted, and added to the rows that do see them at the end.
+// The maximum that P is taken relative to follows the running one only when
+// that has grown by more than 2^8 (P stays far inside fp16's range, and the
+// sums are fp32), so O is rescaled a few times per row at most.
+//
+// Tensor memory: S of tile t at column 128 t (P in its first 64), O at
+// 256 + HD t.  Shared memory: tiles of 128 rows of 64 elements (128 bytes,
+// 128-byte swizzle), HD / 64 of them side by side; Q and K are K-major
+// operands, V (keys x dimensions) is read MN-major.
+#pragma once
+#include "ecu_kv4.cuh"
+#include "ecu_pipe.cuh"
+
+#include <cuda.h>
+
+#define PA_THREADS 384
+#define PA_BOX 16384                       // 128 rows x 128 bytes
+
+template <int HD> struct PaShape {
+    static constexpr int B = HD / 64;              // boxes of a tile
+    static constexpr int TILE = B * PA_BOX;
+    // at hd 64 more stages than the walk needs: one CTA an SM, which takes all of tensor memory
+    static constexpr int STAGES = HD == 128 ? 4 : 6;
+    static constexpr size_t smem = 1024 + (size_t)(2 + STAGES) * TILE;
+};
+
+struct PromptArgs {
+    const void *v;
+    void       *out;
+    long        v_stride, out_stride;
+    int         n_kv, n_rep;
+    float       scale;
+};
+
+// Sequences of one launch by value, the longest first: where their rows lie
+// and the CTA that begins them.
+template <int N> struct PromptSeqs {
+    int n;
+    int q0[N], nq[N], k0[N], nk[N], cta[N + 1];
+};
+
+__device__ __forceinline__ void pa_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void pa_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void pa_commit(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+__device__ __forceinline__ void pa_tma(uint32_t dst, const CUtensorMap *map, int x, int head, int row, uint64_t *bar)
+{
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(head), "r"(row), "r"(smem_addr(bar))
+                 : "memory");
+}
+
+// Shared-memory operand: K-major rows 128 B apart, groups of 8 rows 1024 B
+// (SBO); MN-major: 64 elements a row, groups of 8 k 1024 B apart (SBO), the
+// next 64 elements a box further (LBO).  Version 1, 128-byte swizzle.
+__device__ __forceinline__ uint64_t pa_desc(uint32_t addr, uint32_t lbo)
+{
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+__device__ __forceinline__ void pa_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+                 : "memory");
+}
+
+__device__ __forceinline__ void pa_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+                 : "memory");
+}
+
+#define PA_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
+#define PA_W8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
+
+// 32 columns of this thread's row (its warp's 32 lanes)
+__device__ __forceinline__ void pa_ld32(uint32_t (&v)[32], uint32_t addr)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+                 "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : PA_R8(v, 0), PA_R8(v, 8), PA_R8(v, 16), PA_R8(v, 24)
+                 : "r"(addr)
+                 : "memory");
+}
+
+__device__ __forceinline__ void pa_st32(uint32_t addr, const uint32_t (&v)[32])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+                 "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+                 PA_W8(v, 0), PA_W8(v, 8), PA_W8(v, 16), PA_W8(v, 24)
+                 : "memory");
+}
+
+__device__ __forceinline__ void pa_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// the loaded values are used after the wait only
+__device__ __forceinline__ void pa_pin(uint32_t (&v)[32])
+{
+#pragma unroll
+    for (int x = 0; x < 32; x++) asm volatile("" : "+r"(v[x]));
+}
+__device__ __forceinline__ void pa_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t pa_pair(__half, float lo, float hi)
+{
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pa_pair(__nv_bfloat16, float lo, float hi)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+template <typename T> struct PaBits;     // exponent mask of two elements, and what carries it into the sign when it is full
+template <> struct PaBits<__half> { static constexpr uint32_t exp = 0x7C007C00u, one = 0x04000400u, fmt = 0; };
+template <> struct PaBits<__nv_bfloat16> { static constexpr uint32_t exp = 0x7F807F80u, one = 0x00800080u, fmt = 1; };
+
+template <typename T, int HD, int N>
+__global__ void __launch_bounds__(PA_THREADS, 1)
+k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+              const PromptArgs a, const PromptSeqs<N> list)
+{
+    using S = PaShape<HD>;
+    constexpr int ST = S::STAGES, B = S::B;
+    extern __shared__ uint8_t raw[];
+    uint8_t *sm = reinterpret_cast<uint8_t *>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    uint8_t *ring = sm + 2 * S::TILE;
+    __shared__ __align__(8) uint64_t q_full, full[ST], empty[ST], s_full[2], p_full[2], due[4], clean[4], drain;
+    __shared__ uint32_t              tmem_s, bad[4][4];       // keys of the partly seen tiles with cleaned elements
+    __shared__ int                   any_bad, dead;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    // this CTA's pair: the sequence, the KV head, the two items (tile, head); the
+    // latest tiles, which have most keys, come first
+    int lo = 0, hi = list.n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (list.cta[mid] <= (int)blockIdx.x) lo = mid;
+        else hi = mid;
+    }
+    const int nq = list.nq[lo], nk = list.nk[lo], q0 = list.q0[lo], k0 = list.k0[lo];
+    const int items = (nq + 127) / 128 * a.n_rep, pairs = (items + 1) / 2;
+    const int at = (int)blockIdx.x - list.cta[lo], kvh = at % a.n_kv, item = 2 * (pairs - 1 - at / a.n_kv);
+    const int n_tile = min(2, items - item);
+    auto tile_of = [&](int t) { return (item + t) / a.n_rep; };
+    auto head_of = [&](int t) { return kvh * a.n_rep + (item + t) % a.n_rep; };
+    auto seen = [&](int row) { return min(nk, max(0, row + 1 + nk - nq)); };    // keys that a row sees
+    // key tiles: n in all, those below n_plain seen whole by every row; the rows
+    // of a pair end at most 255 keys apart, so at most 3 are seen in part
+    const int n = (seen(min(tile_of(n_tile - 1) * 128 + 128, nq) - 1) + 127) / 128;
+    const int n_plain = seen(tile_of(0) * 128) / 128;
+
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_s)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (tid == 0) {
+        mbar_init(&q_full, 1);
+        for (int s = 0; s < ST; s++) {
+            mbar_init(full + s, 1);
+            mbar_init(empty + s, 1);
+        }
+        for (int t = 0; t < 2; t++) {
+            mbar_init(s_full + t, 1);
+            mbar_init(p_full + t, 4);
+        }
+        for (int j = 0; j < 4; j++) {
+            mbar_init(due + j, 1);
+            mbar_init(clean + j, 2);
+        }
+        mbar_init(&drain, 1);
+        mbar_init_fence();
+        any_bad = dead = 0;
+    }
+    if (tid < 16) bad[tid >> 2][tid & 3] = 0;
+    pa_fence_before();
+    __syncthreads();
+    pa_fence_after();
+    const uint32_t tmem = tmem_s;
+    // every wait is bounded; one that gives up lets the others give up too
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+        if (mbar_try_wait(bar, parity)) return;
+        if (!mbar_wait<true>(bar, parity, &dead)) atomicExch(&dead, 1);
+    };
+    auto gone = [&] { return *reinterpret_cast<volatile int *>(&dead) != 0; };
+
+    if (warp == 8) {
+        if (lane == 0 && n > 0) {
+            mbar_expect_tx(&q_full, (uint32_t)n_tile * S::TILE);
+            for (int t = 0; t < n_tile; t++)
+                for (int b = 0; b < B; b++)
+                    pa_tma(smem_addr(sm + t * S::TILE + b * PA_BOX), &mq, b * 64, head_of(t), q0 + tile_of(t) * 128, &q_full);
+            int i = 0;
+            for (; i < 2 * n; i++) {              // K and V of key tile i / 2
+                const int s = i % ST;
+                if (i >= ST) wait(empty + s, (uint32_t)(i / ST - 1) & 1u);
+                if (gone()) break;
+                mbar_expect_tx(full + s, S::TILE);
+                for (int b = 0; b < B; b++)
+                    pa_tma(smem_addr(ring + s * S::TILE + b * PA_BOX), (i & 1) ? &mv : &mk, b * 64, kvh, k0 + i / 2 * 128, full + s);
+                // the cleaners may look at the stage's barrier only now that it
+                // counts this tile: its phase's parity would fit an earlier one too
+                if ((i & 1) && i / 2 >= n_plain) mbar_arrive(due + (i / 2 - n_plain));
+            }
+            if (gone()) {                         // nothing may still be on its way into shared memory
+                mbar_drain(&q_full, 0, wait_limit_ns());
+                for (int x = i > ST ? i - ST : 0; x < i; x++) mbar_drain(full + x % ST, (uint32_t)(x / ST) & 1u, wait_limit_ns());
+            }
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        if (lane == 0 && n > 0) {
+            // fp32 sums, M = 128; S: N = 128 keys; O: N = HD dimensions, V MN-major
+            const uint32_t ids = (1u << 4) | (PaBits<T>::fmt << 7) | (PaBits<T>::fmt << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+            const uint32_t ido = (1u << 4) | (PaBits<T>::fmt << 7) | (PaBits<T>::fmt << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((128u >> 4) << 24);
+            auto qk = [&](int t, int s) {
+                const uint32_t q = smem_addr(sm + t * S::TILE), k = smem_addr(ring + s * S::TILE);
+#pragma unroll
+                for (int x = 0; x < HD / 16; x++) {
+                    const uint32_t off = (uint32_t)(x / 4) * PA_BOX + (uint32_t)(x % 4) * 32;
+                    pa_mma_ss(tmem + 128 * t, pa_desc(q + off, 16), pa_desc(k + off, 16), ids, x > 0);
+                }
+            };
+            auto pv = [&](int t, int s, bool more) {
+                const uint32_t v = smem_addr(ring + s * S::TILE);
+#pragma unroll
+                for (int x = 0; x < 8; x++)
+                    pa_mma_ts(tmem + 256 + HD * t, tmem + 128 * t + 8 * x, pa_desc(v + x * 2048, PA_BOX), ido, more || x > 0);
+            };
+            wait(&q_full, 0);
+            wait(full + 0, 0);
+            pa_fence_after();
+            for (int t = 0; t < n_tile && !gone(); t++) {
+                qk(t, 0);
+                pa_commit(s_full + t);
+            }
+            pa_commit(empty + 0);
+            for (int j = 0; j < n && !gone(); j++) {
+                const int iv = 2 * j + 1, sv = iv % ST, ik = iv + 1, sk = ik % ST;
+                wait(full + sv, (uint32_t)(iv / ST) & 1u);
+                if (j >= n_plain) wait(clean + (j - n_plain), 0);
+                if (j + 1 < n) wait(full + sk, (uint32_t)(ik / ST) & 1u);
+                for (int t = 0; t < n_tile; t++) {
+                    wait(p_full + t, (uint32_t)j & 1u);
+                    if (gone()) break;
+                    pa_fence_after();
+                    pv(t, sv, j > 0);
+                    if (t + 1 == n_tile) pa_commit(empty + sv);
+                    if (j + 1 < n) {
+                        qk(t, sk);
+                        if (t + 1 == n_tile) pa_commit(empty + sk);
+                    }
+                    pa_commit(s_full + t);        // the next scores, or at the end the sums, and all before
+                }
+            }
+            pa_commit(&drain);
+            mbar_drain(&drain, 0, wait_limit_ns());       // no product in flight when tensor memory is given back
+        }
+        __syncwarp();
+    } else if (warp >= 10) {
+        const int me = tid - 320;
+        for (int j = n_plain; j < n; j++) {
+            const int iv = 2 * j + 1;
+            wait(due + (j - n_plain), 0);
+            wait(full + iv % ST, (uint32_t)(iv / ST) & 1u);
+            if (__any_sync(0xffffffffu, gone())) break;
+            uint4 *v = reinterpret_cast<uint4 *>(ring + (iv % ST) * S::TILE);
+            for (int i = me; i < S::TILE / 16; i += 64) {
+                uint4     x = v[i];
+                uint32_t *w = reinterpret_cast<uint32_t *>(&x);
+                uint32_t  full_exp = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++) full_exp |= (w[e] & PaBits<T>::exp) + PaBits<T>::one;
+                if (full_exp & 0x80008000u) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const uint32_t f = (w[e] & PaBits<T>::exp) + PaBits<T>::one;
+                        w[e] &= (f & 0x8000u ? 0u : 0xFFFFu) | (f & 0x80000000u ? 0u : 0xFFFF0000u);
+                    }
+                    v[i] = x;
+                    const int key = (i % (PA_BOX / 16)) / 8;
+                    atomicOr(&bad[j - n_plain][key >> 5], 1u << (key & 31));
+                    any_bad = 1;
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(clean + (j - n_plain));
+        }
+    } else {
+        const int      t = warp >> 2, r = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lanes + 128 * t, to = tmem + lanes + 256 + HD * t;
+        if (t < n_tile) {
+            const int   row = tile_of(t) * 128 + r, vis = seen(row);
+            const float sl = a.scale * 1.4426950408889634f;
+            float       m = -INFINITY, l = 0.0f;          // the maximum that P is relative to; the weights' sum
+            for (int j = 0; j < n; j++) {
+                wait(s_full + t, (uint32_t)j & 1u);
+                if (__any_sync(0xffffffffu, gone())) break;
+                pa_fence_after();
+                uint32_t s[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; c++) pa_ld32(s[c], ts + 32 * c);
+                pa_ld_wait();
+#pragma unroll
+                for (int c = 0; c < 4; c++) pa_pin(s[c]);
+                if (j >= n_plain) {
+                    const int left = vis - j * 128;
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+#pragma unroll
+                        for (int x = 0; x < 32; x++)
+                            if (32 * c + x >= left) s[c][x] = 0xFF800000u;
+                }
+                float top[4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    top[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+                    for (int x = 1; x < 32; x++) top[c] = fmaxf(top[c], __uint_as_float(s[c][x]));
+                }
+                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                if (j == 0) m = mx;
+                else {
+                    const bool grow = mx > m && !((mx - m) * sl <= 8.0f);
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float f = grow ? kv4_ex2((m - mx) * sl) : 1.0f;
+                        if (grow) m = mx;
+                        l *= f;
+#pragma unroll
+                        for (int c = 0; c < HD / 32; c++) {
+                            uint32_t o[32];
+                            pa_ld32(o, to + 32 * c);
+                            pa_ld_wait();
+                            pa_pin(o);
+#pragma unroll
+                            for (int x = 0; x < 32; x++) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                            pa_st32(to + 32 * c, o);
+                        }
+                    }
+                }
+                const float mb = m == -INFINITY ? 0.0f : m * sl;
+                float       sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int x = 0; x < 32; x++) {
+                        const float e0 = kv4_ex2(fmaf(__uint_as_float(s[2 * h + x / 16][(2 * x) & 31]), sl, -mb));
+                        const float e1 = kv4_ex2(fmaf(__uint_as_float(s[2 * h + x / 16][(2 * x + 1) & 31]), sl, -mb));
+                        sum[(2 * x) & 3] += e0;
+                        sum[(2 * x + 1) & 3] += e1;
+                        p[x] = pa_pair(T(), e0, e1);
+                    }
+                    pa_st32(ts + 32 * h, p);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                pa_st_wait();
+                pa_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + t);
+            }
+            // the output: this thread's row
+            if (n > 0) wait(s_full + t, (uint32_t)n & 1u);
+            for (int j = n_plain; j < n; j++) wait(clean + (j - n_plain), 0);
+            pa_fence_after();
+            const float inv = gone() ? NAN : 1.0f / l;
+            T          *out = (T *)a.out + (size_t)(q0 + row) * a.out_stride + (size_t)head_of(t) * HD;
+            for (int c = 0; c < HD / 32; c++) {
+                uint32_t o[32];
+                if (n > 0) {
+                    pa_ld32(o, to + 32 * c);
+                    pa_ld_wait();
+                    pa_pin(o);
+                }
+                if (row < nq) {
+                    float y[32];
+#pragma unroll
+                    for (int x = 0; x < 32; x++) y[x] = vis > 0 ? __uint_as_float(o[x]) * inv : 0.0f;
+                    if (any_bad)                          // cleaned elements of keys that the row sees
+                        for (int w = 0; w < 16; w++)
+                            for (uint32_t left = bad[w >> 2][w & 3]; left; left &= left - 1) {
+                                const int key = (n_plain + (w >> 2)) * 128 + (w & 3) * 32 + __ffs(left) - 1;
+                                if (key >= vis) continue;
+                                const T *v = (const T *)a.v + (size_t)(k0 + key) * a.v_stride + (size_t)kvh * HD + 32 * c;
+#pragma unroll
+                                for (int x = 0; x < 32; x++) {
+                                    const float e = kv4_float(v[x]);
+                                    if (!(fabsf(e) < INFINITY)) y[x] += e;
+                                }
+                            }
+#pragma unroll
+                    for (int x = 0; x < 32; x += 8) {
+                        uint4 w;
+                        w.x = pa_pair(T(), y[x], y[x + 1]);
+                        w.y = pa_pair(T(), y[x + 2], y[x + 3]);
+                        w.z = pa_pair(T(), y[x + 4], y[x + 5]);
+                        w.w = pa_pair(T(), y[x + 6], y[x + 7]);
+                        *reinterpret_cast<uint4 *>(out + 32 * c + x) = w;
+                    }
+                }
+            }
+        }
+    }
+    pa_fence_before();
+    __syncthreads();
+    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}

@@ -415,7 +415,7 @@ int    ecu_kv_read(ecu_kv *kv, int layer, int seq, int pos, int n, float *k, flo
  * queries').  The last query sees every key of its sequence, each earlier one
  * one key less; a row that sees none becomes zeros.  q, k, v, out: device,
  * `dtype` (ECU_F16 or ECU_BF16), 16-byte aligned, a row's heads one after the
- * other, rows a multiple of 8 elements apart; head_dim 64 or 128.  What lies
+ * other, rows a multiple of 8 elements apart; head_dim 64 or 128; scale > 0.  What lies
  * behind the last row, or in keys that a row does not see (NaN and infinities
  * too), has no effect.  Sums and the softmax are fp32; the weights are
  * rounded to `dtype` before their product with V. */

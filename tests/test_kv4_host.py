@@ -231,7 +231,8 @@ def prompt(dtype=1, q=A, k=A, v=A, out=A, heads=4, kv=2, hd=64, st=(256, 128, 12
     (dict(cu_q=(0, 5), cu_k=(0, -1)), "decrease"), (dict(q=0), "null rows"), (dict(v=0), "null rows"),
     (dict(st=(248, 128, 128, 256)), "rows overlap"), (dict(st=(256, 120, 128, 256)), "rows overlap"),
     (dict(st=(260, 128, 128, 256)), "not 16-byte aligned"), (dict(k=A + 8), "not 16-byte aligned"),
-    (dict(scale=float("inf")), "not finite"), (dict(n=-1), "negative count"), (dict(), "device 99 not available")])
+    (dict(scale=float("inf")), "positive finite"), (dict(scale=0.0), "positive finite"), (dict(n=-1), "negative count"),
+    (dict(), "device 99 not available")])
 def test_prompt_refuses(over, why):
     assert prompt(**over) == -1
     assert why in engine.last_error()
