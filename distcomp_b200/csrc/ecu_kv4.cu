@@ -134,6 +134,7 @@ void ecu_kv_close(ecu_kv *kv)
     if (kv->device >= 0) {
         DeviceScope d(kv->device);
         for (auto &w : kv->ws) cudaFree(w.second);
+        if (kv->spare) cudaFree(kv->spare);
         if (kv->meta) cudaFree(kv->meta);
         if (kv->own_data && kv->data) cudaFree(kv->data);
     }
@@ -185,12 +186,14 @@ int ecu_kv_open(ecu_kv **out, int n_layer, int n_head_kv, int head_dim, int n_pa
                     kv->own_data = true;
                 }
             }
-            if (!kv->meta || !kv->data) {
+            if (cudaMalloc(&p, ecu_kv_ws_bytes(kv.get())) == cudaSuccess) kv->spare = p;
+            if (!kv->meta || !kv->data || !kv->spare) {
                 cudaGetLastError();
                 ecu_set_error(err, errlen, "out of device memory for a pool of %zu bytes", bytes);
                 return -1;
             }
-            kv->device_bytes = words * sizeof(int) + (data ? 0 : bytes);
+            kv->device_bytes = words * sizeof(int) + (data ? 0 : bytes) + ecu_kv_ws_bytes(kv.get());
+            cudaMemset(kv->spare, 0, ecu_kv_ws_bytes(kv.get()));
             // -1 in the table, 0 in the lengths
             cudaMemset(kv->meta, 0xFF, (size_t)n_seq * max_pages * sizeof(int));
             cudaMemset(kv->len(), 0, (size_t)n_seq * sizeof(int));
@@ -517,6 +520,7 @@ extern "C" int ecu_kv_attend(ecu_kv *kv, int layer, int dtype, const void *q, vo
         if (cap) return say(what, "a captured call needs a workspace of its own");
         try {
             void *&own = kv->ws[stream];
+            if (!own) std::swap(own, kv->spare);
             if (!own) {
                 const size_t bytes = ecu_kv_ws_bytes(kv);
                 void        *p = nullptr;

@@ -5,6 +5,7 @@
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <type_traits>
 
 #define KV4_PAGE 64
 
@@ -253,26 +254,26 @@ struct KvAttendArgs {
 // one position, and transposed the V codes of 4 dimensions of two positions:
 // both are the operand layouts of the products, in the stored order.
 //
-// Work is cut into units of 32 positions of one KV head of one sequence,
-// numbered sequence by sequence, head by head, and dealt out evenly: CTAs get
+// Work is cut into units, a page's 64 positions of one KV head of one
+// sequence, numbered sequence by sequence, head by head, and dealt out evenly: CTAs get
 // equal runs of units, and within a CTA the warps do, whatever the lengths.
 // Each warp streams its units through a ring of its own (bulk copies; no
 // barrier between warps) and keeps its own softmax.  A row that several warps
 // share is merged in shared memory, one that several CTAs share through the
 // workspace by whichever CTA ends last, in the order of the CTAs, so that the
 // result does not depend on timing.
-#define KV4_UNIT 32
+#define KV4_UNIT KV4_PAGE
 #define KV4_STAGES 2
 
 template <typename T> struct KvSplit { static constexpr int N = 1; };
 template <> struct KvSplit<float> { static constexpr int N = 2; };
 
-template <int NT> struct KvWarps { static constexpr int N = NT == 1 ? 16 : 8; };
+#define KV4_WARPS 8
 
 template <typename T, int NB, int NT> struct KvShape {
-    static constexpr int HD = NB * 32, P = KvSplit<T>::N, W = KvWarps<NT>::N;
+    static constexpr int HD = NB * 32, P = KvSplit<T>::N, W = KV4_WARPS;
     static constexpr int HG = 8 * NT / P;                 // query heads of a group
-    static constexpr int STAGE = 36 * HD;                 // one unit: K codes, V codes, K scales, V scales
+    static constexpr int STAGE = 72 * HD;                 // one unit: a KV head's part of a page
     static constexpr int ENTRY = HG * (HD + 2);           // a partial: per head the sums, M and the weights' sum
     static constexpr size_t ring = (size_t)W * KV4_STAGES * STAGE, heads = (size_t)W * ENTRY * 4;
     static constexpr size_t smem(int n) { return ring + heads + W * KV4_STAGES * 8 + (size_t)(n + 1) * 8; }
@@ -292,6 +293,15 @@ __device__ __forceinline__ void kv4_mma(float (&d)[4], uint32_t a0, uint32_t a1,
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// the same from zero
+__device__ __forceinline__ void kv4_mma0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 // Four nibbles of each half of w, minus 8, as fp16 pairs (low half, high half).
@@ -351,7 +361,7 @@ struct KvCursor {
 };
 
 template <typename T, int NB, int NT, int N>
-__global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvAttendArgs a, const KvSeqs<N> list)
+__global__ void __launch_bounds__(KV4_WARPS * 32, 1) k_kv4_attend(const KvAttendArgs a, const KvSeqs<N> list)
 {
     using S = KvShape<T, NB, NT>;
     constexpr int HD = S::HD, P = S::P, W = S::W, HG = S::HG, STAGE = S::STAGE, ENTRY = S::ENTRY;
@@ -430,20 +440,14 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
         p.nu = p.i < n ? pre[p.i + 1] - pre[p.i] : 1;
     };
     auto page_of = [&](const KvCursor &p) {
-        return __ldg(a.table + (size_t)list.seq[p.i] * a.max_pages + p.j / (KV4_PAGE / KV4_UNIT));
+        return __ldg(a.table + (size_t)list.seq[p.i] * a.max_pages + p.j);
     };
-    // the unit's four pieces of its page (held inside the pool whatever the table says)
+    // a unit's copy (from inside the pool whatever the table says)
     auto issue = [&](const KvCursor &p, int page, int k) {
         if (lane) return;
         page = min(max(page, 0), a.n_pages - 1);
-        const int      half = p.j & 1;
-        const uint8_t *src = a.layer + (size_t)page * a.page_bytes + (size_t)(p.r / n_grp) * 72 * HD;
-        uint8_t       *dst = ring + (size_t)k * STAGE;
         mbar_expect_tx(bar + k, STAGE);
-        bulk_g2s(dst, src + half * 16 * HD, 16 * HD, bar + k);
-        bulk_g2s(dst + 16 * HD, src + (32 + half * 16) * HD, 16 * HD, bar + k);
-        bulk_g2s(dst + 32 * HD, src + (64 + half * 2) * HD, 2 * HD, bar + k);
-        bulk_g2s(dst + 34 * HD, src + (68 + half * 2) * HD, 2 * HD, bar + k);
+        bulk_g2s(ring + (size_t)k * STAGE, a.layer + (size_t)page * a.page_bytes + (size_t)(p.r / n_grp) * STAGE, STAGE, bar + k);
     };
 
     uint32_t qf[NT][NB][4];                               // the query columns, as the products' B operands
@@ -511,45 +515,50 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
 #pragma unroll
                 for (int k = 0; k < 4; k++) O[nt][b][0][k] = O[nt][b][1][k] = 0.0f;
     };
-    // NB fp16 scales of one position, as pairs; zeros for a position past the end
-    auto scales = [&](const uint8_t *base, int t, bool live, uint32_t (&w)[(NB + 1) / 2]) {
+    // NB fp16 scales of one position, as pairs
+    auto scales = [&](const uint8_t *base, int t, uint32_t (&w)[(NB + 1) / 2]) {
         if (NB == 4) {
             const uint2 v = *reinterpret_cast<const uint2 *>(base + t * 8);
-            w[0] = live ? v.x : 0u;
-            w[(NB + 1) / 2 - 1] = live ? v.y : 0u;
+            w[0] = v.x;
+            w[(NB + 1) / 2 - 1] = v.y;
         } else if (NB == 2) {
-            w[0] = live ? *reinterpret_cast<const uint32_t *>(base + t * 4) : 0u;
+            w[0] = *reinterpret_cast<const uint32_t *>(base + t * 4);
         } else {
             const uint16_t *p = reinterpret_cast<const uint16_t *>(base) + t * NB;
 #pragma unroll
-            for (int k = 0; k < (NB + 1) / 2; k++)
-                w[k] = live ? (uint32_t)p[2 * k] | (2 * k + 1 < NB ? (uint32_t)p[2 * k + 1] << 16 : 0u) : 0u;
+            for (int k = 0; k < (NB + 1) / 2; k++) w[k] = (uint32_t)p[2 * k] | (2 * k + 1 < NB ? (uint32_t)p[2 * k + 1] << 16 : 0u);
         }
     };
-    auto half_of = [](uint32_t w, int k) { return __half2float(__ushort_as_half((unsigned short)(k ? w >> 16 : w & 0xFFFFu))); };
+    auto half_of = [](uint32_t w, int k) {
+        const __half2 h = *reinterpret_cast<const __half2 *>(&w);
+        return k ? __high2float(h) : __low2float(h);
+    };
+    const int mt_row = (lane & 7) + ((lane >> 3) & 1) * 8, mt_blk = lane >> 4;     // this lane's row of an ldmatrix
 
-    auto unit = [&](const uint8_t *st, int j, int len) {
-        const uint32_t kaddr = smem_addr(st), vaddr = kaddr + 16 * HD;
-        const int      mt_row = (lane & 7) + ((lane >> 3) & 1) * 8, mt_blk = lane >> 4;
-        float          sc[2][2][HL];
-        uint32_t       vs[2][2][(NB + 1) / 2];
-        float          top[HL], vmax = 0.0f;
+    // One unit.  left: positions of it inside the sequence; CUT: not all are
+    auto unit = [&](const uint8_t *st, int left, auto cut) {
+        constexpr bool CUT = decltype(cut)::value;
+        constexpr int  MT = KV4_UNIT / 16;
+        const uint32_t kaddr = smem_addr(st), vaddr = kaddr + 32 * HD;
+        float          sc[MT][2][HL];
+        uint32_t       vs[MT][2][(NB + 1) / 2];
+        float          top[HL];
+        __half2        vm = __float2half2_rn(0.0f);
 #pragma unroll
         for (int h = 0; h < HL; h++) top[h] = -INFINITY;
 #pragma unroll
-        for (int mt = 0; mt < 2; mt++) {
+        for (int mt = 0; mt < MT; mt++) {
             float acc[NT][4];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int k = 0; k < 4; k++) acc[nt][k] = 0.0f;
-            const int  t = mt * 16 + g, t2 = mt * 16 + mt_row;
-            const bool live0 = j * KV4_UNIT + t < len, live1 = j * KV4_UNIT + t + 8 < len;
-            uint32_t   ks0[(NB + 1) / 2], ks1[(NB + 1) / 2];
-            scales(st + 32 * HD, t, true, ks0);
-            scales(st + 32 * HD, t + 8, true, ks1);
-            scales(st + 34 * HD, t, live0, vs[mt][0]);
-            scales(st + 34 * HD, t + 8, live1, vs[mt][1]);
+            const int t = mt * 16 + g, t2 = mt * 16 + mt_row;
+            uint32_t  ks0[(NB + 1) / 2], ks1[(NB + 1) / 2];
+            scales(st + 64 * HD, t, ks0);
+            scales(st + 64 * HD, t + 8, ks1);
+            scales(st + 68 * HD, t, vs[mt][0]);
+            scales(st + 68 * HD, t + 8, vs[mt][1]);
 #pragma unroll
             for (int b = 0; b < NB; b += 2) {
                 uint32_t r[4];
@@ -564,8 +573,8 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
                     const float s0 = half_of(ks0[(b + d) / 2], (b + d) & 1), s1 = half_of(ks1[(b + d) / 2], (b + d) & 1);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        kv4_mma(e, x[0], y[0], x[1], y[1], qf[nt][b + d][0], qf[nt][b + d][1]);
+                        float e[4];
+                        kv4_mma0(e, x[0], y[0], x[1], y[1], qf[nt][b + d][0], qf[nt][b + d][1]);
                         kv4_mma(e, x[2], y[2], x[3], y[3], qf[nt][b + d][2], qf[nt][b + d][3]);
                         acc[nt][0] = fmaf(s0, e[0], acc[nt][0]);
                         acc[nt][1] = fmaf(s0, e[1], acc[nt][1]);
@@ -579,16 +588,19 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
                 const int nt = P == 2 ? h : h >> 1, k = h & 1;
                 sc[mt][0][h] = (P == 2 ? acc[nt][0] + acc[nt][1] : acc[nt][k]) * fac[h];
                 sc[mt][1][h] = (P == 2 ? acc[nt][2] + acc[nt][3] : acc[nt][2 + k]) * fac[h];
-                if (!live0) sc[mt][0][h] = -INFINITY;
-                if (!live1) sc[mt][1][h] = -INFINITY;
+                if (CUT && t >= left) sc[mt][0][h] = -INFINITY;
+                if (CUT && t + 8 >= left) sc[mt][1][h] = -INFINITY;
                 top[h] = fmaxf(top[h], fmaxf(sc[mt][0][h], sc[mt][1][h]));
             }
 #pragma unroll
             for (int x = 0; x < 2; x++)
 #pragma unroll
-                for (int k = 0; k < (NB + 1) / 2; k++)
-                    vmax = fmaxf(vmax, fmaxf(fabsf(half_of(vs[mt][x][k], 0)), fabsf(half_of(vs[mt][x][k], 1))));
+                for (int k = 0; k < (NB + 1) / 2; k++) {
+                    if (CUT && t + 8 * x >= left) vs[mt][x][k] = 0u;      // whatever lies past the end
+                    vm = __hmax2(vm, __habs2(*reinterpret_cast<const __half2 *>(&vs[mt][x][k])));
+                }
         }
+        float vmax = fmaxf(__low2float(vm), __high2float(vm));
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
             vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
@@ -600,42 +612,35 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
         float       alpha[HL];
 #pragma unroll
         for (int h = 0; h < HL; h++) {
-            const float m = fmaxf(M[h], top[h] + ve);
+            const float m = fmaxf(M[h], top[h] + ve), m14 = m - 14.0f;
             alpha[h] = kv4_ex2(M[h] - m);
             M[h] = m;
             float sum = 0.0f;
 #pragma unroll
-            for (int mt = 0; mt < 2; mt++)
+            for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
-                    const bool live = j * KV4_UNIT + mt * 16 + g + 8 * x < len;
-                    sc[mt][x][h] = live ? kv4_ex2(sc[mt][x][h] - m + 14.0f) : 0.0f;
+                    sc[mt][x][h] = kv4_ex2(sc[mt][x][h] - m14);
+                    if (CUT && mt * 16 + g + 8 * x >= left) sc[mt][x][h] = 0.0f;
                     sum += sc[mt][x][h];
                 }
             l[h] = fmaf(l[h], alpha[h], sum);
         }
 #pragma unroll
         for (int b = 0; b < NB; b += 2) {
-            uint32_t r[2][4];
+            float e[2][NT][2][4];
 #pragma unroll
-            for (int mt = 0; mt < 2; mt++) {
+            for (int mt = 0; mt < MT; mt++) {
                 const int t2 = mt * 16 + mt_row;
-                if (b + 1 < NB) kv4_ldsm<true, true>(r[mt], vaddr + t2 * (HD / 2) + kv4_place(t2, b + mt_blk, NB) * 16);
-                else kv4_ldsm<true, false>(r[mt], vaddr + t2 * (HD / 2) + kv4_place(t2, b, NB) * 16);
-            }
+                uint32_t  r[4];
+                if (b + 1 < NB) kv4_ldsm<true, true>(r, vaddr + t2 * (HD / 2) + kv4_place(t2, b + mt_blk, NB) * 16);
+                else kv4_ldsm<true, false>(r, vaddr + t2 * (HD / 2) + kv4_place(t2, b, NB) * 16);
 #pragma unroll
-            for (int d = 0; d < 2; d++) {
-                if (b + d >= NB) continue;
-                float e[NT][2][4];
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++) e[nt][0][k] = e[nt][1][k] = 0.0f;
-#pragma unroll
-                for (int mt = 0; mt < 2; mt++) {
+                for (int d = 0; d < 2; d++) {
+                    if (b + d >= NB) continue;
                     uint32_t x[4], y[4];
-                    kv4_unpack(r[mt][2 * d], x);
-                    kv4_unpack(r[mt][2 * d + 1], y);
+                    kv4_unpack(r[2 * d], x);
+                    kv4_unpack(r[2 * d + 1], y);
                     const float v0 = half_of(vs[mt][0][(b + d) / 2], (b + d) & 1), v1 = half_of(vs[mt][1][(b + d) / 2], (b + d) & 1);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
@@ -652,17 +657,26 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
                             p1 = *reinterpret_cast<const uint32_t *>(&h1);
                         }
                         const uint32_t b0 = kv4_turn(p0), b1 = kv4_turn(p1);
-                        kv4_mma(e[nt][0], x[0], x[1], y[0], y[1], b0, b1);
-                        kv4_mma(e[nt][1], x[2], x[3], y[2], y[3], b0, b1);
+                        if (mt == 0) {
+                            kv4_mma0(e[d][nt][0], x[0], x[1], y[0], y[1], b0, b1);
+                            kv4_mma0(e[d][nt][1], x[2], x[3], y[2], y[3], b0, b1);
+                        } else {
+                            kv4_mma(e[d][nt][0], x[0], x[1], y[0], y[1], b0, b1);
+                            kv4_mma(e[d][nt][1], x[2], x[3], y[2], y[3], b0, b1);
+                        }
                     }
                 }
+            }
+#pragma unroll
+            for (int d = 0; d < 2; d++) {
+                if (b + d >= NB) continue;
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int s = 0; s < 2; s++)
 #pragma unroll
                         for (int k = 0; k < 4; k++)
-                            O[nt][b + d][s][k] = fmaf(O[nt][b + d][s][k], alpha[P == 2 ? nt : 2 * nt + (k & 1)], e[nt][s][k]);
+                            O[nt][b + d][s][k] = fmaf(O[nt][b + d][s][k], alpha[P == 2 ? nt : 2 * nt + (k & 1)], e[d][nt][s][k]);
             }
         }
     };
@@ -731,7 +745,9 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
             // a wait that gives up leaves NaN behind (the copies are this
             // warp's own, so it never should)
             const bool come = mbar_wait(bar + k, phase, nullptr);
-            unit(ring + (size_t)k * STAGE, at.j, len);
+            const int left = len - at.j * KV4_UNIT;
+            if (left >= KV4_UNIT) unit(ring + (size_t)k * STAGE, left, std::false_type());
+            else unit(ring + (size_t)k * STAGE, left, std::true_type());
             if (!come) l[0] = NAN;
             __syncwarp();
             if (u + KV4_STAGES < u1) {

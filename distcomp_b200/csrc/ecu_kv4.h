@@ -53,6 +53,7 @@ struct ecu_kv {
     int     *meta = nullptr;          // device: table, then len
     KvBook   book;
     std::map<void *, void *> ws;      // stream -> its attention workspace
+    void *spare = nullptr;            // the first stream's, allocated with the pool
     int *table() const { return meta; }
     int *len() const { return meta ? meta + (size_t)book.n_seq * book.max_pages : nullptr; }
 };

@@ -35,30 +35,34 @@ def page_bytes(n_head_kv: int, head_dim: int) -> int:
 
 
 def _ints(a) -> np.ndarray:
+    if type(a) is np.ndarray and a.dtype == np.int32 and a.ndim == 1 and a.flags.c_contiguous:
+        return a
     b = np.ascontiguousarray(a, dtype=np.int32)
-    if b.ndim != 1:
-        raise EngineError("a list of whole numbers is wanted")
-    if b is not a and not np.array_equal(b, a):
+    if b.ndim != 1 or not np.array_equal(b, a):
         raise EngineError("a list of whole numbers in 32 bits is wanted")
     return b
 
 
 def _row(t: torch.Tensor, what: str, heads: int | None, hd: int, device: int) -> tuple[int, int]:
     """(heads, row stride) of rows [n, heads, hd] or [n, heads * hd]."""
-    if t.dtype not in _DTYPES or not t.is_cuda or t.device.index != device:
+    if t.dtype not in _DTYPES or not t.is_cuda or t.get_device() != device:
         raise EngineError(f"{what}: rows of float32, float16 or bfloat16 on CUDA device {device} are wanted")
-    if t.dim() == 3:
-        h, d = t.shape[1], t.shape[2]
-        packed = (d <= 1 or t.stride(2) == 1) and (h <= 1 or t.stride(1) == d)
-    elif t.dim() == 2:
-        h, d = (t.shape[1] // hd, hd) if t.shape[1] % hd == 0 else (0, 0)
-        packed = t.shape[1] <= 1 or t.stride(1) == 1
+    shape, st = t.shape, t.stride()
+    if len(shape) == 3:
+        h = shape[1]
+        good = shape[2] == hd and st[2] == 1 and (st[1] == hd or h == 1)
     else:
-        h, d, packed = 0, 0, False
-    if d != hd or h < 1 or (heads is not None and h != heads) or not packed:
-        raise EngineError(f"{what}: rows {tuple(t.shape)} with strides {t.stride()} are not [n, "
+        good = len(shape) == 2 and shape[1] % hd == 0 and st[1] == 1
+        h = shape[1] // hd if good else 0
+    if not good or h < 1 or (heads is not None and h != heads):
+        raise EngineError(f"{what}: rows {tuple(shape)} with strides {st} are not [n, "
                           f"{'heads' if heads is None else heads}, {hd}] with their heads one after the other")
-    return h, t.stride(0) if t.shape[0] > 1 else h * hd
+    return h, st[0] if shape[0] > 1 else h * hd
+
+
+def _current(device: int) -> int:
+    """torch's current stream of a device."""
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 class _Memory:
@@ -81,7 +85,7 @@ class KvPool:
         self.h = C.c_void_p()
         if data is not None:
             want = n_layer * n_pages * page_bytes(n_head_kv, head_dim)
-            if device < 0 or not data.is_cuda or data.device.index != device or not data.is_contiguous() or \
+            if device < 0 or not data.is_cuda or data.get_device() != device or not data.is_contiguous() or \
                     data.numel() * data.element_size() < want:
                 raise EngineError(f"data: {want} contiguous bytes on CUDA device {device} are wanted")
         err = C.create_string_buffer(512)
@@ -128,9 +132,9 @@ class KvPool:
         return [int(p) for p in buf]
 
     def _stream(self, stream):
-        if stream is not None:
+        if stream is not None or self.device < 0:
             return stream
-        return torch.cuda.current_stream(self.device).cuda_stream if self.device >= 0 else None
+        return _current(self.device)
 
     def _change(self, f, a, b, stream) -> None:
         a, b = _ints(a), _ints(b)
@@ -200,7 +204,7 @@ class KvPool:
         s = None if seq is None else _ints(seq)
         if out.dtype != q.dtype or out.shape[0] != q.shape[0] or (s is not None and len(s) != q.shape[0]):
             raise EngineError("out and the sequences: one for each row of q, of its type")
-        if ws is not None and (not ws.is_cuda or ws.device.index != self.device or not ws.is_contiguous() or
+        if ws is not None and (not ws.is_cuda or ws.get_device() != self.device or not ws.is_contiguous() or
                                ws.numel() * ws.element_size() < self.ws_bytes()):
             raise EngineError(f"ws: {self.ws_bytes()} contiguous bytes on CUDA device {self.device} are wanted")
         if lib().ecu_kv_attend(self.h, layer, _DTYPES[q.dtype], q.data_ptr(), out.data_ptr(), heads, qs, os_,
@@ -243,7 +247,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q, cu
     head_dim], offsets cu_q (and cu_k, where sequences have more keys than queries) of each sequence's rows."""
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3 or not q.is_cuda:
         raise EngineError("q, k and v: CUDA tensors [rows, heads, head_dim] are wanted")
-    dev, hd = q.device.index, q.shape[2]
+    dev, hd = q.get_device(), q.shape[2]
     heads, qs = _row(q, "q", None, hd, dev)
     kv, ks = _row(k, "k", None, hd, dev)
     _, vs = _row(v, "v", kv, hd, dev)
@@ -257,7 +261,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q, cu
     if len(cq) < 1 or len(cq) != len(ck) or cq[-1] != q.shape[0] or ck[-1] != k.shape[0] or k.shape[0] != v.shape[0]:
         raise EngineError("cu_q and cu_k: one offset more than sequences, the last one the rows of q and of k and v")
     if stream is None:
-        stream = torch.cuda.current_stream(dev).cuda_stream
+        stream = _current(dev)
     if lib().ecu_attn_prompt(_DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), heads, kv, hd, qs,
                              ks, vs, os_, cq.ctypes.data, ck.ctypes.data, len(cq) - 1,
                              hd ** -0.5 if scale is None else scale, dev, stream) != 0:
