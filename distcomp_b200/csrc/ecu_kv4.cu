@@ -439,7 +439,7 @@ static int attend_launch(ecu_kv *kv, const KvAttendArgs &a, const int *seq, int 
     for (int i = 0; i < n; i++) {
         list.seq[i] = (uint16_t)(seq ? seq[i] : first + i);
         const long long u = (kv->book.seq[list.seq[i]].len + KV4_UNIT - 1) / KV4_UNIT;
-        units += u * rows_seq;
+        units += (u + (u > 0)) * rows_seq;
         rows += u ? rows_seq : 0;
     }
     // one CTA per SM, fewer where the warps would find less than a unit each;

@@ -241,12 +241,14 @@ struct KvAttendArgs {
 // one column (exact after scaling by a power of two), and so are their
 // weights (one rounding to 11 bits, which fp16 and bf16 outputs do not see).
 // To stay in fp16's range a query is scaled by the power of two that brings
-// its largest element to 2^13, and a weight is 2^(score - M + 14) with M the
-// running maximum of score + log2 of the tile's largest V scale, so that
-// weight * scale never passes 2^14 and loses nothing above 2^-38 of that.
-// Every unit's V product starts from zero and is added to the running sums
-// by one fma with the rescaling factor: no long chains inside the tensor core,
-// which cuts off instead of rounding.
+// its largest element to 2^13, and a weight is 2^(score - M + KV4_BASE), where
+// M follows the largest score + log2 of the tile's largest V scale whenever
+// that has passed M by KV4_SLACK: weight * scale never passes 2^14, and loses
+// nothing above 2^-32 of 2^KV4_BASE.  M is common to a warp, so following it
+// takes shuffles and a rescaling of the sums: with the slack both are rare.
+// In fp32 every unit's V product starts from zero and is added to the running
+// sums outside: the tensor core cuts off where fp32 addition rounds, which
+// 16-bit outputs do not see but long fp32 sums would.
 //
 // Unpacking a word of 8 codes: (w & 0xF000F) | 0x64006400 is 1024 + code in
 // each half, (w & 0xF000F0) | ... 1024 + 16 * code; one fp16x2 subtraction or
@@ -254,26 +256,30 @@ struct KvAttendArgs {
 // one position, and transposed the V codes of 4 dimensions of two positions:
 // both are the operand layouts of the products, in the stored order.
 //
-// Work is cut into units, a page's 64 positions of one KV head of one
-// sequence, numbered sequence by sequence, head by head, and dealt out evenly: CTAs get
-// equal runs of units, and within a CTA the warps do, whatever the lengths.
+// Work is cut into units, 32 positions of one KV head of one sequence, and
+// numbered sequence by sequence, head by head; a row (a sequence's KV head)
+// opens with a place of its own, about what its queries cost.  Places are
+// dealt out evenly: CTAs get equal runs of them, and within a CTA the warps
+// do, whatever the lengths.
 // Each warp streams its units through a ring of its own (bulk copies; no
 // barrier between warps) and keeps its own softmax.  A row that several warps
 // share is merged in shared memory, one that several CTAs share through the
 // workspace by whichever CTA ends last, in the order of the CTAs, so that the
 // result does not depend on timing.
-#define KV4_UNIT KV4_PAGE
+#define KV4_BASE 8.0f
+#define KV4_SLACK 6.0f
+#define KV4_UNIT 32
 #define KV4_STAGES 2
 
 template <typename T> struct KvSplit { static constexpr int N = 1; };
 template <> struct KvSplit<float> { static constexpr int N = 2; };
 
-#define KV4_WARPS 8
+template <int NT> struct KvWarps { static constexpr int N = NT == 1 ? 16 : 8; };
 
 template <typename T, int NB, int NT> struct KvShape {
-    static constexpr int HD = NB * 32, P = KvSplit<T>::N, W = KV4_WARPS;
+    static constexpr int HD = NB * 32, P = KvSplit<T>::N, W = KvWarps<NT>::N;
     static constexpr int HG = 8 * NT / P;                 // query heads of a group
-    static constexpr int STAGE = 72 * HD;                 // one unit: a KV head's part of a page
+    static constexpr int STAGE = 36 * HD;                 // one unit: K codes, V codes, K scales, V scales
     static constexpr int ENTRY = HG * (HD + 2);           // a partial: per head the sums, M and the weights' sum
     static constexpr size_t ring = (size_t)W * KV4_STAGES * STAGE, heads = (size_t)W * ENTRY * 4;
     static constexpr size_t smem(int n) { return ring + heads + W * KV4_STAGES * 8 + (size_t)(n + 1) * 8; }
@@ -290,7 +296,7 @@ __device__ __forceinline__ float kv4_ex2(float x)
 __device__ __forceinline__ void kv4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -299,26 +305,42 @@ __device__ __forceinline__ void kv4_mma(float (&d)[4], uint32_t a0, uint32_t a1,
 __device__ __forceinline__ void kv4_mma0(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
-// Four nibbles of each half of w, minus 8, as fp16 pairs (low half, high half).
-__device__ __forceinline__ void kv4_unpack(uint32_t w, uint32_t (&n)[4])
+// Four nibbles of each half of w, minus 8, as fp16 pairs (low half, high
+// half).  and-or as one lop3: left to itself the compiler makes two of it.
+__device__ __forceinline__ uint32_t kv4_and_or(uint32_t x, uint32_t mask, uint32_t bits)
 {
-    const __half2 off = __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));     // 1032
-    const __half2 six = __halves2half2(__ushort_as_half(0x2C00), __ushort_as_half(0x2C00));     // 1 / 16
-    const __half2 low = __halves2half2(__ushort_as_half(0xD480), __ushort_as_half(0xD480));     // -72
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-        const uint32_t x = w >> (8 * k), a = (x & 0x000F000Fu) | 0x64006400u, b = (x & 0x00F000F0u) | 0x64006400u;
-        const __half2  p = __hsub2(*reinterpret_cast<const __half2 *>(&a), off);
-        const __half2  q = __hfma2(*reinterpret_cast<const __half2 *>(&b), six, low);
-        n[2 * k] = *reinterpret_cast<const uint32_t *>(&p);
-        n[2 * k + 1] = *reinterpret_cast<const uint32_t *>(&q);
-    }
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
+    return y;
 }
+
+struct KvMagic {
+    uint32_t mask0, mask1, bits;
+    __device__ __forceinline__ KvMagic()
+    {
+        // opaque, so that they stay in registers
+        asm volatile("mov.u32 %0, 0x000F000F;\n\tmov.u32 %1, 0x00F000F0;\n\tmov.u32 %2, 0x64006400;" : "=r"(mask0), "=r"(mask1), "=r"(bits));
+    }
+    __device__ __forceinline__ void unpack(uint32_t w, uint32_t (&n)[4]) const
+    {
+        const __half2 off = __halves2half2(__ushort_as_half(0x6408), __ushort_as_half(0x6408));     // 1032
+        const __half2 six = __halves2half2(__ushort_as_half(0x2C00), __ushort_as_half(0x2C00));     // 1 / 16
+        const __half2 low = __halves2half2(__ushort_as_half(0xD480), __ushort_as_half(0xD480));     // -72
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const uint32_t x = w >> (8 * k), a = kv4_and_or(x, mask0, bits), b = kv4_and_or(x, mask1, bits);
+            const __half2  p = __hsub2(*reinterpret_cast<const __half2 *>(&a), off);
+            const __half2  q = __hfma2(*reinterpret_cast<const __half2 *>(&b), six, low);
+            n[2 * k] = *reinterpret_cast<const uint32_t *>(&p);
+            n[2 * k + 1] = *reinterpret_cast<const uint32_t *>(&q);
+        }
+    }
+};
 
 __device__ __forceinline__ uint32_t kv4_pack(__half lo, __half hi)
 {
@@ -328,7 +350,7 @@ __device__ __forceinline__ uint32_t kv4_pack(__half lo, __half hi)
 __device__ __forceinline__ uint32_t kv4_turn(uint32_t x)
 {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 
@@ -339,29 +361,30 @@ template <bool TRANS, bool PAIR> __device__ __forceinline__ void kv4_ldsm(uint32
     if (PAIR) {
         if (TRANS)
             asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+                         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
         else
             asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+                         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
     } else {
         if (TRANS)
             asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
-                         : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+                         : "=r"(r[0]), "=r"(r[1]) : "r"(addr));
         else
             asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];"
-                         : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+                         : "=r"(r[0]), "=r"(r[1]) : "r"(addr));
     }
 }
 
-// A place in the numbering of units: sequence i of the list, row r of its
-// KV heads and head groups, unit j of the row's nu.
+// A place in the numbering: place u is sequence i of the list, row r of its
+// KV heads and head groups, place j of the row's nu; place 0 opens the row
+// (its queries are loaded), place j > 0 is unit j - 1.
 struct KvCursor {
     int       i, r, j;
-    long long nu;
+    long long nu, u;
 };
 
 template <typename T, int NB, int NT, int N>
-__global__ void __launch_bounds__(KV4_WARPS * 32, 1) k_kv4_attend(const KvAttendArgs a, const KvSeqs<N> list)
+__global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvAttendArgs a, const KvSeqs<N> list)
 {
     using S = KvShape<T, NB, NT>;
     constexpr int HD = S::HD, P = S::P, W = S::W, HG = S::HG, STAGE = S::STAGE, ENTRY = S::ENTRY;
@@ -370,7 +393,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 1) k_kv4_attend(const KvAttend
     float     *tails = reinterpret_cast<float *>(smem);   // after the loop: tail partials, in the ring's place
     float     *heads = reinterpret_cast<float *>(smem + S::ring);
     uint64_t  *bars = reinterpret_cast<uint64_t *>(smem + S::ring + S::heads);
-    long long *pre = reinterpret_cast<long long *>(bars + W * KV4_STAGES);     // units of a KV head before sequence i
+    long long *pre = reinterpret_cast<long long *>(bars + W * KV4_STAGES);     // places of a row before sequence i
     __shared__ long long rid[2 * W];                      // the row of each warp's head and tail partial, -1: none
     __shared__ int       last_s;
 
@@ -383,12 +406,13 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 1) k_kv4_attend(const KvAttend
     if (lane == 0)
         for (int k = 0; k < KV4_STAGES; k++) mbar_init(bar + k, 1);
     if (tid < 2 * W) rid[tid] = -1;
-    // units before each sequence: every warp scans 32 at a time, the last one's sums carried on
+    // places before each sequence: one warp scans 32 at a time, the last one's sums carried on
     if (warp == 0) {
         long long run = 0;
         for (int i0 = 0; i0 < n; i0 += 32) {
             const int i = i0 + lane;
             long long u = i < n ? (min(max(__ldg(a.len + list.seq[i]), 0), cap) + KV4_UNIT - 1) / KV4_UNIT : 0;
+            u += u > 0;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const long long v = __shfl_up_sync(0xffffffffu, u, o);
@@ -424,6 +448,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 1) k_kv4_attend(const KvAttend
             else hi = mid;
         }
         p.i = lo;
+        p.u = u;
         p.nu = pre[lo + 1] - pre[lo];
         const long long v = u - pre[lo] * R;
         p.r = (int)(v / p.nu);
@@ -431,6 +456,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 1) k_kv4_attend(const KvAttend
         return p;
     };
     auto next = [&](KvCursor &p) {
+        p.u++;
         if (++p.j < p.nu) return;
         p.j = 0;
         if (++p.r < R) return;
@@ -439,17 +465,24 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 1) k_kv4_attend(const KvAttend
         while (p.i < n && pre[p.i + 1] == pre[p.i]);
         p.nu = p.i < n ? pre[p.i + 1] - pre[p.i] : 1;
     };
-    auto page_of = [&](const KvCursor &p) {
-        return __ldg(a.table + (size_t)list.seq[p.i] * a.max_pages + p.j);
+    // the page of the first unit at or after p inside this warp's run; p moves there
+    auto page_at = [&](KvCursor &p) {
+        if (p.u < u1 && p.j == 0) next(p);
+        return p.u < u1 ? __ldg(a.table + (size_t)list.seq[p.i] * a.max_pages + (p.j - 1) / (KV4_PAGE / KV4_UNIT)) : 0;
     };
-    // a unit's copy (from inside the pool whatever the table says)
+    // the unit's four pieces of its page, a lane each (from inside the pool whatever the table says)
     auto issue = [&](const KvCursor &p, int page, int k) {
-        if (lane) return;
+        if (lane == 0) mbar_expect_tx(bar + k, STAGE);
+        __syncwarp();
+        if (lane >= 4) return;
         page = min(max(page, 0), a.n_pages - 1);
-        mbar_expect_tx(bar + k, STAGE);
-        bulk_g2s(ring + (size_t)k * STAGE, a.layer + (size_t)page * a.page_bytes + (size_t)(p.r / n_grp) * STAGE, STAGE, bar + k);
+        const int      half = (p.j - 1) & 1, bytes = lane < 2 ? 16 * HD : 2 * HD;
+        const uint8_t *src = a.layer + (size_t)page * a.page_bytes + (size_t)(p.r / n_grp) * 72 * HD;
+        const int      from = lane < 2 ? 32 * HD * lane : 64 * HD + 4 * HD * (lane - 2), to = lane < 2 ? 16 * HD * lane : 32 * HD + 2 * HD * (lane - 2);
+        bulk_g2s(ring + (size_t)k * STAGE + to, src + from + half * bytes, bytes, bar + k);
     };
 
+    const KvMagic magic;
     uint32_t qf[NT][NB][4];                               // the query columns, as the products' B operands
     float    fac[HL];                                     // score * fac: in units of log2
     float    O[NT][NB][2][4], M[HL], l[HL];
@@ -480,8 +513,9 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 1) k_kv4_attend(const KvAttend
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
             // 2^sh brings m to [2^13, 2^14); held where both it and its inverse are normal numbers
             const int sh = min(126, max(-126, 140 - (int)((__float_as_uint(fmaxf(m, 1e-38f)) >> 23) & 255)));
-            const float up = __uint_as_float((uint32_t)(sh + 127) << 23);
-            f[nt] = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - sh) << 23);
+            // (with the scale's sign, so that fac is not negative)
+            const float up = copysignf(__uint_as_float((uint32_t)(sh + 127) << 23), a.scale);
+            f[nt] = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - sh) << 23);
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 __half h[8];
@@ -539,7 +573,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 1) k_kv4_attend(const KvAttend
     auto unit = [&](const uint8_t *st, int left, auto cut) {
         constexpr bool CUT = decltype(cut)::value;
         constexpr int  MT = KV4_UNIT / 16;
-        const uint32_t kaddr = smem_addr(st), vaddr = kaddr + 32 * HD;
+        const uint32_t kaddr = smem_addr(st), vaddr = kaddr + 16 * HD;
         float          sc[MT][2][HL];
         uint32_t       vs[MT][2][(NB + 1) / 2];
         float          top[HL];
@@ -555,10 +589,10 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 1) k_kv4_attend(const KvAttend
                 for (int k = 0; k < 4; k++) acc[nt][k] = 0.0f;
             const int t = mt * 16 + g, t2 = mt * 16 + mt_row;
             uint32_t  ks0[(NB + 1) / 2], ks1[(NB + 1) / 2];
-            scales(st + 64 * HD, t, ks0);
-            scales(st + 64 * HD, t + 8, ks1);
-            scales(st + 68 * HD, t, vs[mt][0]);
-            scales(st + 68 * HD, t + 8, vs[mt][1]);
+            scales(st + 32 * HD, t, ks0);
+            scales(st + 32 * HD, t + 8, ks1);
+            scales(st + 34 * HD, t, vs[mt][0]);
+            scales(st + 34 * HD, t + 8, vs[mt][1]);
 #pragma unroll
             for (int b = 0; b < NB; b += 2) {
                 uint32_t r[4];
@@ -568,8 +602,8 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 1) k_kv4_attend(const KvAttend
                 for (int d = 0; d < 2; d++) {
                     if (b + d >= NB) continue;
                     uint32_t x[4], y[4];
-                    kv4_unpack(r[2 * d], x);
-                    kv4_unpack(r[2 * d + 1], y);
+                    magic.unpack(r[2 * d], x);
+                    magic.unpack(r[2 * d + 1], y);
                     const float s0 = half_of(ks0[(b + d) / 2], (b + d) & 1), s1 = half_of(ks1[(b + d) / 2], (b + d) & 1);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
@@ -586,11 +620,10 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 1) k_kv4_attend(const KvAttend
 #pragma unroll
             for (int h = 0; h < HL; h++) {
                 const int nt = P == 2 ? h : h >> 1, k = h & 1;
-                sc[mt][0][h] = (P == 2 ? acc[nt][0] + acc[nt][1] : acc[nt][k]) * fac[h];
-                sc[mt][1][h] = (P == 2 ? acc[nt][2] + acc[nt][3] : acc[nt][2 + k]) * fac[h];
-                if (CUT && t >= left) sc[mt][0][h] = -INFINITY;
-                if (CUT && t + 8 >= left) sc[mt][1][h] = -INFINITY;
-                top[h] = fmaxf(top[h], fmaxf(sc[mt][0][h], sc[mt][1][h]));
+                sc[mt][0][h] = P == 2 ? acc[nt][0] + acc[nt][1] : acc[nt][k];
+                sc[mt][1][h] = P == 2 ? acc[nt][2] + acc[nt][3] : acc[nt][2 + k];
+                if (!CUT || t < left) top[h] = fmaxf(top[h], sc[mt][0][h]);
+                if (!CUT || t + 8 < left) top[h] = fmaxf(top[h], sc[mt][1][h]);
             }
 #pragma unroll
             for (int x = 0; x < 2; x++)
@@ -600,47 +633,72 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 1) k_kv4_attend(const KvAttend
                     vm = __hmax2(vm, __habs2(*reinterpret_cast<const __half2 *>(&vs[mt][x][k])));
                 }
         }
-        float vmax = fmaxf(__low2float(vm), __high2float(vm));
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-            vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
-#pragma unroll
-            for (int h = 0; h < HL; h++) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], o));
-        }
-        // every V scale of the unit is below 2^ve (scales below 2^-24 are zeros)
+        // this thread's V scales are below 2^ve (scales below 2^-24 are zeros)
+        float       vmax = fmaxf(__low2float(vm), __high2float(vm));
         const float ve = (float)max((int)(__float_as_uint(vmax) >> 23) - 126, -24);
-        float       alpha[HL];
+        bool        calm = true;
 #pragma unroll
         for (int h = 0; h < HL; h++) {
-            const float m = fmaxf(M[h], top[h] + ve), m14 = m - 14.0f;
-            alpha[h] = kv4_ex2(M[h] - m);
-            M[h] = m;
-            float sum = 0.0f;
+            top[h] *= fac[h];
+            calm = calm && top[h] + ve <= M[h] + KV4_SLACK;
+        }
+        if (!__all_sync(0xffffffffu, calm)) {
+            // M follows the largest score + log2 of the largest V scale
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+#pragma unroll
+                for (int h = 0; h < HL; h++) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], o));
+            }
+            const float vw = (float)max((int)(__float_as_uint(vmax) >> 23) - 126, -24);
+            float       alpha[HL];
+#pragma unroll
+            for (int h = 0; h < HL; h++) {
+                const float m = fmaxf(M[h], top[h] + vw);
+                alpha[h] = kv4_ex2(M[h] - m);
+                M[h] = m;
+                l[h] *= alpha[h];
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        O[nt][b][0][k] *= alpha[P == 2 ? nt : 2 * nt + (k & 1)];
+                        O[nt][b][1][k] *= alpha[P == 2 ? nt : 2 * nt + (k & 1)];
+                    }
+        }
+#pragma unroll
+        for (int h = 0; h < HL; h++) {
+            const float base = KV4_BASE - M[h];
 #pragma unroll
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
-                    sc[mt][x][h] = kv4_ex2(sc[mt][x][h] - m14);
+                    sc[mt][x][h] = kv4_ex2(fmaf(sc[mt][x][h], fac[h], base));
                     if (CUT && mt * 16 + g + 8 * x >= left) sc[mt][x][h] = 0.0f;
-                    sum += sc[mt][x][h];
+                    l[h] += sc[mt][x][h];
                 }
-            l[h] = fmaf(l[h], alpha[h], sum);
         }
 #pragma unroll
         for (int b = 0; b < NB; b += 2) {
-            float e[2][NT][2][4];
+            uint32_t r[MT][4];
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) {
                 const int t2 = mt * 16 + mt_row;
-                uint32_t  r[4];
-                if (b + 1 < NB) kv4_ldsm<true, true>(r, vaddr + t2 * (HD / 2) + kv4_place(t2, b + mt_blk, NB) * 16);
-                else kv4_ldsm<true, false>(r, vaddr + t2 * (HD / 2) + kv4_place(t2, b, NB) * 16);
+                if (b + 1 < NB) kv4_ldsm<true, true>(r[mt], vaddr + t2 * (HD / 2) + kv4_place(t2, b + mt_blk, NB) * 16);
+                else kv4_ldsm<true, false>(r[mt], vaddr + t2 * (HD / 2) + kv4_place(t2, b, NB) * 16);
+            }
 #pragma unroll
-                for (int d = 0; d < 2; d++) {
-                    if (b + d >= NB) continue;
+            for (int d = 0; d < 2; d++) {
+                if (b + d >= NB) continue;
+                float e[NT][2][4];
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) {
                     uint32_t x[4], y[4];
-                    kv4_unpack(r[2 * d], x);
-                    kv4_unpack(r[2 * d + 1], y);
+                    magic.unpack(r[mt][2 * d], x);
+                    magic.unpack(r[mt][2 * d + 1], y);
                     const float v0 = half_of(vs[mt][0][(b + d) / 2], (b + d) & 1), v1 = half_of(vs[mt][1][(b + d) / 2], (b + d) & 1);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
@@ -657,26 +715,26 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 1) k_kv4_attend(const KvAttend
                             p1 = *reinterpret_cast<const uint32_t *>(&h1);
                         }
                         const uint32_t b0 = kv4_turn(p0), b1 = kv4_turn(p1);
-                        if (mt == 0) {
-                            kv4_mma0(e[d][nt][0], x[0], x[1], y[0], y[1], b0, b1);
-                            kv4_mma0(e[d][nt][1], x[2], x[3], y[2], y[3], b0, b1);
+                        if (P == 1) {
+                            kv4_mma(O[nt][b + d][0], x[0], x[1], y[0], y[1], b0, b1);
+                            kv4_mma(O[nt][b + d][1], x[2], x[3], y[2], y[3], b0, b1);
+                        } else if (mt == 0) {
+                            kv4_mma0(e[nt][0], x[0], x[1], y[0], y[1], b0, b1);
+                            kv4_mma0(e[nt][1], x[2], x[3], y[2], y[3], b0, b1);
                         } else {
-                            kv4_mma(e[d][nt][0], x[0], x[1], y[0], y[1], b0, b1);
-                            kv4_mma(e[d][nt][1], x[2], x[3], y[2], y[3], b0, b1);
+                            kv4_mma(e[nt][0], x[0], x[1], y[0], y[1], b0, b1);
+                            kv4_mma(e[nt][1], x[2], x[3], y[2], y[3], b0, b1);
                         }
                     }
                 }
-            }
+                if (P == 2)
 #pragma unroll
-            for (int d = 0; d < 2; d++) {
-                if (b + d >= NB) continue;
+                    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int s = 0; s < 2; s++)
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            O[nt][b + d][s][k] = fmaf(O[nt][b + d][s][k], alpha[P == 2 ? nt : 2 * nt + (k & 1)], e[d][nt][s][k]);
+                        for (int k = 0; k < 4; k++) {
+                            O[nt][b + d][0][k] += e[nt][0][k];
+                            O[nt][b + d][1][k] += e[nt][1][k];
+                        }
             }
         }
     };
@@ -721,72 +779,69 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 1) k_kv4_attend(const KvAttend
     bool tail = false;                                    // this warp ends inside a row that began in its run
     if (u0 < u1) {
         KvCursor at = locate(u0), ahead = at;
-        int      pages[KV4_STAGES + 1];
-        {
-            KvCursor p = at;
+        KvCursor first[KV4_STAGES];
+        int      page[KV4_STAGES + 1];
 #pragma unroll
-            for (int k = 0; k <= KV4_STAGES; k++) {       // independent loads
-                pages[k] = u0 + k < u1 ? page_of(p) : 0;
-                if (u0 + k + 1 < u1) next(p);
-            }
+        for (int k = 0; k < KV4_STAGES; k++) {            // independent loads
+            page[k] = page_at(ahead);
+            first[k] = ahead;
+            if (ahead.u < u1) next(ahead);
         }
+        page[KV4_STAGES] = page_at(ahead);                // of the unit that is issued next
 #pragma unroll
         for (int k = 0; k < KV4_STAGES; k++)
-            if (u0 + k < u1) {
-                issue(ahead, pages[k], k);
-                if (u0 + k + 1 < u1) next(ahead);
-            }
-        int page = pages[KV4_STAGES];                     // of the unit that is issued next
+            if (first[k].u < u1) issue(first[k], page[k], k);
         load_q(at);
-        int  j0 = at.j, k = 0;
+        int      j0 = at.j, k = 0, len = min(__ldg(a.len + list.seq[at.i]), cap);
         unsigned phase = 0;
-        int  len = min(__ldg(a.len + list.seq[at.i]), cap);
-        for (long long u = u0; u < u1; u++) {
-            // a wait that gives up leaves NaN behind (the copies are this
-            // warp's own, so it never should)
-            const bool come = mbar_wait(bar + k, phase, nullptr);
-            const int left = len - at.j * KV4_UNIT;
-            if (left >= KV4_UNIT) unit(ring + (size_t)k * STAGE, left, std::false_type());
-            else unit(ring + (size_t)k * STAGE, left, std::true_type());
-            if (!come) l[0] = NAN;
-            __syncwarp();
-            if (u + KV4_STAGES < u1) {
-                issue(ahead, page, k);
-                if (u + KV4_STAGES + 1 < u1) {
+        for (;;) {
+            if (at.j > 0) {
+                // a wait that gives up leaves NaN behind (the copies are this
+                // warp's own, so it never should)
+                const bool come = mbar_wait(bar + k, phase, nullptr);
+                const int  left = len - (at.j - 1) * KV4_UNIT;
+                if (left >= KV4_UNIT) unit(ring + (size_t)k * STAGE, left, std::false_type());
+                else unit(ring + (size_t)k * STAGE, left, std::true_type());
+                if (!come) l[0] = NAN;
+                __syncwarp();
+                if (ahead.u < u1) {
+                    issue(ahead, page[KV4_STAGES], k);
                     next(ahead);
-                    page = page_of(ahead);
+                    page[KV4_STAGES] = page_at(ahead);
+                }
+                if (++k == KV4_STAGES) {
+                    k = 0;
+                    phase ^= 1;
                 }
             }
-            if (++k == KV4_STAGES) {
-                k = 0;
-                phase ^= 1;
-            }
-            const bool row_end = at.j + 1 == at.nu, run_end = u + 1 == u1;
-            if (row_end || run_end) {
-                sum_l();
-                const long long row = (long long)at.i * R + at.r;
-                if (j0 > 0) {
-                    store_part(heads + warp * ENTRY);
-                    if (lane == 0) rid[2 * warp] = row;
-                } else if (!row_end) {
-                    tail = true;
-                    if (lane == 0) rid[2 * warp + 1] = row;
-                } else {
-                    const int kvh = at.r / n_grp, grp = at.r - kvh * n_grp;
-                    T        *o = (T *)a.out + (size_t)at.i * a.out_stride + (size_t)kvh * a.n_rep * HD;
-                    each([&](int h, int hl, int d, float v) {
-                        if (grp * HG + h < a.n_rep) o[(size_t)(grp * HG + h) * HD + d] = kv4_from<T>(v / l[hl]);
-                    });
-                }
-                if (!run_end) {
-                    next(at);
-                    j0 = 0;
-                    load_q(at);
-                    len = min(__ldg(a.len + list.seq[at.i]), cap);
-                }
-            } else {
+            const bool row_end = at.j + 1 == at.nu, run_end = at.u + 1 == u1;
+            if (!row_end && !run_end) {
                 at.j++;
+                at.u++;
+                continue;
             }
+            sum_l();
+            const long long row = (long long)at.i * R + at.r;
+            if (j0 > 0) {
+                store_part(heads + warp * ENTRY);
+                if (lane == 0) rid[2 * warp] = row;
+            } else if (!row_end) {
+                tail = true;
+                if (lane == 0) rid[2 * warp + 1] = row;
+            } else {
+                const int kvh = at.r / n_grp, grp = at.r - kvh * n_grp;
+                T        *o = (T *)a.out + (size_t)at.i * a.out_stride + (size_t)kvh * a.n_rep * HD;
+#pragma unroll
+                for (int h = 0; h < HL; h++) l[h] = __frcp_rn(l[h]);
+                each([&](int h, int hl, int d, float v) {
+                    if (grp * HG + h < a.n_rep) o[(size_t)(grp * HG + h) * HD + d] = kv4_from<T>(v * l[hl]);
+                });
+            }
+            if (run_end) break;
+            next(at);
+            j0 = 0;
+            load_q(at);
+            len = min(__ldg(a.len + list.seq[at.i]), cap);
         }
     }
     __syncthreads();                                      // every ring is idle
@@ -816,7 +871,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 1) k_kv4_attend(const KvAttend
                 if (rid[k] >= 0) m = fmaxf(m, entry(k)[at + HD]);
             for (int k = e; k < end; k++)
                 if (rid[k] >= 0) {
-                    const float w = kv4_ex2(entry(k)[at + HD] - m);
+                    const float w = entry(k)[at + HD + 1] == 0.0f ? 0.0f : kv4_ex2(entry(k)[at + HD] - m);   // (no unit: no weight)
                     L = fmaf(w, entry(k)[at + HD + 1], L);
                     v = fmaf(w, entry(k)[at + x % HD], v);
                 }
@@ -852,7 +907,7 @@ __global__ void __launch_bounds__(KV4_WARPS * 32, 1) k_kv4_attend(const KvAttend
                     for (int b = c0; b <= c1; b++) m = fmaxf(m, __ldcg(part(b) + HD));
 #pragma unroll 8
                     for (int b = c0; b <= c1; b++) {
-                        const float w = kv4_ex2(__ldcg(part(b) + HD) - m);
+                        const float w = __ldcg(part(b) + HD + 1) == 0.0f ? 0.0f : kv4_ex2(__ldcg(part(b) + HD) - m);
                         L = fmaf(w, __ldcg(part(b) + HD + 1), L);
                         v = fmaf(w, __ldcg(part(b) + x % HD), v);
                     }
