@@ -261,8 +261,8 @@ struct KvAttendArgs {
 // opens with a place of its own, about what its queries cost.  Places are
 // dealt out evenly: CTAs get equal runs of them, and within a CTA the warps
 // do, whatever the lengths.
-// Each warp streams its units through a ring of its own (bulk copies; no
-// barrier between warps) and keeps its own softmax.  A row that several warps
+// Each warp streams its units through a ring of its own (16-byte asynchronous
+// copies; no barrier between warps) and keeps its own softmax.  A row that several warps
 // share is merged in shared memory, one that several CTAs share through the
 // workspace by whichever CTA ends last, in the order of the CTAs, so that the
 // result does not depend on timing.
@@ -282,7 +282,7 @@ template <typename T, int NB, int NT> struct KvShape {
     static constexpr int STAGE = 36 * HD;                 // one unit: K codes, V codes, K scales, V scales
     static constexpr int ENTRY = HG * (HD + 2);           // a partial: per head the sums, M and the weights' sum
     static constexpr size_t ring = (size_t)W * KV4_STAGES * STAGE, heads = (size_t)W * ENTRY * 4;
-    static constexpr size_t smem(int n) { return ring + heads + W * KV4_STAGES * 8 + (size_t)(n + 1) * 8; }
+    static constexpr size_t smem(int n) { return ring + heads + (size_t)(n + 1) * 8; }
     static_assert(ring >= heads, "the tail partials take the ring's place");
 };
 
@@ -375,12 +375,17 @@ template <bool TRANS, bool PAIR> __device__ __forceinline__ void kv4_ldsm(uint32
     }
 }
 
+__device__ __forceinline__ void kv4_cp16(uint32_t dst, const void *src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
 // A place in the numbering: place u is sequence i of the list, row r of its
 // KV heads and head groups, place j of the row's nu; place 0 opens the row
 // (its queries are loaded), place j > 0 is unit j - 1.
 struct KvCursor {
-    int       i, r, j;
-    long long nu, u;
+    int i, r, j, nu;
+    int left;                                             // places of this warp's run from here on
 };
 
 template <typename T, int NB, int NT, int N>
@@ -392,8 +397,7 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
     extern __shared__ __align__(128) uint8_t smem[];
     float     *tails = reinterpret_cast<float *>(smem);   // after the loop: tail partials, in the ring's place
     float     *heads = reinterpret_cast<float *>(smem + S::ring);
-    uint64_t  *bars = reinterpret_cast<uint64_t *>(smem + S::ring + S::heads);
-    long long *pre = reinterpret_cast<long long *>(bars + W * KV4_STAGES);     // places of a row before sequence i
+    long long *pre = reinterpret_cast<long long *>(smem + S::ring + S::heads);     // places of a row before sequence i
     __shared__ long long rid[2 * W];                      // the row of each warp's head and tail partial, -1: none
     __shared__ int       last_s;
 
@@ -401,10 +405,7 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
     const int n = list.n, n_grp = (a.n_rep + HG - 1) / HG, R = a.n_kv * n_grp;
     const int cap = a.max_pages * KV4_PAGE;
     uint8_t  *ring = smem + (size_t)warp * KV4_STAGES * STAGE;
-    uint64_t *bar = bars + warp * KV4_STAGES;
 
-    if (lane == 0)
-        for (int k = 0; k < KV4_STAGES; k++) mbar_init(bar + k, 1);
     if (tid < 2 * W) rid[tid] = -1;
     // places before each sequence: one warp scans 32 at a time, the last one's sums carried on
     if (warp == 0) {
@@ -423,7 +424,6 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
         }
         if (lane == 0) pre[0] = 0;
     }
-    mbar_init_fence();
     __syncthreads();
 
     // an empty sequence's row is zeros
@@ -448,38 +448,43 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
             else hi = mid;
         }
         p.i = lo;
-        p.u = u;
-        p.nu = pre[lo + 1] - pre[lo];
+        p.nu = (int)(pre[lo + 1] - pre[lo]);
         const long long v = u - pre[lo] * R;
         p.r = (int)(v / p.nu);
-        p.j = (int)(v - p.r * p.nu);
+        p.j = (int)(v - (long long)p.r * p.nu);
+        p.left = (int)(u1 - u);
         return p;
     };
     auto next = [&](KvCursor &p) {
-        p.u++;
+        p.left--;
         if (++p.j < p.nu) return;
         p.j = 0;
         if (++p.r < R) return;
         p.r = 0;
         do p.i++;
         while (p.i < n && pre[p.i + 1] == pre[p.i]);
-        p.nu = p.i < n ? pre[p.i + 1] - pre[p.i] : 1;
+        p.nu = p.i < n ? (int)(pre[p.i + 1] - pre[p.i]) : 1;
     };
     // the page of the first unit at or after p inside this warp's run; p moves there
     auto page_at = [&](KvCursor &p) {
-        if (p.u < u1 && p.j == 0) next(p);
-        return p.u < u1 ? __ldg(a.table + (size_t)list.seq[p.i] * a.max_pages + (p.j - 1) / (KV4_PAGE / KV4_UNIT)) : 0;
+        if (p.left > 0 && p.j == 0) next(p);
+        return p.left > 0 ? __ldg(a.table + (size_t)list.seq[p.i] * a.max_pages + (p.j - 1) / (KV4_PAGE / KV4_UNIT)) : 0;
     };
-    // the unit's four pieces of its page, a lane each (from inside the pool whatever the table says)
+    // the unit's pieces of its page, 16 bytes a lane and copy (from inside the pool whatever the table says)
+    const bool     vside = lane >= 4 * NB;
+    const uint32_t ring_lane = smem_addr(ring) + lane * 16;
+    const uint8_t *code_lane = a.layer + lane * 16, *scale_lane = a.layer + 64 * HD + (vside ? 4 * HD : 0) + (lane - (vside ? 4 * NB : 0)) * 16;
     auto issue = [&](const KvCursor &p, int page, int k) {
-        if (lane == 0) mbar_expect_tx(bar + k, STAGE);
-        __syncwarp();
-        if (lane >= 4) return;
-        page = min(max(page, 0), a.n_pages - 1);
-        const int      half = (p.j - 1) & 1, bytes = lane < 2 ? 16 * HD : 2 * HD;
-        const uint8_t *src = a.layer + (size_t)page * a.page_bytes + (size_t)(p.r / n_grp) * 72 * HD;
-        const int      from = lane < 2 ? 32 * HD * lane : 64 * HD + 4 * HD * (lane - 2), to = lane < 2 ? 16 * HD * lane : 32 * HD + 2 * HD * (lane - 2);
-        bulk_g2s(ring + (size_t)k * STAGE + to, src + from + half * bytes, bytes, bar + k);
+        const size_t   at = (size_t)min(max(page, 0), a.n_pages - 1) * a.page_bytes + (unsigned)((n_grp == 1 ? p.r : p.r / n_grp) * 72 * HD);
+        const int      half = (p.j - 1) & 1;
+        const uint8_t *src = code_lane + at + half * 16 * HD;
+        const uint32_t dst = ring_lane + k * STAGE;
+#pragma unroll
+        for (int x = 0; x < NB; x++) {
+            kv4_cp16(dst + 512 * x, src + 512 * x);
+            kv4_cp16(dst + 16 * HD + 512 * x, src + 32 * HD + 512 * x);
+        }
+        if (lane < 8 * NB) kv4_cp16(dst + 32 * HD, scale_lane + at + half * 2 * HD);
     };
 
     const KvMagic magic;
@@ -704,10 +709,12 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
                     for (int nt = 0; nt < NT; nt++) {
                         uint32_t p0, p1;
                         if (P == 2) {
-                            const float  w0 = sc[mt][0][nt] * v0, w1 = sc[mt][1][nt] * v1;
-                            const __half h0 = __float2half_rn(w0), h1 = __float2half_rn(w1);
-                            p0 = kv4_pack(h0, __float2half_rn(w0 - __half2float(h0)));
-                            p1 = kv4_pack(h1, __float2half_rn(w1 - __half2float(h1)));
+                            const float    w0 = sc[mt][0][nt] * v0, w1 = sc[mt][1][nt] * v1;
+                            const __half2  hi = __floats2half2_rn(w0, w1);
+                            const __half2  lo = __floats2half2_rn(w0 - __low2float(hi), w1 - __high2float(hi));
+                            const uint32_t hb = *reinterpret_cast<const uint32_t *>(&hi), lb = *reinterpret_cast<const uint32_t *>(&lo);
+                            p0 = __byte_perm(hb, lb, 0x5410);
+                            p1 = __byte_perm(hb, lb, 0x7632);
                         } else {
                             const __half2 h0 = __floats2half2_rn(sc[mt][0][2 * nt] * v0, sc[mt][0][(2 * nt + 1) % HL] * v0);
                             const __half2 h1 = __floats2half2_rn(sc[mt][1][2 * nt] * v1, sc[mt][1][(2 * nt + 1) % HL] * v1);
@@ -785,39 +792,36 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
         for (int k = 0; k < KV4_STAGES; k++) {            // independent loads
             page[k] = page_at(ahead);
             first[k] = ahead;
-            if (ahead.u < u1) next(ahead);
+            if (ahead.left > 0) next(ahead);
         }
         page[KV4_STAGES] = page_at(ahead);                // of the unit that is issued next
 #pragma unroll
-        for (int k = 0; k < KV4_STAGES; k++)
-            if (first[k].u < u1) issue(first[k], page[k], k);
+        for (int k = 0; k < KV4_STAGES; k++) {
+            if (first[k].left > 0) issue(first[k], page[k], k);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
         load_q(at);
         int      j0 = at.j, k = 0, len = min(__ldg(a.len + list.seq[at.i]), cap);
-        unsigned phase = 0;
         for (;;) {
             if (at.j > 0) {
-                // a wait that gives up leaves NaN behind (the copies are this
-                // warp's own, so it never should)
-                const bool come = mbar_wait(bar + k, phase, nullptr);
-                const int  left = len - (at.j - 1) * KV4_UNIT;
+                asm volatile("cp.async.wait_group %0;" ::"n"(KV4_STAGES - 1) : "memory");
+                __syncwarp();
+                const int left = len - (at.j - 1) * KV4_UNIT;
                 if (left >= KV4_UNIT) unit(ring + (size_t)k * STAGE, left, std::false_type());
                 else unit(ring + (size_t)k * STAGE, left, std::true_type());
-                if (!come) l[0] = NAN;
                 __syncwarp();
-                if (ahead.u < u1) {
+                if (ahead.left > 0) {
                     issue(ahead, page[KV4_STAGES], k);
                     next(ahead);
                     page[KV4_STAGES] = page_at(ahead);
                 }
-                if (++k == KV4_STAGES) {
-                    k = 0;
-                    phase ^= 1;
-                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                k = k + 1 == KV4_STAGES ? 0 : k + 1;
             }
-            const bool row_end = at.j + 1 == at.nu, run_end = at.u + 1 == u1;
+            const bool row_end = at.j + 1 == at.nu, run_end = at.left == 1;
             if (!row_end && !run_end) {
                 at.j++;
-                at.u++;
+                at.left--;
                 continue;
             }
             sum_l();
