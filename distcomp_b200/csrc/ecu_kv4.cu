@@ -176,6 +176,7 @@ int ecu_kv_open(ecu_kv **out, int n_layer, int n_head_kv, int head_dim, int n_pa
             if (!d.ok) { ecu_set_error(err, errlen, "cudaSetDevice(%d) failed", device); return -1; }
             kv->device = device;
             cudaDeviceGetAttribute(&kv->sms, cudaDevAttrMultiProcessorCount, device);
+            kv->sms = std::min(kv->sms, KV4_MAX_CTAS);
             const size_t words = (size_t)n_seq * max_pages + n_seq, bytes = kv->page_bytes * n_pages * n_layer;
             void *p = nullptr;
             if (cudaMalloc(&p, words * sizeof(int)) == cudaSuccess) {

@@ -270,6 +270,7 @@ struct KvAttendArgs {
 #define KV4_SLACK 6.0f
 #define KV4_UNIT 32
 #define KV4_STAGES 2
+#define KV4_MAX_CTAS 192
 
 template <typename T> struct KvSplit { static constexpr int N = 1; };
 template <> struct KvSplit<float> { static constexpr int N = 2; };
@@ -281,9 +282,10 @@ template <typename T, int NB, int NT> struct KvShape {
     static constexpr int HG = 8 * NT / P;                 // query heads of a group
     static constexpr int STAGE = 36 * HD;                 // one unit: K codes, V codes, K scales, V scales
     static constexpr int ENTRY = HG * (HD + 2);           // a partial: per head the sums, M and the weights' sum
-    static constexpr size_t ring = (size_t)W * KV4_STAGES * STAGE, heads = (size_t)W * ENTRY * 4;
+    static constexpr size_t heads = (size_t)W * ENTRY * 4, join = 2 * KV4_MAX_CTAS * HG * 4;
+    // the rings; later the tail partials and what is joined across CTAs
+    static constexpr size_t rings = (size_t)W * KV4_STAGES * STAGE, ring = rings > heads + join ? rings : heads + join;
     static constexpr size_t smem(int n) { return ring + heads + (size_t)(n + 1) * 8; }
-    static_assert(ring >= heads, "the tail partials take the ring's place");
 };
 
 __device__ __forceinline__ float kv4_ex2(float x)
@@ -399,7 +401,9 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
     float     *heads = reinterpret_cast<float *>(smem + S::ring);
     long long *pre = reinterpret_cast<long long *>(smem + S::ring + S::heads);     // places of a row before sequence i
     __shared__ long long rid[2 * W];                      // the row of each warp's head and tail partial, -1: none
-    __shared__ int       last_s;
+    __shared__ float     wgt[2 * W][HG], top_s[2 * W][HG];
+    __shared__ int       last_s, c0_s, np_s;
+    float *joinM = tails + W * ENTRY, *joinL = joinM + KV4_MAX_CTAS * HG;     // of a row's CTAs, behind the tails
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int n = list.n, n_grp = (a.n_rep + HG - 1) / HG, R = a.n_kv * n_grp;
@@ -852,17 +856,32 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
     if (tail) store_part(tails + warp * ENTRY);
     __syncthreads();
 
-    // rows that this CTA's warps share
+    // Rows that this CTA's warps share.  A partial's weight is 2^(its M - the
+    // row's M); one without a unit (its sum is zero) has none.
     auto entry = [&](int e) { return (e & 1) ? tails + (e >> 1) * ENTRY : heads + (e >> 1) * ENTRY; };
+    auto weight = [](float M, float m, float l) { return l == 0.0f ? 0.0f : kv4_ex2(M - m); };
     auto write = [&](long long row, int x, float v) {
         const int i = (int)(row / R), r = (int)(row - (long long)i * R), kvh = r / n_grp, grp = r - kvh * n_grp, h = grp * HG + x / HD;
         if (h < a.n_rep)
             ((T *)a.out)[(size_t)i * a.out_stride + (size_t)(kvh * a.n_rep + h) * HD + x % HD] = kv4_from<T>(v);
     };
+    for (int x = tid; x < 2 * W * HG; x += W * 32) {
+        const int e = x / HG, at = x % HG * (HD + 2) + HD;
+        if (rid[e] < 0) continue;
+        int lo = e, hi = e + 1;                           // the row's partials (-1 between them)
+        while (lo > 0 && (rid[lo - 1] < 0 || rid[lo - 1] == rid[e])) lo--;
+        while (hi < 2 * W && (rid[hi] < 0 || rid[hi] == rid[e])) hi++;
+        float m = -INFINITY;
+        for (int k = lo; k < hi; k++)
+            if (rid[k] >= 0) m = fmaxf(m, entry(k)[at]);
+        wgt[e][x % HG] = weight(entry(e)[at], m, entry(e)[at + 1]);
+        top_s[e][x % HG] = m;
+    }
+    __syncthreads();
     for (int e = 0; e < 2 * W; e++) {
         const long long row = rid[e];
         if (row < 0) continue;
-        int end = e + 1;                                  // the row's partials: e .. end - 1 (-1 between them)
+        int end = e + 1;
         while (end < 2 * W && (rid[end] < 0 || rid[end] == row)) end++;
         const int       i = (int)(row / R);
         const long long nu = pre[i + 1] - pre[i], first = pre[i] * R + (row - (long long)i * R) * nu;
@@ -870,12 +889,10 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
         float          *out = a.part + ((size_t)blockIdx.x * 2 + (first >= cu0)) * ENTRY;
         for (int x = tid; x < HG * HD; x += W * 32) {
             const int h = x / HD, at = h * (HD + 2);
-            float     m = -INFINITY, L = 0.0f, v = 0.0f;
-            for (int k = e; k < end; k++)
-                if (rid[k] >= 0) m = fmaxf(m, entry(k)[at + HD]);
+            float     L = 0.0f, v = 0.0f;
             for (int k = e; k < end; k++)
                 if (rid[k] >= 0) {
-                    const float w = entry(k)[at + HD + 1] == 0.0f ? 0.0f : kv4_ex2(entry(k)[at + HD] - m);   // (no unit: no weight)
+                    const float w = wgt[k][h];
                     L = fmaf(w, entry(k)[at + HD + 1], L);
                     v = fmaf(w, entry(k)[at + x % HD], v);
                 }
@@ -883,37 +900,45 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
             else {
                 out[at + x % HD] = v;
                 if (x % HD == 0) {
-                    out[at + HD] = m;
+                    out[at + HD] = top_s[e][h];
                     out[at + HD + 1] = L;
                 }
             }
         }
         if (!whole) {
-            // the CTAs of the row: those whose runs hold its units
+            // the CTAs of the row: those whose runs hold its places
             auto cta_of = [&](long long u) {
                 long long b = u * ctas / total;
                 while (total * (b + 1) / ctas <= u) b++;
                 while (total * b / ctas > u) b--;
                 return (int)b;
             };
-            const int c0 = cta_of(first), c1 = cta_of(first + nu - 1);
-            __threadfence();
             __syncthreads();
-            if (tid == 0) last_s = atomicAdd(a.count + c0, 1u) == (unsigned)(c1 - c0);
+            if (tid == 0) {
+                c0_s = cta_of(first);
+                np_s = cta_of(first + nu - 1) - c0_s + 1;
+                __threadfence();
+                last_s = atomicAdd(a.count + c0_s, 1u) == (unsigned)(np_s - 1);
+                __threadfence();
+            }
             __syncthreads();
             if (last_s) {
-                __threadfence();
+                const int c0 = c0_s, np = np_s;
+                auto part = [&](int b) { return a.part + ((size_t)(c0 + b) * 2 + (b == 0)) * ENTRY; };
+                for (int x = tid; x < np * HG; x += W * 32) {
+                    joinM[x] = __ldcg(part(x / HG) + x % HG * (HD + 2) + HD);
+                    joinL[x] = __ldcg(part(x / HG) + x % HG * (HD + 2) + HD + 1);
+                }
+                __syncthreads();
                 for (int x = tid; x < HG * HD; x += W * 32) {
-                    const int h = x / HD, at = h * (HD + 2);
-                    auto      part = [&](int b) { return a.part + ((size_t)b * 2 + (b == c0)) * ENTRY + at; };
+                    const int h = x / HD, at = h * (HD + 2) + x % HD;
                     float     m = -INFINITY, L = 0.0f, v = 0.0f;
+                    for (int b = 0; b < np; b++) m = fmaxf(m, joinM[b * HG + h]);
 #pragma unroll 8
-                    for (int b = c0; b <= c1; b++) m = fmaxf(m, __ldcg(part(b) + HD));
-#pragma unroll 8
-                    for (int b = c0; b <= c1; b++) {
-                        const float w = __ldcg(part(b) + HD + 1) == 0.0f ? 0.0f : kv4_ex2(__ldcg(part(b) + HD) - m);
-                        L = fmaf(w, __ldcg(part(b) + HD + 1), L);
-                        v = fmaf(w, __ldcg(part(b) + x % HD), v);
+                    for (int b = 0; b < np; b++) {
+                        const float w = weight(joinM[b * HG + h], m, joinL[b * HG + h]);
+                        L = fmaf(w, joinL[b * HG + h], L);
+                        v = fmaf(w, __ldcg(part(b) + at), v);
                     }
                     write(row, x, v / L);
                 }
