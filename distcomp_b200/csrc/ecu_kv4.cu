@@ -458,8 +458,13 @@ static int attend_launch(ecu_kv *kv, const KvAttendArgs &a, const int *seq, int 
 template <typename T, int NB, int NT>
 static int attend_list(ecu_kv *kv, KvAttendArgs a, const int *seq, int n, bool whole, cudaStream_t s)
 {
-    for (int i = 0; i < n; i += KV4_LIST) {
-        const int  m = std::min(KV4_LIST, n - i);
+    // at most 2^31 - 1 places in a launch, however the sequences may grow
+    const long long places = (long long)kv->n_head_kv * ((a.n_rep + KvShape<T, NB, NT>::HG - 1) / KvShape<T, NB, NT>::HG) *
+                             ((long long)kv->book.max_pages * (KV4_PAGE / KV4_UNIT) + 1);
+    if (places > INT_MAX) return say("ecu_kv_attend", "too many positions and heads a sequence");
+    const int most = (int)std::min<long long>(KV4_LIST, INT_MAX / places);
+    for (int i = 0; i < n; i += most) {
+        const int  m = std::min(most, n - i);
         const int *q = seq ? seq + i : nullptr;
         if ((m <= 64 ? attend_launch<T, NB, NT, 64>(kv, a, q, i, m, whole, s)
                      : attend_launch<T, NB, NT, KV4_LIST>(kv, a, q, i, m, whole, s)) != 0)

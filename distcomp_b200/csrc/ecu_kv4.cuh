@@ -285,7 +285,7 @@ template <typename T, int NB, int NT> struct KvShape {
     static constexpr size_t heads = (size_t)W * ENTRY * 4, join = 2 * KV4_MAX_CTAS * HG * 4;
     // the rings; later the tail partials and what is joined across CTAs
     static constexpr size_t rings = (size_t)W * KV4_STAGES * STAGE, ring = rings > heads + join ? rings : heads + join;
-    static constexpr size_t smem(int n) { return ring + heads + (size_t)(n + 1) * 8; }
+    static constexpr size_t smem(int n) { return ring + heads + (size_t)(n + 1) * 4; }
 };
 
 __device__ __forceinline__ float kv4_ex2(float x)
@@ -399,10 +399,11 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
     extern __shared__ __align__(128) uint8_t smem[];
     float     *tails = reinterpret_cast<float *>(smem);   // after the loop: tail partials, in the ring's place
     float     *heads = reinterpret_cast<float *>(smem + S::ring);
-    long long *pre = reinterpret_cast<long long *>(smem + S::ring + S::heads);     // places of a row before sequence i
-    __shared__ long long rid[2 * W];                      // the row of each warp's head and tail partial, -1: none
+    int       *pre = reinterpret_cast<int *>(smem + S::ring + S::heads);     // places of a row before sequence i
+    __shared__ int       rid[2 * W];                      // the row of each warp's head and tail partial, -1: none
     __shared__ float     wgt[2 * W][HG], top_s[2 * W][HG];
-    __shared__ int       last_s, c0_s, np_s;
+    __shared__ unsigned  mates[2 * W], leaders, sums[W];
+    __shared__ int       last_s[2], c0_s[2], np_s[2];     // of the rows shared with CTAs before and after
     float *joinM = tails + W * ENTRY, *joinL = joinM + KV4_MAX_CTAS * HG;     // of a row's CTAs, behind the tails
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
@@ -411,22 +412,36 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
     uint8_t  *ring = smem + (size_t)warp * KV4_STAGES * STAGE;
 
     if (tid < 2 * W) rid[tid] = -1;
-    // places before each sequence: one warp scans 32 at a time, the last one's sums carried on
-    if (warp == 0) {
-        long long run = 0;
-        for (int i0 = 0; i0 < n; i0 += 32) {
-            const int i = i0 + lane;
-            long long u = i < n ? (min(max(__ldg(a.len + list.seq[i]), 0), cap) + KV4_UNIT - 1) / KV4_UNIT : 0;
-            u += u > 0;
+    // places before each sequence: a scan over the list, PER sequences a thread
+    {
+        constexpr int PER = (N + W * 32 - 1) / (W * 32);
+        int           c[PER], sum = 0;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long v = __shfl_up_sync(0xffffffffu, u, o);
-                if (lane >= o) u += v;
-            }
-            if (i < n) pre[i + 1] = run + u;
-            run += __shfl_sync(0xffffffffu, u, 31);
+        for (int k = 0; k < PER; k++) {
+            const int i = tid * PER + k;
+            c[k] = i < n ? (min(max(__ldg(a.len + list.seq[i]), 0), cap) + KV4_UNIT - 1) / KV4_UNIT : 0;
         }
-        if (lane == 0) pre[0] = 0;
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            c[k] += c[k] > 0;
+            sum += c[k];
+        }
+        int run = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += v;
+        }
+        if (lane == 31) sums[warp] = (unsigned)run;
+        __syncthreads();
+        run -= sum;
+        for (int w = 0; w < warp; w++) run += (int)sums[w];
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            if (tid * PER + k <= n) pre[tid * PER + k] = run;
+            run += c[k];
+        }
+        if (tid == W * 32 - 1 && n == W * 32 * PER) pre[n] = run;
     }
     __syncthreads();
 
@@ -436,14 +451,15 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
             for (int x = tid; x < a.n_kv * a.n_rep * HD; x += W * 32)
                 ((T *)a.out)[(size_t)i * a.out_stride + x] = kv4_from<T>(0.0f);
 
-    const long long total = pre[n] * R;
+    const int  total = pre[n] * R;                        // below 2^31: the host sees to it
     // CTAs with a run: none of them empty, since a shared row waits for a ticket from each
-    const long long ctas = min((long long)gridDim.x, total);
-    const bool      busy = blockIdx.x < ctas;
-    const long long cu0 = busy ? total * blockIdx.x / ctas : 0, cu1 = busy ? total * (blockIdx.x + 1) / ctas : 0;
-    const long long u0 = cu0 + (cu1 - cu0) * warp / W, u1 = cu0 + (cu1 - cu0) * (warp + 1) / W;
+    const int  ctas = min((int)gridDim.x, total);
+    const bool busy = (int)blockIdx.x < ctas;
+    auto       begin_of = [&](int b) { return (int)((long long)total * b / ctas); };
+    const int  cu0 = busy ? begin_of(blockIdx.x) : 0, cu1 = busy ? begin_of(blockIdx.x + 1) : 0;
+    const int  u0 = cu0 + (int)((long long)(cu1 - cu0) * warp / W), u1 = cu0 + (int)((long long)(cu1 - cu0) * (warp + 1) / W);
 
-    auto locate = [&](long long u) {
+    auto locate = [&](int u) {
         KvCursor p;
         int      lo = 0, hi = n;                          // the last sequence whose units begin at or before u
         while (hi - lo > 1) {
@@ -452,11 +468,10 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
             else hi = mid;
         }
         p.i = lo;
-        p.nu = (int)(pre[lo + 1] - pre[lo]);
-        const long long v = u - pre[lo] * R;
-        p.r = (int)(v / p.nu);
-        p.j = (int)(v - (long long)p.r * p.nu);
-        p.left = (int)(u1 - u);
+        p.nu = pre[lo + 1] - pre[lo];
+        p.r = (u - pre[lo] * R) / p.nu;
+        p.j = u - pre[lo] * R - p.r * p.nu;
+        p.left = u1 - u;
         return p;
     };
     auto next = [&](KvCursor &p) {
@@ -467,7 +482,7 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
         p.r = 0;
         do p.i++;
         while (p.i < n && pre[p.i + 1] == pre[p.i]);
-        p.nu = p.i < n ? (int)(pre[p.i + 1] - pre[p.i]) : 1;
+        p.nu = p.i < n ? pre[p.i + 1] - pre[p.i] : 1;
     };
     // the page of the first unit at or after p inside this warp's run; p moves there
     auto page_at = [&](KvCursor &p) {
@@ -829,7 +844,7 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
                 continue;
             }
             sum_l();
-            const long long row = (long long)at.i * R + at.r;
+            const int row = at.i * R + at.r;
             if (j0 > 0) {
                 store_part(heads + warp * ENTRY);
                 if (lane == 0) rid[2 * warp] = row;
@@ -854,48 +869,70 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
     }
     __syncthreads();                                      // every ring is idle
     if (tail) store_part(tails + warp * ENTRY);
+    // meanwhile: the rows that this CTA shares with others, slot 0 the one that
+    // began before its run, slot 1 the one that goes on after it, and their CTAs
+    if (lane < 2 && warp == W - 1) {
+        np_s[lane] = last_s[lane] = 0;
+        if (busy) {
+            const KvCursor p = locate(lane ? cu1 - 1 : cu0);
+            const int      first = pre[p.i] * R + p.r * p.nu, end = first + p.nu;
+            if ((lane ? first >= cu0 : first < cu0) && (first < cu0 || end > cu1)) {
+                auto cta_of = [&](int u) {
+                    int b = (int)((long long)u * ctas / total);
+                    while (begin_of(b + 1) <= u) b++;
+                    while (begin_of(b) > u) b--;
+                    return b;
+                };
+                c0_s[lane] = cta_of(first);
+                np_s[lane] = cta_of(end - 1) - c0_s[lane] + 1;
+            }
+        }
+    }
     __syncthreads();
 
     // Rows that this CTA's warps share.  A partial's weight is 2^(its M - the
     // row's M); one without a unit (its sum is zero) has none.
     auto entry = [&](int e) { return (e & 1) ? tails + (e >> 1) * ENTRY : heads + (e >> 1) * ENTRY; };
     auto weight = [](float M, float m, float l) { return l == 0.0f ? 0.0f : kv4_ex2(M - m); };
-    auto write = [&](long long row, int x, float v) {
-        const int i = (int)(row / R), r = (int)(row - (long long)i * R), kvh = r / n_grp, grp = r - kvh * n_grp, h = grp * HG + x / HD;
+    auto write = [&](int row, int x, float v) {
+        const int i = row / R, r = row - i * R, kvh = r / n_grp, grp = r - kvh * n_grp, h = grp * HG + x / HD;
         if (h < a.n_rep)
             ((T *)a.out)[(size_t)i * a.out_stride + (size_t)(kvh * a.n_rep + h) * HD + x % HD] = kv4_from<T>(v);
     };
-    for (int x = tid; x < 2 * W * HG; x += W * 32) {
-        const int e = x / HG, at = x % HG * (HD + 2) + HD;
-        if (rid[e] < 0) continue;
-        int lo = e, hi = e + 1;                           // the row's partials (-1 between them)
-        while (lo > 0 && (rid[lo - 1] < 0 || rid[lo - 1] == rid[e])) lo--;
-        while (hi < 2 * W && (rid[hi] < 0 || rid[hi] == rid[e])) hi++;
-        float m = -INFINITY;
-        for (int k = lo; k < hi; k++)
-            if (rid[k] >= 0) m = fmaxf(m, entry(k)[at]);
-        wgt[e][x % HG] = weight(entry(e)[at], m, entry(e)[at + 1]);
-        top_s[e][x % HG] = m;
+    if (warp < HG) {                                      // a warp per head, a lane per partial
+        const int      row = lane < 2 * W ? rid[lane % (2 * W)] : -1;
+        const unsigned same = __match_any_sync(0xffffffffu, row);
+        const float   *e = entry(lane % (2 * W)) + warp * (HD + 2) + HD;
+        const float    M = row >= 0 ? e[0] : -INFINITY;
+        // floats in the order of their bits as whole numbers
+        const int      bits = __float_as_int(M), key = bits ^ ((bits >> 31) & 0x7FFFFFFF);
+        const int      most = __reduce_max_sync(same, key);
+        const float    m = __int_as_float(most ^ ((most >> 31) & 0x7FFFFFFF));
+        if (lane < 2 * W) {
+            wgt[lane][warp] = row >= 0 ? weight(M, m, e[1]) : 0.0f;
+            top_s[lane][warp] = m;
+            mates[lane] = same;
+        }
+        const unsigned lead = __ballot_sync(0xffffffffu, row >= 0 && __ffs(same) - 1 == lane);
+        if (tid == 0) leaders = lead;
     }
     __syncthreads();
-    for (int e = 0; e < 2 * W; e++) {
-        const long long row = rid[e];
-        if (row < 0) continue;
-        int end = e + 1;
-        while (end < 2 * W && (rid[end] < 0 || rid[end] == row)) end++;
-        const int       i = (int)(row / R);
-        const long long nu = pre[i + 1] - pre[i], first = pre[i] * R + (row - (long long)i * R) * nu;
-        const bool      whole = first >= cu0 && first + nu <= cu1;
-        float          *out = a.part + ((size_t)blockIdx.x * 2 + (first >= cu0)) * ENTRY;
+    for (unsigned todo = leaders; todo; todo &= todo - 1) {
+        const int e = __ffs(todo) - 1, end = 32 - __clz(mates[e]), row = rid[e];
+        const int i = row / R, nu = pre[i + 1] - pre[i], first = pre[i] * R + (row - i * R) * nu;
+        const bool whole = first >= cu0 && first + nu <= cu1;
+        float     *out = a.part + ((size_t)blockIdx.x * 2 + (first >= cu0)) * ENTRY;
         for (int x = tid; x < HG * HD; x += W * 32) {
             const int h = x / HD, at = h * (HD + 2);
             float     L = 0.0f, v = 0.0f;
-            for (int k = e; k < end; k++)
-                if (rid[k] >= 0) {
-                    const float w = wgt[k][h];
-                    L = fmaf(w, entry(k)[at + HD + 1], L);
-                    v = fmaf(w, entry(k)[at + x % HD], v);
+#pragma unroll 4
+            for (int k = e; k < end; k++) {
+                const float w = wgt[k][h], ln = entry(k)[at + HD + 1], vn = entry(k)[at + x % HD];
+                if (w != 0.0f) {                          // (an unused place holds anything)
+                    L = fmaf(w, ln, L);
+                    v = fmaf(w, vn, v);
                 }
+            }
             if (whole) write(row, x, v / L);
             else {
                 out[at + x % HD] = v;
@@ -905,47 +942,39 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
                 }
             }
         }
-        if (!whole) {
-            // the CTAs of the row: those whose runs hold its places
-            auto cta_of = [&](long long u) {
-                long long b = u * ctas / total;
-                while (total * (b + 1) / ctas <= u) b++;
-                while (total * b / ctas > u) b--;
-                return (int)b;
-            };
-            __syncthreads();
-            if (tid == 0) {
-                c0_s = cta_of(first);
-                np_s = cta_of(first + nu - 1) - c0_s + 1;
-                __threadfence();
-                last_s = atomicAdd(a.count + c0_s, 1u) == (unsigned)(np_s - 1);
-                __threadfence();
-            }
-            __syncthreads();
-            if (last_s) {
-                const int c0 = c0_s, np = np_s;
-                auto part = [&](int b) { return a.part + ((size_t)(c0 + b) * 2 + (b == 0)) * ENTRY; };
-                for (int x = tid; x < np * HG; x += W * 32) {
-                    joinM[x] = __ldcg(part(x / HG) + x % HG * (HD + 2) + HD);
-                    joinL[x] = __ldcg(part(x / HG) + x % HG * (HD + 2) + HD + 1);
-                }
-                __syncthreads();
-                for (int x = tid; x < HG * HD; x += W * 32) {
-                    const int h = x / HD, at = h * (HD + 2) + x % HD;
-                    float     m = -INFINITY, L = 0.0f, v = 0.0f;
-                    for (int b = 0; b < np; b++) m = fmaxf(m, joinM[b * HG + h]);
-#pragma unroll 8
-                    for (int b = 0; b < np; b++) {
-                        const float w = weight(joinM[b * HG + h], m, joinL[b * HG + h]);
-                        L = fmaf(w, joinL[b * HG + h], L);
-                        v = fmaf(w, __ldcg(part(b) + at), v);
-                    }
-                    write(row, x, v / L);
-                }
-                if (tid == 0) a.count[c0] = 0;            // as the next call finds it
-            }
-            __syncthreads();
+    }
+    if (np_s[0] == 0 && np_s[1] == 0) return;
+    __syncthreads();
+    // a ticket for each shared row (released after, and acquired before, the partials)
+    if (lane == 0 && warp < 2 && np_s[warp]) {
+        unsigned t;
+        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(t) : "l"(a.count + c0_s[warp]) : "memory");
+        last_s[warp] = t == (unsigned)(np_s[warp] - 1);
+    }
+    __syncthreads();
+    for (int s = 0; s < 2; s++) {
+        if (!last_s[s]) continue;
+        const int c0 = c0_s[s], np = np_s[s], row_at = s ? cu1 - 1 : cu0;
+        auto      part = [&](int b) { return a.part + ((size_t)(c0 + b) * 2 + (b == 0)) * ENTRY; };
+        for (int x = tid; x < np * HG; x += W * 32) {
+            joinM[x] = __ldcg(part(x / HG) + x % HG * (HD + 2) + HD);
+            joinL[x] = __ldcg(part(x / HG) + x % HG * (HD + 2) + HD + 1);
         }
-        e = end - 1;
+        __syncthreads();
+        const KvCursor p = locate(row_at);
+        for (int x = tid; x < HG * HD; x += W * 32) {
+            const int h = x / HD, at = h * (HD + 2) + x % HD;
+            float     m = -INFINITY, L = 0.0f, v = 0.0f;
+            for (int b = 0; b < np; b++) m = fmaxf(m, joinM[b * HG + h]);
+#pragma unroll 8
+            for (int b = 0; b < np; b++) {
+                const float w = weight(joinM[b * HG + h], m, joinL[b * HG + h]), vn = __ldcg(part(b) + at);
+                L = fmaf(w, joinL[b * HG + h], L);
+                v = fmaf(w, vn, v);
+            }
+            write(p.i * R + p.r, x, v / L);
+        }
+        if (tid == 0) a.count[c0] = 0;                    // as the next call finds it
+        __syncthreads();
     }
 }
