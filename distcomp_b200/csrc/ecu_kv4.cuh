@@ -282,7 +282,7 @@ template <typename T, int NB, int NT> struct KvShape {
     static constexpr int HG = 8 * NT / P;                 // query heads of a group
     static constexpr int STAGE = 36 * HD;                 // one unit: K codes, V codes, K scales, V scales
     static constexpr int ENTRY = HG * (HD + 2);           // a partial: per head the sums, M and the weights' sum
-    static constexpr size_t heads = (size_t)W * ENTRY * 4, join = 2 * KV4_MAX_CTAS * HG * 4;
+    static constexpr size_t heads = (size_t)W * ENTRY * 4, join = KV4_MAX_CTAS * HG * 4;
     // the rings; later the tail partials and what is joined across CTAs
     static constexpr size_t rings = (size_t)W * KV4_STAGES * STAGE, ring = rings > heads + join ? rings : heads + join;
     static constexpr size_t smem(int n) { return ring + heads + (size_t)(n + 1) * 4; }
@@ -402,9 +402,11 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
     int       *pre = reinterpret_cast<int *>(smem + S::ring + S::heads);     // places of a row before sequence i
     __shared__ int       rid[2 * W];                      // the row of each warp's head and tail partial, -1: none
     __shared__ float     wgt[2 * W][HG], top_s[2 * W][HG];
-    __shared__ unsigned  mates[2 * W], leaders, sums[W];
+    __shared__ unsigned  mates[2 * W], sums[W];
+    __shared__ int       lead_s[2 * W], n_lead;
+    __shared__ float     joinL[HG];
     __shared__ int       last_s[2], c0_s[2], np_s[2];     // of the rows shared with CTAs before and after
-    float *joinM = tails + W * ENTRY, *joinL = joinM + KV4_MAX_CTAS * HG;     // of a row's CTAs, behind the tails
+    float *joinW = tails + W * ENTRY;                     // the weights of a row's CTAs, behind the tails
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int n = list.n, n_grp = (a.n_rep + HG - 1) / HG, R = a.n_kv * n_grp;
@@ -511,6 +513,13 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
     float    fac[HL];                                     // score * fac: in units of log2
     float    O[NT][NB][2][4], M[HL], l[HL];
 
+    // row p's queries on their way into the cache, before load_q wants them
+    auto fetch_q = [&](const KvCursor &p) {
+        const int kvh = p.r / n_grp, grp = p.r - kvh * n_grp;
+        const T  *q = (const T *)a.q + (size_t)p.i * a.q_stride + (size_t)(kvh * a.n_rep + grp * HG) * HD;
+        for (int x = lane * (128 / (int)sizeof(T)); x < min(HG, a.n_rep - grp * HG) * HD; x += 32 * (128 / (int)sizeof(T)))
+            asm volatile("prefetch.global.L1 [%0];" ::"l"(q + x));
+    };
     // the queries of row p.r: column col is query head HG * group + col / P, part col % P
     auto load_q = [&](const KvCursor &p) {
         const int kvh = p.r / n_grp, grp = p.r - kvh * n_grp;
@@ -807,6 +816,7 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
         KvCursor at = locate(u0), ahead = at;
         KvCursor first[KV4_STAGES];
         int      page[KV4_STAGES + 1];
+        fetch_q(at);
 #pragma unroll
         for (int k = 0; k < KV4_STAGES; k++) {            // independent loads
             page[k] = page_at(ahead);
@@ -832,6 +842,7 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
                 if (ahead.left > 0) {
                     issue(ahead, page[KV4_STAGES], k);
                     next(ahead);
+                    if (ahead.j == 0 && ahead.left > 0) fetch_q(ahead);
                     page[KV4_STAGES] = page_at(ahead);
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
@@ -913,33 +924,34 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
             top_s[lane][warp] = m;
             mates[lane] = same;
         }
-        const unsigned lead = __ballot_sync(0xffffffffu, row >= 0 && __ffs(same) - 1 == lane);
-        if (tid == 0) leaders = lead;
+        const bool     first = row >= 0 && __ffs(same) - 1 == lane;
+        const unsigned lead = __ballot_sync(0xffffffffu, first);
+        if (warp == 0 && first) lead_s[__popc(lead & ((1u << lane) - 1))] = lane;
+        if (tid == 0) n_lead = __popc(lead);
     }
     __syncthreads();
-    for (unsigned todo = leaders; todo; todo &= todo - 1) {
-        const int e = __ffs(todo) - 1, end = 32 - __clz(mates[e]), row = rid[e];
+    // a warp per row and 32 dimensions of a head
+    for (int task = warp; task < n_lead * HG * NB; task += W) {
+        const int e = lead_s[task / (HG * NB)], end = 32 - __clz(mates[e]), row = rid[e];
         const int i = row / R, nu = pre[i + 1] - pre[i], first = pre[i] * R + (row - i * R) * nu;
         const bool whole = first >= cu0 && first + nu <= cu1;
-        float     *out = a.part + ((size_t)blockIdx.x * 2 + (first >= cu0)) * ENTRY;
-        for (int x = tid; x < HG * HD; x += W * 32) {
-            const int h = x / HD, at = h * (HD + 2);
-            float     L = 0.0f, v = 0.0f;
+        const int  x = task % (HG * NB) * 32 + lane, h = x / HD, at = h * (HD + 2);
+        float      L = 0.0f, v = 0.0f;
 #pragma unroll 4
-            for (int k = e; k < end; k++) {
-                const float w = wgt[k][h], ln = entry(k)[at + HD + 1], vn = entry(k)[at + x % HD];
-                if (w != 0.0f) {                          // (an unused place holds anything)
-                    L = fmaf(w, ln, L);
-                    v = fmaf(w, vn, v);
-                }
+        for (int k = e; k < end; k++) {
+            const float w = wgt[k][h], ln = entry(k)[at + HD + 1], vn = entry(k)[at + x % HD];
+            if (w != 0.0f) {                              // (an unused place holds anything)
+                L = fmaf(w, ln, L);
+                v = fmaf(w, vn, v);
             }
-            if (whole) write(row, x, v / L);
-            else {
-                out[at + x % HD] = v;
-                if (x % HD == 0) {
-                    out[at + HD] = top_s[e][h];
-                    out[at + HD + 1] = L;
-                }
+        }
+        if (whole) write(row, x, v / L);
+        else {                                            // sums [HG][HD], then M and the weights' sum of each head
+            float *out = a.part + ((size_t)blockIdx.x * 2 + (first >= cu0)) * ENTRY;
+            out[x] = v;
+            if (x % HD == 0) {
+                out[HG * HD + h] = top_s[e][h];
+                out[HG * HD + HG + h] = L;
             }
         }
     }
@@ -954,25 +966,58 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
     __syncthreads();
     for (int s = 0; s < 2; s++) {
         if (!last_s[s]) continue;
-        const int c0 = c0_s[s], np = np_s[s], row_at = s ? cu1 - 1 : cu0;
-        auto      part = [&](int b) { return a.part + ((size_t)(c0 + b) * 2 + (b == 0)) * ENTRY; };
-        for (int x = tid; x < np * HG; x += W * 32) {
-            joinM[x] = __ldcg(part(x / HG) + x % HG * (HD + 2) + HD);
-            joinL[x] = __ldcg(part(x / HG) + x % HG * (HD + 2) + HD + 1);
+        // GR partials at a time, four sums a thread, up to eight partials in flight
+        constexpr int V4 = HG * HD / 4, GR = W * 32 / V4;
+        const int     c0 = c0_s[s], np = np_s[s], grp = tid / V4, x4 = tid % V4;
+        auto          part = [&](int b) { return a.part + ((size_t)(c0 + b) * 2 + (b == 0)) * ENTRY; };
+        float4        v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int b = grp + k * GR;
+            v[k] = grp < GR && b < np ? __ldcg(reinterpret_cast<const float4 *>(part(b)) + x4) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        if (warp < HG) {
+            float m = -INFINITY, L = 0.0f;
+            for (int b = lane; b < np; b += 32) m = fmaxf(m, __ldcg(part(b) + HG * HD + warp));
+#pragma unroll
+            for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            for (int b = lane; b < np; b += 32) {
+                const float ln = __ldcg(part(b) + HG * HD + HG + warp), w = weight(__ldcg(part(b) + HG * HD + warp), m, ln);
+                joinW[b * HG + warp] = w;
+                L = fmaf(w, ln, L);
+            }
+            L = warp_sum(L);
+            if (lane == 0) joinL[warp] = L;
         }
         __syncthreads();
-        const KvCursor p = locate(row_at);
-        for (int x = tid; x < HG * HD; x += W * 32) {
-            const int h = x / HD, at = h * (HD + 2) + x % HD;
-            float     m = -INFINITY, L = 0.0f, v = 0.0f;
-            for (int b = 0; b < np; b++) m = fmaxf(m, joinM[b * HG + h]);
-#pragma unroll 8
-            for (int b = 0; b < np; b++) {
-                const float w = weight(joinM[b * HG + h], m, joinL[b * HG + h]), vn = __ldcg(part(b) + at);
-                L = fmaf(w, joinL[b * HG + h], L);
-                v = fmaf(w, vn, v);
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int b0 = 0; b0 < np; b0 += 8 * GR) {
+            if (b0)
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const int b = b0 + grp + k * GR;
+                    if (grp < GR && b < np) v[k] = __ldcg(reinterpret_cast<const float4 *>(part(b)) + x4);
+                }
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int b = b0 + grp + k * GR;
+                if (grp < GR && b < np) {
+                    const float w = joinW[b * HG + x4 * 4 / HD];
+                    sum.x = fmaf(w, v[k].x, sum.x);
+                    sum.y = fmaf(w, v[k].y, sum.y);
+                    sum.z = fmaf(w, v[k].z, sum.z);
+                    sum.w = fmaf(w, v[k].w, sum.w);
+                }
             }
-            write(p.i * R + p.r, x, v / L);
+        }
+        if (grp < GR) reinterpret_cast<float4 *>(heads)[tid] = sum;
+        __syncthreads();
+        const KvCursor p = locate(s ? cu1 - 1 : cu0);
+        for (int x = tid; x < HG * HD; x += W * 32) {
+            float y = 0.0f;
+#pragma unroll
+            for (int k = 0; k < GR; k++) y += heads[k * HG * HD + x];
+            write(p.i * R + p.r, x, y / joinL[x / HD]);
         }
         if (tid == 0) a.count[c0] = 0;                    // as the next call finds it
         __syncthreads();
