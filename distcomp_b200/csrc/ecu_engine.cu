@@ -9,6 +9,7 @@
 // StepState, so the graph is position independent.
 #include "../../include/engine_cuda.h"
 #include "ecu_attn.cuh"
+#include "ecu_batch.cuh"
 #include "ecu_gemv.cuh"
 #include "ecu_kv4.h"
 #include "ecu_mega.cuh"
@@ -23,10 +24,13 @@
 #include <sys/mman.h>
 #include <sys/stat.h>
 #include <unistd.h>
+#include <algorithm>
+#include <climits>
 #include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <exception>
 #include <memory>
 #include <string>
 #include <thread>
@@ -448,6 +452,11 @@ struct ecu_ctx {
         __half *ah = nullptr, *al = nullptr, *wh = nullptr, *wl = nullptr;
         int    *tok = nullptr;
     } pf;
+    // fp16 rows of the tensor-core prompt attention, grown on use
+    struct Halves {
+        size_t  qcap = 0, kcap = 0;
+        __half *q = nullptr, *k = nullptr, *v = nullptr;
+    } hf;
     cudaStream_t stream = nullptr;
     bool        pdl = true, use_graph = true;
     std::vector<void *> allocs;           // this context's own buffers
@@ -737,7 +746,8 @@ static void ctx_free(ecu_ctx *c)
     if (c->link_peer) cudaIpcCloseMemHandle(c->link_peer);
     if (c->ev_step) cudaEventDestroy(c->ev_step);
     for (void *p : {(void *)c->pf.X, (void *)c->pf.QKV, (void *)c->pf.ATT, (void *)c->pf.GU, (void *)c->pf.H,
-                    (void *)c->pf.ah, (void *)c->pf.al, (void *)c->pf.wh, (void *)c->pf.wl, (void *)c->pf.tok})
+                    (void *)c->pf.ah, (void *)c->pf.al, (void *)c->pf.wh, (void *)c->pf.wl, (void *)c->pf.tok,
+                    (void *)c->hf.q, (void *)c->hf.k, (void *)c->hf.v})
         if (p) cudaFree(p);
     for (void *p : c->allocs) cudaFree(p);
     if (c->h_st) cudaFreeHost(c->h_st);
@@ -3193,6 +3203,11 @@ static int pf_gemm(ecu_ctx *c, const DevMat &m, int n, float *C, const float *R)
     return 0;
 }
 
+// ECU_PF_ATTN=2: the prompt's attention on the tensor cores (ecu_attn_prompt)
+// with fp16 operands.  Their rounding, 2^-12 of each element, is far inside
+// the prompt's 1e-3 bar, but not the fp32 attention's results: off by default.
+static bool pf_attn_tc() { const char *e = getenv("ECU_PF_ATTN"); return e && e[0] == '2'; }
+
 // Can the batched kernels run this context's prompt (else: token by token)?
 static bool pf_batched(const ecu_ctx *c, bool &attn2)
 {
@@ -3201,7 +3216,7 @@ static bool pf_batched(const ecu_ctx *c, bool &attn2)
     // one-query-per-CTA kernel keeps its scores in a PF_ATT_MAXPOS array
     const char *ae = getenv("ECU_PF_ATTN");
     attn2 = PF_QB % g.n_rep == 0 && !(ae && ae[0] == '0');
-    bool batched = c->tp.world == 1 && (attn2 || g.n_ctx <= PF_ATT_MAXPOS) && (g.head_dim == 64 || g.head_dim == 128) &&
+    bool batched = c->tp.world == 1 && (attn2 || pf_attn_tc() || g.n_ctx <= PF_ATT_MAXPOS) && (g.head_dim == 64 || g.head_dim == 128) &&
                    g.n_embd % 8 == 0 && g.n_ff % 8 == 0;
     for (auto &ly : c->layers) batched = batched && (!ly.ha || ly.qkv.size() == 1) && (!ly.hf || ly.gu_fused);
     return batched;
@@ -3217,6 +3232,50 @@ static int pf_attrs(const ecu_ctx *c)
         CK(cudaFuncSetAttribute(k_pf_attn2<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pf_attn2_smem<64>()));
         if (c->device < 32) attr_done.fetch_or(1u << c->device);
     }
+    return 0;
+}
+
+// fp16 rows for the tensor-core prompt attention: q elements of queries, k of
+// keys and of values.
+static int hf_reserve(ecu_ctx *c, size_t q, size_t k)
+{
+    auto &H = c->hf;
+    if (q > H.qcap) {
+        if (H.q) cudaFree(H.q);
+        H.q = nullptr;
+        H.qcap = 0;
+        CK(cudaMalloc((void **)&H.q, q * sizeof(__half)));
+        H.qcap = q;
+    }
+    if (k > H.kcap) {
+        if (H.k) cudaFree(H.k);
+        if (H.v) cudaFree(H.v);
+        H.k = H.v = nullptr;
+        H.kcap = 0;
+        CK(cudaMalloc((void **)&H.k, k * sizeof(__half)));
+        CK(cudaMalloc((void **)&H.v, k * sizeof(__half)));
+        H.kcap = k;
+    }
+    return 0;
+}
+
+// Attention of the n rows of P.QKV over positions 0..pos0+n-1 of the cache
+// planes, its fp16 output as the O projection's operand (its low part zero).
+static int pf_attention_tc(ecu_ctx *c, int n, int pos0, int ldq, const float *kc, const float *vc)
+{
+    const EcuGeom &g = c->g;
+    const int hd = g.head_dim, qd = g.n_head * hd, kvd = g.n_head_kv * hd, np = pos0 + n;
+    if (hf_reserve(c, (size_t)n * qd, (size_t)np * kvd) != 0) return -1;
+    k_bt_half<<<4 * c->sms, 256, 0, c->stream>>>(c->pf.QKV, ldq, (size_t)n, qd, c->hf.q);
+    k_bt_plane_half<<<4 * c->sms, 256, 0, c->stream>>>(kc, g.n_ctx, g.n_head_kv, hd, np, c->hf.k);
+    k_bt_plane_half<<<4 * c->sms, 256, 0, c->stream>>>(vc, g.n_ctx, g.n_head_kv, hd, np, c->hf.v);
+    CK(cudaGetLastError());
+    g_launches += 3;
+    const int cq[2] = {0, n}, ck[2] = {0, np};
+    if (ecu_attn_prompt(ECU_F16, c->hf.q, c->hf.k, c->hf.v, c->pf.ah, g.n_head, g.n_head_kv, hd, qd, kvd, kvd, qd, cq, ck, 1,
+                        1.0f / sqrtf((float)hd), c->device, c->stream) != 0)
+        return -1;
+    CK(cudaMemsetAsync(c->pf.al, 0, (size_t)n * qd * sizeof(__half), c->stream));
     return 0;
 }
 
@@ -3237,7 +3296,10 @@ static int pf_layers(ecu_ctx *c, int n, int pos0, bool attn2)
             if (pf_gemm(c, ly.qkv[0], n, P.QKV, nullptr)) return -1;
             k_pf_rope_kv<<<n, 128, 0, c->stream>>>(P.QKV, ldq, g.n_head, g.n_head_kv, hd, pos0, c->rope_cs, ly.bq, ly.bk,
                                                    ly.bv, c->kc + li * plane, c->vc + li * plane, g.n_ctx);
-            if (attn2) {
+            if (pf_attn_tc()) {
+                if (pf_attention_tc(c, n, pos0, ldq, c->kc + li * plane, c->vc + li * plane) != 0) return -1;
+                if (pf_gemm(c, ly.o, n, P.X, P.X)) return -1;
+            } else if (attn2) {
                 // tiled over tokens: 64 query vectors a CTA
                 dim3 ag((unsigned)g.n_head_kv, (unsigned)((n + PF_QB / g.n_rep - 1) / (PF_QB / g.n_rep)));
                 if (hd == 128)
@@ -3257,8 +3319,10 @@ static int pf_layers(ecu_ctx *c, int n, int pos0, bool attn2)
                     k_pf_attn<64><<<ag, 64, 0, c->stream>>>(P.QKV, ldq, g.n_head, g.n_rep, pos0, c->kc + li * plane,
                                                             c->vc + li * plane, g.n_ctx, kscale, P.ATT);
             }
-            k_pf_split<<<4 * c->sms, 256, 0, c->stream>>>(P.ATT, (size_t)n * qd, P.ah, P.al);
-            if (pf_gemm(c, ly.o, n, P.X, P.X)) return -1;
+            if (!pf_attn_tc()) {
+                k_pf_split<<<4 * c->sms, 256, 0, c->stream>>>(P.ATT, (size_t)n * qd, P.ah, P.al);
+                if (pf_gemm(c, ly.o, n, P.X, P.X)) return -1;
+            }
         }
         if (ly.hf) {
             k_pf_norm_split<<<n, 256, 0, c->stream>>>(P.X, ly.ffn_norm, E, g.eps, P.ah, P.al);
@@ -3445,4 +3509,270 @@ int ecu_prefill(ecu_ctx *c, const int *tokens, int n, float *out)
     g_launches += 1;
     if (pf_layers(c, n, pos0, attn2) != 0) return -1;
     return pf_head(c, P.X + (size_t)(n - 1) * E, pos0 + n - 1, tokens[n - 1], out);
+}
+
+// ------------------------------------------------ many sequences at once ---
+
+struct ecu_batch {
+    ecu_ctx *c = nullptr;         // the weights, a stream, the head's buffers; no cache of its own
+    ecu_kv  *kv = nullptr;
+    int     *pos = nullptr;       // device: the position of each row
+    float   *pick = nullptr;      // device: each sequence's picked token
+    int      rows_cap = 0, seq_cap = 0;
+};
+
+extern "C" void ecu_batch_close(ecu_batch *b)
+{
+    if (!b) return;
+    if (b->c) {
+        cudaSetDevice(b->c->device);
+        if (b->c->stream) cudaStreamSynchronize(b->c->stream);
+    }
+    if (b->pos) cudaFree(b->pos);
+    if (b->pick) cudaFree(b->pick);
+    ecu_kv_close(b->kv);
+    if (b->c) ctx_free(b->c);
+    delete b;
+}
+
+extern "C" int ecu_batch_open(ecu_batch **out, ecu_ctx *base, int n_seq, int n_pages, char *err, size_t errlen)
+{
+    if (err && errlen) err[0] = '\0';
+    if (!out || !base) { ecu_set_error(err, errlen, "null argument"); return -1; }
+    *out = nullptr;
+    bool attn2 = false;
+    if (base->stage != ECU_STAGE_FULL || base->tp.world > 1) {
+        ecu_set_error(err, errlen, "a batch needs a FULL context that is not tensor-parallel");
+        return -1;
+    }
+    if (!pf_batched(base, attn2)) {
+        ecu_set_error(err, errlen, "the batched kernels do not cover this model's shapes (head_dim %d)", base->g.head_dim);
+        return -1;
+    }
+    if (cudaSetDevice(base->device) != cudaSuccess) { ecu_set_error(err, errlen, "cudaSetDevice(%d) failed", base->device); return -1; }
+    try {
+        std::unique_ptr<ecu_batch, void (*)(ecu_batch *)> b(new ecu_batch(), ecu_batch_close);
+        ecu_ctx *c = b->c = new ecu_ctx();
+        c->device = base->device;
+        c->sms = base->sms;
+        c->stage = base->stage;
+        c->first = base->first;
+        c->last = base->last;
+        c->g = base->g;
+        c->tp = base->tp;
+        c->pdl = base->pdl;
+        c->shared = base->shared;
+        c->layers = base->layers;
+        c->emb = base->emb;
+        c->out = base->out;
+        c->out_norm = base->out_norm;
+        c->rope_cs = base->rope_cs;
+        if (cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking) != cudaSuccess) {
+            cudaGetLastError();
+            ecu_set_error(err, errlen, "cudaStreamCreate failed");
+            return -1;
+        }
+        if (const char *what = alloc_buffers(c, false, true)) {
+            cudaGetLastError();
+            ecu_set_error(err, errlen, "out of device memory (%s)", what);
+            return -1;
+        }
+        if (ecu_kv_open(&b->kv, (int)c->layers.size(), c->g.n_head_kv, c->g.head_dim, n_pages, n_seq,
+                        (c->g.n_ctx + ECU_KV4_PAGE - 1) / ECU_KV4_PAGE, c->device, nullptr, err, errlen) != 0)
+            return -1;
+        if (cudaDeviceSynchronize() != cudaSuccess || cudaGetLastError() != cudaSuccess) {
+            ecu_set_error(err, errlen, "opening the batch failed: %s", cudaGetErrorString(cudaGetLastError()));
+            return -1;
+        }
+        *out = b.release();
+        return 0;
+    } catch (const std::exception &e) {
+        ecu_set_error(err, errlen, "out of memory (%s)", e.what());
+        return -1;
+    }
+}
+
+extern "C" ecu_kv *ecu_batch_kv(ecu_batch *b) { return b ? b->kv : nullptr; }
+extern "C" void   *ecu_batch_stream(ecu_batch *b) { return b ? (void *)b->c->stream : nullptr; }
+
+// One fed sequence: its place in the caller's list, its slot, its tokens, the
+// positions it held before, its first row.
+struct BatchPart { int at, seq, n, past, row; const int *tok; };
+
+// The layers over `rows` rows of P.X: the first n_step rows are single tokens
+// of sequences with a cache, the others prompt pieces.
+static int batch_layers(ecu_batch *b, const std::vector<BatchPart> &part, int n_step, int rows)
+{
+    ecu_ctx          *c = b->c;
+    ecu_ctx::Prefill &P = c->pf;
+    const EcuGeom    &g = c->g;
+    const int hd = g.head_dim, qd = g.n_head * hd, kvd = g.n_head_kv * hd, ldq = qd + 2 * kvd, E = g.n_embd;
+    const float scale = 1.0f / sqrtf((float)hd);
+    std::vector<int> seq, n_new, cq{0}, ck{0};
+    bool             fresh = true;                        // no prompt piece has a past
+    for (auto &p : part) {
+        seq.push_back(p.seq);
+        n_new.push_back(p.n);
+        if ((int)seq.size() <= n_step) continue;
+        cq.push_back(cq.back() + p.n);
+        ck.push_back(ck.back() + p.past + p.n);
+        fresh = fresh && p.past == 0;
+    }
+    const int n_prompt = (int)part.size() - n_step, prompt_rows = rows - n_step;
+    if (n_prompt && hf_reserve(c, (size_t)prompt_rows * qd, (size_t)ck.back() * kvd) != 0) return -1;
+    for (size_t li = 0; li < c->layers.size(); li++) {
+        LayerDev &ly = c->layers[li];
+        float    *k = P.QKV + qd, *v = k + kvd;
+        k_pf_norm_split<<<rows, 256, 0, c->stream>>>(P.X, ly.attn_norm, E, g.eps, P.ah, P.al);
+        if (pf_gemm(c, ly.qkv[0], rows, P.QKV, nullptr)) return -1;
+        k_bt_rope<<<rows, 128, 0, c->stream>>>(P.QKV, ldq, g.n_head, g.n_head_kv, hd, b->pos, c->rope_cs, ly.bq, ly.bk, ly.bv);
+        if (n_step) {
+            if (ecu_kv_append(b->kv, (int)li, ECU_F32, k, v, ldq, ldq, seq.data(), n_new.data(), n_step, ECU_F32, nullptr, nullptr,
+                              c->stream) != 0 ||
+                ecu_kv_attend(b->kv, (int)li, ECU_F32, P.QKV, P.ATT, g.n_head, ldq, qd, seq.data(), n_step, scale, nullptr,
+                              c->stream) != 0)
+                return -1;
+            k_pf_split<<<4 * c->sms, 256, 0, c->stream>>>(P.ATT, (size_t)n_step * qd, P.ah, P.al);
+        }
+        if (n_prompt) {
+            // the prompt attends to its keys and values as the cache holds
+            // them, like the steps that follow it; fresh ones come straight
+            // from the append, earlier ones are read back
+            const size_t r0 = (size_t)n_step * ldq;
+            if (ecu_kv_append(b->kv, (int)li, ECU_F32, k + r0, v + r0, ldq, ldq, seq.data() + n_step, n_new.data() + n_step, n_prompt,
+                              ECU_F16, fresh ? c->hf.k : nullptr, fresh ? c->hf.v : nullptr, c->stream) != 0)
+                return -1;
+            for (int i = 0; !fresh && i < n_prompt; i++)
+                if (ecu_kv_rows(b->kv, (int)li, seq[n_step + i], ck[i + 1] - ck[i], c->hf.k + (size_t)ck[i] * kvd,
+                                c->hf.v + (size_t)ck[i] * kvd, c->stream) != 0)
+                    return -1;
+            k_bt_half<<<4 * c->sms, 256, 0, c->stream>>>(P.QKV + r0, ldq, (size_t)prompt_rows, qd, c->hf.q);
+            if (ecu_attn_prompt(ECU_F16, c->hf.q, c->hf.k, c->hf.v, P.ah + (size_t)n_step * qd, g.n_head, g.n_head_kv, hd, qd, kvd, kvd,
+                                qd, cq.data(), ck.data(), n_prompt, scale, c->device, c->stream) != 0)
+                return -1;
+            CK(cudaMemsetAsync(P.al + (size_t)n_step * qd, 0, (size_t)prompt_rows * qd * sizeof(__half), c->stream));
+        }
+        if (pf_gemm(c, ly.o, rows, P.X, P.X)) return -1;
+        k_pf_norm_split<<<rows, 256, 0, c->stream>>>(P.X, ly.ffn_norm, E, g.eps, P.ah, P.al);
+        if (pf_gemm(c, ly.gu, rows, P.GU, nullptr)) return -1;
+        k_pf_swiglu<<<4 * c->sms, 256, 0, c->stream>>>(P.GU, (size_t)rows, g.n_ff, P.H);
+        k_pf_split<<<4 * c->sms, 256, 0, c->stream>>>(P.H, (size_t)rows * g.n_ff, P.ah, P.al);
+        if (pf_gemm(c, ly.d, rows, P.X, P.X)) return -1;
+        CK(cudaGetLastError());
+    }
+    g_launches += 14 * c->layers.size();
+    return 0;
+}
+
+static int batch_run(ecu_batch *b, const std::vector<BatchPart> &part, int n_step, int rows, int *picked, float *logits)
+{
+    ecu_ctx      *c = b->c;
+    const size_t  ne = (size_t)c->g.n_embd;
+    const int     n = (int)part.size();
+    std::vector<int> tok((size_t)rows), pos((size_t)rows);
+    for (auto &p : part)
+        for (int i = 0; i < p.n; i++) {
+            tok[p.row + i] = p.tok[i];
+            pos[p.row + i] = p.past + i;
+        }
+    // synchronous: the host vectors may go afterwards
+    CK(cudaMemcpyAsync(c->pf.tok, tok.data(), sizeof(int) * rows, cudaMemcpyHostToDevice, c->stream));
+    CK(cudaMemcpyAsync(b->pos, pos.data(), sizeof(int) * rows, cudaMemcpyHostToDevice, c->stream));
+    k_pf_embed<<<4 * c->sms, 256, 0, c->stream>>>(c->emb, c->pf.tok, rows, c->pf.X, c->g.n_embd);
+    g_launches += 1;
+    if (batch_layers(b, part, n_step, rows) != 0) return -1;
+    // each sequence's last row through the decode step's head
+    c->h_st[0].pos = c->h_st[0].token = 0;
+    CK(cudaMemcpyAsync(c->st, c->h_st, 2 * sizeof(int), cudaMemcpyHostToDevice, c->stream));
+    for (auto &p : part) {
+        CK(cudaMemcpyAsync(c->state, c->pf.X + (size_t)(p.row + p.n - 1) * ne, sizeof(float) * ne, cudaMemcpyDeviceToDevice, c->stream));
+        Launcher L{c->stream, false};
+        enqueue_head(c, L, false);
+        g_launches += (uint64_t)L.count;
+        CK(L.err);
+        CK(cudaMemcpyAsync(b->pick + p.at, c->state + ne, sizeof(float), cudaMemcpyDeviceToDevice, c->stream));
+        if (logits)
+            CK(cudaMemcpyAsync(logits + (size_t)p.at * c->g.n_vocab, c->logits, sizeof(float) * (size_t)c->g.n_vocab,
+                               cudaMemcpyDeviceToHost, c->stream));
+    }
+    std::vector<float> got((size_t)n);
+    CK(cudaMemcpyAsync(got.data(), b->pick, sizeof(float) * n, cudaMemcpyDeviceToHost, c->stream));
+    if (check_status(c) != 0) return -1;
+    for (int i = 0; i < n; i++) picked[i] = (int)got[i];
+    return 0;
+}
+
+extern "C" int ecu_batch_feed(ecu_batch *b, const int *seq, const int *n_tok, int n, const int *tokens, int *picked, float *logits)
+{
+    auto bad = [](const char *why) {
+        ecu_set_error(nullptr, 0, "ecu_batch_feed: %s", why);
+        return -1;
+    };
+    if (!b || n < 0 || (n > 0 && (!seq || !n_tok || !tokens || !picked))) return bad("null argument or negative count");
+    if (n == 0) return 0;
+    ecu_ctx *c = b->c;
+    cudaSetDevice(c->device);
+    try {
+        ecu_kv_info info;
+        ecu_kv_get_info(b->kv, &info);
+        std::vector<bool>      seen((size_t)info.n_seq, false);
+        std::vector<BatchPart> part;
+        std::vector<int>       slots, counts, before;
+        long long              rows = 0;
+        for (int i = 0; i < n; i++) {
+            const int past = ecu_kv_len(b->kv, seq[i], nullptr, 0);
+            if (past < 0) return -1;
+            if (seen[seq[i]] || n_tok[i] < 1) return bad("a sequence comes twice, or without tokens");
+            seen[seq[i]] = true;
+            if ((long long)past + n_tok[i] > c->g.n_ctx) {
+                ecu_set_error(nullptr, 0, "ecu_batch_feed: %d tokens at position %d exceed the context (%d)", n_tok[i], past, c->g.n_ctx);
+                return -1;
+            }
+            for (int j = 0; j < n_tok[i]; j++)
+                if (tokens[rows + j] < 0 || tokens[rows + j] >= c->g.n_vocab) {
+                    ecu_set_error(nullptr, 0, "token %d outside the vocabulary (%d)", tokens[rows + j], c->g.n_vocab);
+                    return -1;
+                }
+            part.push_back({i, seq[i], n_tok[i], past, 0, tokens + rows});
+            slots.push_back(seq[i]);
+            counts.push_back(n_tok[i]);
+            before.push_back(past);
+            rows += n_tok[i];
+        }
+        if (rows > INT_MAX / 4) return bad("too many tokens");
+        // single tokens first: their rows go to the cache's attention, the others to the prompt's
+        std::stable_partition(part.begin(), part.end(), [](const BatchPart &p) { return p.n == 1; });
+        int n_step = 0, row = 0;
+        for (auto &p : part) {
+            n_step += p.n == 1;
+            p.row = row;
+            row += p.n;
+        }
+        if (pf_attrs(c) != 0 || pf_reserve(c, (int)rows) != 0) return -1;
+        if ((int)rows > b->rows_cap) {
+            if (b->pos) cudaFree(b->pos);
+            b->pos = nullptr;
+            b->rows_cap = 0;
+            CK(cudaMalloc((void **)&b->pos, sizeof(int) * rows));
+            b->rows_cap = (int)rows;
+        }
+        if (n > b->seq_cap) {
+            if (b->pick) cudaFree(b->pick);
+            b->pick = nullptr;
+            b->seq_cap = 0;
+            CK(cudaMalloc((void **)&b->pick, sizeof(float) * n));
+            b->seq_cap = n;
+        }
+        if (ecu_kv_extend(b->kv, slots.data(), counts.data(), n, c->stream) != 0) return -1;
+        if (batch_run(b, part, n_step, (int)rows, picked, logits) != 0) {
+            // the sequences keep what they held before
+            const std::string why = ecu_get_error();
+            ecu_kv_truncate(b->kv, slots.data(), before.data(), n, c->stream);
+            ecu_set_error(nullptr, 0, "%s", why.c_str());
+            return -1;
+        }
+        return 0;
+    } catch (const std::exception &e) {
+        return bad(e.what());
+    }
 }

@@ -423,6 +423,19 @@ extern "C" int ecu_kv_read(ecu_kv *kv, int layer, int seq, int pos, int n, float
     return rc;
 }
 
+int ecu_kv_rows(ecu_kv *kv, int layer, int seq, int n, void *k, void *v, cudaStream_t s)
+{
+    const size_t   vecs = (size_t)n * kv->n_head_kv * kv->head_dim / 8;
+    const uint8_t *lay = kv->data + (size_t)layer * kv->book.n_pages * kv->page_bytes;
+    for (int side = 0; side < 2; side++) {
+        k_kv4_read<__half><<<(unsigned)((vecs + 255) / 256), 256, 0, s>>>(
+            lay, kv->page_bytes, kv->table() + (size_t)seq * kv->book.max_pages, 0, n, kv->n_head_kv, kv->head_dim / 32,
+            kv->book.n_pages, side, (__half *)(side ? v : k));
+        if (launched("ecu_kv_rows") != 0) return -1;
+    }
+    return 0;
+}
+
 // ---------------------------------------------------------------- attend ---
 
 // Heads of a group: one 8-column tile, two where an fp32 query has more than

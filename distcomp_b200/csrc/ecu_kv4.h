@@ -74,3 +74,7 @@ struct DeviceScope {
 };
 
 void ecu_count_launches(int n);       // ecu_kernel_launches()
+
+// Positions 0..n-1 of a sequence as fp16 rows [n][n_head_kv * head_dim] in
+// device memory, as the cache holds them.
+int ecu_kv_rows(ecu_kv *kv, int layer, int seq, int n, void *k, void *v, cudaStream_t s);

@@ -140,6 +140,11 @@ SIGNATURES = [
     ("ecu_attn_prompt", C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
                                   C.c_long, C.c_long, C.c_long, C.c_long, C.c_void_p, C.c_void_p, C.c_int, C.c_float,
                                   C.c_int, C.c_void_p]),
+    ("ecu_batch_open", C.c_int, [C.POINTER(C.c_void_p), C.c_void_p, C.c_int, C.c_int, C.c_char_p, C.c_size_t]),
+    ("ecu_batch_close", None, [C.c_void_p]),
+    ("ecu_batch_kv", C.c_void_p, [C.c_void_p]),
+    ("ecu_batch_stream", C.c_void_p, [C.c_void_p]),
+    ("ecu_batch_feed", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
     ("ecu_last_error", C.c_char_p, []),
     ("ecu_kernel_launches", C.c_uint64, []),
     ("ecu_version", C.c_char_p, []),
@@ -431,6 +436,83 @@ class LlmCtx:
     def close(self) -> None:
         if self.h:
             lib().ecu_ctx_close(self.h)
+            self.h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class LlmBatch:
+    """Many sequences over a FULL context's weights, their K/V in a pool of
+    4-bit pages (ecu_batch)."""
+
+    def __init__(self, base: LlmCtx, n_seq: int, n_pages: int):
+        self.h = C.c_void_p()
+        err = C.create_string_buffer(512)
+        if lib().ecu_batch_open(C.byref(self.h), base.h, int(n_seq), int(n_pages), err, 512) != 0:
+            raise EngineError(err.value.decode(errors="replace") or last_error())
+        self.n_vocab = base.n_vocab
+        self.kv = C.c_void_p(lib().ecu_batch_kv(self.h))
+        self.stream = C.c_void_p(lib().ecu_batch_stream(self.h))
+
+    def feed(self, seq, tokens, logits: bool = False):
+        """Each sequence's next tokens (a list of them per sequence); the picked token of each, and with
+        logits=True its head's output [n, n_vocab]."""
+        s = np.ascontiguousarray(seq, dtype=np.int32)
+        if len(s) != len(tokens):
+            raise EngineError(f"{len(s)} sequences and {len(tokens)} lists of tokens")
+        cnt = np.array([len(t) for t in tokens], dtype=np.int32)
+        tok = np.concatenate([np.asarray(t, dtype=np.int32) for t in tokens]) if len(s) else np.zeros(0, np.int32)
+        out = np.zeros(len(s), dtype=np.int32)
+        lg = np.empty((len(s), self.n_vocab), dtype=np.float32) if logits else None
+        if lib().ecu_batch_feed(self.h, _ptr(s), _ptr(cnt), len(s), _ptr(tok), _ptr(out), None if lg is None else _ptr(lg)) != 0:
+            raise EngineError(last_error())
+        picked = [int(t) for t in out]
+        return (picked, lg) if logits else picked
+
+    def _list(self, f, a, b) -> None:
+        a, b = np.ascontiguousarray(a, dtype=np.int32), np.ascontiguousarray(b, dtype=np.int32)
+        if a.shape != b.shape:
+            raise EngineError(f"lists of {a.size} and {b.size}")
+        if f(self.kv, _ptr(a), _ptr(b), a.size, self.stream) != 0:
+            raise EngineError(last_error())
+
+    def fork(self, src, dst) -> None:
+        """Empty slots dst become copies of src, sharing its pages."""
+        self._list(lib().ecu_kv_fork, src, dst)
+
+    def truncate(self, seq, length) -> None:
+        self._list(lib().ecu_kv_truncate, seq, length)
+
+    def free(self, seq) -> None:
+        a = np.ascontiguousarray(seq, dtype=np.int32)
+        if lib().ecu_kv_free(self.kv, _ptr(a), a.size, self.stream) != 0:
+            raise EngineError(last_error())
+
+    def compact(self) -> int:
+        n = int(lib().ecu_kv_compact(self.kv, self.stream))
+        if n < 0:
+            raise EngineError(last_error())
+        return n
+
+    def length(self, seq: int) -> int:
+        n = int(lib().ecu_kv_len(self.kv, int(seq), None, 0))
+        if n < 0:
+            raise EngineError(last_error())
+        return n
+
+    def used(self) -> int:
+        """Pages that some sequence holds."""
+        i = EcuKvInfo()
+        lib().ecu_kv_get_info(self.kv, C.byref(i))
+        return int(i.used)
+
+    def close(self) -> None:
+        if self.h:
+            lib().ecu_batch_close(self.h)
             self.h = C.c_void_p()
 
     def __del__(self):

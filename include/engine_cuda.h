@@ -423,6 +423,34 @@ int  ecu_attn_prompt(int dtype, const void *q, const void *k, const void *v, voi
                      int head_dim, long q_stride, long k_stride, long v_stride, long out_stride, const int *cu_q,
                      const int *cu_k, int n_seq, float scale, int device, void *stream);
 
+/* ---- many sequences over one model (serving) ---- */
+
+/* Sequences with the weights of a FULL context and their K/V in a pool of
+ * 4-bit pages: prompts and single tokens of any of them in one call.  No
+ * counterpart in the reference, which serves one sequence a process
+ * (src/daemon.c:757).  For the shapes that ecu_prefill runs as a batch (and
+ * head_dim 64 or 128); others are refused, and so are tensor-parallel and
+ * staged contexts.  n_seq slots of the base's n_ctx positions, n_pages pages
+ * of ECU_KV4_PAGE positions between them.  The base may be closed first. */
+typedef struct ecu_batch ecu_batch;
+int  ecu_batch_open(ecu_batch **out, ecu_ctx *base, int n_seq, int n_pages, char *err, size_t errlen);
+void ecu_batch_close(ecu_batch *b);
+/* The batch's pool, to fork, truncate and free its sequences and to compact
+ * it (ecu_kv_*), on the batch's stream. */
+ecu_kv *ecu_batch_kv(ecu_batch *b);
+void   *ecu_batch_stream(ecu_batch *b);
+/* Sequence seq[i] (no slot twice) takes the next n_tok[i] >= 1 of `tokens`
+ * at its end; picked[i] is the token that its last position's head picks
+ * (llm_pick's rule), logits (NULL: none wanted; host, n rows of n_vocab) that
+ * head's output.  The rows of all sequences go through the layers together
+ * (ecu_prefill's GEMMs); a sequence with one token attends through
+ * ecu_kv_attend, the others through ecu_attn_prompt, all to keys and values
+ * as the cache holds them, so a prompt leaves the same state however it is
+ * cut.  Against the fp32 cache of ecu_forward the states differ by the
+ * cache's 4-bit rounding.  On an error the sequences keep what they held.
+ * Synchronises the batch's stream. */
+int  ecu_batch_feed(ecu_batch *b, const int *seq, const int *n_tok, int n, const int *tokens, int *picked, float *logits);
+
 /* ---- failure-path testing ------------------------------------------------ */
 
 /* No counterpart in the reference, whose failure paths are host retries and

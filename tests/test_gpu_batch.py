@@ -1,0 +1,204 @@
+"""Many sequences over one model (ecu_batch): prompts, single tokens, forks and
+the pool's upkeep against a plain 64-bit forward of the same model whose keys
+and values go through the cache's 4-bit definition.
+
+The bar: the GEMMs keep about 22 bits, the prompt attention's operands 11
+(2^-12 of each element, averaged over keys and dimensions), so states agree to
+a few 1e-4 of the vector's scale; where a key or value lies that near to the
+border of two codes it may take the other one, a step of 1/8 of its block's
+largest value in one of thousands of products.  1e-2 of the scale covers both;
+the 4-bit cache itself moves these logits by more, which the test checks too.
+"""
+import numpy as np
+import pytest
+
+from distcomp_b200 import gguf as G
+from distcomp_b200 import synth
+from test_gpu_kv4 import stored
+
+pytestmark = pytest.mark.gpu
+REL = 1e-2
+
+
+class Plain:
+    """A llama forward in 64 bits; 4-bit keys and values unless told otherwise."""
+
+    def __init__(self, key, buf, port, four_bits=True):
+        self.s, self.port, self.four = synth.spec(key), port, four_bits
+        self.tab = G.read_tensor_table(buf)
+        self.dims = {name: (dims, t) for name, dims, t in synth.tensor_list(self.s)}
+        self.w = {}
+
+    def weight(self, name):
+        if name not in self.w:
+            dims, t = self.dims[name]
+            n = int(np.prod(dims))
+            rc, v = self.port.dequant(t, np.frombuffer(self.tab[name][2], np.uint8), n, 0, n)
+            assert rc == 0
+            self.w[name] = np.asarray(v, dtype=np.float64).reshape(dims[::-1])
+        return self.w[name]
+
+    def keep(self, x):
+        import torch
+        return stored(torch.from_numpy(x.astype(np.float32))) if self.four else x
+
+    def forward(self, tokens, cache=None):
+        """Logits of every position of `tokens` after those in `cache` (grown in place)."""
+        s = self.s
+        hd, H, KV = s.head_dim or s.n_embd // s.n_head, s.n_head, s.n_head_kv
+        cache = {} if cache is None else cache
+        x = self.weight("token_embd.weight")[list(tokens)]
+        pos0 = len(cache.get((0, "k"), ()))
+        pos = pos0 + np.arange(len(tokens))
+        ang = pos[:, None] * s.rope_base ** (-2.0 * np.arange(hd // 2) / hd)[None]
+        c, sn = np.cos(ang)[:, None], np.sin(ang)[:, None]
+
+        def norm(x):
+            return x / np.sqrt((x * x).mean(-1, keepdims=True) + s.eps)
+
+        def turn(x):
+            a, b = x[..., :hd // 2], x[..., hd // 2:]
+            return np.concatenate([a * c - b * sn, b * c + a * sn], -1)
+
+        for l in range(s.n_layer):
+            y = norm(x) * self.weight(f"blk.{l}.attn_norm.weight")
+            q, k, v = (y @ self.weight(f"blk.{l}.attn_{n}.weight").T for n in "qkv")
+            q, k, v = turn(q.reshape(-1, H, hd)), turn(k.reshape(-1, KV, hd)), v.reshape(-1, KV, hd)
+            for n, r in (("k", k), ("v", v)):
+                old = cache.get((l, n))
+                cache[(l, n)] = self.keep(r) if old is None else np.concatenate([old, self.keep(r)])
+            K, V = cache[(l, "k")], cache[(l, "v")]
+            o = np.empty_like(q)
+            seen = np.arange(len(K))[None] <= pos[:, None]
+            for h in range(H):
+                w = np.where(seen, q[:, h] @ K[:, h // (H // KV)].T / np.sqrt(hd), -np.inf)
+                w = np.exp(w - w.max(1, keepdims=True))
+                o[:, h] = w @ V[:, h // (H // KV)] / w.sum(1, keepdims=True)
+            x = x + o.reshape(len(tokens), -1) @ self.weight(f"blk.{l}.attn_output.weight").T
+            y = norm(x) * self.weight(f"blk.{l}.ffn_norm.weight")
+            g, u = y @ self.weight(f"blk.{l}.ffn_gate.weight").T, y @ self.weight(f"blk.{l}.ffn_up.weight").T
+            x = x + (g / (1 + np.exp(-g)) * u) @ self.weight(f"blk.{l}.ffn_down.weight").T
+        return (norm(x) * self.weight("output_norm.weight")) @ self.weight("output.weight").T
+
+
+def close(got, want, rel=REL):
+    err = float(np.max(np.abs(got.astype(np.float64) - want)) / np.max(np.abs(want)))
+    assert err <= rel, f"off by {err:.2e} of the scale"
+    return err
+
+
+@pytest.fixture(scope="module")
+def setup(eng, oracle_port, model_buf):
+    def get(key):
+        buf = model_buf(key)
+        base = eng.LlmCtx(eng.GgufModel(buf), eng.STAGE_FULL)
+        return base, Plain(key, buf, oracle_port), Plain(key, buf, oracle_port, four_bits=False)
+    return get
+
+
+@pytest.mark.parametrize("key", ["mini-q4", "mini-q8", "mini-q4k"])
+def test_feed_matches_the_plain_forward(eng, setup, key):
+    """Prompts of different lengths in one call, then single tokens and prompt pieces mixed, 20 steps of them."""
+    base, plain, dense = setup(key)
+    b = eng.LlmBatch(base, 4, 12)
+    r = np.random.default_rng(1)
+    V = base.n_vocab
+    text = [list(map(int, r.integers(3, V, n))) for n in (40, 1, 17)]
+    caches = [{} for _ in text]
+    picked, lg = b.feed([2, 0, 1], text, logits=True)
+    for i in range(3):
+        want = plain.forward(text[i], caches[i])[-1]
+        close(lg[i], want)
+        assert picked[i] == int(np.argmax(lg[i]))
+        far = dense.forward(text[i])[-1]
+        if len(text[i]) > 1:
+            assert np.max(np.abs(far - want)) / np.max(np.abs(want)) > 1e-3     # the 4-bit cache is in the values
+    for step in range(20):
+        nxt = [[picked[0]], [int(v) for v in r.integers(3, V, 3)] if step % 5 == 2 else [picked[1]], [picked[2]]]
+        picked, lg = b.feed([2, 0, 1], nxt, logits=True)
+        for i in range(3):
+            close(lg[i], plain.forward(nxt[i], caches[i])[-1])
+    assert [b.length(s) for s in (2, 0, 1, 3)] == [60, 29, 37, 0]
+
+
+def test_prompt_pieces_forks_and_upkeep(eng, setup):
+    """A prompt in pieces (a later one over a page's border), forks that go different ways, a freed slot fed anew, the
+    pool closed up between the steps."""
+    base, plain, _ = setup("mini-q4")
+    b = eng.LlmBatch(base, 5, 10)
+    r = np.random.default_rng(2)
+    p = [int(v) for v in r.integers(3, base.n_vocab, 75)]
+    b.feed([0], [p[:30]])
+    b.feed([0], [p[30:31]])
+    picked, lg = b.feed([0], [p[31:]], logits=True)
+    cache = {}
+    close(lg[0], plain.forward(p, cache)[-1])
+    b.fork([0, 0], [3, 1])
+    assert b.used() == 2
+    tails = {s: [int(v) for v in r.integers(3, base.n_vocab, 6)] for s in (0, 3, 1)}
+    caches = {s: dict(cache) for s in tails}
+    for j in range(6):
+        if j == 3:
+            b.truncate([1], [70])
+            caches[1] = {k: v[:70] for k, v in caches[1].items()}
+        if j == 4:
+            b.free([0])
+            tails.pop(0)
+            assert b.compact() >= 0 and b.used() == 3
+            picked, lg = b.feed([0], [p[:5]], logits=True)
+            close(lg[0], plain.forward(p[:5])[-1])
+        _, lg = b.feed(list(tails), [[t[j]] for t in tails.values()], logits=True)
+        for i, s in enumerate(tails):
+            close(lg[i], plain.forward([tails[s][j]], caches[s])[-1])
+
+
+def test_feed_refuses_and_keeps_what_it_held(eng, setup):
+    base, plain, _ = setup("mini-q4")
+    b = eng.LlmBatch(base, 3, 3)
+    b.feed([0], [[5] * 60])
+    for seq, tok, why in (([0, 0], [[1], [2]], "comes twice"), ([1], [[]], "without tokens"), ([3], [[1]], "no sequence 3"),
+                          ([1], [[base.n_vocab]], "outside the vocabulary"), ([0], [[1] * 69], "exceed the context"),
+                          ([1, 2], [[1] * 70, [2] * 70], "no free page")):
+        with pytest.raises(eng.EngineError, match=why):
+            b.feed(seq, tok)
+        assert [b.length(s) for s in range(3)] == [60, 0, 0] and b.used() == 1
+    assert b.feed([], []) == []
+    _, lg = b.feed([0], [[7]], logits=True)
+    close(lg[0], plain.forward([5] * 60 + [7])[-1])
+
+
+def test_batch_refuses_bases(eng, model_buf):
+    m = eng.GgufModel(model_buf("tiny"))
+    with pytest.raises(eng.EngineError, match="do not cover"):
+        eng.LlmBatch(eng.LlmCtx(m, eng.STAGE_FULL), 2, 4)          # head_dim 32
+    m4 = eng.GgufModel(model_buf("mini-q4"))
+    with pytest.raises(eng.EngineError, match="FULL context"):
+        eng.LlmBatch(eng.LlmCtx(m4, eng.STAGE_LAYERS, 0, 1), 2, 4)
+    base = eng.LlmCtx(m4, eng.STAGE_FULL)
+    for n_seq, n_pages in ((0, 4), (2, 0), (70000, 4)):
+        with pytest.raises(eng.EngineError):
+            eng.LlmBatch(base, n_seq, n_pages)
+
+
+def test_batch_outlives_its_base(eng, setup, model_buf):
+    base = eng.LlmCtx(eng.GgufModel(model_buf("mini-q4")), eng.STAGE_FULL)
+    b = eng.LlmBatch(base, 1, 2)
+    first = b.feed([0], [[9, 8, 7]])
+    base.close()
+    b.free([0])
+    assert b.feed([0], [[9, 8, 7]]) == first
+
+
+@pytest.mark.parametrize("key,n_prompt", [("mini-q4", 100), ("mini-q8", 33), ("mini-q4k", 90)])
+def test_prefill_with_tensor_core_attention(eng, model_buf, monkeypatch, key, n_prompt):
+    """ECU_PF_ATTN=2 keeps ecu_prefill within its 1e-3 bar of the default, also for a second piece."""
+    s = synth.spec(key)
+    m = eng.GgufModel(model_buf(key))
+    prompt = synth.prompt_tokens(n_prompt, s.n_vocab, seed=4)
+    a, b = eng.LlmCtx(m, eng.STAGE_FULL), eng.LlmCtx(m, eng.STAGE_FULL)
+    first = a.prefill(prompt)
+    want = a.logits().astype(np.float64)
+    monkeypatch.setenv("ECU_PF_ATTN", "2")
+    b.prefill(prompt[: n_prompt // 3])
+    assert b.prefill(prompt[n_prompt // 3:]) == first
+    close(b.logits(), want, 1e-3)
