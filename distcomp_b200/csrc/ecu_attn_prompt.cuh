@@ -6,17 +6,23 @@
 // rounded to 16 bits over S's place, O += P V (fp32, tensor memory).  The two
 // tiles take turns: while one's softmax runs, the tensor core computes the
 // other's products.  Roles by warp:
-//   0-3, 4-7  softmax of tile 0 and 1, a thread per row; O's rescaling and
-//             the output at the end
-//   8         copies: Q once, K and V tiles through a ring (TMA)
-//   9         issues the products (one thread)
-//   10, 11    clean V tiles that some row sees only in part: an element that
+//   0-7, 8-15 softmax of tile 0 and 1, two threads per row (64 keys each, so
+//             that a tile's softmax is short beside the other tile's
+//             products); O's rescaling and the output at the end
+//   16        copies: Q once, K and V tiles through a ring (TMA)
+//   17        issues the products (one thread)
+//   18, 19    clean V tiles that some row sees only in part: an element that
 //             is not finite would turn 0 * element into NaN for rows that do
 //             not see it.  Such elements are zeroed in shared memory, their
 //             keys noted, and added to the rows that do see them at the end.
 // The maximum that P is taken relative to follows the running one only when
 // that has grown by more than 2^8 (P stays far inside fp16's range, and the
-// sums are fp32), so O is rescaled a few times per row at most.
+// sums are fp32), so O is rescaled a few times per row at most, and a row's
+// two threads exchange maxima only then: one barrier with a vote a tile.
+// The exponentials of a pair of tiles, 32768 at 16 a clock, take as long as
+// its products at full rate; a quarter of them is computed on the FMA units
+// instead (2^x = 2^n p(f), p a polynomial fitted to the relative error: 7.5e-5
+// for bf16, whose own step is 2^-8, 2.7e-6 for fp16).
 //
 // Tensor memory: S of tile t at column 128 t (P in its first 64), O at
 // 256 + HD t.  Shared memory: tiles of 128 rows of 64 elements (128 bytes,
@@ -28,7 +34,7 @@
 
 #include <cuda.h>
 
-#define PA_THREADS 384
+#define PA_THREADS 640
 #define PA_BOX 16384                       // 128 rows x 128 bytes
 
 template <int HD> struct PaShape {
@@ -113,12 +119,28 @@ __device__ __forceinline__ void pa_st32(uint32_t addr, const uint32_t (&v)[32])
                  : "memory");
 }
 
+// the same of 16 columns: where 32 more values would not fit the registers
+__device__ __forceinline__ void pa_ld16(uint32_t (&v)[16], uint32_t addr)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : PA_R8(v, 0), PA_R8(v, 8)
+                 : "r"(addr)
+                 : "memory");
+}
+
+__device__ __forceinline__ void pa_st16(uint32_t addr, const uint32_t (&v)[16])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+                 PA_W8(v, 0), PA_W8(v, 8)
+                 : "memory");
+}
+
 __device__ __forceinline__ void pa_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 // the loaded values are used after the wait only
-__device__ __forceinline__ void pa_pin(uint32_t (&v)[32])
+template <int N> __device__ __forceinline__ void pa_pin(uint32_t (&v)[N])
 {
 #pragma unroll
-    for (int x = 0; x < 32; x++) asm volatile("" : "+r"(v[x]));
+    for (int x = 0; x < N; x++) asm volatile("" : "+r"(v[x]));
 }
 __device__ __forceinline__ void pa_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -131,6 +153,77 @@ __device__ __forceinline__ uint32_t pa_pair(__nv_bfloat16, float lo, float hi)
 {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Two fp32 values in one register pair, for the packed fp32 units.
+__device__ __forceinline__ uint64_t pa_two(float a, float b)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void pa_untwo(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t pa_fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t pa_add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// max that a NaN survives
+__device__ __forceinline__ float pa_max(float a, float b)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float pa_max3(float a, float b, float c)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// 2^t of two values on the FMA units: t = n + f with |f| <= 1/2, n added to the
+// polynomial's exponent.  t is held at -126, where P rounds to nothing.
+template <int DEG> __device__ __forceinline__ void pa_ex2_fma(uint64_t t2, float &e0, float &e1)
+{
+    float t0, t1, r0, r1, p0, p1;
+    pa_untwo(t2, t0, t1);
+    const uint64_t t = pa_two(fmaxf(t0, -126.0f), fmaxf(t1, -126.0f));
+    const uint64_t r = pa_add2(t, pa_two(12582912.0f, 12582912.0f));                   // 1.5 * 2^23: n in the low bits
+    const uint64_t f = pa_fma2(pa_add2(r, pa_two(-12582912.0f, -12582912.0f)), pa_two(-1.0f, -1.0f), t);
+    uint64_t       p;
+    if (DEG == 3) {
+        p = pa_fma2(f, pa_two(0.055171668529510498f, 0.055171668529510498f), pa_two(0.24261112511157990f, 0.24261112511157990f));
+        p = pa_fma2(f, p, pa_two(0.69326096773147583f, 0.69326096773147583f));
+        p = pa_fma2(f, p, pa_two(0.99992805719375610f, 0.99992805719375610f));
+    } else {
+        p = pa_fma2(f, pa_two(0.0095701021f, 0.0095701021f), pa_two(0.0559178628f, 0.0559178628f));
+        p = pa_fma2(f, p, pa_two(0.2402474433f, 0.2402474433f));
+        p = pa_fma2(f, p, pa_two(0.6931217909f, 0.6931217909f));
+        p = pa_fma2(f, p, pa_two(0.9999992847f, 0.9999992847f));
+    }
+    pa_untwo(r, r0, r1);
+    pa_untwo(p, p0, p1);
+    e0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(r0) << 23));
+    e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(r1) << 23));
+}
+
+// Does any of the 256 threads at barrier `id` say so?
+__device__ __forceinline__ bool pa_any(int id, bool mine)
+{
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+                 "barrier.cta.red.or.pred q, %2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(any) : "r"((uint32_t)mine), "r"(id) : "memory");
+    return any != 0;
 }
 
 template <typename T> struct PaBits;     // exponent mask of two elements, and what carries it into the sign when it is full
@@ -150,6 +243,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     __shared__ __align__(8) uint64_t q_full, full[ST], empty[ST], s_full[2], p_full[2], due[4], clean[4], drain;
     __shared__ uint32_t              tmem_s, bad[4][4];       // keys of the partly seen tiles with cleaned elements
     __shared__ int                   any_bad, dead;
+    __shared__ float                 half_s[2][2][128];       // what a row's two threads tell each other
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     // this CTA's pair: the sequence, the KV head, the two items (tile, head); the
@@ -172,7 +266,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     const int n = (seen(min(tile_of(n_tile - 1) * 128 + 128, nq) - 1) + 127) / 128;
     const int n_plain = seen(tile_of(0) * 128) / 128;
 
-    if (warp == 9) {
+    if (warp == 17) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_s)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -184,7 +278,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         }
         for (int t = 0; t < 2; t++) {
             mbar_init(s_full + t, 1);
-            mbar_init(p_full + t, 4);
+            mbar_init(p_full + t, 8);
         }
         for (int j = 0; j < 4; j++) {
             mbar_init(due + j, 1);
@@ -206,7 +300,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     };
     auto gone = [&] { return *reinterpret_cast<volatile int *>(&dead) != 0; };
 
-    if (warp == 8) {
+    if (warp == 16) {
         if (lane == 0 && n > 0) {
             mbar_expect_tx(&q_full, (uint32_t)n_tile * S::TILE);
             for (int t = 0; t < n_tile; t++)
@@ -230,7 +324,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
             }
         }
         __syncwarp();
-    } else if (warp == 9) {
+    } else if (warp == 17) {
         if (lane == 0 && n > 0) {
             // fp32 sums, M = 128; S: N = 128 keys; O: N = HD dimensions, V MN-major
             const uint32_t ids = (1u << 4) | (PaBits<T>::fmt << 7) | (PaBits<T>::fmt << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
@@ -279,8 +373,8 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
             mbar_drain(&drain, 0, wait_limit_ns());       // no product in flight when tensor memory is given back
         }
         __syncwarp();
-    } else if (warp >= 10) {
-        const int me = tid - 320;
+    } else if (warp >= 18) {
+        const int me = tid - 576;
         for (int j = n_plain; j < n; j++) {
             const int iv = 2 * j + 1;
             wait(due + (j - n_plain), 0);
@@ -310,115 +404,132 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
             if (lane == 0) mbar_arrive(clean + (j - n_plain));
         }
     } else {
-        const int      t = warp >> 2, r = (warp & 3) * 32 + lane;
+        // Nothing here leaves the loop early, whatever gave up: the tile's 256
+        // threads meet at its barrier in every turn.
+        const int      t = warp >> 3, hf = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lanes + 128 * t, to = tmem + lanes + 256 + HD * t;
         if (t < n_tile) {
             const int   row = tile_of(t) * 128 + r, vis = seen(row);
             const float sl = a.scale * 1.4426950408889634f;
-            float       m = -INFINITY, l = 0.0f;          // the maximum that P is relative to; the weights' sum
+            float       m = -INFINITY, l = 0.0f;          // the maximum that P is relative to; this half's weights' sum
             for (int j = 0; j < n; j++) {
                 wait(s_full + t, (uint32_t)j & 1u);
-                if (__any_sync(0xffffffffu, gone())) break;
                 pa_fence_after();
-                uint32_t s[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; c++) pa_ld32(s[c], ts + 32 * c);
+                uint32_t s[2][32];
+                pa_ld32(s[0], ts + 64 * hf);
+                pa_ld32(s[1], ts + 64 * hf + 32);
                 pa_ld_wait();
-#pragma unroll
-                for (int c = 0; c < 4; c++) pa_pin(s[c]);
+                pa_pin(s[0]);
+                pa_pin(s[1]);
                 if (j >= n_plain) {
-                    const int left = vis - j * 128;
+                    const int left = vis - j * 128 - 64 * hf;
 #pragma unroll
-                    for (int c = 0; c < 4; c++)
+                    for (int c = 0; c < 2; c++)
 #pragma unroll
                         for (int x = 0; x < 32; x++)
                             if (32 * c + x >= left) s[c][x] = 0xFF800000u;
                 }
                 float top[4];
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    top[c] = __uint_as_float(s[c][0]);
+                for (int q = 0; q < 4; q++) {
+                    auto v = [&](int x) { return __uint_as_float(s[q >> 1][(q & 1) * 16 + x]); };
+                    top[q] = pa_max3(v(0), v(1), v(2));
 #pragma unroll
-                    for (int x = 1; x < 32; x++) top[c] = fmaxf(top[c], __uint_as_float(s[c][x]));
+                    for (int x = 3; x < 15; x += 2) top[q] = pa_max3(top[q], v(x), v(x + 1));
+                    top[q] = pa_max(top[q], v(15));
                 }
-                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                if (j == 0) m = mx;
-                else {
-                    const bool grow = mx > m && !((mx - m) * sl <= 8.0f);
-                    if (__any_sync(0xffffffffu, grow)) {
-                        const float f = grow ? kv4_ex2((m - mx) * sl) : 1.0f;
-                        if (grow) m = mx;
-                        l *= f;
-#pragma unroll
-                        for (int c = 0; c < HD / 32; c++) {
-                            uint32_t o[32];
-                            pa_ld32(o, to + 32 * c);
+                float mx = pa_max(pa_max3(top[0], top[1], top[2]), top[3]);
+                // not (mx within 2^8 of m): a NaN grows, and turns its whole row into NaN
+                auto grows = [&] { return !(mx <= m) && !((mx - m) * sl <= 8.0f); };
+                // (the barrier also lets P take the place of scores that all have read)
+                if (pa_any(1 + t, grows())) {
+                    half_s[t][hf][r] = mx;
+                    named_bar(1 + t, 256);
+                    mx = pa_max(mx, half_s[t][hf ^ 1][r]);
+                    const bool  grow = grows();
+                    const float f = grow && j > 0 ? kv4_ex2((m - mx) * sl) : 1.0f;
+                    if (grow) m = mx;
+                    l *= f;
+                    if (j > 0)
+#pragma unroll 1
+                        for (int c = 0; c < HD / 2; c += 16) {
+                            uint32_t o[16];
+                            pa_ld16(o, to + HD / 2 * hf + c);
                             pa_ld_wait();
                             pa_pin(o);
 #pragma unroll
-                            for (int x = 0; x < 32; x++) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-                            pa_st32(to + 32 * c, o);
+                            for (int x = 0; x < 16; x++) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                            pa_st16(to + HD / 2 * hf + c, o);
                         }
-                    }
                 }
-                const float mb = m == -INFINITY ? 0.0f : m * sl;
-                float       sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const float    mb = m == -INFINITY ? 0.0f : m * sl;
+                const uint64_t sl2 = pa_two(sl, sl), mb2 = pa_two(-mb, -mb);
+                uint64_t       sum[2] = {pa_two(0.0f, 0.0f), pa_two(0.0f, 0.0f)};
+                uint32_t       p[32];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    uint32_t p[32];
-#pragma unroll
-                    for (int x = 0; x < 32; x++) {
-                        const float e0 = kv4_ex2(fmaf(__uint_as_float(s[2 * h + x / 16][(2 * x) & 31]), sl, -mb));
-                        const float e1 = kv4_ex2(fmaf(__uint_as_float(s[2 * h + x / 16][(2 * x + 1) & 31]), sl, -mb));
-                        sum[(2 * x) & 3] += e0;
-                        sum[(2 * x + 1) & 3] += e1;
-                        p[x] = pa_pair(T(), e0, e1);
+                for (int x = 0; x < 32; x++) {
+                    const uint32_t *v = &s[x >> 4][2 * (x & 15)];
+                    const uint64_t  t2 = pa_fma2(pa_two(__uint_as_float(v[0]), __uint_as_float(v[1])), sl2, mb2);
+                    float           e0, e1;
+                    if (x % 4 == 3) pa_ex2_fma<PaBits<T>::fmt ? 3 : 4>(t2, e0, e1);
+                    else {
+                        pa_untwo(t2, e0, e1);
+                        e0 = kv4_ex2(e0);
+                        e1 = kv4_ex2(e1);
                     }
-                    pa_st32(ts + 32 * h, p);
+                    sum[x & 1] = pa_add2(sum[x & 1], pa_two(e0, e1));
+                    p[x] = pa_pair(T(), e0, e1);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                pa_st32(ts + 32 * hf, p);
+                float a0, a1;
+                pa_untwo(pa_add2(sum[0], sum[1]), a0, a1);
+                l += a0 + a1;
                 pa_st_wait();
                 pa_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full + t);
             }
-            // the output: this thread's row
+            // the output: this thread's half of the row's dimensions
             if (n > 0) wait(s_full + t, (uint32_t)n & 1u);
             for (int j = n_plain; j < n; j++) wait(clean + (j - n_plain), 0);
             pa_fence_after();
-            const float inv = gone() ? NAN : 1.0f / l;
-            T          *out = (T *)a.out + (size_t)(q0 + row) * a.out_stride + (size_t)head_of(t) * HD;
-            for (int c = 0; c < HD / 32; c++) {
-                uint32_t o[32];
+            named_bar(1 + t, 256);
+            half_s[t][hf][r] = l;
+            named_bar(1 + t, 256);
+            const float inv = gone() ? NAN : 1.0f / (half_s[t][0][r] + half_s[t][1][r]);
+            T          *out = (T *)a.out + (size_t)(q0 + row) * a.out_stride + (size_t)head_of(t) * HD + HD / 2 * hf;
+#pragma unroll 1
+            for (int c = 0; c < HD / 2; c += 16) {
+                uint32_t o[16];
                 if (n > 0) {
-                    pa_ld32(o, to + 32 * c);
+                    pa_ld16(o, to + HD / 2 * hf + c);
                     pa_ld_wait();
                     pa_pin(o);
                 }
                 if (row < nq) {
-                    float y[32];
+                    float y[16];
 #pragma unroll
-                    for (int x = 0; x < 32; x++) y[x] = vis > 0 ? __uint_as_float(o[x]) * inv : 0.0f;
+                    for (int x = 0; x < 16; x++) y[x] = vis > 0 ? __uint_as_float(o[x]) * inv : 0.0f;
                     if (any_bad)                          // cleaned elements of keys that the row sees
                         for (int w = 0; w < 16; w++)
                             for (uint32_t left = bad[w >> 2][w & 3]; left; left &= left - 1) {
                                 const int key = (n_plain + (w >> 2)) * 128 + (w & 3) * 32 + __ffs(left) - 1;
                                 if (key >= vis) continue;
-                                const T *v = (const T *)a.v + (size_t)(k0 + key) * a.v_stride + (size_t)kvh * HD + 32 * c;
+                                const T *v = (const T *)a.v + (size_t)(k0 + key) * a.v_stride + (size_t)kvh * HD + HD / 2 * hf + c;
 #pragma unroll
-                                for (int x = 0; x < 32; x++) {
+                                for (int x = 0; x < 16; x++) {
                                     const float e = kv4_float(v[x]);
                                     if (!(fabsf(e) < INFINITY)) y[x] += e;
                                 }
                             }
 #pragma unroll
-                    for (int x = 0; x < 32; x += 8) {
+                    for (int x = 0; x < 16; x += 8) {
                         uint4 w;
                         w.x = pa_pair(T(), y[x], y[x + 1]);
                         w.y = pa_pair(T(), y[x + 2], y[x + 3]);
                         w.z = pa_pair(T(), y[x + 4], y[x + 5]);
                         w.w = pa_pair(T(), y[x + 6], y[x + 7]);
-                        *reinterpret_cast<uint4 *>(out + 32 * c + x) = w;
+                        *reinterpret_cast<uint4 *>(out + c + x) = w;
                     }
                 }
             }
@@ -426,5 +537,5 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     }
     pa_fence_before();
     __syncthreads();
-    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (warp == 17) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
