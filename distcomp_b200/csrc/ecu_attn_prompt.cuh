@@ -63,9 +63,16 @@ template <int N> struct PromptSeqs {
 __device__ __forceinline__ void pa_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void pa_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-__device__ __forceinline__ void pa_commit(uint64_t *bar)
+// The products and their commits are issued by the one thread with `me` set,
+// but by a whole warp's control flow: a predicate on the instruction instead
+// of a branch around it keeps the descriptors in uniform registers (inside
+// `if (lane == 0)` every operand of every product is moved there first, 85
+// cycles a product where it runs for 64).
+__device__ __forceinline__ void pa_commit(uint64_t *bar, uint32_t me)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)), "r"(me)
+                 : "memory");
 }
 
 __device__ __forceinline__ void pa_tma(uint32_t dst, const CUtensorMap *map, int x, int head, int row, uint64_t *bar)
@@ -84,17 +91,17 @@ __device__ __forceinline__ uint64_t pa_desc(uint32_t addr, uint32_t lbo)
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
-__device__ __forceinline__ void pa_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+__device__ __forceinline__ void pa_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t me)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(me)
                  : "memory");
 }
 
-__device__ __forceinline__ void pa_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+__device__ __forceinline__ void pa_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t me)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(me)
                  : "memory");
 }
 
@@ -325,51 +332,59 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         }
         __syncwarp();
     } else if (warp == 17) {
-        if (lane == 0 && n > 0) {
+        if (n > 0) {
+            const uint32_t me = lane == 0;
             // fp32 sums, M = 128; S: N = 128 keys; O: N = HD dimensions, V MN-major
             const uint32_t ids = (1u << 4) | (PaBits<T>::fmt << 7) | (PaBits<T>::fmt << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
             const uint32_t ido = (1u << 4) | (PaBits<T>::fmt << 7) | (PaBits<T>::fmt << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((128u >> 4) << 24);
+            const uint64_t qd = pa_desc(smem_addr(sm), 16), kd = pa_desc(smem_addr(ring), 16), vd = pa_desc(smem_addr(ring), PA_BOX);
             auto qk = [&](int t, int s) {
-                const uint32_t q = smem_addr(sm + t * S::TILE), k = smem_addr(ring + s * S::TILE);
+                const uint64_t q = qd + (uint64_t)(t * (S::TILE >> 4)), k = kd + (uint64_t)(s * (S::TILE >> 4));
 #pragma unroll
                 for (int x = 0; x < HD / 16; x++) {
-                    const uint32_t off = (uint32_t)(x / 4) * PA_BOX + (uint32_t)(x % 4) * 32;
-                    pa_mma_ss(tmem + 128 * t, pa_desc(q + off, 16), pa_desc(k + off, 16), ids, x > 0);
+                    const uint64_t off = (uint64_t)(((x / 4) * PA_BOX + (x % 4) * 32) >> 4);
+                    pa_mma_ss(tmem + 128 * t, q + off, k + off, ids, x > 0, me);
                 }
             };
             auto pv = [&](int t, int s, bool more) {
-                const uint32_t v = smem_addr(ring + s * S::TILE);
+                const uint64_t v = vd + (uint64_t)(s * (S::TILE >> 4));
 #pragma unroll
                 for (int x = 0; x < 8; x++)
-                    pa_mma_ts(tmem + 256 + HD * t, tmem + 128 * t + 8 * x, pa_desc(v + x * 2048, PA_BOX), ido, more || x > 0);
+                    pa_mma_ts(tmem + 256 + HD * t, tmem + 128 * t + 8 * x, v + (uint64_t)(x * 2048 >> 4), ido, more || x > 0, me);
             };
-            wait(&q_full, 0);
-            wait(full + 0, 0);
+            // (all lanes wait, and are together again for what follows)
+            auto until = [&](uint64_t *bar, uint32_t parity) {
+                wait(bar, parity);
+                __syncwarp();
+            };
+            until(&q_full, 0);
+            until(full + 0, 0);
             pa_fence_after();
-            for (int t = 0; t < n_tile && !gone(); t++) {
+            for (int t = 0; t < n_tile; t++) {
                 qk(t, 0);
-                pa_commit(s_full + t);
+                pa_commit(s_full + t, me);
             }
-            pa_commit(empty + 0);
-            for (int j = 0; j < n && !gone(); j++) {
+            pa_commit(empty + 0, me);
+            for (int j = 0; j < n; j++) {
                 const int iv = 2 * j + 1, sv = iv % ST, ik = iv + 1, sk = ik % ST;
-                wait(full + sv, (uint32_t)(iv / ST) & 1u);
-                if (j >= n_plain) wait(clean + (j - n_plain), 0);
-                if (j + 1 < n) wait(full + sk, (uint32_t)(ik / ST) & 1u);
+                until(full + sv, (uint32_t)(iv / ST) & 1u);
+                if (j >= n_plain) until(clean + (j - n_plain), 0);
+                if (j + 1 < n) until(full + sk, (uint32_t)(ik / ST) & 1u);
                 for (int t = 0; t < n_tile; t++) {
-                    wait(p_full + t, (uint32_t)j & 1u);
-                    if (gone()) break;
+                    until(p_full + t, (uint32_t)j & 1u);
+                    if (__any_sync(0xffffffffu, gone())) break;
                     pa_fence_after();
                     pv(t, sv, j > 0);
-                    if (t + 1 == n_tile) pa_commit(empty + sv);
+                    if (t + 1 == n_tile) pa_commit(empty + sv, me);
                     if (j + 1 < n) {
                         qk(t, sk);
-                        if (t + 1 == n_tile) pa_commit(empty + sk);
+                        if (t + 1 == n_tile) pa_commit(empty + sk, me);
                     }
-                    pa_commit(s_full + t);        // the next scores, or at the end the sums, and all before
+                    pa_commit(s_full + t, me);    // the next scores, or at the end the sums, and all before
                 }
+                if (__any_sync(0xffffffffu, gone())) break;
             }
-            pa_commit(&drain);
+            pa_commit(&drain, me);
             mbar_drain(&drain, 0, wait_limit_ns());       // no product in flight when tensor memory is given back
         }
         __syncwarp();
