@@ -63,15 +63,15 @@ template <int N> struct PromptSeqs {
 __device__ __forceinline__ void pa_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void pa_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// The products and their commits are issued by the one thread with `me` set,
-// but by a whole warp's control flow: a predicate on the instruction instead
-// of a branch around it keeps the descriptors in uniform registers (inside
-// `if (lane == 0)` every operand of every product is moved there first, 85
-// cycles a product where it runs for 64).
-__device__ __forceinline__ void pa_commit(uint64_t *bar, uint32_t me)
+// The products and their commits are issued by one elected thread, but by a
+// whole warp's control flow: elect.sync's predicate on the instruction itself
+// keeps the descriptors in uniform registers (behind any other predicate or
+// branch every operand of every product is moved there first, for each thread
+// that might issue it).
+__device__ __forceinline__ void pa_commit(uint64_t *bar)
 {
-    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)), "r"(me)
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xFFFFFFFF;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar))
                  : "memory");
 }
 
@@ -91,18 +91,40 @@ __device__ __forceinline__ uint64_t pa_desc(uint32_t addr, uint32_t lbo)
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
-__device__ __forceinline__ void pa_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t me)
+__device__ __forceinline__ void pa_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
 {
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(me)
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xFFFFFFFF;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
                  : "memory");
 }
 
-__device__ __forceinline__ void pa_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t me)
+__device__ __forceinline__ void pa_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc)
 {
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(me)
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xFFFFFFFF;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
                  : "memory");
+}
+
+// Waits that sleep: up to 20 us at a time inside the barrier's own wait, so
+// that waiting warps leave the issue slots to the others.
+__device__ __forceinline__ bool pa_try(uint64_t *bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(smem_addr(bar)), "r"(parity), "r"(20000u) : "memory");
+    return ok != 0;
+}
+
+// False when the limit of every wait ran out, or *dead says that another's has.
+__device__ __forceinline__ bool pa_wait(uint64_t *bar, uint32_t parity, int *dead)
+{
+    if (pa_try(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    while (!pa_try(bar, parity)) {
+        if (*reinterpret_cast<volatile int *>(dead)) return false;
+        if (globaltimer_ns() - t0 > wait_limit_ns()) return false;
+    }
+    return true;
 }
 
 #define PA_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
@@ -302,8 +324,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     const uint32_t tmem = tmem_s;
     // every wait is bounded; one that gives up lets the others give up too
     auto wait = [&](uint64_t *bar, uint32_t parity) {
-        if (mbar_try_wait(bar, parity)) return;
-        if (!mbar_wait<true>(bar, parity, &dead)) atomicExch(&dead, 1);
+        if (!pa_wait(bar, parity, &dead)) atomicExch(&dead, 1);
     };
     auto gone = [&] { return *reinterpret_cast<volatile int *>(&dead) != 0; };
 
@@ -333,7 +354,6 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         __syncwarp();
     } else if (warp == 17) {
         if (n > 0) {
-            const uint32_t me = lane == 0;
             // fp32 sums, M = 128; S: N = 128 keys; O: N = HD dimensions, V MN-major
             const uint32_t ids = (1u << 4) | (PaBits<T>::fmt << 7) | (PaBits<T>::fmt << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
             const uint32_t ido = (1u << 4) | (PaBits<T>::fmt << 7) | (PaBits<T>::fmt << 10) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((128u >> 4) << 24);
@@ -343,14 +363,14 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
 #pragma unroll
                 for (int x = 0; x < HD / 16; x++) {
                     const uint64_t off = (uint64_t)(((x / 4) * PA_BOX + (x % 4) * 32) >> 4);
-                    pa_mma_ss(tmem + 128 * t, q + off, k + off, ids, x > 0, me);
+                    pa_mma_ss(tmem + 128 * t, q + off, k + off, ids, x > 0);
                 }
             };
             auto pv = [&](int t, int s, bool more) {
                 const uint64_t v = vd + (uint64_t)(s * (S::TILE >> 4));
 #pragma unroll
                 for (int x = 0; x < 8; x++)
-                    pa_mma_ts(tmem + 256 + HD * t, tmem + 128 * t + 8 * x, v + (uint64_t)(x * 2048 >> 4), ido, more || x > 0, me);
+                    pa_mma_ts(tmem + 256 + HD * t, tmem + 128 * t + 8 * x, v + (uint64_t)(x * 2048 >> 4), ido, more || x > 0);
             };
             // (all lanes wait, and are together again for what follows)
             auto until = [&](uint64_t *bar, uint32_t parity) {
@@ -362,9 +382,9 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
             pa_fence_after();
             for (int t = 0; t < n_tile; t++) {
                 qk(t, 0);
-                pa_commit(s_full + t, me);
+                pa_commit(s_full + t);
             }
-            pa_commit(empty + 0, me);
+            pa_commit(empty + 0);
             for (int j = 0; j < n; j++) {
                 const int iv = 2 * j + 1, sv = iv % ST, ik = iv + 1, sk = ik % ST;
                 until(full + sv, (uint32_t)(iv / ST) & 1u);
@@ -375,16 +395,16 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                     if (__any_sync(0xffffffffu, gone())) break;
                     pa_fence_after();
                     pv(t, sv, j > 0);
-                    if (t + 1 == n_tile) pa_commit(empty + sv, me);
+                    if (t + 1 == n_tile) pa_commit(empty + sv);
                     if (j + 1 < n) {
                         qk(t, sk);
-                        if (t + 1 == n_tile) pa_commit(empty + sk, me);
+                        if (t + 1 == n_tile) pa_commit(empty + sk);
                     }
-                    pa_commit(s_full + t, me);    // the next scores, or at the end the sums, and all before
+                    pa_commit(s_full + t);    // the next scores, or at the end the sums, and all before
                 }
                 if (__any_sync(0xffffffffu, gone())) break;
             }
-            pa_commit(&drain, me);
+            pa_commit(&drain);
             mbar_drain(&drain, 0, wait_limit_ns());       // no product in flight when tensor memory is given back
         }
         __syncwarp();
