@@ -18,13 +18,13 @@
 // The maximum that P is taken relative to follows the running one only when
 // that has grown by more than 2^8 (P stays far inside fp16's range, and the
 // sums are fp32), so O is rescaled a few times per row at most, and a row's
-// two threads exchange maxima only then: one barrier with a vote a tile.
+// two threads exchange maxima only then: a vote between their two warps.
 // The exponentials of a pair of tiles, 32768 at 16 a clock, take as long as
-// its products at full rate; a quarter of them is computed on the FMA units
+// its products at full rate; an eighth of them is computed on the FMA units
 // instead (2^x = 2^n p(f), p a polynomial fitted to the relative error: 7.5e-5
 // for bf16, whose own step is 2^-8, 2.7e-6 for fp16).
 //
-// Tensor memory: S of tile t at column 128 t (P in its first 64), O at
+// Tensor memory: S of tile t at column 128 t (P in the first 32 of each 64), O at
 // 256 + HD t.  Shared memory: tiles of 128 rows of 64 elements (128 bytes,
 // 128-byte swizzle), HD / 64 of them side by side; Q and K are K-major
 // operands, V (keys x dimensions) is read MN-major.
@@ -35,6 +35,7 @@
 #include <cuda.h>
 
 #define PA_THREADS 640
+#define PA_FMA 8                           // every PA_FMA-th pair of exponentials goes to the FMA units
 #define PA_BOX 16384                       // 128 rows x 128 bytes
 
 template <int HD> struct PaShape {
@@ -130,25 +131,7 @@ __device__ __forceinline__ bool pa_wait(uint64_t *bar, uint32_t parity, int *dea
 #define PA_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
 #define PA_W8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
 
-// 32 columns of this thread's row (its warp's 32 lanes)
-__device__ __forceinline__ void pa_ld32(uint32_t (&v)[32], uint32_t addr)
-{
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-                 "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                 : PA_R8(v, 0), PA_R8(v, 8), PA_R8(v, 16), PA_R8(v, 24)
-                 : "r"(addr)
-                 : "memory");
-}
-
-__device__ __forceinline__ void pa_st32(uint32_t addr, const uint32_t (&v)[32])
-{
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-                 "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
-                 PA_W8(v, 0), PA_W8(v, 8), PA_W8(v, 16), PA_W8(v, 24)
-                 : "memory");
-}
-
-// the same of 16 columns: where 32 more values would not fit the registers
+// 16 columns of this thread's row (its warp's 32 lanes)
 __device__ __forceinline__ void pa_ld16(uint32_t (&v)[16], uint32_t addr)
 {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -245,12 +228,12 @@ template <int DEG> __device__ __forceinline__ void pa_ex2_fma(uint64_t t2, float
     e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(r1) << 23));
 }
 
-// Does any of the 256 threads at barrier `id` say so?
+// Does any of the 64 threads at barrier `id` say so?
 __device__ __forceinline__ bool pa_any(int id, bool mine)
 {
     uint32_t any;
     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-                 "barrier.cta.red.or.pred q, %2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 "barrier.cta.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
                  : "=r"(any) : "r"((uint32_t)mine), "r"(id) : "memory");
     return any != 0;
 }
@@ -370,7 +353,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                 const uint64_t v = vd + (uint64_t)(s * (S::TILE >> 4));
 #pragma unroll
                 for (int x = 0; x < 8; x++)
-                    pa_mma_ts(tmem + 256 + HD * t, tmem + 128 * t + 8 * x, v + (uint64_t)(x * 2048 >> 4), ido, more || x > 0);
+                    pa_mma_ts(tmem + 256 + HD * t, tmem + 128 * t + 64 * (x / 4) + 8 * (x % 4), v + (uint64_t)(x * 2048 >> 4), ido, more || x > 0);
             };
             // (all lanes wait, and are together again for what follows)
             auto until = [&](uint64_t *bar, uint32_t parity) {
@@ -389,7 +372,6 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                 const int iv = 2 * j + 1, sv = iv % ST, ik = iv + 1, sk = ik % ST;
                 until(full + sv, (uint32_t)(iv / ST) & 1u);
                 if (j >= n_plain) until(clean + (j - n_plain), 0);
-                if (j + 1 < n) until(full + sk, (uint32_t)(ik / ST) & 1u);
                 for (int t = 0; t < n_tile; t++) {
                     until(p_full + t, (uint32_t)j & 1u);
                     if (__any_sync(0xffffffffu, gone())) break;
@@ -397,6 +379,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                     pv(t, sv, j > 0);
                     if (t + 1 == n_tile) pa_commit(empty + sv);
                     if (j + 1 < n) {
+                        if (t == 0) until(full + sk, (uint32_t)(ik / ST) & 1u);
                         qk(t, sk);
                         if (t + 1 == n_tile) pa_commit(empty + sk);
                     }
@@ -439,9 +422,9 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
             if (lane == 0) mbar_arrive(clean + (j - n_plain));
         }
     } else {
-        // Nothing here leaves the loop early, whatever gave up: the tile's 256
-        // threads meet at its barrier in every turn.
-        const int      t = warp >> 3, hf = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;
+        // Nothing here leaves the loop early, whatever gave up: the two warps of
+        // 32 rows meet at their barrier in every turn.
+        const int      t = warp >> 3, hf = (warp >> 2) & 1, r = (warp & 3) * 32 + lane, pair = 1 + 4 * t + (warp & 3);
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lanes + 128 * t, to = tmem + lanes + 256 + HD * t;
         if (t < n_tile) {
             const int   row = tile_of(t) * 128 + r, vis = seen(row);
@@ -450,24 +433,24 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
             for (int j = 0; j < n; j++) {
                 wait(s_full + t, (uint32_t)j & 1u);
                 pa_fence_after();
-                uint32_t s[2][32];
-                pa_ld32(s[0], ts + 64 * hf);
-                pa_ld32(s[1], ts + 64 * hf + 32);
+                uint32_t s[4][16];
+#pragma unroll
+                for (int c = 0; c < 4; c++) pa_ld16(s[c], ts + 64 * hf + 16 * c);
                 pa_ld_wait();
-                pa_pin(s[0]);
-                pa_pin(s[1]);
+#pragma unroll
+                for (int c = 0; c < 4; c++) pa_pin(s[c]);
                 if (j >= n_plain) {
                     const int left = vis - j * 128 - 64 * hf;
 #pragma unroll
-                    for (int c = 0; c < 2; c++)
+                    for (int c = 0; c < 4; c++)
 #pragma unroll
-                        for (int x = 0; x < 32; x++)
-                            if (32 * c + x >= left) s[c][x] = 0xFF800000u;
+                        for (int x = 0; x < 16; x++)
+                            if (16 * c + x >= left) s[c][x] = 0xFF800000u;
                 }
                 float top[4];
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
-                    auto v = [&](int x) { return __uint_as_float(s[q >> 1][(q & 1) * 16 + x]); };
+                    auto v = [&](int x) { return __uint_as_float(s[q][x]); };
                     top[q] = pa_max3(v(0), v(1), v(2));
 #pragma unroll
                     for (int x = 3; x < 15; x += 2) top[q] = pa_max3(top[q], v(x), v(x + 1));
@@ -476,10 +459,9 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                 float mx = pa_max(pa_max3(top[0], top[1], top[2]), top[3]);
                 // not (mx within 2^8 of m): a NaN grows, and turns its whole row into NaN
                 auto grows = [&] { return !(mx <= m) && !((mx - m) * sl <= 8.0f); };
-                // (the barrier also lets P take the place of scores that all have read)
-                if (pa_any(1 + t, grows())) {
+                if (pa_any(pair, grows())) {
                     half_s[t][hf][r] = mx;
-                    named_bar(1 + t, 256);
+                    named_bar(pair, 64);
                     mx = pa_max(mx, half_s[t][hf ^ 1][r]);
                     const bool  grow = grows();
                     const float f = grow && j > 0 ? kv4_ex2((m - mx) * sl) : 1.0f;
@@ -500,22 +482,25 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                 const float    mb = m == -INFINITY ? 0.0f : m * sl;
                 const uint64_t sl2 = pa_two(sl, sl), mb2 = pa_two(-mb, -mb);
                 uint64_t       sum[2] = {pa_two(0.0f, 0.0f), pa_two(0.0f, 0.0f)};
-                uint32_t       p[32];
 #pragma unroll
-                for (int x = 0; x < 32; x++) {
-                    const uint32_t *v = &s[x >> 4][2 * (x & 15)];
-                    const uint64_t  t2 = pa_fma2(pa_two(__uint_as_float(v[0]), __uint_as_float(v[1])), sl2, mb2);
-                    float           e0, e1;
-                    if (x % 4 == 3) pa_ex2_fma<PaBits<T>::fmt ? 3 : 4>(t2, e0, e1);
-                    else {
-                        pa_untwo(t2, e0, e1);
-                        e0 = kv4_ex2(e0);
-                        e1 = kv4_ex2(e1);
+                for (int h = 0; h < 2; h++) {
+                    uint32_t p[16];
+#pragma unroll
+                    for (int x = 0; x < 16; x++) {
+                        const uint32_t *v = &s[2 * h + (x >> 3)][2 * (x & 7)];
+                        const uint64_t  t2 = pa_fma2(pa_two(__uint_as_float(v[0]), __uint_as_float(v[1])), sl2, mb2);
+                        float           e0, e1;
+                        if (x % PA_FMA == PA_FMA - 1) pa_ex2_fma<PaBits<T>::fmt ? 3 : 4>(t2, e0, e1);
+                        else {
+                            pa_untwo(t2, e0, e1);
+                            e0 = kv4_ex2(e0);
+                            e1 = kv4_ex2(e1);
+                        }
+                        sum[x & 1] = pa_add2(sum[x & 1], pa_two(e0, e1));
+                        p[x] = pa_pair(T(), e0, e1);
                     }
-                    sum[x & 1] = pa_add2(sum[x & 1], pa_two(e0, e1));
-                    p[x] = pa_pair(T(), e0, e1);
+                    pa_st16(ts + 64 * hf + 16 * h, p);    // over scores that this thread alone has read
                 }
-                pa_st32(ts + 32 * hf, p);
                 float a0, a1;
                 pa_untwo(pa_add2(sum[0], sum[1]), a0, a1);
                 l += a0 + a1;
@@ -528,9 +513,9 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
             if (n > 0) wait(s_full + t, (uint32_t)n & 1u);
             for (int j = n_plain; j < n; j++) wait(clean + (j - n_plain), 0);
             pa_fence_after();
-            named_bar(1 + t, 256);
+            named_bar(pair, 64);
             half_s[t][hf][r] = l;
-            named_bar(1 + t, 256);
+            named_bar(pair, 64);
             const float inv = gone() ? NAN : 1.0f / (half_s[t][0][r] + half_s[t][1][r]);
             T          *out = (T *)a.out + (size_t)(q0 + row) * a.out_stride + (size_t)head_of(t) * HD + HD / 2 * hf;
 #pragma unroll 1
