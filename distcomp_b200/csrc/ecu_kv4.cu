@@ -281,7 +281,7 @@ static int append_launch(ecu_kv *kv, const KvAppendArgs &a, const int *seq, int 
         r.seq[i] = (uint16_t)(seq ? seq[i] : first + i);
         r.row0[i + 1] = r.row0[i] + n_new[i];
     }
-    const long long threads = (long long)r.row0[n] * 2 * a.n_kv * a.nb * 4;
+    const long long threads = (long long)r.row0[n] * a.n_kv * a.nb * 4;
     if (threads == 0) return 0;
     k_kv4_append<T, O, N><<<(unsigned)((threads + 255) / 256), 256, 0, s>>>(a, r);
     return launched("ecu_kv_append");
@@ -353,7 +353,7 @@ extern "C" int ecu_kv_append(ecu_kv *kv, int layer, int dtype, const void *k, co
             rows += n_new[i];
         }
         if (rows == 0) return 0;
-        if (rows > INT_MAX) return say(what, "too many rows");
+        if (rows > INT_MAX / (row / 8)) return say(what, "too many rows");            // a thread for eight values
         if (!k || !v || (!k_out) != (!v_out)) return say(what, "null rows, or one of k_out and v_out alone");
         if (rows > 1 && (k_stride < row || v_stride < row)) return say(what, "rows overlap: a stride below n_head_kv * head_dim");
         if (((uintptr_t)k | (uintptr_t)v) % es || (k_out && ((uintptr_t)k_out | (uintptr_t)v_out) % os))
@@ -376,6 +376,7 @@ extern "C" int ecu_kv_append(ecu_kv *kv, int layer, int dtype, const void *k, co
         a.n_pages = kv->book.n_pages;
         a.n_kv = kv->n_head_kv;
         a.nb = kv->head_dim / 32;
+        a.nb_inv = (65536 + a.nb - 1) / a.nb;             // exact below 32768: at most 4096 heads of 4 blocks
         a.wide = !(((uintptr_t)k | (uintptr_t)v | (uintptr_t)(k_stride * (long)es) | (uintptr_t)(v_stride * (long)es)) & 15);
         a.wide_out = !(((uintptr_t)k_out | (uintptr_t)v_out) & 15);
         const cudaStream_t s = (cudaStream_t)stream;

@@ -73,28 +73,88 @@ struct KvAppendArgs {
     size_t      page_bytes;
     const int  *table, *len;
     int         max_pages, n_pages, n_kv, nb;
+    unsigned    nb_inv;           // x / nb = x * nb_inv >> 16 for the blocks of a row
     bool        wide, wide_out;
 };
 
-// Four lanes to a block of 32 values, eight values each.  A block's value of
-// largest magnitude is found with two shuffles on (magnitude, first place)
-// keys.  The code is decided exactly: the quotient's rounding can only be off
-// near k + 1/2, and (k + 1/2) * scale has 5 + 11 bits, exact in fp32, so one
-// comparison on either side settles it.  Bound by memory: 2 * (4 or 2) bytes
-// of row read and 1.125 written per pair of K and V values.
+// The larger, or NaN where either is.
+__device__ __forceinline__ float kv4_max(float a, float b)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// Eight of a block's 32 values (the other 24 with the group's other lanes):
+// the scale, and this lane's word of codes and values as stored.
+//
+// With u = x * sign(scale) and d = |scale|, the code is 8 + the k of
+// (k - 1/2) d <= u < (k + 1/2) d.  k is guessed from u * (1 / d) - 2^-18, which
+// is never too high and too low by one at most, and settled by r = u - k d, one
+// fma: where r is near d / 2 it is exact (u and k d are multiples of 2^-24 of
+// the power of two below d, and |r| is below it), so the comparison with d / 2
+// decides as exact arithmetic would.
+__device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[8], unsigned mask, int c, __half &dh, float (&y)[8])
+{
+    // the largest value and the largest negated one say the sign, unless they
+    // are equal: then the first of them does
+    float p = x[0], q = -x[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) {
+        p = kv4_max(p, x[i]);
+        q = kv4_max(q, -x[i]);
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        p = kv4_max(p, __shfl_xor_sync(mask, p, o));
+        q = kv4_max(q, __shfl_xor_sync(mask, q, o));
+    }
+    float m = p > q ? p : -q;
+    if (p == q) {                                                // (the same in the group's four lanes)
+        int at = 64;                                             // 2 * place of the first, odd for a negative value
+#pragma unroll
+        for (int i = 7; i >= 0; i--)
+            if (fabsf(x[i]) == p) at = 2 * (8 * c + i) + (x[i] < 0.0f);
+        at = min(at, __shfl_xor_sync(mask, at, 1));
+        at = min(at, __shfl_xor_sync(mask, at, 2));
+        m = at & 1 ? -p : p;
+    }
+    const bool fine = fabsf(m) < INFINITY && p == p;
+    dh = __float2half_rn(fminf(fmaxf(m * -0.125f, -65504.0f), 65504.0f));
+    if (!fine) dh = __ushort_as_half(0x7FFF);
+    else if (__half2float(dh) == 0.0f) dh = __ushort_as_half(0);
+    const float d = __half2float(dh), sign = copysignf(1.0f, d);
+    // a scale of zero: every guess is 0, and nothing reaches the half step
+    const float inv = d != 0.0f ? __frcp_rn(d) : 0.0f, half = d != 0.0f ? 0.5f * fabsf(d) : INFINITY;
+    uint32_t    w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        // rounded to a whole number by adding 1.5 * 2^23 and taking it off again
+        float k = __fsub_rn(__fadd_rn(__fmaf_rn(x[i], inv, -3.814697265625e-6f), 12582912.0f), 12582912.0f);
+        if (__fmul_rn(__fmaf_rn(-k, d, x[i]), sign) >= half) k += 1.0f;
+        k = fminf(fmaxf(k, -8.0f), 7.0f);
+        // 2^23 + 8 + k has the bits 0x4B000000 + code: eight of them, 4 bits apart, add up to the
+        // word and 0xFB000000
+        w += __float_as_uint(k + 8388616.0f) << (4 * i);
+        y[i] = k * d;
+    }
+    return fine ? w - 0xFB000000u : 0x88888888u;
+}
+
+// Four lanes to a block of 32 dimensions, eight values of K and of V each.
+// Bound by memory: 4 or 2 bytes a value read, 0.5625 written, and 4 or 2 where
+// the values are handed back.
 template <typename T, typename O, int N>
 __global__ void __launch_bounds__(256) k_kv4_append(const KvAppendArgs a, const KvRows<N> rows)
 {
-    const int per_row = 2 * a.n_kv * a.nb;                       // blocks of a row: K then V
-    const long long blk = ((long long)blockIdx.x * 256 + threadIdx.x) >> 2;
-    const int c = threadIdx.x & 3;
-    const long long r = blk / per_row;
+    const unsigned per_row = a.n_kv * a.nb;                      // blocks of a row
+    const unsigned blk = (blockIdx.x * 256u + threadIdx.x) >> 2; // below 2^31: the host sees to it
+    const int      c = threadIdx.x & 3, r = (int)(blk / per_row);
     if (r >= rows.row0[rows.n]) return;                          // whole groups of four leave together
-    const int in_row = (int)(blk - r * per_row), side = in_row >= a.n_kv * a.nb;
-    const int hb = in_row - side * a.n_kv * a.nb, h = hb / a.nb, b = hb - h * a.nb;
-    const T  *src = side ? (const T *)a.v + (size_t)r * a.v_stride : (const T *)a.k + (size_t)r * a.k_stride;
-    float     x[8];
-    kv4_load8(src + (size_t)hb * 32 + 8 * c, a.wide, x);
+    const int hb = (int)(blk - r * per_row), h = (int)((unsigned)hb * a.nb_inv >> 16), b = hb - h * a.nb;
+    float     x[2][8];
+    kv4_load8((const T *)a.k + (size_t)r * a.k_stride + (size_t)hb * 32 + 8 * c, a.wide, x[0]);
+    kv4_load8((const T *)a.v + (size_t)r * a.v_stride + (size_t)hb * 32 + 8 * c, a.wide, x[1]);
     // the sequence of row r: the last whose first row is not past it
     int lo = 0, hi = rows.n;
     while (hi - lo > 1) {
@@ -102,56 +162,24 @@ __global__ void __launch_bounds__(256) k_kv4_append(const KvAppendArgs a, const 
         if (rows.row0[mid] <= r) lo = mid;
         else hi = mid;
     }
-    const int s = rows.seq[lo];
-    const int pos = __ldg(a.len + s) - (rows.row0[lo + 1] - (int)r);
-
+    const int  s = rows.seq[lo], pos = __ldg(a.len + s) - (rows.row0[lo + 1] - r);
+    const bool placed = pos >= 0 && pos < a.max_pages * KV4_PAGE;
+    const int  page = placed ? __ldg(a.table + (size_t)s * a.max_pages + pos / KV4_PAGE) : -1;
+    const int  hd = a.nb * 32, t = pos % KV4_PAGE;
+    const bool wr = (unsigned)page < (unsigned)a.n_pages;        // no page: nothing to write to
+    uint8_t   *p = a.layer + (size_t)(wr ? page : 0) * a.page_bytes + (size_t)h * 72 * hd;
     const unsigned mask = 0xFu << (threadIdx.x & 28);
-    float          m = x[0];
-    int            at = 8 * c;
-    bool           fine = true;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        if (fabsf(x[i]) > fabsf(m)) { m = x[i]; at = 8 * c + i; }
-        fine = fine && fabsf(x[i]) < INFINITY;
+    for (int side = 0; side < 2; side++) {
+        float          y[8];
+        __half         d;
+        const uint32_t w = kv4_quantise(x[side], mask, c, d, y);
+        if (a.k_out)
+            kv4_store8((O *)(side ? a.v_out : a.k_out) + (size_t)r * per_row * 32 + (size_t)hb * 32 + 8 * c, a.wide_out, y);
+        if (!wr) continue;
+        *reinterpret_cast<uint32_t *>(p + side * 32 * hd + t * (hd / 2) + kv4_place(t, b, a.nb) * 16 + 4 * c) = w;
+        if (c == 0) *reinterpret_cast<__half *>(p + 64 * hd + side * 4 * hd + (t * a.nb + b) * 2) = d;
     }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        const float m2 = __shfl_xor_sync(mask, m, o);
-        const int   a2 = __shfl_xor_sync(mask, at, o);
-        fine = __shfl_xor_sync(mask, (int)fine, o) && fine;
-        if (fabsf(m2) > fabsf(m) || (fabsf(m2) == fabsf(m) && a2 < at)) { m = m2; at = a2; }
-    }
-    __half dh = __float2half_rn(fminf(fmaxf(m * -0.125f, -65504.0f), 65504.0f));
-    if (!fine) dh = __ushort_as_half(0x7FFF);
-    else if (__half2float(dh) == 0.0f) dh = __ushort_as_half(0);
-    const float d = __half2float(dh);
-    const bool  flat = !fine || d == 0.0f;
-    const float sg = d < 0.0f ? -1.0f : 1.0f, ad = fabsf(d);
-    uint32_t    w = 0;
-    float       y[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        int code = 8;
-        if (!flat) {
-            // floor(x / d + 8.5) with x, d -> x * sign(d), |d|
-            const float u = x[i] * sg;
-            float       k = floorf(__fadd_rn(fminf(fmaxf(__fdiv_rn(u, ad), -16.0f), 16.0f), 0.5f));
-            if (u < (k - 0.5f) * ad) k -= 1.0f;
-            else if (u >= (k + 0.5f) * ad) k += 1.0f;
-            code = min(15, max(0, (int)k + 8));
-        }
-        w |= (uint32_t)code << (4 * i);
-        y[i] = (float)(code - 8) * d;
-    }
-    const int nkvhd = a.n_kv * a.nb * 32;
-    if (a.k_out) kv4_store8((O *)(side ? a.v_out : a.k_out) + (size_t)r * nkvhd + (size_t)hb * 32 + 8 * c, a.wide_out, y);
-    if (pos < 0 || pos >= a.max_pages * KV4_PAGE) return;
-    const int page = __ldg(a.table + (size_t)s * a.max_pages + pos / KV4_PAGE);
-    if ((unsigned)page >= (unsigned)a.n_pages) return;           // no page: nothing to write to
-    const int hd = a.nb * 32, t = pos % KV4_PAGE;
-    uint8_t  *p = a.layer + (size_t)page * a.page_bytes + (size_t)h * 72 * hd;
-    *reinterpret_cast<uint32_t *>(p + side * 32 * hd + t * (hd / 2) + kv4_place(t, b, a.nb) * 16 + 4 * c) = w;
-    if (c == 0) *reinterpret_cast<__half *>(p + 64 * hd + side * 4 * hd + (t * a.nb + b) * 2) = dh;
 }
 
 // ----------------------------------------------------------- page upkeep ---
