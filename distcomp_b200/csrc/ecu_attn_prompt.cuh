@@ -252,7 +252,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     extern __shared__ uint8_t raw[];
     uint8_t *sm = reinterpret_cast<uint8_t *>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     uint8_t *ring = sm + 2 * S::TILE;
-    __shared__ __align__(8) uint64_t q_full, full[ST], empty[ST], s_full[2], p_full[2], due[4], clean[4], drain;
+    __shared__ __align__(8) uint64_t q_full[2], full[ST], empty[ST], s_full[2], p_full[2], due[4], clean[4], drain;
     __shared__ uint32_t              tmem_s, bad[4][4];       // keys of the partly seen tiles with cleaned elements
     __shared__ int                   any_bad, dead;
     __shared__ float                 half_s[2][2][128];       // what a row's two threads tell each other
@@ -282,13 +282,23 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_s)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (tid == 0) {
-        mbar_init(&q_full, 1);
+    // one tile of K (x even) or V of key tile x / 2 into the ring's place x % ST
+    auto copy_kv = [&](int x) {
+        mbar_expect_tx(full + x % ST, S::TILE);
+        for (int b = 0; b < B; b++)
+            pa_tma(smem_addr(ring + x % ST * S::TILE + b * PA_BOX), (x & 1) ? &mv : &mk, b * 64, kvh, k0 + x / 2 * 128, full + x % ST);
+        // the cleaners may look at the stage's barrier only now that it
+        // counts this tile: its phase's parity would fit an earlier one too
+        if ((x & 1) && x / 2 >= n_plain) mbar_arrive(due + (x / 2 - n_plain));
+    };
+    if (tid == 512) {                                     // the first copies are on their way before the block meets
+        for (const CUtensorMap *m : {&mq, &mk, &mv}) asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
         for (int s = 0; s < ST; s++) {
             mbar_init(full + s, 1);
             mbar_init(empty + s, 1);
         }
         for (int t = 0; t < 2; t++) {
+            mbar_init(q_full + t, 1);
             mbar_init(s_full + t, 1);
             mbar_init(p_full + t, 8);
         }
@@ -299,6 +309,15 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         mbar_init(&drain, 1);
         mbar_init_fence();
         any_bad = dead = 0;
+        if (n > 0) {
+            for (int t = 0; t < n_tile; t++) {
+                mbar_expect_tx(q_full + t, S::TILE);
+                for (int b = 0; b < B; b++)
+                    pa_tma(smem_addr(sm + t * S::TILE + b * PA_BOX), &mq, b * 64, head_of(t), q0 + tile_of(t) * 128, q_full + t);
+                if (t == 0) copy_kv(0);
+            }
+            for (int x = 1; x < min(ST, 2 * n); x++) copy_kv(x);
+        }
     }
     if (tid < 16) bad[tid >> 2][tid & 3] = 0;
     pa_fence_before();
@@ -312,26 +331,16 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     auto gone = [&] { return *reinterpret_cast<volatile int *>(&dead) != 0; };
 
     if (warp == 16) {
-        if (lane == 0 && n > 0) {
-            mbar_expect_tx(&q_full, (uint32_t)n_tile * S::TILE);
-            for (int t = 0; t < n_tile; t++)
-                for (int b = 0; b < B; b++)
-                    pa_tma(smem_addr(sm + t * S::TILE + b * PA_BOX), &mq, b * 64, head_of(t), q0 + tile_of(t) * 128, &q_full);
-            int i = 0;
-            for (; i < 2 * n; i++) {              // K and V of key tile i / 2
-                const int s = i % ST;
-                if (i >= ST) wait(empty + s, (uint32_t)(i / ST - 1) & 1u);
+        if (lane == 0) {
+            int x = min(ST, 2 * n);
+            for (; x < 2 * n; x++) {
+                wait(empty + x % ST, (uint32_t)(x / ST - 1) & 1u);
                 if (gone()) break;
-                mbar_expect_tx(full + s, S::TILE);
-                for (int b = 0; b < B; b++)
-                    pa_tma(smem_addr(ring + s * S::TILE + b * PA_BOX), (i & 1) ? &mv : &mk, b * 64, kvh, k0 + i / 2 * 128, full + s);
-                // the cleaners may look at the stage's barrier only now that it
-                // counts this tile: its phase's parity would fit an earlier one too
-                if ((i & 1) && i / 2 >= n_plain) mbar_arrive(due + (i / 2 - n_plain));
+                copy_kv(x);
             }
             if (gone()) {                         // nothing may still be on its way into shared memory
-                mbar_drain(&q_full, 0, wait_limit_ns());
-                for (int x = i > ST ? i - ST : 0; x < i; x++) mbar_drain(full + x % ST, (uint32_t)(x / ST) & 1u, wait_limit_ns());
+                for (int t = 0; t < n_tile && n > 0; t++) mbar_drain(q_full + t, 0, wait_limit_ns());
+                for (int y = x > ST ? x - ST : 0; y < x; y++) mbar_drain(full + y % ST, (uint32_t)(y / ST) & 1u, wait_limit_ns());
             }
         }
         __syncwarp();
@@ -360,10 +369,10 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                 wait(bar, parity);
                 __syncwarp();
             };
-            until(&q_full, 0);
             until(full + 0, 0);
-            pa_fence_after();
             for (int t = 0; t < n_tile; t++) {
+                until(q_full + t, 0);
+                pa_fence_after();
                 qk(t, 0);
                 pa_commit(s_full + t);
             }
@@ -517,7 +526,10 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
             half_s[t][hf][r] = l;
             named_bar(pair, 64);
             const float inv = gone() ? NAN : 1.0f / (half_s[t][0][r] + half_s[t][1][r]);
-            T          *out = (T *)a.out + (size_t)(q0 + row) * a.out_stride + (size_t)head_of(t) * HD + HD / 2 * hf;
+            // through the place of the tile's queries, 16-byte chunk j of row r at
+            // j ^ (r & 7), so that rows leave whole: 2.5 us a pair where every
+            // thread writes its own row
+            uint8_t *rows_s = sm + t * S::TILE + (size_t)(warp & 3) * 32 * HD * 2;
 #pragma unroll 1
             for (int c = 0; c < HD / 2; c += 16) {
                 uint32_t o[16];
@@ -526,7 +538,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                     pa_ld_wait();
                     pa_pin(o);
                 }
-                if (row < nq) {
+                {
                     float y[16];
 #pragma unroll
                     for (int x = 0; x < 16; x++) y[x] = vis > 0 ? __uint_as_float(o[x]) * inv : 0.0f;
@@ -549,9 +561,17 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                         w.y = pa_pair(T(), y[x + 2], y[x + 3]);
                         w.z = pa_pair(T(), y[x + 4], y[x + 5]);
                         w.w = pa_pair(T(), y[x + 6], y[x + 7]);
-                        *reinterpret_cast<uint4 *>(out + c + x) = w;
+                        *reinterpret_cast<uint4 *>(rows_s + lane * HD * 2 + (((HD / 2 * hf + c + x) / 8 ^ (lane & 7)) * 16)) = w;
                     }
                 }
+            }
+            named_bar(pair, 64);
+            T *out = (T *)a.out + (size_t)(q0 + tile_of(t) * 128 + (warp & 3) * 32) * a.out_stride + (size_t)head_of(t) * HD;
+            const int rows = nq - tile_of(t) * 128 - (warp & 3) * 32;       // of these 32
+#pragma unroll
+            for (int x = hf * 32 + lane; x < 32 * HD / 8; x += 64) {
+                const int y = x / (HD / 8), j = x % (HD / 8);
+                if (y < rows) *reinterpret_cast<uint4 *>(out + (size_t)y * a.out_stride + j * 8) = *reinterpret_cast<const uint4 *>(rows_s + y * HD * 2 + ((j ^ (y & 7)) * 16));
             }
         }
     }
