@@ -548,24 +548,32 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
         for (int x = lane * (128 / (int)sizeof(T)); x < min(HG, a.n_rep - grp * HG) * HD; x += 32 * (128 / (int)sizeof(T)))
             asm volatile("prefetch.global.L1 [%0];" ::"l"(q + x));
     };
-    // the queries of row p.r: column col is query head HG * group + col / P, part col % P
-    auto load_q = [&](const KvCursor &p) {
+    // this lane's elements of the query columns of row p.r: column col is query
+    // head HG * group + col / P
+    auto read_q = [&](const KvCursor &p, float (&x)[NT][NB][8]) {
         const int kvh = p.r / n_grp, grp = p.r - kvh * n_grp;
-        float     f[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const int col = nt * 8 + g, hh = grp * HG + col / P;
-            float     x[NB][8], m = 0.0f;
-            if (hh < a.n_rep) {
-                const T *q = (const T *)a.q + (size_t)p.i * a.q_stride + (size_t)(kvh * a.n_rep + hh) * HD + 8 * c;
+            const int hh = grp * HG + (nt * 8 + g) / P;
+            const T  *q = (const T *)a.q + (size_t)p.i * a.q_stride + (size_t)(kvh * a.n_rep + hh) * HD + 8 * c;
 #pragma unroll
-                for (int b = 0; b < NB; b++) kv4_load8(q + 32 * b, a.wide_q, x[b]);
-            } else {
+            for (int b = 0; b < NB; b++) {
+                if (hh < a.n_rep) kv4_load8(q + 32 * b, a.wide_q, x[nt][b]);
+                else
 #pragma unroll
-                for (int b = 0; b < NB; b++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[b][e] = 0.0f;
+                    for (int e = 0; e < 8; e++) x[nt][b][e] = 0.0f;
             }
+        }
+    };
+    // them as the products' operands (column col: part col % P of its head's
+    // query), and the row's softmax from nothing
+    auto load_q = [&](const float (&xs)[NT][NB][8]) {
+        float f[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const int    col = nt * 8 + g;
+            const float(&x)[NB][8] = xs[nt];
+            float        m = 0.0f;
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -844,7 +852,8 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
         KvCursor at = locate(u0), ahead = at;
         KvCursor first[KV4_STAGES];
         int      page[KV4_STAGES + 1];
-        fetch_q(at);
+        float    xq[NT][NB][8];
+        read_q(at, xq);                                   // (all of these loads are in flight together)
 #pragma unroll
         for (int k = 0; k < KV4_STAGES; k++) {            // independent loads
             page[k] = page_at(ahead);
@@ -857,7 +866,7 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
             if (first[k].left > 0) issue(first[k], page[k], k);
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
-        load_q(at);
+        load_q(xq);
         int      j0 = at.j, k = 0, len = min(__ldg(a.len + list.seq[at.i]), cap);
         for (;;) {
             if (at.j > 0) {
@@ -902,7 +911,9 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
             if (run_end) break;
             next(at);
             j0 = 0;
-            load_q(at);
+            float x2[NT][NB][8];
+            read_q(at, x2);
+            load_q(x2);
             len = min(__ldg(a.len + list.seq[at.i]), cap);
         }
     }
@@ -958,26 +969,41 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
         if (tid == 0) n_lead = __popc(lead);
     }
     __syncthreads();
-    // a warp per row and 32 dimensions of a head
-    for (int task = warp; task < n_lead * HG * NB; task += W) {
-        const int e = lead_s[task / (HG * NB)], end = 32 - __clz(mates[e]), row = rid[e];
+    // a warp per row and head, or, of few rows, per 32 dimensions of one
+    const int span = n_lead * HG >= W ? NB : 1, parts = NB / span;
+    for (int task = warp; task < n_lead * HG * parts; task += W) {
+        const int e = lead_s[task / (HG * parts)], end = 32 - __clz(mates[e]), row = rid[e];
         const int i = row / R, nu = pre[i + 1] - pre[i], first = pre[i] * R + (row - i * R) * nu;
         const bool whole = first >= cu0 && first + nu <= cu1;
-        const int  x = task % (HG * NB) * 32 + lane, h = x / HD, at = h * (HD + 2);
-        float      L = 0.0f, v = 0.0f;
+        const int  h = task / parts % HG, d0 = task % parts * 32 + lane;
+        float      L = 0.0f, v[NB];
+#pragma unroll
+        for (int x = 0; x < NB; x++) v[x] = 0.0f;
 #pragma unroll 4
         for (int k = e; k < end; k++) {
-            const float w = wgt[k][h], ln = entry(k)[at + HD + 1], vn = entry(k)[at + x % HD];
+            const float  w = wgt[k][h];
+            const float *from = entry(k) + h * (HD + 2);
             if (w != 0.0f) {                              // (an unused place holds anything)
-                L = fmaf(w, ln, L);
-                v = fmaf(w, vn, v);
+                L = fmaf(w, from[HD + 1], L);
+#pragma unroll
+                for (int x = 0; x < NB; x++)
+                    if (x < span) v[x] = fmaf(w, from[d0 + 32 * x], v[x]);
             }
         }
-        if (whole) write(row, x, v / L);
-        else {                                            // sums [HG][HD], then M and the weights' sum of each head
+        if (whole) {
+            const float inv = 1.0f / L;
+            const int   r = row - i * R, kvh = r / n_grp, hh = (r - kvh * n_grp) * HG + h;
+            if (hh < a.n_rep)
+#pragma unroll
+                for (int x = 0; x < NB; x++)
+                    if (x < span)
+                        ((T *)a.out)[(size_t)i * a.out_stride + (size_t)(kvh * a.n_rep + hh) * HD + d0 + 32 * x] = kv4_from<T>(v[x] * inv);
+        } else {                                          // sums [HG][HD], then M and the weights' sum of each head
             float *out = a.part + ((size_t)blockIdx.x * 2 + (first >= cu0)) * ENTRY;
-            out[x] = v;
-            if (x % HD == 0) {
+#pragma unroll
+            for (int x = 0; x < NB; x++)
+                if (x < span) out[h * HD + d0 + 32 * x] = v[x];
+            if (d0 == 0) {
                 out[HG * HD + h] = top_s[e][h];
                 out[HG * HD + HG + h] = L;
             }
