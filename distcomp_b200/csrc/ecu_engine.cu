@@ -3599,6 +3599,12 @@ extern "C" void   *ecu_batch_stream(ecu_batch *b) { return b ? (void *)b->c->str
 // positions it held before, its first row.
 struct BatchPart { int at, seq, n, past, row; const int *tok; };
 
+// Up to this many single tokens go through the projections row by row, as the
+// decode step's matrix-vector products: on the 8B shape a step takes 1.1 ms and
+// 1.8 ms a row (12 rows 22.9 ms), with the GEMMs 31 ms for 1 to 13 rows and 39
+// for 64, most of it spent on their dequantised weight operands.
+#define BT_GEMV_ROWS 16
+
 // The layers over `rows` rows of P.X: the first n_step rows are single tokens
 // of sequences with a cache, the others prompt pieces.
 static int batch_layers(ecu_batch *b, const std::vector<BatchPart> &part, int n_step, int rows)
@@ -3620,11 +3626,24 @@ static int batch_layers(ecu_batch *b, const std::vector<BatchPart> &part, int n_
     }
     const int n_prompt = (int)part.size() - n_step, prompt_rows = rows - n_step;
     if (n_prompt && hf_reserve(c, (size_t)prompt_rows * qd, (size_t)ck.back() * kvd) != 0) return -1;
+    const bool by_row = n_prompt == 0 && rows <= BT_GEMV_ROWS;
+    Launcher   L{c->stream, false};
+    auto gemv = [&](const DevMat &m, const float *x, int ldx, const float *norm, float *y, int ldy, int epi) {
+        for (int r = 0; r < rows; r++) {
+            GemvArgs a = {};
+            a.st = c->st;
+            enqueue_gemv(L, c->sms, m, x + (size_t)r * ldx, norm, g.eps, y + (size_t)r * ldy, epi, c->scr, a);
+        }
+    };
     for (size_t li = 0; li < c->layers.size(); li++) {
         LayerDev &ly = c->layers[li];
         float    *k = P.QKV + qd, *v = k + kvd;
-        k_pf_norm_split<<<rows, 256, 0, c->stream>>>(P.X, ly.attn_norm, E, g.eps, P.ah, P.al);
-        if (pf_gemm(c, ly.qkv[0], rows, P.QKV, nullptr)) return -1;
+        if (by_row) {
+            gemv(ly.qkv[0], P.X, E, ly.attn_norm, P.QKV, ldq, EPI_STORE);
+        } else {
+            k_pf_norm_split<<<rows, 256, 0, c->stream>>>(P.X, ly.attn_norm, E, g.eps, P.ah, P.al);
+            if (pf_gemm(c, ly.qkv[0], rows, P.QKV, nullptr)) return -1;
+        }
         k_bt_rope<<<rows, 128, 0, c->stream>>>(P.QKV, ldq, g.n_head, g.n_head_kv, hd, b->pos, c->rope_cs, ly.bq, ly.bk, ly.bv);
         if (n_step) {
             if (ecu_kv_append(b->kv, (int)li, ECU_F32, k, v, ldq, ldq, seq.data(), n_new.data(), n_step, ECU_F32, nullptr, nullptr,
@@ -3632,7 +3651,14 @@ static int batch_layers(ecu_batch *b, const std::vector<BatchPart> &part, int n_
                 ecu_kv_attend(b->kv, (int)li, ECU_F32, P.QKV, P.ATT, g.n_head, ldq, qd, seq.data(), n_step, scale, nullptr,
                               c->stream) != 0)
                 return -1;
-            k_pf_split<<<4 * c->sms, 256, 0, c->stream>>>(P.ATT, (size_t)n_step * qd, P.ah, P.al);
+            if (!by_row) k_pf_split<<<4 * c->sms, 256, 0, c->stream>>>(P.ATT, (size_t)n_step * qd, P.ah, P.al);
+        }
+        if (by_row) {
+            gemv(ly.o, P.ATT, qd, nullptr, P.X, E, EPI_ADD);
+            gemv(ly.gu, P.X, E, ly.ffn_norm, P.H, g.n_ff, EPI_SWIGLU);
+            gemv(ly.d, P.H, g.n_ff, nullptr, P.X, E, EPI_ADD);
+            CK(L.err);
+            continue;
         }
         if (n_prompt) {
             // the prompt attends to its keys and values as the cache holds
@@ -3660,7 +3686,7 @@ static int batch_layers(ecu_batch *b, const std::vector<BatchPart> &part, int n_
         if (pf_gemm(c, ly.d, rows, P.X, P.X)) return -1;
         CK(cudaGetLastError());
     }
-    g_launches += 14 * c->layers.size();
+    g_launches += by_row ? (uint64_t)L.count + c->layers.size() : 14 * c->layers.size();
     return 0;
 }
 

@@ -443,7 +443,8 @@ void   *ecu_batch_stream(ecu_batch *b);
  * at its end; picked[i] is the token that its last position's head picks
  * (llm_pick's rule), logits (NULL: none wanted; host, n rows of n_vocab) that
  * head's output.  The rows of all sequences go through the layers together
- * (ecu_prefill's GEMMs); a sequence with one token attends through
+ * (ecu_prefill's GEMMs; a few single tokens alone as the decode step's
+ * matrix-vector products); a sequence with one token attends through
  * ecu_kv_attend, the others through ecu_attn_prompt, all to keys and values
  * as the cache holds them, so a prompt leaves the same state however it is
  * cut.  Against the fp32 cache of ecu_forward the states differ by the

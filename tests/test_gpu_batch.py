@@ -152,6 +152,31 @@ def test_prompt_pieces_forks_and_upkeep(eng, setup):
             close(lg[i], plain.forward([tails[s][j]], caches[s])[-1])
 
 
+def test_steps_of_many_sequences(eng, setup):
+    """More single tokens than go through the projections row by row, forks of one prompt among them, and a prompt
+    in the same call."""
+    base, plain, _ = setup("mini-q4")
+    n = 20
+    b = eng.LlmBatch(base, n + 1, 60)
+    r = np.random.default_rng(5)
+    p = [int(v) for v in r.integers(3, base.n_vocab, 66)]
+    cache = {}
+    plain.forward(p, cache)
+    b.feed([0], [p])
+    b.fork([0] * (n - 1), range(1, n))
+    tok = [int(v) for v in r.integers(3, base.n_vocab, n)]
+    more = [int(v) for v in r.integers(3, base.n_vocab, 9)]
+    for seqs, toks in ((list(range(n)), [[t] for t in tok]), (list(range(n + 1)), [[t + 1] for t in tok] + [more])):
+        picked, lg = b.feed(seqs, toks, logits=True)
+        for i in (0, 1, 7, n - 1):
+            c = dict(cache)
+            if len(seqs) > n:
+                plain.forward([tok[i]], c)
+            close(lg[i], plain.forward(toks[i], c)[-1])
+            assert picked[i] == int(np.argmax(lg[i]))
+    close(lg[n], plain.forward(more)[-1])
+
+
 def test_feed_refuses_and_keeps_what_it_held(eng, setup):
     base, plain, _ = setup("mini-q4")
     b = eng.LlmBatch(base, 3, 3)
