@@ -56,7 +56,7 @@ static int make_map(CUtensorMap *m, int dtype, const void *p, int head_dim, int 
 
 template <typename T, int HD, int N>
 static int launch(const CUtensorMap (&m)[3], const PromptArgs &a, const int *cu_q, const int *cu_k, const int *order, int n,
-                  cudaStream_t s)
+                  int device, cudaStream_t s)
 {
     PromptSeqs<N> list;
     list.n = n;
@@ -73,7 +73,8 @@ static int launch(const CUtensorMap (&m)[3], const PromptArgs &a, const int *cu_
     if (ctas > INT_MAX) return say("too many rows and heads");
     list.cta[n] = (int)ctas;
     auto kern = k_attn_prompt<T, HD, N>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PaShape<HD>::smem);
+    static std::atomic<unsigned> done{0};
+    cudaError_t e = ecu_allow_smem(kern, PaShape<HD>::smem, device, done);
     if (e == cudaSuccess) {
         kern<<<(unsigned)ctas, PA_THREADS, PaShape<HD>::smem, s>>>(m[0], m[1], m[2], a, list);
         e = cudaGetLastError();
@@ -88,7 +89,7 @@ static int launch(const CUtensorMap (&m)[3], const PromptArgs &a, const int *cu_
 
 template <typename T>
 static int launch_all(const CUtensorMap (&m)[3], const PromptArgs &a, int head_dim, const int *cu_q, const int *cu_k, int n_seq,
-                      cudaStream_t s)
+                      int device, cudaStream_t s)
 {
     // sequences with query rows, the most keys first: their last tiles are the longest walks
     std::vector<int> order;
@@ -99,8 +100,8 @@ static int launch_all(const CUtensorMap (&m)[3], const PromptArgs &a, int head_d
     for (int i = 0; i < (int)order.size(); i += PA_LIST) {
         const int  c = std::min<int>(PA_LIST, (int)order.size() - i);
         const int *o = order.data() + i;
-        const int  rc = head_dim == 128 ? (c <= 32 ? launch<T, 128, 32>(m, a, cu_q, cu_k, o, c, s) : launch<T, 128, PA_LIST>(m, a, cu_q, cu_k, o, c, s))
-                                        : (c <= 32 ? launch<T, 64, 32>(m, a, cu_q, cu_k, o, c, s) : launch<T, 64, PA_LIST>(m, a, cu_q, cu_k, o, c, s));
+        const int  rc = head_dim == 128 ? (c <= 32 ? launch<T, 128, 32>(m, a, cu_q, cu_k, o, c, device, s) : launch<T, 128, PA_LIST>(m, a, cu_q, cu_k, o, c, device, s))
+                                        : (c <= 32 ? launch<T, 64, 32>(m, a, cu_q, cu_k, o, c, device, s) : launch<T, 64, PA_LIST>(m, a, cu_q, cu_k, o, c, device, s));
         if (rc != 0) return rc;
     }
     return 0;
@@ -154,8 +155,8 @@ extern "C" int ecu_attn_prompt(int dtype, const void *q, const void *k, const vo
         return -1;
     const cudaStream_t s = (cudaStream_t)stream;
     try {
-        return dtype == ECU_F16 ? launch_all<__half>(m, a, head_dim, cu_q, cu_k, n_seq, s)
-                                : launch_all<__nv_bfloat16>(m, a, head_dim, cu_q, cu_k, n_seq, s);
+        return dtype == ECU_F16 ? launch_all<__half>(m, a, head_dim, cu_q, cu_k, n_seq, device, s)
+                                : launch_all<__nv_bfloat16>(m, a, head_dim, cu_q, cu_k, n_seq, device, s);
     } catch (const std::exception &e) {
         return say(e.what());
     }

@@ -24,6 +24,10 @@
 // instead (2^x = 2^n p(f), p a polynomial fitted to the relative error: 7.5e-5
 // for bf16, whose own step is 2^-8, 2.7e-6 for fp16).
 //
+// 8192 tokens, 32 heads of 128 over 8: 554 us, 993 TFLOP/s; the walk's turn of
+// two tiles takes 1.5 times its products' time, the softmax of a tile being
+// longer than the other tile's products, and a pair 7 us beside its walk.
+//
 // Tensor memory: S of tile t at column 128 t (P in the first 32 of each 64), O at
 // 256 + HD t.  Shared memory: tiles of 128 rows of 64 elements (128 bytes,
 // 128-byte swizzle), HD / 64 of them side by side; Q and K are K-major

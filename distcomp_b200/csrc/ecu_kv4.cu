@@ -464,7 +464,8 @@ static int attend_launch(ecu_kv *kv, const KvAttendArgs &a, const int *seq, int 
     const int       grid = whole ? kv->sms : (int)std::max(1ll, std::min<long long>(kv->sms, want));
     const size_t    smem = S::smem(n);
     auto            kern = k_kv4_attend<T, NB, NT, N>;
-    CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::smem(N)));
+    static std::atomic<unsigned> done{0};
+    CK(ecu_allow_smem(kern, S::smem(N), kv->device, done));
     kern<<<grid, S::W * 32, smem, s>>>(a, list);
     return launched("ecu_kv_attend");
 }

@@ -142,8 +142,9 @@ __device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[8], unsigned m
 }
 
 // Four lanes to a block of 32 dimensions, eight values of K and of V each.
-// Bound by memory: 4 or 2 bytes a value read, 0.5625 written, and 4 or 2 where
-// the values are handed back.
+// Read are 4 or 2 bytes a value, written 0.5625, and 4 or 2 where the values
+// are handed back; what bounds it is instruction issue (39 a value): 8310 bf16
+// rows of 8 heads of 128, handed back, 28.7 us, 2.7 TB/s.
 template <typename T, typename O, int N>
 __global__ void __launch_bounds__(256) k_kv4_append(const KvAppendArgs a, const KvRows<N> rows)
 {
@@ -192,7 +193,9 @@ template <int N> struct KvUpdate {
 #define KV4_COPY_VECS 8           // 16-byte words a thread copies
 
 // Blocks below copy_blocks copy 256 * KV4_COPY_VECS words of one page of one
-// layer; the others set words.  Sources and destinations never overlap.
+// layer; the others set words.  Sources and destinations never overlap.  Bound
+// by memory: 64 pages of 32 layers (8 heads of 128) in 42 us, 7.1 TB/s of reads
+// and writes.
 template <int N>
 __global__ void __launch_bounds__(256) k_kv4_update(uint8_t *data, size_t page_bytes, size_t layer_bytes, int n_layer,
                                                     int blocks_page, unsigned copy_blocks, int *meta,
@@ -294,6 +297,10 @@ struct KvAttendArgs {
 // share is merged in shared memory, one that several CTAs share through the
 // workspace by whichever CTA ends last, in the order of the CTAs, so that the
 // result does not depend on timing.
+//
+// One sequence of 131089 positions, 8 KV heads of 128, fp32 queries: 44 us, of
+// which 26 stream the 151 MB (5.8 TB/s), bound by the instructions that unpack
+// and multiply (about 800 a unit and warp); 64 sequences of 1 to 4096: 51 us.
 #define KV4_BASE 8.0f
 #define KV4_SLACK 6.0f
 #define KV4_UNIT 32

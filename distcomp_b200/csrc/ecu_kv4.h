@@ -3,6 +3,7 @@
 #pragma once
 #include "../../include/engine_cuda.h"
 
+#include <atomic>
 #include <cuda_runtime.h>
 #include <cstdint>
 #include <map>
@@ -72,6 +73,16 @@ struct DeviceScope {
         if (old >= 0) cudaSetDevice(old);
     }
 };
+
+// A kernel's dynamic shared memory limit, set once per kernel (`done`: a bit
+// per device) on the current device `dev`.
+template <typename F> cudaError_t ecu_allow_smem(F kern, size_t bytes, int dev, std::atomic<unsigned> &done)
+{
+    if (dev < 32 && (done.load(std::memory_order_relaxed) >> dev & 1u)) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && dev < 32) done.fetch_or(1u << dev);
+    return e;
+}
 
 void ecu_count_launches(int n);       // ecu_kernel_launches()
 

@@ -43,6 +43,17 @@ def _ints(a) -> np.ndarray:
     return b
 
 
+_INT_AT = C.c_int.from_buffer
+
+
+def _at(a: np.ndarray) -> int:
+    """The address of an array's numbers."""
+    try:
+        return C.addressof(_INT_AT(a))        # a third of what a.ctypes.data takes
+    except (TypeError, ValueError):           # read-only, or empty
+        return a.ctypes.data
+
+
 def _row(t: torch.Tensor, what: str, heads: int | None, hd: int, device: int) -> tuple[int, int]:
     """(heads, row stride) of rows [n, heads, hd] or [n, heads * hd]."""
     if t.dtype not in _DTYPES or not t.is_cuda or t.get_device() != device:
@@ -63,6 +74,12 @@ def _row(t: torch.Tensor, what: str, heads: int | None, hd: int, device: int) ->
 def _current(device: int) -> int:
     """torch's current stream of a device."""
     return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _like(t: torch.Tensor, of: torch.Tensor) -> bool:
+    """Of the type, device, shape and strides of another, which has been checked."""
+    return t.dtype is of.dtype and t.shape == of.shape and t.stride() == of.stride() and t.is_cuda and \
+        t.get_device() == of.get_device()
 
 
 class _Memory:
@@ -140,7 +157,7 @@ class KvPool:
         a, b = _ints(a), _ints(b)
         if len(a) != len(b):
             raise EngineError(f"{len(a)} sequences and {len(b)} values for them")
-        if f(self.h, a.ctypes.data, b.ctypes.data, len(a), self._stream(stream)) != 0:
+        if f(self.h, _at(a), _at(b), len(a), self._stream(stream)) != 0:
             raise EngineError(last_error())
 
     def extend(self, seq, n_new, stream: int | None = None) -> None:
@@ -157,7 +174,7 @@ class KvPool:
 
     def free(self, seq, stream: int | None = None) -> None:
         a = _ints(seq)
-        if lib().ecu_kv_free(self.h, a.ctypes.data, len(a), self._stream(stream)) != 0:
+        if lib().ecu_kv_free(self.h, _at(a), len(a), self._stream(stream)) != 0:
             raise EngineError(last_error())
 
     def compact(self, stream: int | None = None) -> int:
@@ -171,25 +188,29 @@ class KvPool:
                v_out: torch.Tensor | None = None, stream: int | None = None) -> None:
         """The newest n_new[i] positions' rows of sequences seq[i] (ecu_kv_append); k_out, v_out: contiguous
         rows that receive the values as the cache holds them."""
-        _, ks = _row(k, "k", self.n_head_kv, self.head_dim, self.device)
-        _, vs = _row(v, "v", self.n_head_kv, self.head_dim, self.device)
+        heads, hd, dev = self.n_head_kv, self.head_dim, self.device
+        _, ks = _row(k, "k", heads, hd, dev)
+        vs = ks if _like(v, k) else _row(v, "v", heads, hd, dev)[1]
         n_new = _ints(n_new)
         s = None if seq is None else _ints(seq)
-        rows = int(n_new.sum(dtype=np.int64))
-        if (s is not None and len(s) != len(n_new)) or k.shape[0] != rows or v.shape[0] != rows or k.dtype != v.dtype:
+        n = len(n_new)
+        rows = sum(n_new.tolist()) if n <= 256 else int(n_new.sum(dtype=np.int64))
+        if (s is not None and len(s) != n) or k.shape[0] != rows or v.shape[0] != rows or k.dtype != v.dtype:
             raise EngineError(f"k and v: {rows} rows of one type are wanted, and a count for each sequence")
         if (k_out is None) != (v_out is None):
             raise EngineError("k_out and v_out come together")
         ko = vo = None
         od = k.dtype
         if k_out is not None:
-            for t, what in ((k_out, "k_out"), (v_out, "v_out")):
-                _row(t, what, self.n_head_kv, self.head_dim, self.device)
-                if t.shape[0] != rows or not t.is_contiguous() or t.dtype != k_out.dtype:
-                    raise EngineError(f"{what}: {rows} contiguous rows of one type are wanted")
+            _row(k_out, "k_out", heads, hd, dev)
+            if not _like(v_out, k_out):
+                _row(v_out, "v_out", heads, hd, dev)
+            if k_out.shape[0] != rows or v_out.shape[0] != rows or k_out.dtype != v_out.dtype or \
+                    not k_out.is_contiguous() or not v_out.is_contiguous():
+                raise EngineError(f"k_out and v_out: {rows} contiguous rows of one type are wanted")
             ko, vo, od = k_out.data_ptr(), v_out.data_ptr(), k_out.dtype
         if lib().ecu_kv_append(self.h, layer, _DTYPES[k.dtype], k.data_ptr(), v.data_ptr(), ks, vs,
-                               None if s is None else s.ctypes.data, n_new.ctypes.data, len(n_new), _DTYPES[od], ko, vo,
+                               None if s is None else _at(s), _at(n_new), n, _DTYPES[od], ko, vo,
                                self._stream(stream)) != 0:
             raise EngineError(last_error())
 
@@ -200,7 +221,7 @@ class KvPool:
         heads, qs = _row(q, "q", None, self.head_dim, self.device)
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _, os_ = _row(out, "out", heads, self.head_dim, self.device)
+        os_ = qs if _like(out, q) else _row(out, "out", heads, self.head_dim, self.device)[1]
         s = None if seq is None else _ints(seq)
         if out.dtype != q.dtype or out.shape[0] != q.shape[0] or (s is not None and len(s) != q.shape[0]):
             raise EngineError("out and the sequences: one for each row of q, of its type")
@@ -208,7 +229,7 @@ class KvPool:
                                ws.numel() * ws.element_size() < self.ws_bytes()):
             raise EngineError(f"ws: {self.ws_bytes()} contiguous bytes on CUDA device {self.device} are wanted")
         if lib().ecu_kv_attend(self.h, layer, _DTYPES[q.dtype], q.data_ptr(), out.data_ptr(), heads, qs, os_,
-                               None if s is None else s.ctypes.data, q.shape[0],
+                               None if s is None else _at(s), q.shape[0],
                                self.head_dim ** -0.5 if scale is None else scale,
                                None if ws is None else ws.data_ptr(), self._stream(stream)) != 0:
             raise EngineError(last_error())
@@ -250,10 +271,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q, cu
     dev, hd = q.get_device(), q.shape[2]
     heads, qs = _row(q, "q", None, hd, dev)
     kv, ks = _row(k, "k", None, hd, dev)
-    _, vs = _row(v, "v", kv, hd, dev)
+    vs = ks if _like(v, k) else _row(v, "v", kv, hd, dev)[1]
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _, os_ = _row(out, "out", heads, hd, dev)
+    os_ = qs if _like(out, q) else _row(out, "out", heads, hd, dev)[1]
     cq = _ints(cu_q)
     ck = cq if cu_k is None else _ints(cu_k)
     if q.dtype != k.dtype or q.dtype != v.dtype or q.dtype != out.dtype or out.shape[0] != q.shape[0]:
@@ -263,7 +284,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q, cu
     if stream is None:
         stream = _current(dev)
     if lib().ecu_attn_prompt(_DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), heads, kv, hd, qs,
-                             ks, vs, os_, cq.ctypes.data, ck.ctypes.data, len(cq) - 1,
+                             ks, vs, os_, _at(cq), _at(ck), len(cq) - 1,
                              hd ** -0.5 if scale is None else scale, dev, stream) != 0:
         raise EngineError(last_error())
     return out
