@@ -466,8 +466,24 @@ static int attend_launch(ecu_kv *kv, const KvAttendArgs &a, const int *seq, int 
     auto            kern = k_kv4_attend<T, NB, NT, N>;
     static std::atomic<unsigned> done{0};
     CK(ecu_allow_smem(kern, S::smem(N), kv->device, done));
-    kern<<<grid, S::W * 32, smem, s>>>(a, list);
-    return launched("ecu_kv_attend");
+    cudaLaunchConfig_t  cfg = {};
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(S::W * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, list);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        ecu_set_error(nullptr, 0, "ecu_kv_attend: launch failed: %s", cudaGetErrorString(e));
+        return -1;
+    }
+    ecu_count_launches(1);
+    return 0;
 }
 
 template <typename T, int NB, int NT>

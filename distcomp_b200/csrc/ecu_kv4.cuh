@@ -449,6 +449,10 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
     uint8_t  *ring = smem + (size_t)warp * KV4_STAGES * STAGE;
 
     if (tid < 2 * W) rid[tid] = -1;
+    // launched while what comes before it in the stream ends: nothing of that is
+    // read, and nothing written, before it has; and so for what comes next
+    pdl_wait();
+    pdl_trigger();
     // places before each sequence: a scan over the list, PER sequences a thread
     {
         constexpr int PER = (N + W * 32 - 1) / (W * 32);

@@ -37,10 +37,13 @@ def page_bytes(n_head_kv: int, head_dim: int) -> int:
 def _ints(a) -> np.ndarray:
     if type(a) is np.ndarray and a.dtype == np.int32 and a.ndim == 1 and a.flags.c_contiguous:
         return a
-    b = np.ascontiguousarray(a, dtype=np.int32)
-    if b.ndim != 1 or not np.array_equal(b, a):
-        raise EngineError("a list of whole numbers in 32 bits is wanted")
-    return b
+    try:
+        b = np.ascontiguousarray(a, dtype=np.int32)
+        if b.ndim == 1 and np.array_equal(b, a):
+            return b
+    except (OverflowError, TypeError, ValueError):
+        pass
+    raise EngineError("a list of whole numbers in 32 bits is wanted")
 
 
 _INT_AT = C.c_int.from_buffer

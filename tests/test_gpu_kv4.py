@@ -641,3 +641,68 @@ def test_prompts_then_steps():
         for i, s in enumerate(live):
             hist[s] = [np.concatenate([a, stored(b[i:i + 1])]) for a, b in zip(hist[s], (k1, v1))]
         attend_check(pool, hist, q1, live, pool.attend(0, q1, live))
+
+
+# -------------------------------------------------------------- refusals ---
+
+def test_wrappers_refuse():
+    """What only the tensors show: types, devices, shapes, strides, sizes."""
+    hd, n_kv = 64, 2
+    pool = kv4.KvPool(1, n_kv, hd, 4, 3, 2)
+    pool.extend([0, 1], [5, 70])
+    k = rows(1, 5, n_kv, hd)
+    cpu, wide = k.cpu(), rows(2, 5, n_kv, 2 * hd)
+    bad = engine.EngineError
+    for kk, vv in ((cpu, k), (k, cpu), (k.double(), k.double()), (k, k.half()), (k[:4], k[:4]), (k[:, :1], k[:, :1]),
+                   (wide[..., :hd], k), (k.transpose(0, 1), k), (k.transpose(1, 2).contiguous().transpose(1, 2), k),
+                   (k[0], k[0]), (k.flatten(1)[:, 1:], k)):
+        with pytest.raises(bad):
+            pool.append(0, kk, vv, [0], [5])
+    for seq, n_new in (([0], [5, 0]), ([0.5], [5]), ([[0]], [[5]]), ([1 << 33], [5]), ([0, 0], [3, 2]), ([2], [5])):
+        with pytest.raises(bad):
+            pool.append(0, k, k, seq, n_new)
+    out = torch.empty_like(k)
+    for ko, vo in ((out, None), (None, out), (out[:4], out[:4]), (out, out.half()), (out.cpu(), out), (wide[..., :hd], out)):
+        with pytest.raises(bad):
+            pool.append(0, k, k, [0], [5], k_out=ko, v_out=vo)
+    q = rows(3, 2, 4, hd)
+    for qq, kw in ((q.cpu(), {}), (q.double(), {}), (q[:, :3], {}), (q, {"out": q.half()}), (q, {"out": q[:1]}),
+                   (q, {"seq": [0]}), (q, {"seq": [0, 3]}), (q, {"ws": torch.zeros(8, device="cuda")}),
+                   (q, {"ws": pool.workspace().cpu()}), (q, {"scale": float("inf")}), (q[..., :32], {})):
+        with pytest.raises(bad):
+            pool.attend(0, qq, **{"seq": [0, 1], **kw})
+    for l in (-1, 1):
+        with pytest.raises(bad):
+            pool.attend(l, q, [0, 1])
+    h = rows(4, 6, 2, hd).half()
+    for a, b, c, cu, kw in ((h.cpu(), h, h, [0, 6], {}), (h.float(), h.float(), h.float(), [0, 6], {}), (h, h, h, [0, 5], {}),
+                            (h, h[:5], h, [0, 6], {}), (h, h, h.bfloat16(), [0, 6], {}), (h, h, h, [0, 6], {"cu_k": [0, 3, 6]}),
+                            (h, h, h, [], {}), (h, h, h, [0, 6], {"out": h[:5]}), (h, h, h, [0, 6], {"scale": -1.0}),
+                            (h[:, :, :32], h, h, [0, 6], {}), (h, h, h, [0, 7, 6], {})):
+        with pytest.raises(bad):
+            kv4.prompt_attention(a, b, c, cu, **kw)
+    flat = torch.zeros(6 * 2 * hd + 1, device="cuda", dtype=torch.float16)[1:].view(6, 2, hd)
+    with pytest.raises(bad, match="16-byte aligned"):
+        kv4.prompt_attention(flat, flat, flat, [0, 6])
+    with pytest.raises(bad):
+        kv4.KvPool(1, n_kv, hd, 4, 3, 2, data=torch.zeros(100, device="cuda"))
+    assert pool.length(0) == 5 and pool.used == 3
+
+
+def test_pool_over_given_memory_and_its_end():
+    """Pages in the caller's memory stay as they are; a closed pool answers with errors."""
+    hd, n_kv = 32, 1
+    data = torch.full((2, 3, kv4.page_bytes(n_kv, hd)), 7, dtype=torch.uint8, device="cuda")
+    pool = kv4.KvPool(2, n_kv, hd, 3, 2, 2, data=data)
+    assert (data == 7).all()
+    pool.extend([1], [3])
+    k = rows(1, 3, n_kv, hd)
+    pool.append(1, k, k, [1], [3])
+    assert (data[0] == 7).all() and (data[1, 1:] == 7).all() and not (data[1, 0] == 7).all()
+    pool.close()
+    pool.close()
+    for f in (pool.info, lambda: pool.length(0), lambda: pool.extend([0], [1]), lambda: pool.compact(),
+              lambda: pool.append(0, k, k, [1], [3]), lambda: pool.attend(0, k, [1, 1, 1])):
+        with pytest.raises(engine.EngineError):
+            f()
+    assert (data[0] == 7).all()
