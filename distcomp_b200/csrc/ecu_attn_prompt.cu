@@ -76,10 +76,10 @@ static int launch(const CUtensorMap (&m)[3], const PromptArgs &a, const int *cu_
     static std::atomic<unsigned> done{0};
     cudaError_t e = ecu_allow_smem(kern, PaShape<HD>::smem, device, done);
     if (e == cudaSuccess) {
-        kern<<<(unsigned)ctas, PA_THREADS, PaShape<HD>::smem, s>>>(m[0], m[1], m[2], a, list);
-        e = cudaGetLastError();
+        e = ecu_launch_early(kern, (unsigned)ctas, PA_THREADS, PaShape<HD>::smem, s, m[0], m[1], m[2], a, list);
     }
     if (e != cudaSuccess) {
+        cudaGetLastError();
         ecu_set_error(nullptr, 0, "ecu_attn_prompt: launch failed: %s", cudaGetErrorString(e));
         return -1;
     }

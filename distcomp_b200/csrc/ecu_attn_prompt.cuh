@@ -313,6 +313,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         mbar_init(&drain, 1);
         mbar_init_fence();
         any_bad = dead = 0;
+        pdl_wait();
         if (n > 0) {
             for (int t = 0; t < n_tile; t++) {
                 mbar_expect_tx(q_full + t, S::TILE);
@@ -324,6 +325,8 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         }
     }
     if (tid < 16) bad[tid >> 2][tid & 3] = 0;
+    pdl_wait();
+    pdl_trigger();
     pa_fence_before();
     __syncthreads();
     pa_fence_after();

@@ -63,10 +63,10 @@ static int capturing(cudaStream_t s, const char *what)
     return st != cudaStreamCaptureStatusNone;
 }
 
-static int launched(const char *what)
+static int launched(const char *what, cudaError_t e)
 {
-    const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) {
+        cudaGetLastError();
         ecu_set_error(nullptr, 0, "%s: launch failed: %s", what, cudaGetErrorString(e));
         return -1;
     }
@@ -94,9 +94,8 @@ template <int N> static int update_launch(ecu_kv *kv, size_t &c0, size_t &s0, cu
     s0 += u.n_set;
     const int      blocks_page = (int)((kv->page_bytes / 16 + 256 * KV4_COPY_VECS - 1) / (256 * KV4_COPY_VECS));
     const unsigned copy_blocks = (unsigned)u.n_copy * kv->n_layer * blocks_page;
-    k_kv4_update<N><<<copy_blocks + (u.n_set + 255) / 256, 256, 0, s>>>(
-        kv->data, kv->page_bytes, kv->page_bytes * B.n_pages, kv->n_layer, blocks_page, copy_blocks, kv->meta, u);
-    return launched("ecu_kv");
+    return launched("ecu_kv", ecu_launch_early(k_kv4_update<N>, copy_blocks + (u.n_set + 255) / 256, 256, 0, s, kv->data, kv->page_bytes,
+                                               kv->page_bytes * B.n_pages, kv->n_layer, blocks_page, copy_blocks, kv->meta, u));
 }
 
 // What the last operation changed, on the device.  The lists travel as kernel
@@ -283,8 +282,7 @@ static int append_launch(ecu_kv *kv, const KvAppendArgs &a, const int *seq, int 
     }
     const long long threads = (long long)r.row0[n] * a.n_kv * a.nb * 4;
     if (threads == 0) return 0;
-    k_kv4_append<T, O, N><<<(unsigned)((threads + 255) / 256), 256, 0, s>>>(a, r);
-    return launched("ecu_kv_append");
+    return launched("ecu_kv_append", ecu_launch_early(k_kv4_append<T, O, N>, (unsigned)((threads + 255) / 256), 256, 0, s, a, r));
 }
 
 template <typename T, typename O>
@@ -413,7 +411,7 @@ extern "C" int ecu_kv_read(ecu_kv *kv, int layer, int seq, int pos, int n, float
         k_kv4_read<float><<<(unsigned)((count / 8 + 255) / 256), 256, 0, s>>>(
             lay, kv->page_bytes, kv->table() + (size_t)seq * kv->book.max_pages, pos, n, kv->n_head_kv, kv->head_dim / 32,
             kv->book.n_pages, side, buf);
-        rc = launched(what);
+        rc = launched(what, cudaGetLastError());
         if (rc == 0 && (cudaMemcpyAsync(host, buf, count * sizeof(float), cudaMemcpyDeviceToHost, s) != cudaSuccess ||
                         cudaStreamSynchronize(s) != cudaSuccess)) {
             ecu_set_error(nullptr, 0, "%s: %s", what, cudaGetErrorString(cudaGetLastError()));
@@ -432,7 +430,7 @@ int ecu_kv_rows(ecu_kv *kv, int layer, int seq, int n, void *k, void *v, cudaStr
         k_kv4_read<__half><<<(unsigned)((vecs + 255) / 256), 256, 0, s>>>(
             lay, kv->page_bytes, kv->table() + (size_t)seq * kv->book.max_pages, 0, n, kv->n_head_kv, kv->head_dim / 32,
             kv->book.n_pages, side, (__half *)(side ? v : k));
-        if (launched("ecu_kv_rows") != 0) return -1;
+        if (launched("ecu_kv_rows", cudaGetLastError()) != 0) return -1;
     }
     return 0;
 }
@@ -466,24 +464,7 @@ static int attend_launch(ecu_kv *kv, const KvAttendArgs &a, const int *seq, int 
     auto            kern = k_kv4_attend<T, NB, NT, N>;
     static std::atomic<unsigned> done{0};
     CK(ecu_allow_smem(kern, S::smem(N), kv->device, done));
-    cudaLaunchConfig_t  cfg = {};
-    cudaLaunchAttribute early;
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(S::W * 32);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cfg.attrs = &early;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, list);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        ecu_set_error(nullptr, 0, "ecu_kv_attend: launch failed: %s", cudaGetErrorString(e));
-        return -1;
-    }
-    ecu_count_launches(1);
-    return 0;
+    return launched("ecu_kv_attend", ecu_launch_early(kern, (unsigned)grid, S::W * 32, smem, s, a, list));
 }
 
 template <typename T, int NB, int NT>

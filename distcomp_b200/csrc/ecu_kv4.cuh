@@ -148,6 +148,8 @@ __device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[8], unsigned m
 template <typename T, typename O, int N>
 __global__ void __launch_bounds__(256) k_kv4_append(const KvAppendArgs a, const KvRows<N> rows)
 {
+    pdl_wait();
+    pdl_trigger();
     const unsigned per_row = a.n_kv * a.nb;                      // blocks of a row
     const unsigned blk = (blockIdx.x * 256u + threadIdx.x) >> 2; // below 2^31: the host sees to it
     const int      c = threadIdx.x & 3, r = (int)(blk / per_row);
@@ -201,6 +203,8 @@ __global__ void __launch_bounds__(256) k_kv4_update(uint8_t *data, size_t page_b
                                                     int blocks_page, unsigned copy_blocks, int *meta,
                                                     const KvUpdate<N> u)
 {
+    pdl_wait();
+    pdl_trigger();
     if (blockIdx.x >= copy_blocks) {
         const int i = (int)(blockIdx.x - copy_blocks) * 256 + (int)threadIdx.x;
         if (i < u.n_set) meta[u.a[u.n_copy + i]] = u.b[u.n_copy + i];
@@ -449,8 +453,6 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
     uint8_t  *ring = smem + (size_t)warp * KV4_STAGES * STAGE;
 
     if (tid < 2 * W) rid[tid] = -1;
-    // launched while what comes before it in the stream ends: nothing of that is
-    // read, and nothing written, before it has; and so for what comes next
     pdl_wait();
     pdl_trigger();
     // places before each sequence: a scan over the list, PER sequences a thread

@@ -84,6 +84,24 @@ template <typename F> cudaError_t ecu_allow_smem(F kern, size_t bytes, int dev, 
     return e;
 }
 
+// A launch that may begin while what comes before it in the stream ends (the
+// kernel waits for that itself, pdl_wait, before it touches global memory).
+template <typename... P, typename... A>
+cudaError_t ecu_launch_early(void (*kern)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t s, const A &...args)
+{
+    cudaLaunchConfig_t  cfg = {};
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
 void ecu_count_launches(int n);       // ecu_kernel_launches()
 
 // Positions 0..n-1 of a sequence as fp16 rows [n][n_head_kv * head_dim] in
