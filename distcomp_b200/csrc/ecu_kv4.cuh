@@ -144,7 +144,7 @@ __device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[8], unsigned m
 // Four lanes to a block of 32 dimensions, eight values of K and of V each.
 // Read are 4 or 2 bytes a value, written 0.5625, and 4 or 2 where the values
 // are handed back; what bounds it is instruction issue (39 a value): 8310 bf16
-// rows of 8 heads of 128, handed back, 28.7 us, 2.7 TB/s.
+// rows of 8 heads of 128, handed back, 26 us, 3.0 TB/s.
 template <typename T, typename O, int N>
 __global__ void __launch_bounds__(256) k_kv4_append(const KvAppendArgs a, const KvRows<N> rows)
 {
@@ -302,9 +302,9 @@ struct KvAttendArgs {
 // workspace by whichever CTA ends last, in the order of the CTAs, so that the
 // result does not depend on timing.
 //
-// One sequence of 131089 positions, 8 KV heads of 128, fp32 queries: 44 us, of
+// One sequence of 131089 positions, 8 KV heads of 128, fp32 queries: 43 us, of
 // which 26 stream the 151 MB (5.8 TB/s), bound by the instructions that unpack
-// and multiply (about 800 a unit and warp); 64 sequences of 1 to 4096: 51 us.
+// and multiply (about 800 a unit and warp); 64 sequences of 1 to 4096: 50 us.
 #define KV4_BASE 8.0f
 #define KV4_SLACK 6.0f
 #define KV4_UNIT 32

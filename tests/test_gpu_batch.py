@@ -23,8 +23,8 @@ REL = 1e-2
 class Plain:
     """A llama forward in 64 bits; 4-bit keys and values unless told otherwise."""
 
-    def __init__(self, key, buf, port, four_bits=True):
-        self.s, self.port, self.four = synth.spec(key), port, four_bits
+    def __init__(self, spec, buf, port, four_bits=True):
+        self.s, self.port, self.four = spec, port, four_bits
         self.tab = G.read_tensor_table(buf)
         self.dims = {name: (dims, t) for name, dims, t in synth.tensor_list(self.s)}
         self.w = {}
@@ -63,6 +63,8 @@ class Plain:
         for l in range(s.n_layer):
             y = norm(x) * self.weight(f"blk.{l}.attn_norm.weight")
             q, k, v = (y @ self.weight(f"blk.{l}.attn_{n}.weight").T for n in "qkv")
+            if s.qkv_bias:
+                q, k, v = (x + self.weight(f"blk.{l}.attn_{n}.bias") for x, n in zip((q, k, v), "qkv"))
             q, k, v = turn(q.reshape(-1, H, hd)), turn(k.reshape(-1, KV, hd)), v.reshape(-1, KV, hd)
             for n, r in (("k", k), ("v", v)):
                 old = cache.get((l, n))
@@ -78,7 +80,7 @@ class Plain:
             y = norm(x) * self.weight(f"blk.{l}.ffn_norm.weight")
             g, u = y @ self.weight(f"blk.{l}.ffn_gate.weight").T, y @ self.weight(f"blk.{l}.ffn_up.weight").T
             x = x + (g / (1 + np.exp(-g)) * u) @ self.weight(f"blk.{l}.ffn_down.weight").T
-        return (norm(x) * self.weight("output_norm.weight")) @ self.weight("output.weight").T
+        return (norm(x) * self.weight("output_norm.weight")) @ self.weight("token_embd.weight" if s.tied else "output.weight").T
 
 
 def close(got, want, rel=REL):
@@ -89,10 +91,10 @@ def close(got, want, rel=REL):
 
 @pytest.fixture(scope="module")
 def setup(eng, oracle_port, model_buf):
-    def get(key):
-        buf = model_buf(key)
+    def get(key, **over):
+        buf, spec = model_buf(key, **over), synth.spec(key, **over)
         base = eng.LlmCtx(eng.GgufModel(buf), eng.STAGE_FULL)
-        return base, Plain(key, buf, oracle_port), Plain(key, buf, oracle_port, four_bits=False)
+        return base, Plain(spec, buf, oracle_port), Plain(spec, buf, oracle_port, four_bits=False)
     return get
 
 
@@ -119,6 +121,23 @@ def test_feed_matches_the_plain_forward(eng, setup, key):
         for i in range(3):
             close(lg[i], plain.forward(nxt[i], caches[i])[-1])
     assert [b.length(s) for s in (2, 0, 1, 3)] == [60, 29, 37, 0]
+
+
+def test_biases_and_a_tied_head(eng, setup):
+    """A qwen2-style model: Q/K/V biases, the embedding as the head; prompts, and few and many steps."""
+    base, plain, _ = setup("mini-q8", arch="qwen2", qkv_bias=True, tied=True)
+    n = 18
+    b = eng.LlmBatch(base, n, 40)
+    r = np.random.default_rng(8)
+    text = [[int(v) for v in r.integers(3, base.n_vocab, 2 + i)] for i in range(n)]
+    caches = [{} for _ in text]
+    for seqs in (range(n), range(n), range(3)):
+        toks = [text[i] for i in seqs]
+        picked, lg = b.feed(list(seqs), toks, logits=True)
+        for i in seqs:
+            want = plain.forward(toks[i], caches[i])[-1]
+            close(lg[i], want)
+            text[i] = [picked[i]]
 
 
 def test_prompt_pieces_forks_and_upkeep(eng, setup):
