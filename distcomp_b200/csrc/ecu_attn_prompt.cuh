@@ -206,30 +206,25 @@ __device__ __forceinline__ float pa_max3(float a, float b, float c)
     return r;
 }
 
-// 2^t of two values on the FMA units: t = n + f with |f| <= 1/2, n added to the
-// polynomial's exponent.  t is held at -126, where P rounds to nothing.
-template <int DEG> __device__ __forceinline__ void pa_ex2_fma(uint64_t t2, float &e0, float &e1)
+// 2^t on the FMA units: t = n + f with |f| <= 1/2, n added to the polynomial's
+// exponent.  t is held at -126, where P rounds to nothing.
+template <int DEG> __device__ __forceinline__ float pa_ex2_fma(float t)
 {
-    float t0, t1, r0, r1, p0, p1;
-    pa_untwo(t2, t0, t1);
-    const uint64_t t = pa_two(fmaxf(t0, -126.0f), fmaxf(t1, -126.0f));
-    const uint64_t r = pa_add2(t, pa_two(12582912.0f, 12582912.0f));                   // 1.5 * 2^23: n in the low bits
-    const uint64_t f = pa_fma2(pa_add2(r, pa_two(-12582912.0f, -12582912.0f)), pa_two(-1.0f, -1.0f), t);
-    uint64_t       p;
+    t = fmaxf(t, -126.0f);
+    const float r = __fadd_rn(t, 12582912.0f);                   // 1.5 * 2^23: n in the low bits
+    const float f = __fsub_rn(t, __fsub_rn(r, 12582912.0f));
+    float       p;
     if (DEG == 3) {
-        p = pa_fma2(f, pa_two(0.055171668529510498f, 0.055171668529510498f), pa_two(0.24261112511157990f, 0.24261112511157990f));
-        p = pa_fma2(f, p, pa_two(0.69326096773147583f, 0.69326096773147583f));
-        p = pa_fma2(f, p, pa_two(0.99992805719375610f, 0.99992805719375610f));
+        p = fmaf(f, 0.055171668529510498f, 0.24261112511157990f);
+        p = fmaf(f, p, 0.69326096773147583f);
+        p = fmaf(f, p, 0.99992805719375610f);
     } else {
-        p = pa_fma2(f, pa_two(0.0095701021f, 0.0095701021f), pa_two(0.0559178628f, 0.0559178628f));
-        p = pa_fma2(f, p, pa_two(0.2402474433f, 0.2402474433f));
-        p = pa_fma2(f, p, pa_two(0.6931217909f, 0.6931217909f));
-        p = pa_fma2(f, p, pa_two(0.9999992847f, 0.9999992847f));
+        p = fmaf(f, 0.0095701021f, 0.0559178628f);
+        p = fmaf(f, p, 0.2402474433f);
+        p = fmaf(f, p, 0.6931217909f);
+        p = fmaf(f, p, 0.9999992847f);
     }
-    pa_untwo(r, r0, r1);
-    pa_untwo(p, p0, p1);
-    e0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(r0) << 23));
-    e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(r1) << 23));
+    return __uint_as_float(__float_as_uint(p) + (__float_as_uint(r) << 23));
 }
 
 // Does any of the 64 threads at barrier `id` say so?
@@ -506,9 +501,11 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                         const uint32_t *v = &s[2 * h + (x >> 3)][2 * (x & 7)];
                         const uint64_t  t2 = pa_fma2(pa_two(__uint_as_float(v[0]), __uint_as_float(v[1])), sl2, mb2);
                         float           e0, e1;
-                        if (x % PA_FMA == PA_FMA - 1) pa_ex2_fma<PaBits<T>::fmt ? 3 : 4>(t2, e0, e1);
-                        else {
-                            pa_untwo(t2, e0, e1);
+                        pa_untwo(t2, e0, e1);
+                        if (x % PA_FMA == PA_FMA - 1) {
+                            e0 = pa_ex2_fma<PaBits<T>::fmt ? 3 : 4>(e0);
+                            e1 = pa_ex2_fma<PaBits<T>::fmt ? 3 : 4>(e1);
+                        } else {
                             e0 = kv4_ex2(e0);
                             e1 = kv4_ex2(e1);
                         }
