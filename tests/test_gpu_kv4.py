@@ -8,7 +8,7 @@ Tolerances, from the arithmetic (h = half a step of a type, relative):
     are at most A = max_t sum_d |q_d k_td|; the split of an fp32 query leaves
     2^-22 of its largest element, 2^-22 * A at most counted twice.  With the
     scale and the base-2 exponential (2^-21 relative each):
-    ds = scale * A * 2^-23 * (hd / 2 + 16) + 2^-20;
+    ds = |scale| * A * 2^-23 * (hd / 2 + 16) + 2^-20;
   * a weight is then off by 2 * ds (numerator and sum), a sum of n weighted
     rows by 2^-23 * (n / 16 + 64): both times max |v|;
   * 16-bit forms round weights once more before their product with V: h of
@@ -100,7 +100,7 @@ def reference(q, k, v, scale, ds_extra, hw, hout, causal_from=None):
         kh, vh = k[:, h // (H // kv)], v[:, h // (H // kv)]
         s = q[:, h] @ kh.T * scale
         A = np.max(np.abs(q[:, h]) @ np.abs(kh).T, axis=1, initial=0.0)
-        ds = scale * A * 2.0 ** -23 * (hd / 2 + 16) + 2.0 ** -20
+        ds = abs(scale) * A * 2.0 ** -23 * (hd / 2 + 16) + 2.0 ** -20
         seen = np.full(r, n) if causal_from is None else np.maximum(0, causal_from + np.arange(r))
         s = np.where(np.arange(n)[None] < seen[:, None], s, -np.inf)
         live = seen > 0
@@ -282,6 +282,35 @@ def test_attend_long(n_kv, rep, lens, dtype):
     attend_check(pool, vals, q, range(len(lens)), out)
     for _ in range(3):                               # the same bits whatever the order in which the CTAs end
         assert torch.equal(pool.attend(0, q), out)
+
+
+@pytest.mark.parametrize("hd, rep", [(32, 3), (64, 8), (96, 5), (96, 1), (128, 9)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_attend_long_other_shapes(hd, rep, dtype):
+    """Rows across many CTAs at every head size, padded head groups, and a negative scale."""
+    lens = [9001, 40, 3000]
+    pool, vals = filled(1, hd, lens, seed=hd)
+    q = rows(8, 3, rep, hd).to(dtype)
+    for scale in (hd ** -0.5, -0.05):
+        attend_check(pool, vals, q, [2, 0, 1], pool.attend(0, q, [2, 0, 1], scale=scale), scale=scale)
+
+
+def test_attend_zero_and_tiny_rows():
+    """Keys, values or queries of zeros, and V scales from fp16's smallest to its largest, in one sequence."""
+    hd, n = 64, 300
+    pool = kv4.KvPool(1, 1, hd, 6, 2, 5)
+    k, v = rows(1, n, 1, hd), rows(2, n, 1, hd)
+    k[:64], v[32:96] = 0, 0
+    v[128:160] *= 1e-6
+    v[200:210] *= 3e4
+    pool.extend([0, 1], [n, 33])
+    pool.append(0, torch.cat([k, torch.zeros(33, 1, hd, device="cuda")]), torch.cat([v, torch.zeros(33, 1, hd, device="cuda")]),
+                [0, 1], [n, 33])
+    q = rows(3, 2, 2, hd)
+    q[:, 1] = 0
+    out = pool.attend(0, q)
+    assert (out[1] == 0).all()
+    attend_check(pool, [(stored(k), stored(v))], q[:1], [0], out[:1])
 
 
 def test_attend_many_short():
