@@ -207,12 +207,14 @@ __device__ __forceinline__ float pa_max3(float a, float b, float c)
 }
 
 // 2^t on the FMA units: t = n + f with |f| <= 1/2, n added to the polynomial's
-// exponent.  t is held at -126, where P rounds to nothing.
+// exponent.  Below -126 it is zero, as ex2's: what a row does not see has
+// t = -inf, and 2^-126 times a large bf16 value would count.  So the result is
+// formed 2^64 too large, with t held at -190, and the last product flushes it.
 template <int DEG> __device__ __forceinline__ float pa_ex2_fma(float t)
 {
-    t = fmaxf(t, -126.0f);
-    const float r = __fadd_rn(t, 12582912.0f);                   // 1.5 * 2^23: n in the low bits
-    const float f = __fsub_rn(t, __fsub_rn(r, 12582912.0f));
+    t = fmaxf(t, -190.0f);
+    const float r = __fadd_rn(t, 12582976.0f);                   // 1.5 * 2^23 + 64: n + 64 in the low bits
+    const float f = __fsub_rn(t, __fsub_rn(r, 12582976.0f));
     float       p;
     if (DEG == 3) {
         p = fmaf(f, 0.055171668529510498f, 0.24261112511157990f);
@@ -224,7 +226,9 @@ template <int DEG> __device__ __forceinline__ float pa_ex2_fma(float t)
         p = fmaf(f, p, 0.6931217909f);
         p = fmaf(f, p, 0.9999992847f);
     }
-    return __uint_as_float(__float_as_uint(p) + (__float_as_uint(r) << 23));
+    float y;
+    asm("mul.ftz.f32 %0, %1, 0f1F800000;" : "=f"(y) : "f"(__uint_as_float(__float_as_uint(p) + (__float_as_uint(r) << 23))));
+    return y;
 }
 
 // Does any of the 64 threads at barrier `id` say so?
@@ -490,7 +494,8 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                             pa_st16(to + HD / 2 * hf + c, o);
                         }
                 }
-                const float    mb = m == -INFINITY ? 0.0f : m * sl;
+                // (an infinite maximum, or product with the scale, makes the row NaN in every weight)
+                const float    mb = m == -INFINITY ? 0.0f : fmaf(m * sl, 0.0f, m * sl);
                 const uint64_t sl2 = pa_two(sl, sl), mb2 = pa_two(-mb, -mb);
                 uint64_t       sum[2] = {pa_two(0.0f, 0.0f), pa_two(0.0f, 0.0f)};
 #pragma unroll

@@ -417,8 +417,10 @@ int    ecu_kv_read(ecu_kv *kv, int layer, int seq, int pos, int n, float *k, flo
  * `dtype` (ECU_F16 or ECU_BF16), 16-byte aligned, a row's heads one after the
  * other, rows a multiple of 8 elements apart; head_dim 64 or 128; scale > 0.  What lies
  * behind the last row, or in keys that a row does not see (NaN and infinities
- * too), has no effect.  Sums and the softmax are fp32; the weights are
- * rounded to `dtype` before their product with V. */
+ * too), has no effect.  Sums and the softmax are fp32, relative to weights of
+ * up to 2^8 (bf16 values near 2^127 / 2^8 / keys can pass fp32's range); the
+ * weights are rounded to `dtype` before their product with V.  out overlaps
+ * none of the others. */
 int  ecu_attn_prompt(int dtype, const void *q, const void *k, const void *v, void *out, int n_head, int n_head_kv,
                      int head_dim, long q_stride, long k_stride, long v_stride, long out_stride, const int *cu_q,
                      const int *cu_k, int n_seq, float scale, int device, void *stream);

@@ -590,6 +590,60 @@ def test_prompt_masked_places_have_no_effect(hd, bad):
         assert (out[60:100, 0, 5] == bad).all() and out[169, 1, 7] == bad
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prompt_masked_places_of_the_largest_values(hd, dtype):
+    """The largest finite keys and values in masked places, one of them at every place of a tile, weigh nothing."""
+    n, big = 300, torch.finfo(dtype).max
+    q, k, v = rows(1, n, 2, hd).to(dtype), rows(2, n, 2, hd).to(dtype), rows(3, n, 2, hd).to(dtype)
+    want = kv4.prompt_attention(q, k, v, [0, n])
+    for first in (40, 150):
+        k2, v2 = k.clone(), v.clone()
+        k2[first:] = big
+        v2[first:] = -big
+        assert torch.equal(kv4.prompt_attention(q, k2, v2, [0, n])[:first], want[:first])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prompt_weights_that_vanish(dtype):
+    """A key 2^369 ahead of all the others: their values, however large, add nothing.  The key lies at every place.
+    (Where it comes in the second tile of 128 keys, the first one's sum comes before it: 128 of the largest bf16
+    values, 2^135, are past fp32, so they are 2^100 there.)"""
+    n, hd = 200, 64
+    q = torch.zeros(n, 1, hd, device="cuda", dtype=dtype)
+    k = torch.zeros(n * n, 1, hd, device="cuda", dtype=dtype)
+    v = torch.full((n * n, 1, hd), torch.finfo(dtype).max, device="cuda", dtype=dtype)
+    at = torch.arange(n, device="cuda") * (n + 1)
+    q[:, 0, 0] = 16
+    k[at, 0, 0] = 16
+    if dtype is torch.bfloat16:
+        v[128 * n:] = 2.0 ** 100
+    v[at] = 1
+    out = kv4.prompt_attention(q, k, v, range(n + 1), range(0, n * n + 1, n), scale=1.0)
+    assert (out == 1).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prompt_infinite_scores(dtype):
+    """A score of -inf weighs nothing; of +inf, or -inf alone, the softmax is NaN.  At every place of a tile."""
+    n, hd = 200, 64
+    cu_q, cu_k = range(n + 1), range(0, n * n + 1, n)
+    q, k, v = rows(1, n, 1, hd), rows(2, n * n, 1, hd), rows(3, n * n, 1, hd).to(dtype)
+    q[:, 0, 0] = q[:, 0, 0].abs() + 0.5
+    q, k = q.to(dtype), k.to(dtype)
+    at = torch.arange(n, device="cuda") * (n + 1)
+    k[at, 0, 0] = float("inf")
+    assert torch.isnan(kv4.prompt_attention(q, k, v, cu_q, cu_k)).all()
+    k[at, 0, 0] = float("-inf")
+    v[at] = torch.finfo(dtype).max
+    out = kv4.prompt_attention(q, k, v, cu_q, cu_k)
+    rest = torch.ones(n * n, dtype=torch.bool, device="cuda")
+    rest[at] = False
+    prompt_check(q, k[rest], v[rest], out, list(cu_q), list(range(0, n * (n - 1) + 1, n - 1)))
+    k[:, 0, 0] = float("-inf")
+    assert torch.isnan(kv4.prompt_attention(q, k, v, cu_q, cu_k)).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_prompt_large_scores(dtype):
     """Scores in the hundreds, one key that takes all, rows of equal scores."""
