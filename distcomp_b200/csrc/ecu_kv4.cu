@@ -21,6 +21,7 @@
     } while (0)
 
 #define KV4_LIST 1024             // sequences of one launch
+#define KV4_STREAMS 16            // streams that a pool keeps a workspace for
 
 static bool shape_ok(int n_head_kv, int head_dim)
 {
@@ -115,8 +116,16 @@ static int change_ok(ecu_kv *kv, const void *list, const void *list2, int n, cud
 {
     if (!kv || n < 0 || (n > 0 && (!list || !list2))) return say(what, "null argument or negative count");
     if (kv->device < 0) return 0;
+    // a launch that failed later would leave the bookkeeping ahead of the device
+    DeviceScope d(kv->device);
+    if (!d.ok) return say(what, "the pool's device cannot be used");
     const int c = capturing(s, what);
     if (c > 0) return say(what, "the pool's bookkeeping cannot be captured");
+    int dev = -1;
+    if (c == 0 && (cudaStreamGetDevice(s, &dev) != cudaSuccess || dev != kv->device)) {
+        cudaGetLastError();
+        return say(what, "the stream is not one of the pool's device");
+    }
     return c;
 }
 
@@ -156,6 +165,11 @@ int ecu_kv_open(ecu_kv **out, int n_layer, int n_head_kv, int head_dim, int n_pa
         ecu_set_error(err, errlen, "a pool of %d layers, %d pages, %d sequences of %d pages", n_layer, n_pages, n_seq, max_pages);
         return -1;
     }
+    size_t bytes = 0;
+    if (__builtin_mul_overflow(ecu_kv4_page_bytes(n_head_kv, head_dim), (size_t)n_pages * n_layer, &bytes)) {
+        ecu_set_error(err, errlen, "a pool of %d layers of %d pages is too large", n_layer, n_pages);
+        return -1;
+    }
     if (data && ((uintptr_t)data & 15)) { ecu_set_error(err, errlen, "the pages' memory is not 16-byte aligned"); return -1; }
     try {
         std::unique_ptr<ecu_kv, void (*)(ecu_kv *)> kv(new ecu_kv(), ecu_kv_close);
@@ -176,7 +190,7 @@ int ecu_kv_open(ecu_kv **out, int n_layer, int n_head_kv, int head_dim, int n_pa
             kv->device = device;
             cudaDeviceGetAttribute(&kv->sms, cudaDevAttrMultiProcessorCount, device);
             kv->sms = std::min(kv->sms, KV4_MAX_CTAS);
-            const size_t words = (size_t)n_seq * max_pages + n_seq, bytes = kv->page_bytes * n_pages * n_layer;
+            const size_t words = (size_t)n_seq * max_pages + n_seq;
             void *p = nullptr;
             if (cudaMalloc(&p, words * sizeof(int)) == cudaSuccess) {
                 kv->meta = (int *)p;
@@ -517,7 +531,7 @@ extern "C" int ecu_kv_attend(ecu_kv *kv, int layer, int dtype, const void *q, vo
     }
     const size_t es = dtype_bytes(dtype);
     if (!es) return say(what, "unknown element type");
-    if (n_head < 1 || n_head % kv->n_head_kv || n_head / kv->n_head_kv > 4096) {
+    if (n_head < 1 || n_head % kv->n_head_kv || n_head / kv->n_head_kv > 4096 || n_head > INT_MAX / kv->head_dim) {
         ecu_set_error(nullptr, 0, "%s: %d query heads for %d KV heads", what, n_head, kv->n_head_kv);
         return -1;
     }
@@ -537,10 +551,24 @@ extern "C" int ecu_kv_attend(ecu_kv *kv, int layer, int dtype, const void *q, vo
     if (!ws) {
         if (cap) return say(what, "a captured call needs a workspace of its own");
         try {
-            void *&own = kv->ws[stream];
+            unsigned long long id = 0;
+            CK(cudaStreamGetId(s, &id));
+            const size_t bytes = ecu_kv_ws_bytes(kv);
+            if (kv->ws.size() >= KV4_STREAMS && !kv->ws.count(id)) {        // streams come and go: start over
+                CK(cudaDeviceSynchronize());
+                for (auto &w : kv->ws) {
+                    if (!w.second) continue;
+                    if (!kv->spare) std::swap(kv->spare, w.second);
+                    else {
+                        cudaFree(w.second);
+                        kv->device_bytes -= bytes;
+                    }
+                }
+                kv->ws.clear();
+            }
+            void *&own = kv->ws[id];
             if (!own) std::swap(own, kv->spare);
             if (!own) {
-                const size_t bytes = ecu_kv_ws_bytes(kv);
                 void        *p = nullptr;
                 CK(cudaMalloc(&p, bytes));
                 cudaMemset(p, 0, bytes);

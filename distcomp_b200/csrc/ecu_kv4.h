@@ -53,7 +53,9 @@ struct ecu_kv {
     bool     own_data = false;
     int     *meta = nullptr;          // device: table, then len
     KvBook   book;
-    std::map<void *, void *> ws;      // stream -> its attention workspace
+    // a stream's id -> its attention workspace (handles are reused, and the
+    // per-thread default stream's names another stream in each thread)
+    std::map<unsigned long long, void *> ws;
     void *spare = nullptr;            // the first stream's, allocated with the pool
     int *table() const { return meta; }
     int *len() const { return meta ? meta + (size_t)book.n_seq * book.max_pages : nullptr; }

@@ -50,6 +50,19 @@ class EcuKprof(C.Structure):
                 ("bytes_per_launch", C.c_double)]
 
 
+def int_list(a) -> np.ndarray:
+    """A list or array as C ints; one of other values, or of more dimensions, is refused."""
+    if type(a) is np.ndarray and a.dtype == np.int32 and a.ndim == 1 and a.flags.c_contiguous:
+        return a
+    try:
+        b = np.ascontiguousarray(a, dtype=np.int32)
+        if b.ndim == 1 and np.array_equal(b, a):
+            return b
+    except (OverflowError, TypeError, ValueError):
+        pass
+    raise EngineError("a list of whole numbers in 32 bits is wanted")
+
+
 class EcuKvInfo(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("n_layer", "n_head_kv", "head_dim", "n_pages", "n_seq", "max_pages", "device",
                                        "used")] + [("page_bytes", C.c_size_t), ("device_bytes", C.c_size_t),
@@ -451,21 +464,29 @@ class LlmBatch:
 
     def __init__(self, base: LlmCtx, n_seq: int, n_pages: int):
         self.h = C.c_void_p()
+        int_list([n_seq, n_pages])
         err = C.create_string_buffer(512)
         if lib().ecu_batch_open(C.byref(self.h), base.h, int(n_seq), int(n_pages), err, 512) != 0:
             raise EngineError(err.value.decode(errors="replace") or last_error())
         self.n_vocab = base.n_vocab
-        self.kv = C.c_void_p(lib().ecu_batch_kv(self.h))
+        self._kv = C.c_void_p(lib().ecu_batch_kv(self.h))
         self.stream = C.c_void_p(lib().ecu_batch_stream(self.h))
+
+    @property
+    def kv(self) -> C.c_void_p:
+        """The batch's pool (ecu_kv)."""
+        if not self.h:
+            raise EngineError("the batch is closed")
+        return self._kv
 
     def feed(self, seq, tokens, logits: bool = False):
         """Each sequence's next tokens (a list of them per sequence); the picked token of each, and with
         logits=True its head's output [n, n_vocab]."""
-        s = np.ascontiguousarray(seq, dtype=np.int32)
+        s = int_list(seq)
         if len(s) != len(tokens):
             raise EngineError(f"{len(s)} sequences and {len(tokens)} lists of tokens")
         cnt = np.array([len(t) for t in tokens], dtype=np.int32)
-        tok = np.concatenate([np.asarray(t, dtype=np.int32) for t in tokens]) if len(s) else np.zeros(0, np.int32)
+        tok = np.concatenate([int_list(t) for t in tokens]) if len(s) else np.zeros(0, np.int32)
         out = np.zeros(len(s), dtype=np.int32)
         lg = np.empty((len(s), self.n_vocab), dtype=np.float32) if logits else None
         if lib().ecu_batch_feed(self.h, _ptr(s), _ptr(cnt), len(s), _ptr(tok), _ptr(out), None if lg is None else _ptr(lg)) != 0:
@@ -474,7 +495,7 @@ class LlmBatch:
         return (picked, lg) if logits else picked
 
     def _list(self, f, a, b) -> None:
-        a, b = np.ascontiguousarray(a, dtype=np.int32), np.ascontiguousarray(b, dtype=np.int32)
+        a, b = int_list(a), int_list(b)
         if a.shape != b.shape:
             raise EngineError(f"lists of {a.size} and {b.size}")
         if f(self.kv, _ptr(a), _ptr(b), a.size, self.stream) != 0:
@@ -488,7 +509,7 @@ class LlmBatch:
         self._list(lib().ecu_kv_truncate, seq, length)
 
     def free(self, seq) -> None:
-        a = np.ascontiguousarray(seq, dtype=np.int32)
+        a = int_list(seq)
         if lib().ecu_kv_free(self.kv, _ptr(a), a.size, self.stream) != 0:
             raise EngineError(last_error())
 
@@ -499,6 +520,7 @@ class LlmBatch:
         return n
 
     def length(self, seq: int) -> int:
+        int_list([seq])
         n = int(lib().ecu_kv_len(self.kv, int(seq), None, 0))
         if n < 0:
             raise EngineError(last_error())

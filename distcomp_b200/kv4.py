@@ -23,7 +23,7 @@ import ctypes as C
 import numpy as np
 import torch
 
-from .engine import EcuKvInfo, EngineError, last_error, lib
+from .engine import EcuKvInfo, EngineError, int_list as _ints, last_error, lib
 
 PAGE = 64
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -31,19 +31,8 @@ _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 def page_bytes(n_head_kv: int, head_dim: int) -> int:
     """Bytes of one page of one layer (0: a shape that is not covered)."""
+    _ints([n_head_kv, head_dim])
     return int(lib().ecu_kv4_page_bytes(n_head_kv, head_dim))
-
-
-def _ints(a) -> np.ndarray:
-    if type(a) is np.ndarray and a.dtype == np.int32 and a.ndim == 1 and a.flags.c_contiguous:
-        return a
-    try:
-        b = np.ascontiguousarray(a, dtype=np.int32)
-        if b.ndim == 1 and np.array_equal(b, a):
-            return b
-    except (OverflowError, TypeError, ValueError):
-        pass
-    raise EngineError("a list of whole numbers in 32 bits is wanted")
 
 
 _INT_AT = C.c_int.from_buffer
@@ -103,6 +92,7 @@ class KvPool:
         the pool as long as it lives), else the pool allocates it.  device -1:
         the bookkeeping alone."""
         self.h = C.c_void_p()
+        _ints([n_layer, n_head_kv, head_dim, n_pages, n_seq, max_pages, device])      # (ctypes drops higher bits)
         if data is not None:
             want = n_layer * n_pages * page_bytes(n_head_kv, head_dim)
             if device < 0 or not data.is_cuda or data.get_device() != device or not data.is_contiguous() or \
@@ -133,14 +123,17 @@ class KvPool:
     @property
     def table(self) -> torch.Tensor:
         """The device's page ids [n_seq, max_pages], -1 where there is none (a view: for reading)."""
+        self.info()
         return torch.as_tensor(_Memory(self._table, (self.n_seq, self.max_pages), self), device=f"cuda:{self.device}")
 
     @property
     def lengths(self) -> torch.Tensor:
         """The device's positions of each sequence [n_seq] (a view: for reading)."""
+        self.info()
         return torch.as_tensor(_Memory(self._len, (self.n_seq,), self), device=f"cuda:{self.device}")
 
     def length(self, seq: int) -> int:
+        _ints([seq])
         n = int(lib().ecu_kv_len(self.h, int(seq), None, 0))
         if n < 0:
             raise EngineError(last_error())
@@ -150,6 +143,11 @@ class KvPool:
         buf = np.zeros((self.length(seq) + PAGE - 1) // PAGE, dtype=np.int32)
         lib().ecu_kv_len(self.h, int(seq), buf.ctypes.data, len(buf))
         return [int(p) for p in buf]
+
+    def _layer(self, layer: int) -> int:
+        if not 0 <= layer < self.n_layer:
+            raise EngineError(f"layer {layer} of {self.n_layer}")
+        return layer
 
     def _stream(self, stream):
         if stream is not None or self.device < 0:
@@ -212,7 +210,7 @@ class KvPool:
                     not k_out.is_contiguous() or not v_out.is_contiguous():
                 raise EngineError(f"k_out and v_out: {rows} contiguous rows of one type are wanted")
             ko, vo, od = k_out.data_ptr(), v_out.data_ptr(), k_out.dtype
-        if lib().ecu_kv_append(self.h, layer, _DTYPES[k.dtype], k.data_ptr(), v.data_ptr(), ks, vs,
+        if lib().ecu_kv_append(self.h, self._layer(layer), _DTYPES[k.dtype], k.data_ptr(), v.data_ptr(), ks, vs,
                                None if s is None else _at(s), _at(n_new), n, _DTYPES[od], ko, vo,
                                self._stream(stream)) != 0:
             raise EngineError(last_error())
@@ -231,7 +229,7 @@ class KvPool:
         if ws is not None and (not ws.is_cuda or ws.get_device() != self.device or not ws.is_contiguous() or
                                ws.numel() * ws.element_size() < self.ws_bytes()):
             raise EngineError(f"ws: {self.ws_bytes()} contiguous bytes on CUDA device {self.device} are wanted")
-        if lib().ecu_kv_attend(self.h, layer, _DTYPES[q.dtype], q.data_ptr(), out.data_ptr(), heads, qs, os_,
+        if lib().ecu_kv_attend(self.h, self._layer(layer), _DTYPES[q.dtype], q.data_ptr(), out.data_ptr(), heads, qs, os_,
                                None if s is None else _at(s), q.shape[0],
                                self.head_dim ** -0.5 if scale is None else scale,
                                None if ws is None else ws.data_ptr(), self._stream(stream)) != 0:
@@ -248,8 +246,9 @@ class KvPool:
     def read(self, layer: int, seq: int, pos: int = 0, n: int | None = None, stream: int | None = None):
         """(K, V) rows [n, n_head_kv, head_dim] of cached positions as numpy arrays (ecu_kv_read)."""
         n = self.length(seq) - pos if n is None else n
+        _ints([pos, n])
         k, v = (np.empty((max(n, 0), self.n_head_kv, self.head_dim), dtype=np.float32) for _ in range(2))
-        if lib().ecu_kv_read(self.h, layer, int(seq), pos, n, k.ctypes.data, v.ctypes.data, self._stream(stream)) != 0:
+        if lib().ecu_kv_read(self.h, self._layer(layer), int(seq), pos, n, k.ctypes.data, v.ctypes.data, self._stream(stream)) != 0:
             raise EngineError(last_error())
         return k, v
 

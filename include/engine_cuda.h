@@ -384,7 +384,8 @@ int  ecu_kv_compact(ecu_kv *kv, void *stream);
  * and v (device, `dtype`, a row's KV heads one after the other, rows k_stride
  * / v_stride elements apart).  The positions' pages must be the sequence's
  * own (freshly extended ones are).  k_out, v_out (or NULL): the values as the
- * cache holds them, `out_dtype`, rows of n_head_kv * head_dim without gaps.
+ * cache holds them, `out_dtype`, rows of n_head_kv * head_dim without gaps,
+ * apart from k and v.
  * The lengths are read on the device when the call runs, so a captured call
  * appends to the then newest positions. */
 int  ecu_kv_append(ecu_kv *kv, int layer, int dtype, const void *k, const void *v, long k_stride, long v_stride,
@@ -400,7 +401,9 @@ int  ecu_kv_append(ecu_kv *kv, int layer, int dtype, const void *k, const void *
  * call runs.
  * ws: ecu_kv_ws_bytes() bytes of device memory, zeroed once before their
  * first use, that no other call uses at the same time; NULL: the pool's own
- * for this stream, which a stream that is being captured must not take. */
+ * for this stream, which a stream that is being captured must not take (made
+ * on its first call; past 16 streams the device is synchronised and they are
+ * made anew).  out and q do not overlap. */
 int    ecu_kv_attend(ecu_kv *kv, int layer, int dtype, const void *q, void *out, int n_head, long q_stride,
                      long out_stride, const int *seq, int n, float scale, void *ws, void *stream);
 size_t ecu_kv_ws_bytes(const ecu_kv *kv);

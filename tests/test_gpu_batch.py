@@ -246,3 +246,19 @@ def test_prefill_with_tensor_core_attention(eng, model_buf, monkeypatch, key, n_
     b.prefill(prompt[: n_prompt // 3])
     assert b.prefill(prompt[n_prompt // 3:]) == first
     close(b.logits(), want, 1e-3)
+
+
+def test_batch_refuses_when_closed_and_what_is_no_list(eng, model_buf):
+    """A closed batch answers with errors; numbers are not cut to 32 bits or to whole ones."""
+    b = eng.LlmBatch(eng.LlmCtx(eng.GgufModel(model_buf("mini-q4")), eng.STAGE_FULL), 2, 4)
+    big = 1 << 32
+    for f in (lambda: b.feed([big], [[1]]), lambda: b.feed(np.array([big]), [[1]]), lambda: b.feed([0], [np.array([big + 1])]),
+              lambda: b.feed([0], [[1.5]]), lambda: b.feed([[0]], [[1]]), lambda: b.length(big), lambda: b.free(np.array([big])),
+              lambda: b.truncate([0], [0.5])):
+        with pytest.raises(eng.EngineError):
+            f()
+    b.close()
+    for f in (lambda: b.feed([0], [[1]]), lambda: b.fork([0], [1]), lambda: b.truncate([0], [0]), lambda: b.free([0]),
+              lambda: b.compact(), lambda: b.length(0), lambda: b.used(), lambda: b.kv):
+        with pytest.raises(eng.EngineError):
+            f()

@@ -445,6 +445,46 @@ def test_attend_on_two_streams():
 
 # ----------------------------------------------------------------- pages ---
 
+def test_attend_keeps_a_workspace_a_stream():
+    """The pool's own workspaces go by the stream, not by its handle: the per-thread default stream has one handle for
+    all threads, and two threads' calls may overlap."""
+    import threading
+    hd, n_kv, n = 64, 2, 3000
+    pool, vals = filled(n_kv, hd, [n], 5)
+    q = rows(6, 1, n_kv, hd)
+    want = pool.attend(0, q, [0])
+    torch.cuda.synchronize()
+    per = pool.ws_bytes()
+    for _ in range(2):
+        pool.attend(0, q, [0], stream=2)                  # this thread's own default stream
+    before = pool.info().device_bytes
+    outs, errors = [torch.zeros_like(q) for _ in range(2)], []
+
+    def work(out):
+        try:
+            for _ in range(20):
+                pool.attend(0, q, [0], out=out, stream=2)
+        except Exception as e:
+            errors.append(e)
+    for o in outs:                                        # one after the other on the host; their kernels may overlap
+        t = threading.Thread(target=work, args=(o,))
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors and all(torch.equal(o, want) for o in outs)
+    assert pool.info().device_bytes == before + 2 * per
+    streams = [torch.cuda.Stream(priority=p) for _ in range(32) for p in (0, -1)]
+    outs = []
+    for s in streams:                                     # more than the pool keeps
+        outs.append(torch.zeros_like(q))
+        s.wait_stream(torch.cuda.current_stream())
+        pool.attend(0, q, [0], out=outs[-1], stream=s.cuda_stream)
+        assert pool.info().device_bytes <= before + 16 * per
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    pool.close()
+
+
 def test_pages_follow_their_sequences():
     """Forks, copies on write, truncations and compactions leave every sequence's rows as they were."""
     hd, n_kv, layers, slots = 64, 2, 3, 6
@@ -789,3 +829,6 @@ def test_pool_over_given_memory_and_its_end():
         with pytest.raises(engine.EngineError):
             f()
     assert (data[0] == 7).all()
+    for f in (lambda: pool.table, lambda: pool.lengths, lambda: pool.read(0, 1)):
+        with pytest.raises(engine.EngineError):
+            f()

@@ -240,3 +240,32 @@ def test_prompt_refuses(over, why):
 
 def test_prompt_of_nothing():
     assert prompt(cu_q=(0,)) == 0 and prompt(cu_q=(0, 0, 0), cu_k=(0, 3, 3)) == 0
+
+
+def test_open_refuses_pools_past_64_bits():
+    """Pages whose bytes pass 2^64 are no pool of what is left of them."""
+    with pytest.raises(engine.EngineError, match="too large"):
+        kv4.KvPool(65535, 4096, 128, 2 ** 31 - 1, 1, 1, device=-1)
+
+
+def test_attend_refuses_rows_past_32_bits():
+    pool = kv4.KvPool(1, 4096, 128, 1, 1, 1, device=-1)
+    assert attend(pool, heads=4096 * 4096) == -1 and "16777216 query heads" in engine.last_error()
+
+
+def test_numbers_past_32_bits():
+    """ctypes passes the low 32 bits of a number: such ones are refused, not taken for others."""
+    big = 1 << 32
+    for at in range(7):
+        size = [1, 2, 64, 8, 2, 4, -1]
+        size[at] += big
+        with pytest.raises(engine.EngineError):
+            kv4.KvPool(*size[:6], device=size[6])
+    pool = kv4.KvPool(1, 2, 64, 8, 2, 4, device=-1)
+    pool.extend([0], [5])
+    for f in (lambda: pool.length(big), lambda: pool.pages(big), lambda: pool.extend([big], [1]), lambda: pool.extend([0], [big + 1]),
+              lambda: pool.read(0, 0, big, 1), lambda: pool.read(big, 0), lambda: kv4.page_bytes(big + 2, 64),
+              lambda: pool.free(np.array([big], dtype=np.int64)), lambda: pool.truncate([0], [big])):
+        with pytest.raises(engine.EngineError):
+            f()
+    assert pool.length(0) == 5
