@@ -954,7 +954,9 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
     __syncthreads();
 
     // Rows that this CTA's warps share.  A partial's weight is 2^(its M - the
-    // row's M); one without a unit (its sum is zero) has none.
+    // row's M); one without a unit (its sums are zeros) has none.  M follows
+    // what is no NaN: a partial of NaN scores alone has M = -inf, weight 0 and
+    // sums of NaN.
     auto entry = [&](int e) { return (e & 1) ? tails + (e >> 1) * ENTRY : heads + (e >> 1) * ENTRY; };
     auto weight = [](float M, float m, float l) { return l == 0.0f ? 0.0f : kv4_ex2(M - m); };
     auto write = [&](int row, int x, float v) {
@@ -985,7 +987,9 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
     // a warp per row and head, or, of few rows, per 32 dimensions of one
     const int span = n_lead * HG >= W ? NB : 1, parts = NB / span;
     for (int task = warp; task < n_lead * HG * parts; task += W) {
-        const int e = lead_s[task / (HG * parts)], end = 32 - __clz(mates[e]), row = rid[e];
+        const int      e = lead_s[task / (HG * parts)], row = rid[e];
+        const unsigned own = mates[e];                    // the row's places
+        const int      end = 32 - __clz(own);
         const int i = row / R, nu = pre[i + 1] - pre[i], first = pre[i] * R + (row - i * R) * nu;
         const bool whole = first >= cu0 && first + nu <= cu1;
         const int  h = task / parts % HG, d0 = task % parts * 32 + lane;
@@ -996,7 +1000,8 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
         for (int k = e; k < end; k++) {
             const float  w = wgt[k][h];
             const float *from = entry(k) + h * (HD + 2);
-            if (w != 0.0f) {                              // (an unused place holds anything)
+            if (own >> k & 1u) {                          // (an unused place holds anything; a weight of 0 does
+                                                          // not take a place out: 0 * NaN is NaN)
                 L = fmaf(w, from[HD + 1], L);
 #pragma unroll
                 for (int x = 0; x < NB; x++)

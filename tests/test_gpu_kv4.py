@@ -365,6 +365,60 @@ def test_attend_nan_rows_stay_in_their_sequence():
     attend_check(pool, vals, q, [0, 1], pool.attend(0, q))
 
 
+def nan_check(pool, vals, q, out):
+    """Sequence 0's row: NaN where the definition is NaN, the rest as without the values that are not finite."""
+    n_kv, rep = pool.n_head_kv, q.shape[1] // pool.n_head_kv
+    k, v = vals
+    for g in range(n_kv):
+        hs = slice(g * rep, (g + 1) * rep)
+        bad_v = np.isnan(v[:, g]).any(0)
+        want_nan = np.broadcast_to(bad_v | np.isnan(k[:, g]).any(), (rep, pool.head_dim))
+        got = out[0, hs].double().cpu().numpy()
+        assert np.array_equal(np.isnan(got), want_nan), f"KV head {g}"
+        if np.isnan(k[:, g]).any():
+            continue
+        half, wide = torch.finfo(q.dtype).eps / 2, q.dtype == torch.float32
+        want, tol = reference(q[:1, hs].double().cpu().numpy(), k[:, g:g + 1], np.nan_to_num(v[:, g:g + 1]), pool.head_dim ** -0.5,
+                              0.0 if wide else 2.0 ** -24, 0.0 if wide else H16, half)
+        fine = ~bad_v
+        assert (np.abs(got[:, fine] - want[0][:, fine]) <= tol[0][:, fine]).all()
+
+
+@pytest.mark.parametrize("n_kv, rep", [(1, 4), (2, 1), (8, 4), (8, 8)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n, first, count", [(33, 32, 1), (65, 64, 1), (65, 0, 1), (96, 32, 32), (5000, 4992, 8), (5000, 1000, 32)])
+def test_attend_keys_that_are_not_finite(n_kv, rep, dtype, n, first, count):
+    """A key that is not finite makes its head's row NaN, wherever it lies: alone in its warp's part of the row, as a
+    whole unit, or in one CTA's part of many."""
+    hd = 64
+    pool = kv4.KvPool(1, n_kv, hd, 80, 1, 80)
+    k, v = rows(n, n, n_kv, hd), rows(n + 1, n, n_kv, hd)
+    k[first:first + count, n_kv - 1, 3] = float("nan")
+    pool.extend([0], [n])
+    pool.append(0, k, v, [0], [n])
+    q = rows(9, 1, rep * n_kv, hd).to(dtype)
+    nan_check(pool, (stored(k), stored(v)), q, pool.attend(0, q))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n, at", [(33, 32), (33, 0), (65, 40), (5000, 4999), (5000, 7)])
+def test_attend_values_that_are_not_finite_and_weigh_nothing(dtype, n, at):
+    """A value that is not finite makes its dimensions NaN however small its weight is: 0 * NaN is NaN."""
+    hd, n_kv = 64, 8
+    pool = kv4.KvPool(1, n_kv, hd, 80, 1, 80)
+    k, v = rows(n, n, n_kv, hd), rows(n + 1, n, n_kv, hd)
+    unit = slice(at // 32 * 32, min(n, at // 32 * 32 + 32))
+    k[unit, 5] = 0
+    k[unit, 5, 0] = -400                             # the whole unit far below the others: its weights are zero
+    v[at, 5, 40] = float("inf")
+    pool.extend([0], [n])
+    pool.append(0, k, v, [0], [n])
+    q = rows(9, 1, 4 * n_kv, hd)
+    q[:, :, 0] = 20                                  # scores of -1000
+    q = q.to(dtype)
+    nan_check(pool, (stored(k), stored(v)), q, pool.attend(0, q))
+
+
 def test_attend_beyond_32_bits():
     """Pages further than 4 GB into the layer."""
     hd, n_kv = 128, 8
