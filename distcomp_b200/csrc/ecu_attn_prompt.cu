@@ -13,6 +13,12 @@
 
 #define PA_LIST 1024              // sequences of one launch
 
+// Set where a wait of a caller's own call gave up (the engine's calls name
+// their context's word), until ecu_attn_prompt_status reads it.
+static __device__ int g_prompt_status;
+
+static std::atomic<unsigned> g_stall{0};        // devices (bits) whose next call's waits run out
+
 static int say(const char *why)
 {
     ecu_set_error(nullptr, 0, "ecu_attn_prompt: %s", why);
@@ -107,9 +113,73 @@ static int launch_all(const CUtensorMap (&m)[3], const PromptArgs &a, int head_d
     return 0;
 }
 
+int ecu_prompt_set_wait(unsigned long long ns) { return set_wait_limit(ns) == cudaSuccess ? 0 : -1; }
+
+// The status word's address on the current device; nullptr: it cannot be had.
+static int *status_word(int device)
+{
+    static std::atomic<int *> at[32];
+    void                     *p = device < 32 ? at[device].load() : nullptr;
+    if (!p) {
+        if (cudaGetSymbolAddress(&p, g_prompt_status) != cudaSuccess) {
+            cudaGetLastError();
+            return nullptr;
+        }
+        if (device < 32) at[device] = (int *)p;
+    }
+    return (int *)p;
+}
+
+extern "C" int ecu_attn_prompt_status(int device, void *stream)
+{
+    int ndev = 0;
+    if (cudaGetDeviceCount(&ndev) != cudaSuccess || device < 0 || device >= ndev) {
+        cudaGetLastError();
+        ecu_set_error(nullptr, 0, "ecu_attn_prompt_status: CUDA device %d not available (%d devices)", device, ndev);
+        return -1;
+    }
+    DeviceScope d(device);
+    if (!d.ok) return say("the device cannot be used");
+    const cudaStream_t      s = (cudaStream_t)stream;
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    cudaError_t             e = cudaStreamIsCapturing(s, &cap);
+    if (e == cudaSuccess && cap != cudaStreamCaptureStatusNone) return say("the status of a stream that is being captured is not known");
+    int *word = status_word(device), flags = 0;
+    if (!word) return say("the status word cannot be read");
+    if (e == cudaSuccess) e = cudaMemcpyAsync(&flags, word, sizeof flags, cudaMemcpyDeviceToHost, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    if (e == cudaSuccess && flags) {
+        e = cudaMemsetAsync(word, 0, sizeof flags, s);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    }
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        ecu_set_error(nullptr, 0, "ecu_attn_prompt_status: %s", cudaGetErrorString(e));
+        return -1;
+    }
+    if (!flags) return 0;
+    ecu_set_error(nullptr, 0, "ecu_attn_prompt: a kernel gave up on a bounded wait (status %d)", flags);
+    return -1;
+}
+
+extern "C" int ecu_inject_prompt_timeout(int device)
+{
+    if (device < 0 || device >= 32) return say("no such device to stall");
+    g_stall.fetch_or(1u << device);
+    return 0;
+}
+
 extern "C" int ecu_attn_prompt(int dtype, const void *q, const void *k, const void *v, void *out, int n_head, int n_head_kv,
                                int head_dim, long q_stride, long k_stride, long v_stride, long out_stride, const int *cu_q,
                                const int *cu_k, int n_seq, float scale, int device, void *stream)
+{
+    return ecu_attn_prompt_on(nullptr, dtype, q, k, v, out, n_head, n_head_kv, head_dim, q_stride, k_stride, v_stride, out_stride, cu_q,
+                              cu_k, n_seq, scale, device, stream);
+}
+
+int ecu_attn_prompt_on(int *status, int dtype, const void *q, const void *k, const void *v, void *out, int n_head, int n_head_kv,
+                       int head_dim, long q_stride, long k_stride, long v_stride, long out_stride, const int *cu_q, const int *cu_k,
+                       int n_seq, float scale, int device, void *stream)
 {
     if (dtype != ECU_F16 && dtype != ECU_BF16) return say("rows are ECU_F16 or ECU_BF16");
     if (head_dim != 64 && head_dim != 128) {
@@ -146,7 +216,8 @@ extern "C" int ecu_attn_prompt(int dtype, const void *q, const void *k, const vo
     }
     DeviceScope d(device);
     if (!d.ok) return say("the device cannot be used");
-    PromptArgs  a{v, out, v_stride, out_stride, n_head_kv, n_head / n_head_kv, scale};
+    if (!status && !(status = status_word(device))) return say("the status word cannot be had");
+    PromptArgs  a{v, out, v_stride, out_stride, n_head_kv, n_head / n_head_kv, scale, status, 0};
     CUtensorMap m[3];
     // a pointer that no row is read from is not mapped: q stands in
     if (make_map(m + 0, dtype, q, head_dim, n_head, cu_q[n_seq], q_stride) != 0 ||
@@ -154,6 +225,8 @@ extern "C" int ecu_attn_prompt(int dtype, const void *q, const void *k, const vo
         make_map(m + 2, dtype, keys ? v : q, head_dim, keys ? n_head_kv : 1, keys ? cu_k[n_seq] : 1, keys ? v_stride : qr) != 0)
         return -1;
     const cudaStream_t s = (cudaStream_t)stream;
+    if (device < 32 && g_stall.load(std::memory_order_relaxed))
+        a.stall = (int)(g_stall.fetch_and(~(1u << device)) >> device & 1u);
     try {
         return dtype == ECU_F16 ? launch_all<__half>(m, a, head_dim, cu_q, cu_k, n_seq, device, s)
                                 : launch_all<__nv_bfloat16>(m, a, head_dim, cu_q, cu_k, n_seq, device, s);

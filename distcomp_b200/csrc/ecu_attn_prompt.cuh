@@ -56,6 +56,8 @@ struct PromptArgs {
     long        v_stride, out_stride;
     int         n_kv, n_rep;
     float       scale;
+    int        *status;           // ECU_STATUS_TIMEOUT where a wait gave up
+    int         stall;            // 1: the first keys are never copied, so that a wait runs out
 };
 
 // Sequences of one launch by value, the longest first: where their rows lie
@@ -120,14 +122,19 @@ __device__ __forceinline__ bool pa_try(uint64_t *bar, uint32_t parity)
     return ok != 0;
 }
 
-// False when the limit of every wait ran out, or *dead says that another's has.
-__device__ __forceinline__ bool pa_wait(uint64_t *bar, uint32_t parity, int *dead)
+// False when the limit of every wait ran out, or another's has: *dead says so
+// of this CTA's, *status (nullptr: not looked at) of another CTA's or
+// kernel's.  It is looked at after a millisecond, a thousand times what a tile
+// takes: one limit, and not one per CTA, passes before a grid ends.
+__device__ __forceinline__ bool pa_wait(uint64_t *bar, uint32_t parity, int *dead, int *status = nullptr)
 {
     if (pa_try(bar, parity)) return true;
     const uint64_t t0 = globaltimer_ns();
     while (!pa_try(bar, parity)) {
         if (*reinterpret_cast<volatile int *>(dead)) return false;
-        if (globaltimer_ns() - t0 > wait_limit_ns()) return false;
+        const uint64_t dt = globaltimer_ns() - t0;
+        if (dt > wait_limit_ns()) return false;
+        if (status && dt > 1000000 && *reinterpret_cast<volatile int *>(status) != 0) return false;
     }
     return true;
 }
@@ -318,7 +325,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                 mbar_expect_tx(q_full + t, S::TILE);
                 for (int b = 0; b < B; b++)
                     pa_tma(smem_addr(sm + t * S::TILE + b * PA_BOX), &mq, b * 64, head_of(t), q0 + tile_of(t) * 128, q_full + t);
-                if (t == 0) copy_kv(0);
+                if (t == 0 && !a.stall) copy_kv(0);
             }
             for (int x = 1; x < min(ST, 2 * n); x++) copy_kv(x);
         }
@@ -330,9 +337,14 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     __syncthreads();
     pa_fence_after();
     const uint32_t tmem = tmem_s;
-    // every wait is bounded; one that gives up lets the others give up too
+    // every wait is bounded; one that gives up lets the others give up too, and
+    // the block's end flags the status (which the softmax warps do not look at:
+    // that made 8192 tokens 1.2 % slower)
     auto wait = [&](uint64_t *bar, uint32_t parity) {
         if (!pa_wait(bar, parity, &dead)) atomicExch(&dead, 1);
+    };
+    auto watch = [&](uint64_t *bar, uint32_t parity) {
+        if (!pa_wait(bar, parity, &dead, a.status)) atomicExch(&dead, 1);
     };
     auto gone = [&] { return *reinterpret_cast<volatile int *>(&dead) != 0; };
 
@@ -340,14 +352,16 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         if (lane == 0) {
             int x = min(ST, 2 * n);
             for (; x < 2 * n; x++) {
-                wait(empty + x % ST, (uint32_t)(x / ST - 1) & 1u);
+                watch(empty + x % ST, (uint32_t)(x / ST - 1) & 1u);
                 if (gone()) break;
                 copy_kv(x);
             }
-            if (gone()) {                         // nothing may still be on its way into shared memory
-                for (int t = 0; t < n_tile && n > 0; t++) mbar_drain(q_full + t, 0, wait_limit_ns());
-                for (int y = x > ST ? x - ST : 0; y < x; y++) mbar_drain(full + y % ST, (uint32_t)(y / ST) & 1u, wait_limit_ns());
-            }
+            // nothing may still be on its way into shared memory when the block
+            // ends, whoever has given up by then or does so later
+            bool landed = true;
+            for (int t = 0; t < n_tile && n > 0; t++) landed &= mbar_drain(q_full + t, 0, wait_limit_ns());
+            for (int y = max(a.stall, x - ST); y < x; y++) landed &= mbar_drain(full + y % ST, (uint32_t)(y / ST) & 1u, wait_limit_ns());
+            if (!landed) atomicExch(&dead, 1);
         }
         __syncwarp();
     } else if (warp == 17) {
@@ -372,7 +386,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
             };
             // (all lanes wait, and are together again for what follows)
             auto until = [&](uint64_t *bar, uint32_t parity) {
-                wait(bar, parity);
+                watch(bar, parity);
                 __syncwarp();
             };
             until(full + 0, 0);
@@ -403,7 +417,8 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                 if (__any_sync(0xffffffffu, gone())) break;
             }
             pa_commit(&drain);
-            mbar_drain(&drain, 0, wait_limit_ns());       // no product in flight when tensor memory is given back
+            // no product in flight when tensor memory is given back
+            if (!mbar_drain(&drain, 0, wait_limit_ns())) atomicExch(&dead, 1);
         }
         __syncwarp();
     } else if (warp >= 18) {
@@ -586,5 +601,6 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     }
     pa_fence_before();
     __syncthreads();
+    if (tid == 512 && gone()) atomicOr(a.status, ECU_STATUS_TIMEOUT);
     if (warp == 17) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }

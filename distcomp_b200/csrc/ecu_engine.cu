@@ -2825,7 +2825,11 @@ int ecu_set_wait_ns(int device, unsigned long long ns)
         return -1;
     }
     CK(cudaSetDevice(device));
-    CK(cudaMemcpyToSymbol(g_wait_ns, &ns, sizeof ns));
+    CK(set_wait_limit(ns));
+    if (ecu_prompt_set_wait(ns) != 0 || ecu_noalloc_set_wait(ns) != 0) {
+        ecu_set_error(nullptr, 0, "ecu_set_wait_ns: %s", cudaGetErrorString(cudaGetLastError()));
+        return -1;
+    }
     return 0;
 }
 
@@ -3272,7 +3276,7 @@ static int pf_attention_tc(ecu_ctx *c, int n, int pos0, int ldq, const float *kc
     CK(cudaGetLastError());
     g_launches += 3;
     const int cq[2] = {0, n}, ck[2] = {0, np};
-    if (ecu_attn_prompt(ECU_F16, c->hf.q, c->hf.k, c->hf.v, c->pf.ah, g.n_head, g.n_head_kv, hd, qd, kvd, kvd, qd, cq, ck, 1,
+    if (ecu_attn_prompt_on(&c->st->status, ECU_F16, c->hf.q, c->hf.k, c->hf.v, c->pf.ah, g.n_head, g.n_head_kv, hd, qd, kvd, kvd, qd, cq, ck, 1,
                         1.0f / sqrtf((float)hd), c->device, c->stream) != 0)
         return -1;
     CK(cudaMemsetAsync(c->pf.al, 0, (size_t)n * qd * sizeof(__half), c->stream));
@@ -3673,7 +3677,7 @@ static int batch_layers(ecu_batch *b, const std::vector<BatchPart> &part, int n_
                                 c->hf.v + (size_t)ck[i] * kvd, c->stream) != 0)
                     return -1;
             k_bt_half<<<4 * c->sms, 256, 0, c->stream>>>(P.QKV + r0, ldq, (size_t)prompt_rows, qd, c->hf.q);
-            if (ecu_attn_prompt(ECU_F16, c->hf.q, c->hf.k, c->hf.v, P.ah + (size_t)n_step * qd, g.n_head, g.n_head_kv, hd, qd, kvd, kvd,
+            if (ecu_attn_prompt_on(&c->st->status, ECU_F16, c->hf.q, c->hf.k, c->hf.v, P.ah + (size_t)n_step * qd, g.n_head, g.n_head_kv, hd, qd, kvd, kvd,
                                 qd, cq.data(), ck.data(), n_prompt, scale, c->device, c->stream) != 0)
                 return -1;
             CK(cudaMemsetAsync(P.al + (size_t)n_step * qd, 0, (size_t)prompt_rows * qd * sizeof(__half), c->stream));

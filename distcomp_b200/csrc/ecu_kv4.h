@@ -106,6 +106,18 @@ cudaError_t ecu_launch_early(void (*kern)(P...), unsigned grid, unsigned block, 
 
 void ecu_count_launches(int n);       // ecu_kernel_launches()
 
+// ecu_attn_prompt with a status word of the caller's on the device (nullptr:
+// the one that ecu_attn_prompt_status reads): ECU_STATUS_TIMEOUT is set in it
+// where a wait gives up.
+int ecu_attn_prompt_on(int *status, int dtype, const void *q, const void *k, const void *v, void *out, int n_head, int n_head_kv,
+                       int head_dim, long q_stride, long k_stride, long v_stride, long out_stride, const int *cu_q, const int *cu_k,
+                       int n_seq, float scale, int device, void *stream);
+
+// ecu_set_wait_ns for the kernels of other translation units, on the current
+// device.
+int ecu_prompt_set_wait(unsigned long long ns);
+int ecu_noalloc_set_wait(unsigned long long ns);
+
 // Positions 0..n-1 of a sequence as fp16 rows [n][n_head_kv * head_dim] in
 // device memory, as the cache holds them.
 int ecu_kv_rows(ecu_kv *kv, int layer, int seq, int n, void *k, void *v, cudaStream_t s);

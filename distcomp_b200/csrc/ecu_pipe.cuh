@@ -15,6 +15,12 @@
 // changes while no kernel runs.
 static __device__ unsigned long long g_wait_ns = ECU_WAIT_NS;
 
+// Sets this translation unit's limit on the current device.
+[[maybe_unused]] static cudaError_t set_wait_limit(unsigned long long ns)
+{
+    return cudaMemcpyToSymbol(g_wait_ns, &ns, sizeof ns);
+}
+
 __device__ __forceinline__ unsigned long long wait_limit_ns() { return __ldg(&g_wait_ns); }
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p)

@@ -126,6 +126,7 @@ SIGNATURES = [
                                             C.c_void_p, C.c_void_p]),
     ("ecu_set_wait_ns", C.c_int, [C.c_int, C.c_ulonglong]),
     ("ecu_inject_wait_timeout", C.c_int, [C.c_void_p]),
+    ("ecu_inject_prompt_timeout", C.c_int, [C.c_int]),
     ("ecu_matvec_bench", C.c_int, [C.c_uint, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int,
                                    C.c_int, C.c_int, C.POINTER(C.c_double)]),
     ("ecu_matvec_stream_bench", C.c_int, [C.c_uint, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
@@ -153,6 +154,7 @@ SIGNATURES = [
     ("ecu_attn_prompt", C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
                                   C.c_long, C.c_long, C.c_long, C.c_long, C.c_void_p, C.c_void_p, C.c_int, C.c_float,
                                   C.c_int, C.c_void_p]),
+    ("ecu_attn_prompt_status", C.c_int, [C.c_int, C.c_void_p]),
     ("ecu_batch_open", C.c_int, [C.POINTER(C.c_void_p), C.c_void_p, C.c_int, C.c_int, C.c_char_p, C.c_size_t]),
     ("ecu_batch_close", None, [C.c_void_p]),
     ("ecu_batch_kv", C.c_void_p, [C.c_void_p]),
@@ -579,6 +581,13 @@ def matvec_bench(gtype: int, raw: np.ndarray, n_in: int, n_out: int, x: np.ndarr
 def set_wait_ns(ns: int, device: int = 0) -> None:
     """The limit after which every bounded wait in the kernels gives up."""
     if lib().ecu_set_wait_ns(device, int(ns)) != 0:
+        raise EngineError(last_error())
+
+
+def inject_prompt_timeout(device: int = 0) -> None:
+    """The next prompt attention on the device waits for keys that are never
+    copied (ecu_inject_prompt_timeout): failure-path testing."""
+    if lib().ecu_inject_prompt_timeout(int(device)) != 0:
         raise EngineError(last_error())
 
 

@@ -290,3 +290,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q, cu
                              hd ** -0.5 if scale is None else scale, dev, stream) != 0:
         raise EngineError(last_error())
     return out
+
+
+def prompt_status(device: int = 0, stream: int | None = None) -> None:
+    """Waits for the stream's work; raises where a prompt attention on the device gave up on a wait since this was
+    last asked: its rows are NaN (ecu_attn_prompt_status)."""
+    if lib().ecu_attn_prompt_status(device, _current(device) if stream is None else stream) != 0:
+        raise EngineError(last_error())

@@ -423,10 +423,18 @@ int    ecu_kv_read(ecu_kv *kv, int layer, int seq, int pos, int n, float *k, flo
  * too), has no effect.  Sums and the softmax are fp32, relative to weights of
  * up to 2^8 (bf16 values near 2^127 / 2^8 / keys can pass fp32's range); the
  * weights are rounded to `dtype` before their product with V.  out overlaps
- * none of the others. */
+ * none of the others.
+ * Every wait in the kernel is bounded (ecu_set_wait_ns): one that gives up
+ * leaves rows of NaN, which ecu_attn_prompt_status reports. */
 int  ecu_attn_prompt(int dtype, const void *q, const void *k, const void *v, void *out, int n_head, int n_head_kv,
                      int head_dim, long q_stride, long k_stride, long v_stride, long out_stride, const int *cu_q,
                      const int *cu_k, int n_seq, float scale, int device, void *stream);
+/* Waits for the stream; -1 where a wait of an ecu_attn_prompt call on
+ * `device` has given up since this was last asked (until then, waits of later
+ * calls that take longer than a millisecond give up with it), or the status
+ * cannot be read.  The calls inside ecu_batch_feed and ecu_prefill report
+ * through those. */
+int  ecu_attn_prompt_status(int device, void *stream);
 
 /* ---- many sequences over one model (serving) ---- */
 
@@ -469,9 +477,14 @@ int  ecu_batch_feed(ecu_batch *b, const int *seq, const int *n_tok, int n, const
  * tagged input, for an input word that no phase writes: its waits run out,
  * that step returns -1 with the timeout in ecu_last_error, and the context
  * steps normally again afterwards (reset it: that step's cache row is not
- * valid).  -1 for a context on the per-kernel step. */
+ * valid).  -1 for a context on the per-kernel step.
+ * ecu_inject_prompt_timeout: the next prompt attention on `device`
+ * (ecu_attn_prompt, or inside ecu_batch_feed or ecu_prefill) never copies its
+ * first keys, so that its waits run out: ecu_attn_prompt_status, or the call
+ * around it, returns -1. */
 int  ecu_set_wait_ns(int device, unsigned long long ns);
 int  ecu_inject_wait_timeout(ecu_ctx *c);
+int  ecu_inject_prompt_timeout(int device);
 
 /* ---- measurement --------------------------------------------------------- */
 

@@ -56,3 +56,64 @@ def test_injection_needs_the_persistent_step(eng, model_buf, monkeypatch):
     with pytest.raises(eng.EngineError, match="positive"):
         eng.set_wait_ns(0)
     c.close()
+
+
+@pytest.fixture
+def short_wait(eng):
+    eng.set_wait_ns(100_000_000)
+    yield
+    eng.set_wait_ns(2_000_000_000)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [40, 700])             # all keys requested at once; keys waiting for a place of the ring
+def test_prompt_attention_gives_up_and_reports(eng, short_wait, hd, n):
+    """Keys that are never copied: the rows become NaN, the status reports it once, and the next call is right."""
+    import torch
+
+    from distcomp_b200 import kv4
+    g = torch.Generator().manual_seed(n + hd)
+    q, k, v = (torch.randn(n, h, hd, generator=g).half().cuda() for h in (8, 2, 2))
+    want = kv4.prompt_attention(q, k, v, [0, n])
+    kv4.prompt_status()
+    for _ in range(2):
+        eng.inject_prompt_timeout()
+        t0 = time.perf_counter()
+        out = kv4.prompt_attention(q, k, v, [0, n])
+        with pytest.raises(eng.EngineError, match="bounded wait"):
+            kv4.prompt_status()
+        dt = time.perf_counter() - t0
+        assert 0.08 <= dt < 5.0, dt
+        assert torch.isnan(out).all()
+        assert torch.equal(kv4.prompt_attention(q, k, v, [0, n]), want)
+        kv4.prompt_status()
+
+
+def test_batch_reports_a_prompt_that_gave_up(eng, short_wait, model_buf):
+    """The feed fails, the sequences keep what they held, and the batch goes on as one that never failed."""
+    m = eng.GgufModel(model_buf("mini-q4"))
+    base = eng.LlmCtx(m, eng.STAGE_FULL)
+    a, b = eng.LlmBatch(base, 3, 9), eng.LlmBatch(base, 3, 9)
+    for x in (a, b):
+        x.feed([0, 1], [[5] * 40, [7, 8, 9]])
+    eng.inject_prompt_timeout()
+    with pytest.raises(eng.EngineError, match="bounded wait"):
+        a.feed([0, 1, 2], [[3], [4] * 70, [6] * 30])
+    assert [a.length(s) for s in range(3)] == [40, 3, 0] and a.used() == b.used()
+    for _ in range(2):
+        (pa, la), (pb, lb) = (x.feed([0, 1, 2], [[3], [4] * 20, [6] * 30], logits=True) for x in (a, b))
+        assert pa == pb and np.array_equal(la, lb)
+
+
+def test_prefill_reports_a_prompt_that_gave_up(eng, short_wait, model_buf, monkeypatch):
+    monkeypatch.setenv("ECU_PF_ATTN", "2")
+    c = eng.LlmCtx(eng.GgufModel(model_buf("mini-q4")), eng.STAGE_FULL, n_ctx=128)
+    prompt = [3, 9, 27] * 20
+    want = c.prefill(prompt)
+    c.reset()
+    eng.inject_prompt_timeout()
+    with pytest.raises(eng.EngineError, match="bounded wait"):
+        c.prefill(prompt)
+    c.reset()
+    assert c.prefill(prompt) == want
+    c.close()

@@ -269,3 +269,12 @@ def test_numbers_past_32_bits():
         with pytest.raises(engine.EngineError):
             f()
     assert pool.length(0) == 5
+
+
+def test_prompt_status_refuses_devices():
+    L = engine.lib()
+    assert L.ecu_attn_prompt_status(99, None) == -1 and "not available" in engine.last_error()
+    assert L.ecu_attn_prompt_status(-1, None) == -1
+    for d in (-1, 32):
+        with pytest.raises(engine.EngineError):
+            engine.inject_prompt_timeout(d)
