@@ -113,10 +113,9 @@ int ecu_attn_prompt_on(int *status, int dtype, const void *q, const void *k, con
                        int head_dim, long q_stride, long k_stride, long v_stride, long out_stride, const int *cu_q, const int *cu_k,
                        int n_seq, float scale, int device, void *stream);
 
-// ecu_set_wait_ns for the kernels of other translation units, on the current
+// ecu_set_wait_ns for the prompt attention's translation unit, on the current
 // device.
 int ecu_prompt_set_wait(unsigned long long ns);
-int ecu_noalloc_set_wait(unsigned long long ns);
 
 // Positions 0..n-1 of a sequence as fp16 rows [n][n_head_kv * head_dim] in
 // device memory, as the cache holds them.

@@ -17,7 +17,6 @@
 // device which loads the library holds until the process exits.
 #include "../../include/engine_cuda.h"
 #include "ecu_gemv.cuh"
-#include "ecu_kv4.h"
 #include "ecu_model.h"
 
 #include <cstddef>
@@ -37,8 +36,6 @@ struct NoallocScratch {
 // The scratch.  In host code this name is only a stand-in for the device
 // symbol: its address must come from cudaGetSymbolAddress on each device.
 static __device__ __align__(256) uint8_t g_noalloc_scratch[sizeof(NoallocScratch)];
-
-int ecu_noalloc_set_wait(unsigned long long ns) { return set_wait_limit(ns) == cudaSuccess ? 0 : -1; }
 
 // Device address of g_noalloc_scratch on the current device.  Looked up on
 // every call (cudaGetSymbolAddress allocates nothing and is cheap): a cached
