@@ -9,6 +9,7 @@
 #include <cmath>
 #include <exception>
 #include <memory>
+#include <optional>
 
 #define CK(call)                                                                        \
     do {                                                                                \
@@ -93,6 +94,7 @@ template <int N> static int update_launch(ecu_kv *kv, size_t &c0, size_t &s0, cu
     }
     c0 += u.n_copy;
     s0 += u.n_set;
+    if (kv->device < 0) return 0;
     const int      blocks_page = (int)((kv->page_bytes / 16 + 256 * KV4_COPY_VECS - 1) / (256 * KV4_COPY_VECS));
     const unsigned copy_blocks = (unsigned)u.n_copy * kv->n_layer * blocks_page;
     return launched("ecu_kv", ecu_launch_early(k_kv4_update<N>, copy_blocks + (u.n_set + 255) / 256, 256, 0, s, kv->data, kv->page_bytes,
@@ -100,21 +102,38 @@ template <int N> static int update_launch(ecu_kv *kv, size_t &c0, size_t &s0, cu
 }
 
 // What the last operation changed, on the device.  The lists travel as kernel
-// arguments: 128 entries in a 1 KB argument, longer ones 2000 at a time.
+// arguments: 128 entries in a 1 KB argument, longer ones 2000 at a time.  A
+// launch that fails takes the operation back where it is the first; where it
+// is not, the device's tables are neither the old nor the new ones, and the
+// pool refuses what comes after.
 static int update(ecu_kv *kv, cudaStream_t s)
 {
     size_t c0 = 0, s0 = 0;
     const size_t nc = kv->book.copies.size(), ns = kv->book.sets.size();
-    if (kv->device < 0) return 0;
-    while (c0 < nc || s0 < ns)
-        if ((nc - c0 + ns - s0 <= 128 ? update_launch<128>(kv, c0, s0, s) : update_launch<2000>(kv, c0, s0, s)) != 0) return -1;
+    const int    fail_at = kv->inject;
+    kv->inject = -1;
+    for (int i = 0; c0 < nc || s0 < ns; i++) {
+        const int rc = i == fail_at ? say("ecu_kv", "launch failed: injected")
+                                    : nc - c0 + ns - s0 <= 128 ? update_launch<128>(kv, c0, s0, s) : update_launch<2000>(kv, c0, s0, s);
+        if (rc == 0) continue;
+        if (i == 0) kv->book.fail();
+        else kv->broken = true;
+        return -1;
+    }
     return 0;
+}
+
+// A pool that a failed launch left between two states takes no more calls.
+static int whole(const ecu_kv *kv, const char *what)
+{
+    return kv->broken ? say(what, "a launch of an earlier change failed: the pool can only be closed") : 0;
 }
 
 // The checks that every change of the pool begins with.
 static int change_ok(ecu_kv *kv, const void *list, const void *list2, int n, cudaStream_t s, const char *what)
 {
     if (!kv || n < 0 || (n > 0 && (!list || !list2))) return say(what, "null argument or negative count");
+    if (whole(kv, what) != 0) return -1;
     if (kv->device < 0) return 0;
     // a launch that failed later would leave the bookkeeping ahead of the device
     DeviceScope d(kv->device);
@@ -244,11 +263,11 @@ int ecu_kv_len(const ecu_kv *kv, int seq, int *pages, int n)
 #define KV_CHANGE(name_, list, list2, op)                                                            \
     if (change_ok(kv, list, list2, n, (cudaStream_t)stream, name_) != 0) return -1;                  \
     try {                                                                                           \
+        std::optional<DeviceScope> d;                                                               \
+        if (kv->device >= 0) d.emplace(kv->device);                                                 \
+        if (d && !d->ok) return say(name_, "the pool's device cannot be used");                      \
         const int r = (op);                                                                         \
-        if (r < 0 || kv->device < 0) return r;                                                      \
-        DeviceScope d(kv->device);                                                                  \
-        if (!d.ok) return say(name_, "the pool's device cannot be used");                            \
-        return update(kv, (cudaStream_t)stream) != 0 ? -1 : r;                                      \
+        return r < 0 ? r : update(kv, (cudaStream_t)stream) != 0 ? -1 : r;                           \
     } catch (const std::exception &e) {                                                             \
         kv->book.fail();                                                                            \
         return say(name_, e.what());                                                                 \
@@ -278,6 +297,13 @@ int ecu_kv_compact(ecu_kv *kv, void *stream)
 {
     const int n = 0;
     KV_CHANGE("ecu_kv_compact", nullptr, nullptr, kv->book.compact())
+}
+
+int ecu_kv_inject_failure(ecu_kv *kv, int launch)
+{
+    if (!kv || launch < 0) return say("ecu_kv_inject_failure", "null argument or negative number");
+    kv->inject = launch;
+    return 0;
 }
 
 } // extern "C"
@@ -340,6 +366,7 @@ extern "C" int ecu_kv_append(ecu_kv *kv, int layer, int dtype, const void *k, co
     }
     const size_t es = dtype_bytes(dtype), os = dtype_bytes(out_dtype);
     if (!es || !os) return say(what, "unknown element type");
+    if (whole(kv, what) != 0) return -1;
     if (slots_ok(kv, seq, n, what) != 0) return -1;
     const long row = (long)kv->n_head_kv * kv->head_dim;
     try {
@@ -407,6 +434,7 @@ extern "C" int ecu_kv_read(ecu_kv *kv, int layer, int seq, int pos, int n, float
     if (layer < 0 || layer >= kv->n_layer || slots_ok(kv, &seq, 1, what) != 0 || pos < 0 || n < 0 ||
         (long long)pos + n > kv->book.seq[seq].len)
         return say(what, "no such layer, sequence or positions");
+    if (whole(kv, what) != 0) return -1;
     if (kv->device < 0) return say(what, "the pool has no device");
     if (n == 0) return 0;
     const cudaStream_t s = (cudaStream_t)stream;
@@ -536,6 +564,7 @@ extern "C" int ecu_kv_attend(ecu_kv *kv, int layer, int dtype, const void *q, vo
         return -1;
     }
     if (!std::isfinite(scale)) return say(what, "the scale is not finite");
+    if (whole(kv, what) != 0) return -1;
     if (slots_ok(kv, seq, n, what) != 0) return -1;
     if (n == 0) return 0;
     const long row = (long)n_head * kv->head_dim;

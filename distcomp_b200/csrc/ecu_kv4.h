@@ -31,18 +31,21 @@ struct KvBook {
     int  fork(const int *src, const int *dst, int n);
     int  truncate(const int *s, const int *len, int n);
     int  compact();
-    int  fail();                      // takes the operation back; -1
+    int  fail();                      // takes the last operation back; -1
 
 private:
     struct Undo { int kind, a, b; };
     std::vector<Undo> log_;
     std::vector<std::pair<int, int>> cell_;    // table cells (sequence, index) that changed
     std::vector<int>                 length_;  // sequences whose length changed
+    std::vector<int>                 move_;    // of each page, where it goes while pages move; else -1
+    bool                             compacted_ = false;       // the last operation is a compaction
     int  take();
     void hold(int p);
     void drop(int p);
     void begin();
     void finish();
+    void move_pages(bool back);
     bool slot(int s, const char *what);
 };
 
@@ -57,6 +60,8 @@ struct ecu_kv {
     // per-thread default stream's names another stream in each thread)
     std::map<unsigned long long, void *> ws;
     void *spare = nullptr;            // the first stream's, allocated with the pool
+    bool  broken = false;             // a change ended between its launches: tables and bookkeeping differ
+    int   inject = -1;                // ecu_kv_inject_failure: the launch of the next change that fails
     int *table() const { return meta; }
     int *len() const { return meta ? meta + (size_t)book.n_seq * book.max_pages : nullptr; }
 };

@@ -3,7 +3,9 @@
 // Free pages are a bitmap and taken lowest id first, so that the same calls
 // always give the same tables and the pool stays packed towards its start.
 // An operation logs what it changes and is undone from the log when a later
-// part of it cannot be done.
+// part of it cannot be done, here or on the device.  Memory for a step and its
+// log is taken before the step, so that one that runs out leaves a log that
+// matches what was done.
 #include "ecu_kv4.h"
 #include "ecu_model.h"
 
@@ -12,6 +14,11 @@
 static int pages_of(long long n) { return (int)((n + ECU_KV4_PAGE - 1) / ECU_KV4_PAGE); }
 
 enum { U_HOLD, U_DROP, U_PUSH, U_POP, U_CELL, U_LEN };
+
+template <typename T> static void room(std::vector<T> &v, size_t n)
+{
+    if (v.capacity() - v.size() < n) v.reserve(std::max(2 * v.capacity(), v.size() + n));
+}
 
 void KvBook::init(int pages, int seqs, int per_seq)
 {
@@ -47,6 +54,7 @@ int KvBook::take()
         if (~taken[hint]) {
             const int p = (int)(hint * 64) + __builtin_ctzll(~taken[hint]);
             if (p >= n_pages) return -1;
+            room(log_, 1);
             hold(p);
             log_.push_back({U_HOLD, p, 0});
             return p;
@@ -61,10 +69,28 @@ void KvBook::begin()
     length_.clear();
     copies.clear();
     sets.clear();
+    compacted_ = false;
+}
+
+// Pages `from` become pages `to` in every table.
+void KvBook::move_pages(bool back)
+{
+    std::vector<int> &to = move_;
+    for (const Copy &c : copies) to[back ? c.to : c.from] = back ? c.from : c.to;
+    for (Seq &q : seq)
+        for (int &p : q.page)
+            if (to[p] >= 0) p = to[p];
+    for (const Copy &c : copies) to[back ? c.to : c.from] = -1;
+    for (const Copy &c : copies) std::swap(ref[c.to], ref[c.from]);
+    std::fill(taken.begin(), taken.end(), 0ull);
+    for (int p = 0; p < n_pages; p++)
+        if (ref[p]) taken[p >> 6] |= 1ull << (p & 63);
+    hint = back ? 0 : (size_t)used >> 6;
 }
 
 int KvBook::fail()
 {
+    if (compacted_) move_pages(true);
     for (size_t i = log_.size(); i-- > 0;) {
         const Undo u = log_[i];
         switch (u.kind) {
@@ -124,22 +150,26 @@ int KvBook::extend(const int *s, const int *n_new, int n)
             const int old = q.page.back(), p = take();
             if (p < 0) return none();
             copies.push_back({old, p});
+            cell_.push_back({s[i], (int)q.page.size() - 1});
+            room(log_, 2);
             drop(old);
             log_.push_back({U_DROP, old, 0});
             log_.push_back({U_CELL, s[i], old});
             q.page.back() = p;
-            cell_.push_back({s[i], (int)q.page.size() - 1});
         }
         while ((int)q.page.size() < pages_of(want)) {
             const int p = take();
             if (p < 0) return none();
+            cell_.push_back({s[i], (int)q.page.size()});
+            room(q.page, 1);
+            room(log_, 1);
             q.page.push_back(p);
             log_.push_back({U_PUSH, s[i], 0});
-            cell_.push_back({s[i], (int)q.page.size() - 1});
         }
+        length_.push_back(s[i]);
+        room(log_, 1);
         log_.push_back({U_LEN, s[i], q.len});
         q.len = (int)want;
-        length_.push_back(s[i]);
     }
     finish();
     return 0;
@@ -155,7 +185,12 @@ int KvBook::fork(const int *src, const int *dst, int n)
             return fail();
         }
         Seq &d = seq[dst[i]];
-        for (int p : seq[src[i]].page) {
+        const std::vector<int> &from = seq[src[i]].page;
+        room(d.page, from.size());
+        room(log_, 2 * from.size() + 1);
+        room(cell_, from.size());
+        room(length_, 1);
+        for (int p : from) {
             hold(p);
             log_.push_back({U_HOLD, p, 0});
             d.page.push_back(p);
@@ -182,6 +217,10 @@ int KvBook::truncate(const int *s, const int *len, int n)
             return fail();
         }
         if (keep == q.len) continue;
+        const size_t gone = q.page.size() - pages_of(keep);
+        room(log_, 2 * gone + 1);
+        room(cell_, gone);
+        room(length_, 1);
         while ((int)q.page.size() > pages_of(keep)) {
             const int p = q.page.back();
             drop(p);
@@ -201,27 +240,21 @@ int KvBook::truncate(const int *s, const int *len, int n)
 int KvBook::compact()
 {
     begin();
-    std::vector<int> to;
-    int              hole = 0;
+    int hole = 0;
     for (int p = used; p < n_pages; p++) {
         if (!ref[p]) continue;
         while (ref[hole]) hole++;
-        if (to.empty()) to.assign((size_t)n_pages, -1);
-        to[p] = hole;
         copies.push_back({p, hole});
         hole++;
     }
     if (copies.empty()) return 0;
     for (int s = 0; s < n_seq; s++)
         for (size_t j = 0; j < seq[s].page.size(); j++)
-            if (to[seq[s].page[j]] >= 0) {
-                seq[s].page[j] = to[seq[s].page[j]];
-                cell_.push_back({s, (int)j});
-            }
-    for (const Copy &c : copies) std::swap(ref[c.to], ref[c.from]);
-    std::fill(taken.begin(), taken.end(), 0ull);
-    for (int p = 0; p < used; p++) taken[p >> 6] |= 1ull << (p & 63);
-    hint = (size_t)used >> 6;
+            if (seq[s].page[j] >= used) cell_.push_back({s, (int)j});
+    room(sets, cell_.size());
+    move_.resize((size_t)n_pages, -1);
+    move_pages(false);
+    compacted_ = true;
     finish();
     return (int)copies.size();
 }

@@ -145,6 +145,7 @@ SIGNATURES = [
     ("ecu_kv_truncate", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
     ("ecu_kv_free", C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
     ("ecu_kv_compact", C.c_int, [C.c_void_p, C.c_void_p]),
+    ("ecu_kv_inject_failure", C.c_int, [C.c_void_p, C.c_int]),
     ("ecu_kv_append", C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_long, C.c_long, C.c_void_p,
                                 C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
     ("ecu_kv_attend", C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_long, C.c_long,

@@ -185,6 +185,12 @@ class KvPool:
             raise EngineError(last_error())
         return n
 
+    def inject_failure(self, launch: int = 0) -> None:
+        """The launch-th device update of the next change fails (ecu_kv_inject_failure): failure-path testing."""
+        _ints([launch])
+        if lib().ecu_kv_inject_failure(self.h, launch) != 0:
+            raise EngineError(last_error())
+
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, seq, n_new, k_out: torch.Tensor | None = None,
                v_out: torch.Tensor | None = None, stream: int | None = None) -> None:
         """The newest n_new[i] positions' rows of sequences seq[i] (ecu_kv_append); k_out, v_out: contiguous

@@ -356,8 +356,12 @@ int  ecu_kv_get_info(const ecu_kv *kv, ecu_kv_info *info);
  * pages[0..n) (NULL: none wanted). */
 int  ecu_kv_len(const ecu_kv *kv, int seq, int *pages, int n);
 
-/* The next four change n sequences in the list's order; each either does all
- * of it or, with -1, nothing.  What they change on the device is enqueued on
+/* The next four, and ecu_kv_compact, change sequences in the list's order;
+ * each either does all of it or, with -1, nothing.  (Long changes take several
+ * launches, about 2000 page copies and table words each.  Where one after the
+ * first fails, which no valid call brings about, the pool refuses every later
+ * call but those that read its bookkeeping, and ecu_kv_close.)  What they
+ * change on the device is enqueued on
  * `stream` (NULL: the legacy default stream); calls on the same pool from
  * different streams are ordered by the caller, and a stream that is being
  * captured is refused (the bookkeeping would not be replayed).
@@ -481,10 +485,13 @@ int  ecu_batch_feed(ecu_batch *b, const int *seq, const int *n_tok, int n, const
  * ecu_inject_prompt_timeout: the next prompt attention on `device`
  * (ecu_attn_prompt, or inside ecu_batch_feed or ecu_prefill) never copies its
  * first keys, so that its waits run out: ecu_attn_prompt_status, or the call
- * around it, returns -1. */
+ * around it, returns -1.  ecu_kv_inject_failure: of the launches with which
+ * the next change of the pool updates the device (a pool without one counts
+ * them alike), number `launch`, from 0, fails. */
 int  ecu_set_wait_ns(int device, unsigned long long ns);
 int  ecu_inject_wait_timeout(ecu_ctx *c);
 int  ecu_inject_prompt_timeout(int device);
+int  ecu_kv_inject_failure(ecu_kv *kv, int launch);
 
 /* ---- measurement --------------------------------------------------------- */
 

@@ -584,6 +584,27 @@ def test_pages_follow_their_sequences():
                     assert np.array_equal(v.astype(np.float64), held[i][l][:, 1]), (step, i, l)
 
 
+def test_pages_of_a_failed_change():
+    """A change whose first launch fails leaves the device's tables and pages to the sequences that had them."""
+    hd, n_kv = 64, 2
+    pool, vals = filled(n_kv, hd, [70, 130, 5], seed=4, gap=8)
+    q = rows(5, 3, 4, hd)
+    want, table, lens = pool.attend(0, q).clone(), pool.table.clone(), pool.lengths.clone()
+    for f in (lambda: pool.extend([0, 2], [100, 1]), lambda: pool.truncate([1], [3]), lambda: pool.free([0, 2])):
+        pool.inject_failure()
+        with pytest.raises(engine.EngineError, match="injected"):
+            f()
+        assert torch.equal(pool.table, table) and torch.equal(pool.lengths, lens)
+        assert torch.equal(pool.attend(0, q), want)
+    pool.free([0])
+    pool.inject_failure()
+    with pytest.raises(engine.EngineError, match="injected"):
+        pool.compact()
+    assert torch.equal(pool.attend(0, q[1:], [1, 2]), want[1:])
+    assert pool.compact() > 0
+    attend_check(pool, vals, q[1:], [1, 2], pool.attend(0, q[1:], [1, 2]))
+
+
 def test_pages_many_at_once():
     """More copies and words than one launch's argument holds."""
     hd, n_kv, n = 32, 1, 1500

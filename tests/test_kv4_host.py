@@ -278,3 +278,65 @@ def test_prompt_status_refuses_devices():
     for d in (-1, 32):
         with pytest.raises(engine.EngineError):
             engine.inject_prompt_timeout(d)
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_a_change_whose_launch_fails_is_taken_back(seed):
+    """Every kind of change, its device update refused, leaves tables, lengths and the pages that come next as they were."""
+    r = random.Random(100 + seed)
+    pages, slots, per = r.choice([40, 70, 200]), 9, 12
+    pool, m = kv4.KvPool(2, 2, 64, pages, slots, per, device=-1), Model(pages, slots, per)
+    failed = {k: 0 for k in ("extend", "fork", "truncate", "free", "compact")}
+    for _ in range(400):
+        what, s = r.choice(list(failed) + ["extend"]), r.randrange(slots)
+        if what == "extend":
+            n = r.choice([1, 2, 64, 65, r.randint(1, 300)])
+            if m.len[s] + n > per * PAGE or m.need(s, n) > m.ref.count(0):
+                continue
+            call, do = (lambda: pool.extend([s], [n])), (lambda: m.extend(s, n))
+        elif what == "fork":
+            d = r.randrange(slots)
+            if d == s or m.len[d] or not m.len[s]:
+                continue
+            call, do = (lambda: pool.fork([s], [d])), (lambda: m.fork(s, d))
+        elif what == "compact":
+            if not any(m.ref[p] and p >= sum(x > 0 for x in m.ref) for p in range(pages)):
+                continue
+            call, do = pool.compact, m.compact
+        else:
+            if not m.len[s]:
+                continue
+            n = 0 if what == "free" else r.randrange(m.len[s])
+            call, do = (lambda: pool.free([s]) if what == "free" else pool.truncate([s], [n])), (lambda: m.truncate(s, n))
+        for _ in range(r.choice([0, 1, 2])):
+            pool.inject_failure()
+            with pytest.raises(engine.EngineError, match="injected"):
+                call()
+            failed[what] += 1
+            same(pool, m)
+        call()
+        do()
+        same(pool, m)
+    assert all(failed.values()), failed
+
+
+def test_a_change_cut_off_between_launches_ends_the_pool():
+    """A later launch of a long list fails: nothing after it works on tables that are neither old nor new."""
+    n = 1500                                         # two words a sequence: two launches
+    pool = kv4.KvPool(1, 1, 64, 2 * n, n, 2, device=-1)
+    with pytest.raises(engine.EngineError):
+        pool.inject_failure(-1)
+    pool.inject_failure(2)
+    pool.extend(range(n), [1] * n)                   # has no third launch
+    pool.extend([0], [1])
+    pool.inject_failure(1)
+    with pytest.raises(engine.EngineError, match="injected"):
+        pool.free(range(n))
+    for f in (lambda: pool.extend([0], [1]), lambda: pool.fork([0], [1]), lambda: pool.truncate([0], [0]), lambda: pool.free([0]),
+              pool.compact, lambda: pool.read(0, 0, 0, 0)):
+        with pytest.raises(engine.EngineError, match="can only be closed"):
+            f()
+    for rc in (append(pool, ks=64, vs=64), attend(pool, heads=1, qs=64, os=64)):
+        assert rc == -1 and "can only be closed" in engine.last_error()
+    pool.length(0), pool.used
+    pool.close()
