@@ -3732,6 +3732,25 @@ static int batch_run(ecu_batch *b, const std::vector<BatchPart> &part, int n_ste
     return 0;
 }
 
+// Takes sequences back to the lengths they had, unless the feed got through:
+// whatever way it ends otherwise.
+struct BatchUndo {
+    ecu_batch              *b;
+    const std::vector<int> &slots, &before;
+    bool                    done = false;
+    ~BatchUndo()
+    {
+        if (done) return;
+        char why[512];
+        snprintf(why, sizeof why, "%s", ecu_get_error());
+        try {
+            ecu_kv_truncate(b->kv, slots.data(), before.data(), (int)slots.size(), b->c->stream);
+            ecu_set_error(nullptr, 0, "%s", why);
+        } catch (...) {               // no memory for the message
+        }
+    }
+};
+
 extern "C" int ecu_batch_feed(ecu_batch *b, const int *seq, const int *n_tok, int n, const int *tokens, int *picked, float *logits)
 {
     auto bad = [](const char *why) {
@@ -3794,14 +3813,9 @@ extern "C" int ecu_batch_feed(ecu_batch *b, const int *seq, const int *n_tok, in
             b->seq_cap = n;
         }
         if (ecu_kv_extend(b->kv, slots.data(), counts.data(), n, c->stream) != 0) return -1;
-        if (batch_run(b, part, n_step, (int)rows, picked, logits) != 0) {
-            // the sequences keep what they held before
-            const std::string why = ecu_get_error();
-            ecu_kv_truncate(b->kv, slots.data(), before.data(), n, c->stream);
-            ecu_set_error(nullptr, 0, "%s", why.c_str());
-            return -1;
-        }
-        return 0;
+        BatchUndo undo{b, slots, before};
+        undo.done = batch_run(b, part, n_step, (int)rows, picked, logits) == 0;
+        return undo.done ? 0 : -1;
     } catch (const std::exception &e) {
         return bad(e.what());
     }

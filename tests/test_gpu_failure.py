@@ -117,3 +117,20 @@ def test_prefill_reports_a_prompt_that_gave_up(eng, short_wait, model_buf, monke
     c.reset()
     assert c.prefill(prompt) == want
     c.close()
+
+
+def test_batch_whose_pool_update_fails(eng, model_buf):
+    """A feed that the pool refuses on the device changes nothing and can be made again."""
+    m = eng.GgufModel(model_buf("mini-q4"))
+    b = eng.LlmBatch(eng.LlmCtx(m, eng.STAGE_FULL), 3, 9)
+    b.feed([0, 1], [[5] * 64, [7, 8, 9]])
+    b.fork([1], [2])
+    want = [b.length(s) for s in range(3)], b.used()
+    assert eng.lib().ecu_kv_inject_failure(b.kv, 0) == 0
+    with pytest.raises(eng.EngineError, match="injected"):
+        b.feed([0, 2, 1], [[3], [4], [6] * 70])
+    assert ([b.length(s) for s in range(3)], b.used()) == want
+    first = b.feed([0, 2, 1], [[3], [4], [6] * 70])
+    b.free([0, 1, 2])
+    b.feed([0, 1, 2], [[5] * 64, [7, 8, 9], [7, 8, 9]])
+    assert b.feed([0, 2, 1], [[3], [4], [6] * 70]) == first
