@@ -3212,6 +3212,15 @@ static int pf_gemm(ecu_ctx *c, const DevMat &m, int n, float *C, const float *R)
 // the prompt's 1e-3 bar, but not the fp32 attention's results: off by default.
 static bool pf_attn_tc() { const char *e = getenv("ECU_PF_ATTN"); return e && e[0] == '2'; }
 
+// Do the batched GEMMs and the tensor-core prompt attention cover the shapes?
+static bool pf_shapes(const ecu_ctx *c)
+{
+    const EcuGeom &g = c->g;
+    bool ok = c->tp.world == 1 && (g.head_dim == 64 || g.head_dim == 128) && g.n_embd % 8 == 0 && g.n_ff % 8 == 0;
+    for (auto &ly : c->layers) ok = ok && (!ly.ha || ly.qkv.size() == 1) && (!ly.hf || ly.gu_fused);
+    return ok;
+}
+
 // Can the batched kernels run this context's prompt (else: token by token)?
 static bool pf_batched(const ecu_ctx *c, bool &attn2)
 {
@@ -3220,10 +3229,7 @@ static bool pf_batched(const ecu_ctx *c, bool &attn2)
     // one-query-per-CTA kernel keeps its scores in a PF_ATT_MAXPOS array
     const char *ae = getenv("ECU_PF_ATTN");
     attn2 = PF_QB % g.n_rep == 0 && !(ae && ae[0] == '0');
-    bool batched = c->tp.world == 1 && (attn2 || pf_attn_tc() || g.n_ctx <= PF_ATT_MAXPOS) && (g.head_dim == 64 || g.head_dim == 128) &&
-                   g.n_embd % 8 == 0 && g.n_ff % 8 == 0;
-    for (auto &ly : c->layers) batched = batched && (!ly.ha || ly.qkv.size() == 1) && (!ly.hf || ly.gu_fused);
-    return batched;
+    return pf_shapes(c) && (attn2 || pf_attn_tc() || g.n_ctx <= PF_ATT_MAXPOS);
 }
 
 static int pf_attrs(const ecu_ctx *c)
@@ -3544,13 +3550,13 @@ extern "C" int ecu_batch_open(ecu_batch **out, ecu_ctx *base, int n_seq, int n_p
     if (err && errlen) err[0] = '\0';
     if (!out || !base) { ecu_set_error(err, errlen, "null argument"); return -1; }
     *out = nullptr;
-    bool attn2 = false;
     if (base->stage != ECU_STAGE_FULL || base->tp.world > 1) {
         ecu_set_error(err, errlen, "a batch needs a FULL context that is not tensor-parallel");
         return -1;
     }
-    if (!pf_batched(base, attn2)) {
-        ecu_set_error(err, errlen, "the batched kernels do not cover this model's shapes (head_dim %d)", base->g.head_dim);
+    if (!pf_shapes(base)) {
+        ecu_set_error(err, errlen, "the batched kernels do not cover this model's shapes (head_dim %d; 64 and 128 are, with Q, K, V and "
+                      "gate, up in one fast format each and widths in eights)", base->g.head_dim);
         return -1;
     }
     if (cudaSetDevice(base->device) != cudaSuccess) { ecu_set_error(err, errlen, "cudaSetDevice(%d) failed", base->device); return -1; }

@@ -445,9 +445,11 @@ int  ecu_attn_prompt_status(int device, void *stream);
 /* Sequences with the weights of a FULL context and their K/V in a pool of
  * 4-bit pages: prompts and single tokens of any of them in one call.  No
  * counterpart in the reference, which serves one sequence a process
- * (src/daemon.c:757).  For the shapes that ecu_prefill runs as a batch (and
- * head_dim 64 or 128); others are refused, and so are tensor-parallel and
- * staged contexts.  n_seq slots of the base's n_ctx positions, n_pages pages
+ * (src/daemon.c:757).  For models of head_dim 64 or 128 whose embedding and
+ * feed-forward widths are multiples of 8 and whose Q, K and V, and gate and
+ * up, share a format of the fast layouts (as the persistent step wants), of
+ * any n_ctx; others are refused, and so are tensor-parallel and staged
+ * contexts.  n_seq slots of the base's n_ctx positions, n_pages pages
  * of ECU_KV4_PAGE positions between them.  The base may be closed first. */
 typedef struct ecu_batch ecu_batch;
 int  ecu_batch_open(ecu_batch **out, ecu_ctx *base, int n_seq, int n_pages, char *err, size_t errlen);

@@ -262,3 +262,71 @@ def test_batch_refuses_when_closed_and_what_is_no_list(eng, model_buf):
               lambda: b.compact(), lambda: b.length(0), lambda: b.used(), lambda: b.kv):
         with pytest.raises(eng.EngineError):
             f()
+
+
+class Held(Plain):
+    """The plain forward over the rows that a batch's pool holds.  Where a key or value lies within the projections'
+    rounding of the border of two codes, either code is right, and the layers after it follow the one taken; so this
+    forward takes the pool's, after checking each against its own value: half a code away, a whole one where the code
+    ends (7, opposite the largest value), and 5e-3 of the block's largest value for what came before."""
+
+    def __init__(self, plain, eng, batch):
+        self.__dict__.update(plain.__dict__)
+        self.eng, self.b = eng, batch
+        self.hd = self.s.head_dim or self.s.n_embd // self.s.n_head
+
+    def rows(self, seq, layer, pos, n):
+        k, v = (np.empty((n, self.s.n_head_kv, self.hd), dtype=np.float32) for _ in range(2))
+        assert self.eng.lib().ecu_kv_read(self.b.kv, layer, seq, pos, n, k.ctypes.data, v.ctypes.data, self.b.stream) == 0
+        return [x.astype(np.float64) for x in (k, v)]
+
+    def keep(self, x):
+        got = self.queue.pop(0)
+        m = np.abs(x.reshape(*x.shape[:-1], -1, 32)).max(-1, keepdims=True)
+        off = np.abs(got - x).reshape(*x.shape[:-1], -1, 32)
+        ends = np.abs(x.reshape(off.shape)) > m * 15 / 16 - 5e-3 * m
+        assert (off <= m * (np.where(ends, 1 / 8, 1 / 16) + 5e-3)).all()
+        return got
+
+    def last(self, seq, tokens):
+        """Logits of the last of `tokens`, a sequence's newest ones, which the pool holds already."""
+        past = self.b.length(seq) - len(tokens)
+        cache = {}
+        self.queue = []
+        for l in range(self.s.n_layer):
+            for n, old, new in zip("kv", self.rows(seq, l, 0, past), self.rows(seq, l, past, len(tokens))):
+                cache[(l, n)] = old
+                self.queue.append(new)
+        return self.forward(tokens, cache)[-1]
+
+
+@pytest.mark.parametrize("kv, attn", [(2, None), (4, "0"), (16, "2")])
+def test_contexts_of_any_size(eng, setup, monkeypatch, kv, attn):
+    """A context past 8192 positions, whatever attention ecu_prefill takes (which the batch does not use): prompts,
+    pieces, few and many steps, 8, 4 and 1 query heads a KV head."""
+    if attn:
+        monkeypatch.setenv("ECU_PF_ATTN", attn)
+    base, plain, _ = setup("mini-q8", n_head_kv=kv, n_ff=1024, n_ctx=9000)
+    b = eng.LlmBatch(base, 20, 300)
+    held = Held(plain, eng, b)
+    r = np.random.default_rng(kv)
+
+    def some(n):
+        return [int(v) for v in r.integers(3, base.n_vocab, n)]
+    text = [some(n) for n in (70, 2, 129)]
+    for toks in (text, [some(1), some(3), some(1)], [some(1), some(1), some(1)]):
+        _, lg = b.feed([4, 0, 9], toks, logits=True)
+        for i, s in enumerate((4, 0, 9)):
+            close(lg[i], held.last(s, toks[i]))
+    b.fork([4] * 17, [s for s in range(20) if s not in (4, 0, 9)])
+    toks = [some(1) for _ in range(20)]
+    _, lg = b.feed(range(20), toks, logits=True)
+    for s in (4, 0, 9, 19):
+        close(lg[s], held.last(s, toks[s]))
+    b.free(range(20))
+    far = some(8300)
+    _, lg = b.feed([0], [far], logits=True)
+    close(lg[0], held.last(0, far[-1:]))
+    b.feed([1], [far[:8250]])
+    _, lg = b.feed([1], [far[8250:]], logits=True)
+    close(lg[0], held.last(1, far[8250:]))
