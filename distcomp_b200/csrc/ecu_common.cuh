@@ -88,6 +88,7 @@ struct StepState {
 
 #define ECU_STATUS_TIMEOUT 1
 #define ECU_STATUS_BADTOKEN 2
+#define ECU_STATUS_RANGE 4          // a prompt operand past fp16's range
 
 // -------------------------------------------------------------- helpers ----
 

@@ -993,6 +993,8 @@ static int check_status(ecu_ctx *c)
         }
         if (s.status & ECU_STATUS_BADTOKEN)
             ecu_set_error(nullptr, 0, "the device-resident token is outside the vocabulary (%d)", c->g.n_vocab);
+        else if (s.status == ECU_STATUS_RANGE)
+            ecu_set_error(nullptr, 0, "a query, key, value or attention row of a prompt or a large batch passes fp16's range (65504)");
         else
             ecu_set_error(nullptr, 0, "a kernel gave up on a bounded wait (status %d)", s.status);
         CK(cudaMemset(&c->st->status, 0, sizeof(int)));
@@ -3276,9 +3278,9 @@ static int pf_attention_tc(ecu_ctx *c, int n, int pos0, int ldq, const float *kc
     const EcuGeom &g = c->g;
     const int hd = g.head_dim, qd = g.n_head * hd, kvd = g.n_head_kv * hd, np = pos0 + n;
     if (hf_reserve(c, (size_t)n * qd, (size_t)np * kvd) != 0) return -1;
-    k_bt_half<<<4 * c->sms, 256, 0, c->stream>>>(c->pf.QKV, ldq, (size_t)n, qd, c->hf.q);
-    k_bt_plane_half<<<4 * c->sms, 256, 0, c->stream>>>(kc, g.n_ctx, g.n_head_kv, hd, np, c->hf.k);
-    k_bt_plane_half<<<4 * c->sms, 256, 0, c->stream>>>(vc, g.n_ctx, g.n_head_kv, hd, np, c->hf.v);
+    k_bt_half<<<4 * c->sms, 256, 0, c->stream>>>(c->pf.QKV, ldq, (size_t)n, qd, c->hf.q, nullptr, nullptr, 0, &c->st->status);
+    k_bt_plane_half<<<4 * c->sms, 256, 0, c->stream>>>(kc, g.n_ctx, g.n_head_kv, hd, np, c->hf.k, &c->st->status);
+    k_bt_plane_half<<<4 * c->sms, 256, 0, c->stream>>>(vc, g.n_ctx, g.n_head_kv, hd, np, c->hf.v, &c->st->status);
     CK(cudaGetLastError());
     g_launches += 3;
     const int cq[2] = {0, n}, ck[2] = {0, np};
@@ -3661,7 +3663,7 @@ static int batch_layers(ecu_batch *b, const std::vector<BatchPart> &part, int n_
                 ecu_kv_attend(b->kv, (int)li, ECU_F32, P.QKV, P.ATT, g.n_head, ldq, qd, seq.data(), n_step, scale, nullptr,
                               c->stream) != 0)
                 return -1;
-            if (!by_row) k_pf_split<<<4 * c->sms, 256, 0, c->stream>>>(P.ATT, (size_t)n_step * qd, P.ah, P.al);
+            if (!by_row) k_bt_split<<<4 * c->sms, 256, 0, c->stream>>>(P.ATT, (size_t)n_step * qd, P.ah, P.al, &c->st->status);
         }
         if (by_row) {
             gemv(ly.o, P.ATT, qd, nullptr, P.X, E, EPI_ADD);
@@ -3682,7 +3684,8 @@ static int batch_layers(ecu_batch *b, const std::vector<BatchPart> &part, int n_
                 if (ecu_kv_rows(b->kv, (int)li, seq[n_step + i], ck[i + 1] - ck[i], c->hf.k + (size_t)ck[i] * kvd,
                                 c->hf.v + (size_t)ck[i] * kvd, c->stream) != 0)
                     return -1;
-            k_bt_half<<<4 * c->sms, 256, 0, c->stream>>>(P.QKV + r0, ldq, (size_t)prompt_rows, qd, c->hf.q);
+            k_bt_half<<<4 * c->sms, 256, 0, c->stream>>>(P.QKV + r0, ldq, (size_t)prompt_rows, qd, c->hf.q, c->hf.k, c->hf.v,
+                                                         (size_t)ck.back() * kvd, &c->st->status);
             if (ecu_attn_prompt_on(&c->st->status, ECU_F16, c->hf.q, c->hf.k, c->hf.v, P.ah + (size_t)n_step * qd, g.n_head, g.n_head_kv, hd, qd, kvd, kvd,
                                 qd, cq.data(), ck.data(), n_prompt, scale, c->device, c->stream) != 0)
                 return -1;

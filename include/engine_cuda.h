@@ -467,8 +467,11 @@ void   *ecu_batch_stream(ecu_batch *b);
  * ecu_kv_attend, the others through ecu_attn_prompt, all to keys and values
  * as the cache holds them, so a prompt leaves the same state however it is
  * cut.  Against the fp32 cache of ecu_forward the states differ by the
- * cache's 4-bit rounding.  On an error the sequences keep what they held.
- * Synchronises the batch's stream. */
+ * cache's 4-bit rounding.  Prompts' queries, keys and values, and the
+ * attention rows of more than 16 single tokens, go through fp16: a finite one
+ * past 65504 in magnitude fails the feed (fed alone, single tokens reach what
+ * the cache holds, 8 * 65504).  On an error the sequences keep what they
+ * held.  Synchronises the batch's stream. */
 int  ecu_batch_feed(ecu_batch *b, const int *seq, const int *n_tok, int n, const int *tokens, int *picked, float *logits);
 
 /* ---- failure-path testing ------------------------------------------------ */

@@ -330,3 +330,42 @@ def test_contexts_of_any_size(eng, setup, monkeypatch, kv, attn):
     b.feed([1], [far[:8250]])
     _, lg = b.feed([1], [far[8250:]], logits=True)
     close(lg[0], held.last(1, far[8250:]))
+
+
+@pytest.mark.parametrize("which, rel", [("q", 0.1), ("k", 0.1), ("v", REL)])
+def test_values_past_fp16(eng, oracle_port, model_buf, monkeypatch, which, rel):
+    """Queries, keys or values of 1e5 (a bias): steps, whose attention is fp32 over the cache's exact values, hold them; a
+    prompt or a batch of more steps, whose operands are fp16, fails and leaves the sequences as they were.  (Scores of
+    some thousands, 8 * 65504 at most in a key: their fp32 rounding moves a weight by up to some percent.)"""
+    over = dict(arch="qwen2", qkv_bias=True)
+    buf = np.frombuffer(bytes(model_buf("mini-q4", **over)), np.uint8).copy()
+    np.frombuffer(G.read_tensor_table(buf)[f"blk.1.attn_{which}.bias"][2], np.float32)[5] = 1e5
+    m = eng.GgufModel(buf)
+    base = eng.LlmCtx(m, eng.STAGE_FULL)
+    b = eng.LlmBatch(base, 20, 30)
+    held = Held(Plain(synth.spec("mini-q4", **over), buf, oracle_port), eng, b)
+    r = np.random.default_rng(3)
+    toks = [int(t) for t in r.integers(3, base.n_vocab, 24)]
+    for i, t in enumerate(toks[:12]):
+        _, lg = b.feed([0], [[t]], logits=True)
+        assert np.isfinite(lg).all()
+        close(lg[0], held.last(0, [t]), rel)
+    b.fork([0] * 17, range(1, 18))
+    state = [b.length(s) for s in range(20)], b.used()
+    for seq, text in (([18], [toks]), ([0], [toks[12:]]), ([0, 18], [toks[12:13], toks])):
+        with pytest.raises(eng.EngineError, match="fp16's range"):
+            b.feed(seq, text)
+        assert [b.length(s) for s in range(20)] == state[0]
+    many = list(range(18)), [[toks[12]]] * 18
+    if which == "v":
+        with pytest.raises(eng.EngineError, match="fp16's range"):
+            b.feed(*many)
+        assert [b.length(s) for s in range(20)] == state[0]
+    else:
+        _, lg = b.feed(*many, logits=True)
+        close(lg[17], held.last(17, [toks[12]]), rel)
+    _, lg = b.feed([3], [[toks[13]]], logits=True)
+    close(lg[0], held.last(3, [toks[13]]), rel)
+    monkeypatch.setenv("ECU_PF_ATTN", "2")
+    with pytest.raises(eng.EngineError, match="fp16's range"):
+        base.prefill(toks)
