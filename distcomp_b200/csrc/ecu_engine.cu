@@ -3612,9 +3612,10 @@ extern "C" void   *ecu_batch_stream(ecu_batch *b) { return b ? (void *)b->c->str
 struct BatchPart { int at, seq, n, past, row; const int *tok; };
 
 // Up to this many single tokens go through the projections row by row, as the
-// decode step's matrix-vector products: on the 8B shape a step takes 1.1 ms and
-// 1.8 ms a row (12 rows 22.9 ms), with the GEMMs 31 ms for 1 to 13 rows and 39
-// for 64, most of it spent on their dequantised weight operands.
+// decode step's matrix-vector products: on the 8B shape a step takes 2.8 ms for
+// 1 row, 8.3 for 4, 22.8 for 12 and 30.2 for 16 (each row reads the weights),
+// with the GEMMs 32.4 ms for 17 rows and 38.9 for 64, most of it spent on their
+// dequantised weight operands.
 #define BT_GEMV_ROWS 16
 
 // The layers over `rows` rows of P.X: the first n_step rows are single tokens

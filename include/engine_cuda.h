@@ -400,9 +400,10 @@ int  ecu_kv_append(ecu_kv *kv, int layer, int dtype, const void *k, const void *
  * (head h reads KV head h / (n_head / n_head_kv)) of sequence seq[i] (NULL:
  * slots 0..n-1; a slot may come twice).  q and out: device, `dtype`, a row's
  * heads one after the other, rows q_stride / out_stride elements apart.  An
- * empty sequence's row becomes zeros.  Sums and the softmax are fp32; fp32
- * queries keep their 24 bits.  The lengths are read on the device when the
- * call runs.
+ * empty sequence's row becomes zeros.  Sums and the softmax are fp32; of fp32
+ * queries, and of their weights, 22 bits count.  A position that is not finite
+ * in K makes its head's rows NaN, one in V its block of 32 dimensions, however
+ * little it weighs.  The lengths are read on the device when the call runs.
  * ws: ecu_kv_ws_bytes() bytes of device memory, zeroed once before their
  * first use, that no other call uses at the same time; NULL: the pool's own
  * for this stream, which a stream that is being captured must not take (made
@@ -464,10 +465,13 @@ void   *ecu_batch_stream(ecu_batch *b);
  * head's output.  The rows of all sequences go through the layers together
  * (ecu_prefill's GEMMs; a few single tokens alone as the decode step's
  * matrix-vector products); a sequence with one token attends through
- * ecu_kv_attend, the others through ecu_attn_prompt, all to keys and values
- * as the cache holds them, so a prompt leaves the same state however it is
- * cut.  Against the fp32 cache of ecu_forward the states differ by the
- * cache's 4-bit rounding.  Prompts' queries, keys and values, and the
+ * ecu_kv_attend, the others through ecu_attn_prompt (in fp16: 11 bits of each
+ * operand and weight), all to keys and values as the cache holds them.  So a
+ * prompt leaves nearly the same state however it is cut, but not the same
+ * bits: where a key or value lies at the border of two 4-bit codes, the
+ * paths' rounding can decide it either way, and later layers follow.  Against
+ * the fp32 cache of ecu_forward the states differ by the cache's 4-bit
+ * rounding.  Prompts' queries, keys and values, and the
  * attention rows of more than 16 single tokens, go through fp16: a finite one
  * past 65504 in magnitude fails the feed (fed alone, single tokens reach what
  * the cache holds, 8 * 65504).  On an error the sequences keep what they

@@ -369,3 +369,24 @@ def test_values_past_fp16(eng, oracle_port, model_buf, monkeypatch, which, rel):
     monkeypatch.setenv("ECU_PF_ATTN", "2")
     with pytest.raises(eng.EngineError, match="fp16's range"):
         base.prefill(toks)
+
+
+def test_a_prompt_however_it_is_cut(eng, setup):
+    """One prompt whole, in pieces and token by token: each agrees with the plain forward over its own pool's rows, and
+    the rows with one another to a code (1/8 of their block's largest value; 1e-2 of it for what came before)."""
+    base, plain, _ = setup("mini-q4")
+    b = eng.LlmBatch(base, 4, 12)
+    held = Held(plain, eng, b)
+    text = [int(t) for t in np.random.default_rng(12).integers(3, base.n_vocab, 90)]
+    for seq, cuts in enumerate(([90], [30, 1, 33, 26], [64, 26], [1] * 90)):
+        at = 0
+        for n in cuts:
+            _, lg = b.feed([seq], [text[at:at + n]], logits=True)
+            close(lg[0], held.last(seq, text[at:at + n]))
+            at += n
+    for layer in range(plain.s.n_layer):
+        first = held.rows(0, layer, 0, 90)
+        for seq in (1, 2, 3):
+            for x, y in zip(first, held.rows(seq, layer, 0, 90)):
+                m = np.abs(x).reshape(90, plain.s.n_head_kv, -1, 32).max(-1, keepdims=True)
+                assert (np.abs(x - y).reshape(90, plain.s.n_head_kv, -1, 32) <= m * (1 / 8 + 1e-2)).all()
