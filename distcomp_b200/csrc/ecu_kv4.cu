@@ -600,8 +600,13 @@ extern "C" int ecu_kv_attend(ecu_kv *kv, int layer, int dtype, const void *q, vo
             if (!own) {
                 void        *p = nullptr;
                 CK(cudaMalloc(&p, bytes));
-                cudaMemset(p, 0, bytes);
-                cudaDeviceSynchronize();
+                const cudaError_t e = cudaMemsetAsync(p, 0, bytes, s);       // ahead of the call that takes it
+                if (e != cudaSuccess) {
+                    cudaGetLastError();
+                    cudaFree(p);
+                    ecu_set_error(nullptr, 0, "%s: clearing a workspace failed: %s", what, cudaGetErrorString(e));
+                    return -1;
+                }
                 own = p;
                 kv->device_bytes += bytes;
             }
