@@ -499,6 +499,7 @@ struct ecu_ctx {
     unsigned long long *mega_ll = nullptr;   // the tagged activation vectors, one block
     size_t      mega_ll_words = 0;
     int         stall_next = -1;          // ecu_inject_wait_timeout: the phase the next launch stalls
+    bool        late_next = false;        // ecu_inject_late_warp: a warp is late in the next launch
     std::vector<MegaPhase> mega_ph;       // host copy of the phase list (pipeline links patch inputs)
     cudaEvent_t ev_step = nullptr;        // ecu_step_dev on a caller's stream: ordering with the own stream
     void       *link_peer = nullptr;      // IPC mapping of the next stage's tagged vectors
@@ -1025,6 +1026,8 @@ template <class F> static int on_stream(ecu_ctx *c, void *stream, F enq)
 typedef void (*MegaFn)(MegaArgs);
 
 // sys: the tagged words cross GPUs (tensor-parallel ranks): system scope
+#define MEGA_LATE_NS 10000           // ecu_inject_late_warp: ten times what a descriptor's copy takes
+
 static MegaFn mega_lookup(int hd, int rep, bool sys)
 {
     if (hd == 128 && rep == 4) return sys ? k_decode_mega<128, 4, true> : k_decode_mega<128, 4, false>;
@@ -1476,7 +1479,9 @@ static int mega_launch(ecu_ctx *c, cudaStream_t s, unsigned long long *phase_ns,
     at.val.cooperative = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    cudaError_t e = mega_launch_serial(c->device, cfg, c->mega_fn, a);
+    const MegaFn fn = c->late_next ? k_decode_mega<128, 4, false, MEGA_LATE_NS> : c->mega_fn;
+    c->late_next = false;
+    cudaError_t e = mega_launch_serial(c->device, cfg, fn, a);
     if (e != cudaSuccess) {
         ecu_set_error(nullptr, 0, "persistent step launch failed: %s", cudaGetErrorString(e));
         return -1;
@@ -2832,6 +2837,19 @@ int ecu_set_wait_ns(int device, unsigned long long ns)
         ecu_set_error(nullptr, 0, "ecu_set_wait_ns: %s", cudaGetErrorString(cudaGetLastError()));
         return -1;
     }
+    return 0;
+}
+
+int ecu_inject_late_warp(ecu_ctx *c)
+{
+    const MegaFn late = k_decode_mega<128, 4, false, MEGA_LATE_NS>;
+    if (!c || !c->mega || c->mega_fn != mega_lookup(128, 4, false)) {
+        ecu_set_error(nullptr, 0, "ecu_inject_late_warp: only a context on the persistent step of one GPU, 4 query heads of 128 a KV head");
+        return -1;
+    }
+    cudaSetDevice(c->device);
+    CK(cudaFuncSetAttribute(late, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)c->mega_smem));
+    c->late_next = true;
     return 0;
 }
 

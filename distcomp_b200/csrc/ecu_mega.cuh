@@ -451,7 +451,7 @@ struct MegaShared {
     int      *dig;
     float    *kvbuf;
     float    *cs;          // RoPE (cos, sin) row of the current position, staged a phase early
-    uint64_t *dbar;        // completes when the next phase's descriptor has arrived
+    uint64_t *dbar;        // [2]: [p & 1] completes when phase p's descriptor has arrived
     double   *dsum;
     ArgBest  *argsh;
     const uint4 *tab;      // the phase table (shared memory)
@@ -909,7 +909,7 @@ __device__ void mega_gemv(const MegaArgs &a, const MegaPhase &ph, const MegaShar
     }
     if (next) {
         // next phase's descriptor: its copy was issued at this phase's start
-        mbar_wait<true>(S.dbar, (unsigned)p_idx & 1u, a.status);
+        mbar_wait<true>(S.dbar + ((p_idx + 1) & 1), (unsigned)p_idx >> 1 & 1u, a.status);
         if (tid == 0 && a.att_l2 == 1) attn_prefetch(a, *next, S.pos, hd);
         if (tid < hd) S.cs[tid] = cs_next;
     }
@@ -1339,7 +1339,10 @@ __device__ void mega_embed(const MegaArgs &a, const MegaShared &S, int p_idx)
     }
 }
 
-template <int HD, int NREP, bool SYS>
+// LATE_NS (failure-path testing): the last warp of every CTA comes this much
+// late to each phase.  A template argument, since a branch here costs the step
+// up to 6 % in register allocation.
+template <int HD, int NREP, bool SYS, int LATE_NS = 0>
 __global__ void __launch_bounds__(MEGA_THREADS, 1) k_decode_mega(MegaArgs a)
 {
     extern __shared__ __align__(128) uint8_t smem[];
@@ -1360,11 +1363,11 @@ __global__ void __launch_bounds__(MEGA_THREADS, 1) k_decode_mega(MegaArgs a)
     __shared__ int pos_s;
     __shared__ unsigned launch_s;
     __shared__ __align__(16) MegaPhase ph_s[2];
-    __shared__ __align__(8) uint64_t desc_bar;
+    __shared__ __align__(8) uint64_t desc_bar[2];
     __shared__ __align__(16) float cs_row[HD];
     S.rc = &ring_state;
     S.cs = cs_row;
-    S.dbar = &desc_bar;
+    S.dbar = desc_bar;
 
     // the phase table into shared memory (the ring cursor reads only it)
     for (int i = threadIdx.x; i < a.n_ph; i += nct) reinterpret_cast<uint4 *>(smem + P.tab)[i] = __ldg(a.tab + i);
@@ -1372,7 +1375,8 @@ __global__ void __launch_bounds__(MEGA_THREADS, 1) k_decode_mega(MegaArgs a)
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.nst; s++) mbar_init(&S.full[s], 1);
         for (int k = 0; k < 5; k++) mbar_init(&S.abar[k], 1);
-        mbar_init(&desc_bar, 1);
+        mbar_init(desc_bar, 1);
+        mbar_init(desc_bar + 1, 1);
         mbar_init_fence();
         pos_s = a.st->pos;            // stable for the whole step
         launch_s = a.bar[3];
@@ -1405,15 +1409,24 @@ __global__ void __launch_bounds__(MEGA_THREADS, 1) k_decode_mega(MegaArgs a)
     for (int p = 0; p < a.n_ph; p++) {
         // descriptors live in shared memory: phase p's arrived by a bulk
         // copy issued at the start of phase p-1, and phase p+1's is issued
-        // now, so no phase starts with a global-memory round trip
-        if (p > 0) mbar_wait<true>(&desc_bar, (unsigned)(p - 1) & 1u, a.status);
+        // now, so no phase starts with a global-memory round trip.  Two
+        // barriers in turn: with one, a warp that comes to this wait after
+        // thread 0's next copy has landed finds it two phases on, which its
+        // parity cannot tell from not yet complete, and the block stands still
+        if constexpr (LATE_NS > 0)
+            if (threadIdx.x >= MEGA_THREADS - 32) {
+                const uint64_t t0 = globaltimer_ns();
+                while (globaltimer_ns() - t0 < LATE_NS) __nanosleep(500);
+            }
+        if (p > 0) mbar_wait<true>(desc_bar + (p & 1), (unsigned)(p - 1) >> 1 & 1u, a.status);
         const MegaPhase &ph = ph_s[p & 1];
         if (threadIdx.x == 0 && p + 1 < a.n_ph) {
             // the reads of that buffer (phase p-1's descriptor) are done:
             // every thread has passed the end of phase p-1
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_expect_tx(&desc_bar, (uint32_t)sizeof(MegaPhase));
-            bulk_g2s(&ph_s[(p + 1) & 1], a.ph + p + 1, (uint32_t)sizeof(MegaPhase), &desc_bar);
+            uint64_t *bar = desc_bar + ((p + 1) & 1);
+            mbar_expect_tx(bar, (uint32_t)sizeof(MegaPhase));
+            bulk_g2s(&ph_s[(p + 1) & 1], a.ph + p + 1, (uint32_t)sizeof(MegaPhase), bar);
         }
         const int kind = ph.kind;
         if (kind == PH_GEMV) {

@@ -126,6 +126,7 @@ SIGNATURES = [
                                             C.c_void_p, C.c_void_p]),
     ("ecu_set_wait_ns", C.c_int, [C.c_int, C.c_ulonglong]),
     ("ecu_inject_wait_timeout", C.c_int, [C.c_void_p]),
+    ("ecu_inject_late_warp", C.c_int, [C.c_void_p]),
     ("ecu_inject_prompt_timeout", C.c_int, [C.c_int]),
     ("ecu_matvec_bench", C.c_int, [C.c_uint, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int,
                                    C.c_int, C.c_int, C.POINTER(C.c_double)]),
@@ -415,6 +416,12 @@ class LlmCtx:
     def step_dev(self, stream: int | None = None) -> None:
         """One step from device-resident input (ecu_step_dev)."""
         if lib().ecu_step_dev(self.h, C.c_void_p(stream or 0)) != 0:
+            raise EngineError(last_error())
+
+    def inject_late_warp(self) -> None:
+        """One warp of every block comes late to each phase of the next
+        persistent step (ecu_inject_late_warp): failure-path testing."""
+        if lib().ecu_inject_late_warp(self.h) != 0:
             raise EngineError(last_error())
 
     def inject_wait_timeout(self) -> None:

@@ -490,7 +490,10 @@ int  ecu_batch_feed(ecu_batch *b, const int *seq, const int *n_tok, int n, const
  * tagged input, for an input word that no phase writes: its waits run out,
  * that step returns -1 with the timeout in ecu_last_error, and the context
  * steps normally again afterwards (reset it: that step's cache row is not
- * valid).  -1 for a context on the per-kernel step.
+ * valid).  -1 for a context on the per-kernel step.  ecu_inject_late_warp:
+ * in the next persistent step of `c` (4 query heads of 128 a KV head, one
+ * GPU) one warp of every block comes 10 us late to each phase, which changes
+ * nothing but the step's time.
  * ecu_inject_prompt_timeout: the next prompt attention on `device`
  * (ecu_attn_prompt, or inside ecu_batch_feed or ecu_prefill) never copies its
  * first keys, so that its waits run out: ecu_attn_prompt_status, or the call
@@ -499,6 +502,7 @@ int  ecu_batch_feed(ecu_batch *b, const int *seq, const int *n_tok, int n, const
  * them alike), number `launch`, from 0, fails. */
 int  ecu_set_wait_ns(int device, unsigned long long ns);
 int  ecu_inject_wait_timeout(ecu_ctx *c);
+int  ecu_inject_late_warp(ecu_ctx *c);
 int  ecu_inject_prompt_timeout(int device);
 int  ecu_kv_inject_failure(ecu_kv *kv, int launch);
 

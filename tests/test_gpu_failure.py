@@ -48,6 +48,36 @@ def test_wait_runs_out_and_context_recovers(eng, oracle_port, model_buf):
     c.close()
 
 
+def test_a_warp_that_comes_late_to_every_phase(eng, model_buf):
+    """A warp that reaches each phase long after the next phase's descriptor has landed: the step takes longer, and its
+    token, state and logits are the same bits."""
+    c = eng.LlmCtx(eng.GgufModel(model_buf("mini-q4", n_layer=4)), eng.STAGE_FULL, n_ctx=64)
+    assert c.path() == "persistent"
+    eng.set_wait_ns(200_000_000)                     # a step that stood still would give up after this
+    try:
+        outs = []
+        for late in (False, True, True, False):
+            c.reset()
+            steps = []
+            for t in (3, 9, 27, 81):
+                out = np.zeros(c.n_embd + 1, dtype=np.float32)
+                if late:
+                    c.inject_late_warp()
+                assert c.forward(t, out) == 0, eng.last_error()
+                steps.append((out.copy(), c.logits().copy()))
+            outs.append(steps)
+        for steps in outs[1:]:
+            for (a, la), (b, lb) in zip(outs[0], steps):
+                assert np.array_equal(a.view(np.uint32), b.view(np.uint32)) and np.array_equal(la.view(np.uint32), lb.view(np.uint32))
+    finally:
+        eng.set_wait_ns(2_000_000_000)
+    c.close()
+    c = eng.LlmCtx(eng.GgufModel(model_buf("mini-q8")), eng.STAGE_FULL, n_ctx=16)
+    with pytest.raises(eng.EngineError, match="4 query heads of 128"):
+        c.inject_late_warp()
+    c.close()
+
+
 def test_injection_needs_the_persistent_step(eng, model_buf, monkeypatch):
     monkeypatch.setenv("ECU_MEGA", "0")
     c = eng.LlmCtx(eng.GgufModel(model_buf("mini-q4")), eng.STAGE_FULL, n_ctx=16)
