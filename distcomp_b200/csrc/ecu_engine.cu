@@ -989,8 +989,11 @@ static int check_status(ecu_ctx *c)
         if (c->mega) {
             // counters and launch number restart at zero: the tagged vectors
             // must not hold words of an earlier launch with the same number
-            CK(cudaMemset(c->margs.bar, 0, (4 + (size_t)c->g.n_head_kv) * sizeof(unsigned)));
-            CK(cudaMemset(c->mega_ll, 0, c->mega_ll_words * sizeof(unsigned long long)));
+            // (on the context's stream: the legacy stream does not order
+            // against it, and a clear that ran into the next step would take
+            // its words away)
+            CK(cudaMemsetAsync(c->margs.bar, 0, (4 + (size_t)c->g.n_head_kv) * sizeof(unsigned), c->stream));
+            CK(cudaMemsetAsync(c->mega_ll, 0, c->mega_ll_words * sizeof(unsigned long long), c->stream));
         }
         if (s.status & ECU_STATUS_BADTOKEN)
             ecu_set_error(nullptr, 0, "the device-resident token is outside the vocabulary (%d)", c->g.n_vocab);
@@ -998,7 +1001,8 @@ static int check_status(ecu_ctx *c)
             ecu_set_error(nullptr, 0, "a query, key, value or attention row of a prompt or a large batch passes fp16's range (65504)");
         else
             ecu_set_error(nullptr, 0, "a kernel gave up on a bounded wait (status %d)", s.status);
-        CK(cudaMemset(&c->st->status, 0, sizeof(int)));
+        CK(cudaMemsetAsync(&c->st->status, 0, sizeof(int), c->stream));
+        CK(cudaStreamSynchronize(c->stream));
         return -1;
     }
     return 0;
@@ -1499,7 +1503,7 @@ static int mega_profile(ecu_ctx *c, int n_steps, ecu_kprof *out, int max_kinds)
     // [np + 1] global ns, [np + 1] CTA 0's SM clock at the same points, [np][4] detail
     const size_t nbuf = 2 * ((size_t)np + 1) + 4 * (size_t)np;
     CK(cudaMalloc(&d_ns, sizeof(unsigned long long) * nbuf));
-    CK(cudaMemset(d_ns, 0, sizeof(unsigned long long) * nbuf));
+    CK(cudaMemsetAsync(d_ns, 0, sizeof(unsigned long long) * nbuf, c->stream));
     std::vector<unsigned long long> ns(nbuf);
     unsigned long long *d_det = d_ns + 2 * (np + 1);
     int nk = 0;
@@ -3129,8 +3133,11 @@ int ecu_link_input(ecu_ctx *c)
             if (q.kind == PH_GEMV && q.in_ep == MEGA_EP_PLAIN) q.in_ep = MEGA_EP_LINK;
             if (q.kind == PH_GEMV && q.epi == EPI_ADD && q.y_ep == MEGA_EP_PLAIN) q.y_ep = MEGA_EP_LINK;
         }
-        CK(cudaMemcpy(const_cast<MegaPhase *>(c->margs.ph), c->mega_ph.data(), c->mega_ph.size() * sizeof(MegaPhase),
-                      cudaMemcpyHostToDevice));
+        // (on the context's stream, which the steps follow; a copy from
+        // pageable memory on the legacy stream may return before it is done)
+        CK(cudaMemcpyAsync(const_cast<MegaPhase *>(c->margs.ph), c->mega_ph.data(), c->mega_ph.size() * sizeof(MegaPhase),
+                           cudaMemcpyHostToDevice, c->stream));
+        CK(cudaStreamSynchronize(c->stream));
     }
     c->linked_in = true;
     return 0;
