@@ -130,6 +130,10 @@ static int *status_word(int device)
     return (int *)p;
 }
 
+// Reads and clears the word in one step, so that no flag that another stream's
+// call sets in between is lost.
+static __global__ void k_take_status(int *out) { *out = atomicExch(&g_prompt_status, 0); }
+
 extern "C" int ecu_attn_prompt_status(int device, void *stream)
 {
     int ndev = 0;
@@ -144,12 +148,13 @@ extern "C" int ecu_attn_prompt_status(int device, void *stream)
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     cudaError_t             e = cudaStreamIsCapturing(s, &cap);
     if (e == cudaSuccess && cap != cudaStreamCaptureStatusNone) return say("the status of a stream that is being captured is not known");
-    int *word = status_word(device), flags = 0;
-    if (!word) return say("the status word cannot be read");
-    if (e == cudaSuccess) e = cudaMemcpyAsync(&flags, word, sizeof flags, cudaMemcpyDeviceToHost, s);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-    if (e == cudaSuccess && flags) {
-        e = cudaMemsetAsync(word, 0, sizeof flags, s);
+    int *taken = nullptr, flags = 0;
+    if (e == cudaSuccess) e = cudaMallocAsync((void **)&taken, sizeof flags, s);
+    if (e == cudaSuccess) {
+        k_take_status<<<1, 1, 0, s>>>(taken);
+        e = cudaGetLastError();
+        if (e == cudaSuccess) e = cudaMemcpyAsync(&flags, taken, sizeof flags, cudaMemcpyDeviceToHost, s);
+        cudaFreeAsync(taken, s);
         if (e == cudaSuccess) e = cudaStreamSynchronize(s);
     }
     if (e != cudaSuccess) {
