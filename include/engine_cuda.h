@@ -391,7 +391,8 @@ int  ecu_kv_compact(ecu_kv *kv, void *stream);
  * cache holds them, `out_dtype`, rows of n_head_kv * head_dim without gaps,
  * apart from k and v.
  * The lengths are read on the device when the call runs, so a captured call
- * appends to the then newest positions. */
+ * appends to the then newest positions (whose pages must then be the
+ * sequence's own: that is checked when the call is made, not at a replay). */
 int  ecu_kv_append(ecu_kv *kv, int layer, int dtype, const void *k, const void *v, long k_stride, long v_stride,
                    const int *seq, const int *n_new, int n, int out_dtype, void *k_out, void *v_out, void *stream);
 
