@@ -25,7 +25,7 @@
 // error by the Remez exchange, whose extremes are equal: 7.5e-5 of degree 3 for
 // bf16, whose own step is 2^-8, 2.7e-6 of degree 4 for fp16).
 //
-// 8192 tokens, 32 heads of 128 over 8: 547 us, 1004 TFLOP/s; the walk's turn of
+// 8192 tokens, 32 heads of 128 over 8: 549 us, 1001 TFLOP/s; the walk's turn of
 // two tiles takes 1.5 times its products' time, the softmax of a tile being
 // longer than the other tile's products, and a pair 7 us beside its walk.
 //
