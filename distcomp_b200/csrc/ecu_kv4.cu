@@ -21,59 +21,10 @@
         }                                                                               \
     } while (0)
 
-#define KV4_LIST 1024             // sequences of one launch
-#define KV4_STREAMS 16            // streams that a pool keeps a workspace for
 
 static bool shape_ok(int n_head_kv, int head_dim)
 {
     return n_head_kv > 0 && n_head_kv <= 4096 && (head_dim == 32 || head_dim == 64 || head_dim == 96 || head_dim == 128);
-}
-
-static size_t dtype_bytes(int t) { return t == ECU_F32 ? 4 : t == ECU_F16 || t == ECU_BF16 ? 2 : 0; }
-
-static int say(const char *what, const char *why)
-{
-    ecu_set_error(nullptr, 0, "%s: %s", what, why);
-    return -1;
-}
-
-// Does [a, a + n) of whole numbers name existing slots?  (NULL: 0..n-1)
-static int slots_ok(const ecu_kv *kv, const int *seq, int n, const char *what)
-{
-    if (!seq && n > kv->book.n_seq) {
-        ecu_set_error(nullptr, 0, "%s: %d sequences of %d slots", what, n, kv->book.n_seq);
-        return -1;
-    }
-    for (int i = 0; seq && i < n; i++)
-        if (seq[i] < 0 || seq[i] >= kv->book.n_seq) {
-            ecu_set_error(nullptr, 0, "%s: no sequence %d (%d slots)", what, seq[i], kv->book.n_seq);
-            return -1;
-        }
-    return 0;
-}
-
-// 1: the stream is being captured, 0: it is not, -1: it cannot be used.
-static int capturing(cudaStream_t s, const char *what)
-{
-    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-    const cudaError_t       e = cudaStreamIsCapturing(s, &st);
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        ecu_set_error(nullptr, 0, "%s: the stream cannot be used: %s", what, cudaGetErrorString(e));
-        return -1;
-    }
-    return st != cudaStreamCaptureStatusNone;
-}
-
-static int launched(const char *what, cudaError_t e)
-{
-    if (e != cudaSuccess) {
-        cudaGetLastError();
-        ecu_set_error(nullptr, 0, "%s: launch failed: %s", what, cudaGetErrorString(e));
-        return -1;
-    }
-    ecu_count_launches(1);
-    return 0;
 }
 
 // ------------------------------------------------------------------ pool ---
@@ -123,12 +74,6 @@ static int update(ecu_kv *kv, cudaStream_t s)
     return 0;
 }
 
-// A pool that a failed launch left between two states takes no more calls.
-static int whole(const ecu_kv *kv, const char *what)
-{
-    return kv->broken ? say(what, "a launch of an earlier change failed: the pool can only be closed") : 0;
-}
-
 // The checks that every change of the pool begins with.
 static int change_ok(ecu_kv *kv, const void *list, const void *list2, int n, cudaStream_t s, const char *what)
 {
@@ -161,6 +106,7 @@ void ecu_kv_close(ecu_kv *kv)
     if (kv->device >= 0) {
         DeviceScope d(kv->device);
         for (auto &w : kv->ws) cudaFree(w.second);
+        for (auto &w : kv->tree_ws) cudaFree(w.second);
         if (kv->spare) cudaFree(kv->spare);
         if (kv->meta) cudaFree(kv->meta);
         if (kv->own_data && kv->data) cudaFree(kv->data);
@@ -298,6 +244,93 @@ int ecu_kv_compact(ecu_kv *kv, void *stream)
     const int n = 0;
     KV_CHANGE("ecu_kv_compact", nullptr, nullptr, kv->book.compact())
 }
+
+} // extern "C"
+
+struct KvMove { int from, to; uint16_t at; };
+
+template <int N>
+static int move_launch(ecu_kv *kv, const std::vector<KvMove> &moves, const std::vector<int> &first, size_t &i, size_t &j, cudaStream_t s)
+{
+    KvMoves<N> m;
+    m.n = 0;
+    m.first[0] = 0;
+    int k = 0;
+    while (k < N && j < moves.size()) {                   // a sequence that does not fit goes on in the next launch
+        const int take = std::min<int>(N - k, first[i + 1] - (int)j);
+        for (int x = 0; x < take; x++, k++, j++) {
+            m.from[k] = moves[j].from;
+            m.to[k] = moves[j].to;
+            m.at[k] = moves[j].at;
+        }
+        m.first[++m.n] = k;
+        if ((int)j == first[i + 1]) i++;
+    }
+    return launched("ecu_kv_keep", ecu_launch_early(k_kv4_move<N>, (unsigned)m.n * kv->n_layer, 256, 0, s, kv->data, kv->page_bytes,
+                                                    kv->page_bytes * kv->book.n_pages, kv->n_layer, kv->n_head_kv, kv->head_dim / 32, m));
+}
+
+extern "C" int ecu_kv_keep(ecu_kv *kv, const int *seq, const int *n_new, const int *kept, const int *n_kept, int n, void *stream)
+{
+    const char *what = "ecu_kv_keep";
+    if (change_ok(kv, seq, n_new, n, (cudaStream_t)stream, what) != 0) return -1;
+    if (n > 0 && !n_kept) return say(what, "null argument or negative count");
+    if (slots_ok(kv, seq, n, what) != 0) return -1;
+    bool changing = false;
+    try {
+        std::vector<bool>   seen((size_t)kv->book.n_seq, false);
+        std::vector<KvMove> moves;
+        std::vector<int>    first{0}, len;
+        for (int i = 0; i < n; i++) {
+            const auto &q = kv->book.seq[seq[i]];
+            if (seen[seq[i]]) {
+                ecu_set_error(nullptr, 0, "%s: sequence %d comes twice", what, seq[i]);
+                return -1;
+            }
+            seen[seq[i]] = true;
+            if (n_new[i] < 0 || n_new[i] > q.len || n_kept[i] < 0 || n_kept[i] > n_new[i] || (n_kept[i] > 0 && !kept)) {
+                ecu_set_error(nullptr, 0, "%s: %d rows of %d new ones of sequence %d of %d positions", what, n_kept[i], n_new[i], seq[i], q.len);
+                return -1;
+            }
+            const int base = q.len - n_new[i];
+            for (int t = 0; t < n_kept[i]; t++, kept++) {
+                if (*kept < t || *kept >= n_new[i] || (t > 0 && *kept <= kept[-1])) {
+                    ecu_set_error(nullptr, 0, "%s: the kept rows of sequence %d are not rising numbers below %d", what, seq[i], n_new[i]);
+                    return -1;
+                }
+                if (*kept == t) continue;
+                const int a = base + *kept, b = base + t, to = q.page[b / ECU_KV4_PAGE];
+                if (kv->book.ref[to] > 1) {
+                    ecu_set_error(nullptr, 0, "%s: positions of sequence %d lie in a page that other sequences hold", what, seq[i]);
+                    return -1;
+                }
+                moves.push_back({q.page[a / ECU_KV4_PAGE], to, (uint16_t)(a % ECU_KV4_PAGE | b % ECU_KV4_PAGE << 8)});
+            }
+            if ((int)moves.size() > first.back()) first.push_back((int)moves.size());
+            len.push_back(base + n_kept[i]);
+        }
+        std::optional<DeviceScope> d;
+        if (kv->device >= 0) d.emplace(kv->device);
+        if (d && !d->ok) return say(what, "the pool's device cannot be used");
+        // The tables first: a launch that fails there is taken back.  The moves
+        // name their pages themselves, and those given back are taken only by
+        // later calls.
+        changing = true;
+        if (kv->book.truncate(seq, len.data(), n) != 0 || update(kv, (cudaStream_t)stream) != 0) return -1;
+        for (size_t i = 0, j = 0; kv->device >= 0 && j < moves.size();)
+            if ((moves.size() - j <= 64 ? move_launch<64>(kv, moves, first, i, j, (cudaStream_t)stream)
+                                        : move_launch<512>(kv, moves, first, i, j, (cudaStream_t)stream)) != 0) {
+                kv->broken = true;
+                return -1;
+            }
+        return 0;
+    } catch (const std::exception &e) {
+        if (changing) kv->book.fail();
+        return say(what, e.what());
+    }
+}
+
+extern "C" {
 
 int ecu_kv_inject_failure(ecu_kv *kv, int launch)
 {

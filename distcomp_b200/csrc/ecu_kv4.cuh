@@ -224,6 +224,64 @@ __global__ void __launch_bounds__(256) k_kv4_update(uint8_t *data, size_t page_b
         if (at + k * 256 < n) dst[at + k * 256] = v[k];
 }
 
+// Rows moved within their sequences, by value: group i (a sequence) has moves
+// first[i] .. first[i + 1] - 1, in the order of its positions, towards lower ones.
+template <int N> struct KvMoves {
+    int      n;
+    int      first[N + 1];
+    int      from[N], to[N];          // pages
+    uint16_t at[N];                   // positions in them: from, and to << 8
+};
+
+#define KV4_MOVE_ITEMS 4          // blocks of 32 dimensions that a thread holds
+
+// A CTA per sequence and layer.  A row may be another's place, so a round of
+// moves is read whole before any of it is written; a later round reads only
+// positions behind all that were written.  A move of a KV head of 128
+// dimensions reads and writes 144 bytes.
+template <int N>
+__global__ void __launch_bounds__(256) k_kv4_move(uint8_t *data, size_t page_bytes, size_t layer_bytes, int n_layer, int n_kv, int nb,
+                                                  const __grid_constant__ KvMoves<N> m)
+{
+    pdl_wait();
+    pdl_trigger();
+    const int  i = blockIdx.x / n_layer, hd = nb * 32;
+    uint8_t   *layer = data + (size_t)(blockIdx.x - i * n_layer) * layer_bytes;
+    const int  heads = min(n_kv, 256 * KV4_MOVE_ITEMS / (2 * nb)), end = m.first[i + 1];
+    for (int h0 = 0; h0 < n_kv; h0 += heads) {
+        const int nh = min(heads, n_kv - h0), per = nh * 2 * nb, round = 256 * KV4_MOVE_ITEMS / per;
+        for (int m0 = m.first[i]; m0 < end; m0 += round) {
+            const int items = min(round, end - m0) * per;
+            uint4     code[KV4_MOVE_ITEMS];
+            uint16_t  scale[KV4_MOVE_ITEMS];
+            auto      each = [&](auto f) {
+#pragma unroll
+                for (int k = 0; k < KV4_MOVE_ITEMS; k++) {
+                    const int x = threadIdx.x + 256 * k;
+                    if (x >= items) continue;
+                    const int b = x % nb, side = x / nb % 2, h = h0 + x / (2 * nb) % nh, j = m0 + x / per;
+                    f(k, j, (size_t)h * 72 * hd, side, b);
+                }
+            };
+            auto code_at = [&](int side, int t, int b) { return side * 32 * hd + t * (hd / 2) + kv4_place(t, b, nb) * 16; };
+            auto scale_at = [&](int side, int t, int b) { return 64 * hd + side * 4 * hd + (t * nb + b) * 2; };
+            each([&](int k, int j, size_t head, int side, int b) {
+                const uint8_t *p = layer + (size_t)m.from[j] * page_bytes + head;
+                const int      t = m.at[j] & 255;
+                code[k] = *reinterpret_cast<const uint4 *>(p + code_at(side, t, b));
+                scale[k] = *reinterpret_cast<const uint16_t *>(p + scale_at(side, t, b));
+            });
+            __syncthreads();
+            each([&](int k, int j, size_t head, int side, int b) {
+                uint8_t  *p = layer + (size_t)m.to[j] * page_bytes + head;
+                const int t = m.at[j] >> 8;
+                *reinterpret_cast<uint4 *>(p + code_at(side, t, b)) = code[k];
+                *reinterpret_cast<uint16_t *>(p + scale_at(side, t, b)) = scale[k];
+            });
+        }
+    }
+}
+
 // ------------------------------------------------------------------ read ---
 // Positions pos .. pos + n - 1 of one sequence as rows of KV heads; a thread
 // per 8 values.  pages: the sequence's table row.

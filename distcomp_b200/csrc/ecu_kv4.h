@@ -2,6 +2,7 @@
 // translation units that use it.
 #pragma once
 #include "../../include/engine_cuda.h"
+#include "ecu_model.h"
 
 #include <atomic>
 #include <cuda_runtime.h>
@@ -60,6 +61,7 @@ struct ecu_kv {
     // per-thread default stream's names another stream in each thread)
     std::map<unsigned long long, void *> ws;
     void *spare = nullptr;            // the first stream's, allocated with the pool
+    std::map<unsigned long long, void *> tree_ws;         // the same for ecu_kv_attend_tree, made on a stream's first call
     bool  broken = false;             // a change ended between its launches: tables and bookkeeping differ
     int   inject = -1;                // ecu_kv_inject_failure: the launch of the next change that fails
     int *table() const { return meta; }
@@ -110,6 +112,62 @@ cudaError_t ecu_launch_early(void (*kern)(P...), unsigned grid, unsigned block, 
 }
 
 void ecu_count_launches(int n);       // ecu_kernel_launches()
+
+#define KV4_LIST 1024             // sequences of one launch
+#define KV4_STREAMS 16            // streams that a pool keeps a workspace for
+
+inline size_t dtype_bytes(int t) { return t == ECU_F32 ? 4 : t == ECU_F16 || t == ECU_BF16 ? 2 : 0; }
+
+inline int say(const char *what, const char *why)
+{
+    ecu_set_error(nullptr, 0, "%s: %s", what, why);
+    return -1;
+}
+
+// Does [a, a + n) of whole numbers name existing slots?  (NULL: 0..n-1)
+inline int slots_ok(const ecu_kv *kv, const int *seq, int n, const char *what)
+{
+    if (!seq && n > kv->book.n_seq) {
+        ecu_set_error(nullptr, 0, "%s: %d sequences of %d slots", what, n, kv->book.n_seq);
+        return -1;
+    }
+    for (int i = 0; seq && i < n; i++)
+        if (seq[i] < 0 || seq[i] >= kv->book.n_seq) {
+            ecu_set_error(nullptr, 0, "%s: no sequence %d (%d slots)", what, seq[i], kv->book.n_seq);
+            return -1;
+        }
+    return 0;
+}
+
+// 1: the stream is being captured, 0: it is not, -1: it cannot be used.
+inline int capturing(cudaStream_t s, const char *what)
+{
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    const cudaError_t       e = cudaStreamIsCapturing(s, &st);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        ecu_set_error(nullptr, 0, "%s: the stream cannot be used: %s", what, cudaGetErrorString(e));
+        return -1;
+    }
+    return st != cudaStreamCaptureStatusNone;
+}
+
+inline int launched(const char *what, cudaError_t e)
+{
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        ecu_set_error(nullptr, 0, "%s: launch failed: %s", what, cudaGetErrorString(e));
+        return -1;
+    }
+    ecu_count_launches(1);
+    return 0;
+}
+
+// A pool that a failed launch left between two states takes no more calls.
+inline int whole(const ecu_kv *kv, const char *what)
+{
+    return kv->broken ? say(what, "a launch of an earlier change failed: the pool can only be closed") : 0;
+}
 
 // ecu_attn_prompt with a status word of the caller's on the device (nullptr:
 // the one that ecu_attn_prompt_status reads): ECU_STATUS_TIMEOUT is set in it

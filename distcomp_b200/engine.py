@@ -153,6 +153,19 @@ SIGNATURES = [
                                 C.c_void_p, C.c_int, C.c_float, C.c_void_p, C.c_void_p]),
     ("ecu_kv_ws_bytes", C.c_size_t, [C.c_void_p]),
     ("ecu_kv_read", C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
+    ("ecu_rope_init", C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_double, C.c_int, C.c_double, C.c_double, C.c_double,
+                                C.c_double]),
+    ("ecu_rope_set", C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_double]),
+    ("ecu_kv_append_rope", C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
+                                     C.c_long, C.c_long, C.c_long, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p,
+                                     C.c_long, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
+    ("ecu_kv_attend_tree", C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_long, C.c_long,
+                                     C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_float, C.c_void_p, C.c_void_p]),
+    ("ecu_kv_tree_ws_bytes", C.c_size_t, [C.c_void_p]),
+    ("ecu_draft_verify", C.c_int, [C.c_int, C.c_void_p, C.c_long, C.c_int, C.c_void_p, C.c_long, C.c_void_p, C.c_void_p,
+                                   C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                   C.c_int, C.c_void_p]),
+    ("ecu_kv_keep", C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
     ("ecu_attn_prompt", C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
                                   C.c_long, C.c_long, C.c_long, C.c_long, C.c_void_p, C.c_void_p, C.c_int, C.c_float,
                                   C.c_int, C.c_void_p]),

@@ -221,6 +221,100 @@ class KvPool:
                                self._stream(stream)) != 0:
             raise EngineError(last_error())
 
+    def append_rope(self, layer: int, rope, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, seq, n_new,
+                    depth: torch.Tensor | None = None, q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None,
+                    v_out: torch.Tensor | None = None, stream: int | None = None) -> torch.Tensor | None:
+        """append() of keys turned by their positions (rope: draft.Rope), and the queries q beside them, turned into
+        q_out (which may be q; ecu_kv_append_rope).  depth: int32, one a row, how far behind the positions held before
+        the row stands; by default its number in its sequence."""
+        heads, hd, dev = self.n_head_kv, self.head_dim, self.device
+        _, ks = _row(k, "k", heads, hd, dev)
+        vs = ks if _like(v, k) else _row(v, "v", heads, hd, dev)[1]
+        n_new = _ints(n_new)
+        s = None if seq is None else _ints(seq)
+        n = len(n_new)
+        rows = sum(n_new.tolist()) if n <= 256 else int(n_new.sum(dtype=np.int64))
+        if (s is not None and len(s) != n) or k.shape[0] != rows or v.shape[0] != rows or k.dtype != v.dtype:
+            raise EngineError(f"k and v: {rows} rows of one type are wanted, and a count for each sequence")
+        qp = qo = None
+        nh = qs = qos = 0
+        if q is not None:
+            nh, qs = _row(q, "q", None, hd, dev)
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            qos = qs if _like(q_out, q) else _row(q_out, "q_out", nh, hd, dev)[1]
+            if q.dtype != k.dtype or q_out.dtype != q.dtype or q.shape[0] != rows or q_out.shape[0] != rows:
+                raise EngineError(f"q and q_out: {rows} rows of k's type are wanted")
+            qp, qo = q.data_ptr(), q_out.data_ptr()
+        elif q_out is not None:
+            raise EngineError("q_out without q")
+        if depth is not None and (depth.dtype != torch.int32 or depth.dim() != 1 or depth.shape[0] != rows or
+                                  not depth.is_contiguous() or not depth.is_cuda or depth.get_device() != dev):
+            raise EngineError(f"depth: {rows} int32 numbers on CUDA device {dev} are wanted")
+        if (k_out is None) != (v_out is None):
+            raise EngineError("k_out and v_out come together")
+        ko = vo = None
+        od = k.dtype
+        if k_out is not None:
+            _row(k_out, "k_out", heads, hd, dev)
+            if not _like(v_out, k_out):
+                _row(v_out, "v_out", heads, hd, dev)
+            if k_out.shape[0] != rows or v_out.shape[0] != rows or k_out.dtype != v_out.dtype or \
+                    not k_out.is_contiguous() or not v_out.is_contiguous():
+                raise EngineError(f"k_out and v_out: {rows} contiguous rows of one type are wanted")
+            ko, vo, od = k_out.data_ptr(), v_out.data_ptr(), k_out.dtype
+        if lib().ecu_kv_append_rope(self.h, self._layer(layer), rope.at, _DTYPES[k.dtype], qp, k.data_ptr(), v.data_ptr(), nh, qs, ks,
+                                    vs, None if s is None else _at(s), _at(n_new), n, None if depth is None else depth.data_ptr(),
+                                    qo, qos, _DTYPES[od], ko, vo, self._stream(stream)) != 0:
+            raise EngineError(last_error())
+        return q_out
+
+    def attend_tree(self, layer: int, q: torch.Tensor, seq, n_new, mask: torch.Tensor | None = None,
+                    out: torch.Tensor | None = None, scale: float | None = None, ws: torch.Tensor | None = None,
+                    stream: int | None = None) -> torch.Tensor:
+        """The newest n_new[i] positions of each sequence over those before them and, of themselves, those whose bit is
+        set in their mask (int64, one a row; draft.tree makes them; by default each row sees those before it;
+        ecu_kv_attend_tree).  ws: tree_workspace() for calls that are captured or may overlap."""
+        heads, qs = _row(q, "q", None, self.head_dim, self.device)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        os_ = qs if _like(out, q) else _row(out, "out", heads, self.head_dim, self.device)[1]
+        n_new = _ints(n_new)
+        s = None if seq is None else _ints(seq)
+        n, rows = len(n_new), int(n_new.sum(dtype=np.int64))
+        if out.dtype != q.dtype or out.shape[0] != rows or q.shape[0] != rows or (s is not None and len(s) != n):
+            raise EngineError(f"q and out: {rows} rows of one type are wanted, and a count for each sequence")
+        if mask is not None and (mask.dtype != torch.int64 or mask.dim() != 1 or mask.shape[0] != rows or
+                                 not mask.is_contiguous() or not mask.is_cuda or mask.get_device() != self.device):
+            raise EngineError(f"mask: {rows} int64 words on CUDA device {self.device} are wanted")
+        if ws is not None and (not ws.is_cuda or ws.get_device() != self.device or not ws.is_contiguous() or
+                               ws.numel() * ws.element_size() < self.tree_ws_bytes()):
+            raise EngineError(f"ws: {self.tree_ws_bytes()} contiguous bytes on CUDA device {self.device} are wanted")
+        if lib().ecu_kv_attend_tree(self.h, self._layer(layer), _DTYPES[q.dtype], q.data_ptr(), out.data_ptr(), heads, qs, os_,
+                                    None if s is None else _at(s), _at(n_new), n, None if mask is None else mask.data_ptr(),
+                                    self.head_dim ** -0.5 if scale is None else scale,
+                                    None if ws is None else ws.data_ptr(), self._stream(stream)) != 0:
+            raise EngineError(last_error())
+        return out
+
+    def tree_ws_bytes(self) -> int:
+        return int(lib().ecu_kv_tree_ws_bytes(self.h))
+
+    def tree_workspace(self) -> torch.Tensor:
+        """A workspace for attend_tree."""
+        return torch.empty(self.tree_ws_bytes(), dtype=torch.uint8, device=f"cuda:{self.device}")
+
+    def keep(self, seq, n_new, kept, stream: int | None = None) -> None:
+        """Of the newest n_new[i] positions of each sequence the rows kept[i] (rising) stay, moved together; the others
+        are given back (ecu_kv_keep)."""
+        s, n_new = _ints(seq), _ints(n_new)
+        if len(s) != len(n_new) or len(s) != len(kept):
+            raise EngineError(f"{len(s)} sequences, {len(n_new)} counts and {len(kept)} lists of rows")
+        count = _ints([len(r) for r in kept])
+        flat = _ints([j for r in kept for j in r])
+        if lib().ecu_kv_keep(self.h, _at(s), _at(n_new), _at(flat), _at(count), len(s), self._stream(stream)) != 0:
+            raise EngineError(last_error())
+
     def attend(self, layer: int, q: torch.Tensor, seq=None, out: torch.Tensor | None = None, scale: float | None = None,
                ws: torch.Tensor | None = None, stream: int | None = None) -> torch.Tensor:
         """One query row per sequence over all of its positions (ecu_kv_attend); ws: workspace() for calls that

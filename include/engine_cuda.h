@@ -418,6 +418,106 @@ size_t ecu_kv_ws_bytes(const ecu_kv *kv);
  * NULL): the cache's ecu_dequant_tensor.  Synchronises `stream`. */
 int    ecu_kv_read(ecu_kv *kv, int layer, int seq, int pos, int n, float *k, float *v, void *stream);
 
+/* ---- steps with drafted tokens ------------------------------------------- */
+
+/* A step may check several drafted tokens of a sequence at once: extend the
+ * sequence by them, write their rows (ecu_kv_append_rope), attend to the cache
+ * and to each other along a tree (ecu_kv_attend_tree), hold them against the
+ * target's probabilities (ecu_draft_verify), and keep what was accepted
+ * (ecu_kv_keep).  The drafted rows are a sequence's newest positions; row 0 is
+ * the token that was picked last, every other row hangs on an earlier one.  No
+ * counterpart in the reference, which feeds one token a step
+ * (src/shard.c:911-917). */
+#define ECU_DRAFT_ROWS 64     /* of a sequence, at most */
+
+/* A rotation: the first `rot` dimensions of a head turn in pairs, (i, i + rot/2)
+ * or, interleaved, (2i, 2i + 1), by the angle pos * w_i; both results are
+ * multiplied by `factor`.  turn[i] is w_i / 2 pi as a 64-bit fraction, so that
+ * pos * turn[i] modulo 2^64 is the fraction of a turn, however far the
+ * position.  Filled by the two functions below; rot 0 turns nothing. */
+typedef struct {
+    int      rot, interleaved;
+    double   factor;
+    uint64_t turn[64];
+} ecu_rope;
+/* w_i = base^(-2i/rot), and of those, for contexts longer than the trained
+ * `context`:  LINEAR  w_i / factor;  BANDS  pairs of fewer than `slow` turns
+ * over `context` w_i / factor, of more than `fast` w_i, between them a blend
+ * linear in the number of turns;  YARN  the same blend linear in the pair's
+ * number i, between the (rounded) numbers at which pairs turn `fast` and `slow`
+ * times, and the result's factor 0.1 ln(factor) + 1. */
+enum { ECU_ROPE_PLAIN = 0, ECU_ROPE_LINEAR = 1, ECU_ROPE_BANDS = 2, ECU_ROPE_YARN = 3 };
+int  ecu_rope_init(ecu_rope *r, int rot, int interleaved, double base, int scaling, double factor, double context,
+                   double slow, double fast);
+/* The caller's own frequencies, radians a position, rot / 2 of them. */
+int  ecu_rope_set(ecu_rope *r, int rot, int interleaved, const double *freq, double factor);
+
+/* ecu_kv_append of keys that are turned by their positions on the way, and of
+ * the queries beside them (q NULL: none): q_out row r = row r of q, turned.
+ * Row r of a sequence that gets n_new[i] rows is written at position len -
+ * n_new[i] + r and turned by the position len - n_new[i] + depth[r] (depth:
+ * device, one number for each row of the call; NULL: r), len read on the device
+ * when the call runs.  A key is turned and quantised in 64-bit arithmetic, its
+ * code that of the exact value; a query is turned in 32 bits and rounded once
+ * to `dtype`.  q_out may be q with its stride; else it is apart from the rows
+ * read.  Everything else as in ecu_kv_append. */
+int  ecu_kv_append_rope(ecu_kv *kv, int layer, const ecu_rope *rope, int dtype, const void *q, const void *k,
+                        const void *v, int n_head, long q_stride, long k_stride, long v_stride, const int *seq,
+                        const int *n_new, int n, const int *depth, void *q_out, long q_out_stride, int out_dtype,
+                        void *k_out, void *v_out, void *stream);
+
+/* Attention of the newest n_new[i] (at most ECU_DRAFT_ROWS) positions of each
+ * sequence seq[i] (NULL: slots 0..n-1; no slot twice) in layer `layer`: a row
+ * sees every position before them, and of them those whose bit is set in its
+ * mask (mask: device, one word for each row of the call, bit j its sequence's
+ * j-th drafted row; NULL: itself and those before it).  q and out: rows of
+ * consecutive sequences one after the other, as in ecu_kv_attend.  A row that
+ * sees nothing becomes zeros.  A position that a row sees and that is not
+ * finite in K makes the row NaN, one in V its block of 32 dimensions; positions
+ * that it does not see have no effect.  ws: ecu_kv_tree_ws_bytes() bytes of
+ * device memory that no other call uses at the same time; NULL: the pool's own
+ * for this stream, as in ecu_kv_attend.  The lengths are read on the device when
+ * the call runs, so a captured call follows its sequences. */
+int    ecu_kv_attend_tree(ecu_kv *kv, int layer, int dtype, const void *q, void *out, int n_head, long q_stride,
+                          long out_stride, const int *seq, const int *n_new, int n, const uint64_t *mask, float scale,
+                          void *ws, void *stream);
+size_t ecu_kv_tree_ws_bytes(const ecu_kv *kv);
+
+/* Drafted tokens held against the target's probabilities with given random
+ * numbers.  Sequence i has n_row[i] (at most ECU_DRAFT_ROWS) consecutive rows:
+ * logits [n_vocab] (`dtype`, rows `stride` elements apart), the token of each
+ * row and its parent, an earlier row of the sequence (row 0's are not looked
+ * at).  From row 0 on, rows are tried in order: one that hangs on the current
+ * row, with token x, is accepted where u[row] q(x) F < f(x), and becomes the
+ * current one.  f is softmax(logits / temperature) of the current row, F its
+ * sum, q the distribution that its children were drawn from: row `current` of
+ * draft (fp32, rows draft_stride apart), or 1 where draft is NULL (the drafter
+ * does not draw).  A rejected row leaves f <- max(f / F - q, 0), or f(x) <- 0;
+ * where nothing is left of f it is softmax(logits / temperature) again.  At the
+ * end next[i] is the first x with f(x) > 0 whose running sum passes
+ * u_next[i] F.  A temperature (one a sequence; NULL: 1) that is not above 0
+ * takes the first of the largest logits instead, and accepts it alone.
+ * Everything compared is 64-bit.  A token outside the vocabulary is not tried.
+ * A row whose logits hold a NaN or +infinity, or -infinity alone, ends the walk
+ * with next[i] = -1 when it becomes the current one.
+ * kept: the accepted rows, numbered within their sequence, row 0 first, in the
+ * first n_kept[i] of the sequence's n_row[i] words, -1 in the others; a
+ * sequence without rows has n_kept 0 and next -1.  All but n_row are device
+ * memory. */
+int  ecu_draft_verify(int dtype, const void *logits, long stride, int n_vocab, const float *draft, long draft_stride,
+                      const int *token, const int *parent, const int *n_row, int n, const float *u, const float *u_next,
+                      const float *temperature, int *kept, int *n_kept, int *next, int device, void *stream);
+
+/* Of the newest n_new[i] positions of sequence seq[i] (no slot twice) the
+ * n_kept[i] rows named in `kept` (host, the sequences' lists one after the
+ * other; rising numbers below n_new[i]) stay, moved together behind the
+ * positions before them in every layer; the others are given back as by
+ * ecu_kv_truncate.  Positions that rows move to must lie in the sequence's own
+ * pages.  A change of the pool like those above. */
+int  ecu_kv_keep(ecu_kv *kv, const int *seq, const int *n_new, const int *kept, const int *n_kept, int n, void *stream);
+
+/* ---- packed prompts ------------------------------------------------------- */
+
 /* Causal attention of packed prompts, on the tensor cores: sequence s has
  * query rows cu_q[s] .. cu_q[s+1]-1 and key/value rows cu_k[s] .. cu_k[s+1]-1
  * (host arrays of n_seq + 1 non-decreasing offsets from 0; cu_k NULL: the
