@@ -14,7 +14,8 @@
 #define PA_LIST 1024              // sequences of one launch
 
 // Set where a wait of a caller's own call gave up (the engine's calls name
-// their context's word), until ecu_attn_prompt_status reads it.
+// their context's word), or one of ecu_kv_attend_tree, until
+// ecu_attn_prompt_status reads it.
 static __device__ int g_prompt_status;
 
 static std::atomic<unsigned> g_stall{0};        // devices (bits) whose next call's waits run out
@@ -115,8 +116,7 @@ static int launch_all(const CUtensorMap (&m)[3], const PromptArgs &a, int head_d
 
 int ecu_prompt_set_wait(unsigned long long ns) { return set_wait_limit(ns) == cudaSuccess ? 0 : -1; }
 
-// The status word's address on the current device; nullptr: it cannot be had.
-static int *status_word(int device)
+int *ecu_prompt_status_word(int device)
 {
     static std::atomic<int *> at[32];
     void                     *p = device < 32 ? at[device].load() : nullptr;
@@ -221,7 +221,7 @@ int ecu_attn_prompt_on(int *status, int dtype, const void *q, const void *k, con
     }
     DeviceScope d(device);
     if (!d.ok) return say("the device cannot be used");
-    if (!status && !(status = status_word(device))) return say("the status word cannot be had");
+    if (!status && !(status = ecu_prompt_status_word(device))) return say("the status word cannot be had");
     PromptArgs  a{v, out, v_stride, out_stride, n_head_kv, n_head / n_head_kv, scale, status, 0};
     CUtensorMap m[3];
     // a pointer that no row is read from is not mapped: q stands in

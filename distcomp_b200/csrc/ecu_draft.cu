@@ -1,10 +1,8 @@
 // ecu_draft.cu -- a step with drafted tokens behind engine_cuda.h: rows turned
-// by their positions and appended, the attention of a tree of drafted rows, and
-// the drafts' verification.  (ecu_kv_keep, a change of the pool, is in
-// ecu_kv4.cu.)
-#include "ecu_kv4.h"
+// by their positions and appended, and the drafts' verification.  (The attention
+// is in ecu_tree.cu, ecu_kv_keep, a change of the pool, in ecu_kv4.cu.)
+#include "ecu_draft.h"
 #include "ecu_rope.cuh"
-#include "ecu_tree.cuh"
 #include "ecu_verify.cuh"
 
 #include <algorithm>
@@ -21,43 +19,6 @@
             return -1;                                                                  \
         }                                                                               \
     } while (0)
-
-static int number_of(int first, const int *seq, int i) { return seq ? seq[i] : first + i; }
-
-// What append_rope and attend_tree ask of their lists: slots that exist, none
-// twice, at most `most` new rows of each and no more than it holds.  The rows
-// in all, or -1.
-static long long rows_ok(const ecu_kv *kv, const int *seq, const int *n_new, int n, int most, const char *what)
-{
-    if (slots_ok(kv, seq, n, what) != 0) return -1;
-    long long         rows = 0;
-    std::vector<bool> seen((size_t)kv->book.n_seq, false);
-    for (int i = 0; i < n; i++) {
-        const int s = number_of(0, seq, i);
-        if (seen[s]) {
-            ecu_set_error(nullptr, 0, "%s: sequence %d comes twice", what, s);
-            return -1;
-        }
-        seen[s] = true;
-        if (n_new[i] < 0 || n_new[i] > kv->book.seq[s].len || n_new[i] > most) {
-            ecu_set_error(nullptr, 0, "%s: %d rows for sequence %d of %d positions%s", what, n_new[i], s, kv->book.seq[s].len,
-                          n_new[i] > most ? " (64 drafted rows at most)" : "");
-            return -1;
-        }
-        rows += n_new[i];
-    }
-    return rows;
-}
-
-template <int N> static void fill_rows(KvRows<N> &r, const int *seq, int first, const int *n_new, int n)
-{
-    r.n = n;
-    r.row0[0] = 0;
-    for (int i = 0; i < n; i++) {
-        r.seq[i] = (uint16_t)number_of(first, seq, i);
-        r.row0[i + 1] = r.row0[i] + n_new[i];
-    }
-}
 
 // -------------------------------------------------------------- rotation ---
 
@@ -254,184 +215,6 @@ extern "C" int ecu_kv_append_rope(ecu_kv *kv, int layer, const ecu_rope *rope, i
         if (dtype == ECU_F32) return rope_out<float>(kv, a, out_dtype, seq, n_new, n, s);
         if (dtype == ECU_F16) return rope_out<__half>(kv, a, out_dtype, seq, n_new, n, s);
         return rope_out<__nv_bfloat16>(kv, a, out_dtype, seq, n_new, n, s);
-    } catch (const std::exception &e) {
-        return say(what, e.what());
-    }
-}
-
-// ------------------------------------------------------------------ tree ---
-
-extern "C" size_t ecu_kv_tree_ws_bytes(const ecu_kv *kv)
-{
-    return kv && kv->device >= 0 ? (size_t)kv->sms * 2 * TREE_MAX_WC * 16 * (kv->head_dim + 2) * sizeof(float) : 0;
-}
-
-// The pool's own workspace for a stream: by the stream's id, since handles are
-// reused and the per-thread default stream's names another in each thread.
-static int tree_workspace(ecu_kv *kv, cudaStream_t s, void **ws)
-{
-    unsigned long long id = 0;
-    CK(cudaStreamGetId(s, &id));
-    const size_t bytes = ecu_kv_tree_ws_bytes(kv);
-    if (kv->tree_ws.size() >= KV4_STREAMS && !kv->tree_ws.count(id)) {       // streams come and go: start over
-        CK(cudaDeviceSynchronize());
-        for (auto &w : kv->tree_ws) {
-            cudaFree(w.second);
-            kv->device_bytes -= bytes;
-        }
-        kv->tree_ws.clear();
-    }
-    auto at = kv->tree_ws.find(id);
-    if (at == kv->tree_ws.end()) {
-        void *p = nullptr;
-        CK(cudaMalloc(&p, bytes));
-        try {
-            at = kv->tree_ws.emplace(id, p).first;
-        } catch (...) {
-            cudaFree(p);
-            throw;
-        }
-        kv->device_bytes += bytes;
-    }
-    *ws = at->second;
-    return 0;
-}
-
-template <typename T, int NB, int N>
-static int tree_launch(ecu_kv *kv, TreeArgs a, const int *seq, int first, const int *n_new, int n, bool captured, cudaStream_t s)
-{
-    using S = TreeShape<T, NB>;
-    KvRows<N> r;
-    fill_rows(r, seq, first, n_new, n);
-    if (r.row0[n] == 0) return 0;
-    // Tiles of a group: the width at which the sequences' units cost least (a
-    // unit of a group of wc warps occupies them all, whether a warp has a tile
-    // or not, and no unit passes faster than its bytes arrive)
-    double best = 0.0;
-    for (int wc = TREE_MAX_WC; wc >= 1; wc--) {
-        double cost = 0.0;
-        for (int i = 0; i < n; i++) {
-            const TreePlan p = tree_plan(kv->book.seq[r.seq[i]].len, n_new[i], a.n_kv, a.n_rep, S::C, wc);
-            cost += (double)p.rows * p.nu * std::max(wc, 1) * (wc == 1 ? 1.2 : 1.0);
-        }
-        if (wc == TREE_MAX_WC || cost < best) {
-            best = cost;
-            a.wc = wc;
-        }
-    }
-    // One CTA an SM; fewer where a group would find less than two units.  Rows
-    // of one length that fill whole CTAs are not shared, and need no join.
-    const int WP = TREE_WARPS / a.wc;
-    long long want = 0, rows = 0, places = -1;
-    bool      even = true;
-    for (int i = 0; i < n; i++) {
-        const TreePlan p = tree_plan(kv->book.seq[r.seq[i]].len, n_new[i], a.n_kv, a.n_rep, S::C, a.wc);
-        if (!p.rows) continue;
-        rows += p.rows;
-        want += (long long)p.rows * std::max(1, p.nu / (2 * WP));
-        even = even && (places < 0 || places == p.nu);
-        places = p.nu;
-    }
-    const int  grid = captured ? kv->sms : (int)std::max(1ll, std::min<long long>(kv->sms, want));
-    const bool shared = captured || !even || rows % grid != 0;
-    const size_t smem = S::smem(n);
-    auto         kern = k_kv4_tree<T, NB, N>;
-    static std::atomic<unsigned> done{0};
-    CK(ecu_allow_smem(kern, S::smem(N), kv->device, done));
-    if (launched("ecu_kv_attend_tree", ecu_launch_early(kern, (unsigned)grid, TREE_WARPS * 32, smem, s, a, r)) != 0) return -1;
-    if (!shared) return 0;
-    const unsigned blocks = (unsigned)grid * ((a.wc * S::C + 7) / 8);
-    return launched("ecu_kv_attend_tree", ecu_launch_early(k_kv4_tree_join<T, NB, N>, blocks, 256, 0, s, a, r, grid));
-}
-
-template <typename T, int NB> static int tree_list(ecu_kv *kv, TreeArgs a, const int *seq, const int *n_new, int n, bool captured, cudaStream_t s)
-{
-    // at most 2^31 - 1 places in a launch, however the sequences may grow
-    const TreePlan  p = tree_plan(kv->book.max_pages * KV4_PAGE, TREE_ROWS, a.n_kv, a.n_rep, TreeShape<T, NB>::C, 1);
-    const long long places = (long long)p.rows * (p.nu + TREE_OPEN);
-    if (places > INT_MAX) return say("ecu_kv_attend_tree", "too many positions and heads a sequence");
-    const int most = (int)std::min<long long>(KV4_LIST, INT_MAX / places);
-    for (int i = 0; i < n; i += most) {
-        const int  m = std::min(most, n - i);
-        const int *q = seq ? seq + i : nullptr;
-        if ((m <= 64 ? tree_launch<T, NB, 64>(kv, a, q, i, n_new + i, m, captured, s)
-                     : tree_launch<T, NB, KV4_LIST>(kv, a, q, i, n_new + i, m, captured, s)) != 0)
-            return -1;
-        size_t rows = 0;
-        for (int j = 0; j < m; j++) rows += n_new[i + j];
-        a.q = (const T *)a.q + rows * a.q_stride;
-        a.out = (T *)a.out + rows * a.out_stride;
-        if (a.mask) a.mask += rows;
-    }
-    return 0;
-}
-
-template <typename T> static int tree_dim(ecu_kv *kv, const TreeArgs &a, const int *seq, const int *n_new, int n, bool captured, cudaStream_t s)
-{
-    switch (kv->head_dim / 32) {
-    case 1: return tree_list<T, 1>(kv, a, seq, n_new, n, captured, s);
-    case 2: return tree_list<T, 2>(kv, a, seq, n_new, n, captured, s);
-    case 3: return tree_list<T, 3>(kv, a, seq, n_new, n, captured, s);
-    default: return tree_list<T, 4>(kv, a, seq, n_new, n, captured, s);
-    }
-}
-
-extern "C" int ecu_kv_attend_tree(ecu_kv *kv, int layer, int dtype, const void *q, void *out, int n_head, long q_stride, long out_stride,
-                                  const int *seq, const int *n_new, int n, const uint64_t *mask, float scale, void *ws, void *stream)
-{
-    const char *what = "ecu_kv_attend_tree";
-    if (!kv || n < 0 || (n > 0 && !n_new)) return say(what, "null argument or negative count");
-    if (layer < 0 || layer >= kv->n_layer) {
-        ecu_set_error(nullptr, 0, "%s: layer %d of %d", what, layer, kv->n_layer);
-        return -1;
-    }
-    const size_t es = dtype_bytes(dtype);
-    if (!es) return say(what, "unknown element type");
-    if (n_head < 1 || n_head % kv->n_head_kv || n_head / kv->n_head_kv > 4096 || n_head > INT_MAX / kv->head_dim) {
-        ecu_set_error(nullptr, 0, "%s: %d query heads for %d KV heads", what, n_head, kv->n_head_kv);
-        return -1;
-    }
-    if (!std::isfinite(scale)) return say(what, "the scale is not finite");
-    if (whole(kv, what) != 0) return -1;
-    try {
-        const long long rows = rows_ok(kv, seq, n_new, n, TREE_ROWS, what);
-        if (rows < 0) return -1;
-        if (rows == 0) return 0;
-        const long row = (long)n_head * kv->head_dim;
-        if (!q || !out) return say(what, "null rows");
-        if (rows > 1 && (q_stride < row || out_stride < row)) return say(what, "rows overlap: a stride below n_head * head_dim");
-        if (((uintptr_t)q | (uintptr_t)out) % es || ((uintptr_t)ws & 15) || ((uintptr_t)mask & 7))
-            return say(what, "rows, masks or workspace are not aligned");
-        if (kv->device < 0) return say(what, "the pool has no device");
-        DeviceScope d(kv->device);
-        if (!d.ok) return say(what, "the pool's device cannot be used");
-        const cudaStream_t s = (cudaStream_t)stream;
-        const int          cap = capturing(s, what);
-        if (cap < 0) return -1;
-        if (!ws) {
-            if (cap) return say(what, "a captured call needs a workspace of its own");
-            if (tree_workspace(kv, s, &ws) != 0) return -1;
-        }
-        TreeArgs a = {};
-        a.q = q;
-        a.out = out;
-        a.q_stride = q_stride;
-        a.out_stride = out_stride;
-        a.layer = kv->data + (size_t)layer * kv->book.n_pages * kv->page_bytes;
-        a.page_bytes = kv->page_bytes;
-        a.table = kv->table();
-        a.len = kv->len();
-        a.mask = (const long long *)mask;
-        a.max_pages = kv->book.max_pages;
-        a.n_pages = kv->book.n_pages;
-        a.n_kv = kv->n_head_kv;
-        a.n_rep = n_head / kv->n_head_kv;
-        a.scale = scale;
-        a.wide_q = !(((uintptr_t)q | (uintptr_t)(q_stride * (long)es)) & 15);
-        a.part = (float *)ws;
-        if (dtype == ECU_F16) return tree_dim<__half>(kv, a, seq, n_new, n, cap, s);
-        if (dtype == ECU_BF16) return tree_dim<__nv_bfloat16>(kv, a, seq, n_new, n, cap, s);
-        return tree_dim<float>(kv, a, seq, n_new, n, cap, s);
     } catch (const std::exception &e) {
         return say(what, e.what());
     }

@@ -2837,7 +2837,7 @@ int ecu_set_wait_ns(int device, unsigned long long ns)
     }
     CK(cudaSetDevice(device));
     CK(set_wait_limit(ns));
-    if (ecu_prompt_set_wait(ns) != 0) {
+    if (ecu_prompt_set_wait(ns) != 0 || ecu_draft_set_wait(ns) != 0) {
         ecu_set_error(nullptr, 0, "ecu_set_wait_ns: %s", cudaGetErrorString(cudaGetLastError()));
         return -1;
     }

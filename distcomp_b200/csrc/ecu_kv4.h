@@ -176,9 +176,14 @@ int ecu_attn_prompt_on(int *status, int dtype, const void *q, const void *k, con
                        int head_dim, long q_stride, long k_stride, long v_stride, long out_stride, const int *cu_q, const int *cu_k,
                        int n_seq, float scale, int device, void *stream);
 
-// ecu_set_wait_ns for the prompt attention's translation unit, on the current
-// device.
+// The word that ecu_attn_prompt_status reads, on the current device; nullptr:
+// it cannot be had.
+int *ecu_prompt_status_word(int device);
+
+// ecu_set_wait_ns for the translation units of the prompt's and the drafts'
+// attention, on the current device.
 int ecu_prompt_set_wait(unsigned long long ns);
+int ecu_draft_set_wait(unsigned long long ns);
 
 // Positions 0..n-1 of a sequence as fp16 rows [n][n_head_kv * head_dim] in
 // device memory, as the cache holds them.

@@ -45,8 +45,10 @@ struct TreeArgs {
     const int     *table, *len;
     const long long *mask;        // nullptr: each row sees those before it
     int            max_pages, n_pages, n_kv, n_rep, wc;
+    int            group;         // columns of a row: wc tiles of them
+    int            entry;         // columns of a partial
     float          scale;
-    bool           wide_q;
+    bool           wide_q, wide_out;
     float         *part;          // workspace: partials of rows that several CTAs share
 };
 
@@ -54,73 +56,141 @@ template <typename T, int NB> struct TreeShape {
     static constexpr int HD = NB * 32, P = KvSplit<T>::N, C = 16 / P;       // columns of a tile
     static constexpr int STAGE = 36 * HD;                                   // one unit
     static constexpr int LD = HD + 4;                                       // a column of a warp's partial
-    static constexpr int ENTRY = TREE_MAX_WC * C * (HD + 2);                // a partial: sums, M and the weights' sum of each column
+    static constexpr int EC = TREE_MAX_WC * C;                              // columns of a partial: sums, then M, then the weights' sum of each
     static constexpr size_t ring = (size_t)24 * STAGE, parts = (size_t)TREE_WARPS * C * LD * 4;
     static constexpr size_t smem(int n) { return ring + parts + (size_t)(n + 1) * 4; }
 };
 
-// Places of one sequence's rows (KV heads times groups of tiles).
+// Places of one sequence's rows (KV heads times groups of columns).
 struct TreePlan {
-    int nu, rows, n_cg;           // units of a row, rows, groups of tiles
+    int nu, rows, n_cg;           // units of a row, rows, groups of columns
 };
-__host__ __device__ inline TreePlan tree_plan(int len, int n_new, int n_kv, int n_rep, int per_tile, int wc)
+// unit: positions of a unit; group: columns of a row
+__host__ __device__ inline TreePlan tree_plan(int len, int n_new, int n_kv, int n_rep, int group, int unit)
 {
     TreePlan p;
-    p.nu = n_new > 0 && len > 0 ? (len + KV4_UNIT - 1) / KV4_UNIT : 0;
-    p.n_cg = (n_new * n_rep + per_tile * wc - 1) / (per_tile * wc);
+    p.nu = n_new > 0 && len > 0 ? (len + unit - 1) / unit : 0;
+    p.n_cg = (n_new * n_rep + group - 1) / group;
     p.rows = p.nu ? n_kv * p.n_cg : 0;
     return p;
 }
 __host__ __device__ inline int tree_places(const TreePlan &p) { return p.rows * (p.nu + TREE_OPEN); }
 
-// pre[i]: places before sequence i, by the whole block of NT threads.
+// pre[i]: places before sequence i, by the first NT threads of a block that
+// meets as a whole.
 template <int NT, int N>
-__device__ __forceinline__ void tree_scan(const TreeArgs &a, const KvRows<N> &rows, int per_tile, int *pre, int *sums)
+__device__ __forceinline__ void tree_scan(const TreeArgs &a, const KvRows<N> &rows, int unit, int *pre, int *sums)
 {
     constexpr int PER = (N + NT - 1) / NT;
     const int     tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = rows.n;
-    int           c[PER], sum = 0;
+    int           c[PER], sum = 0, run = 0;
 #pragma unroll
     for (int k = 0; k < PER; k++) {
         const int i = tid * PER + k;
         c[k] = 0;
-        if (i < n) {
+        if (i < n && tid < NT) {
             const int len = min(max(__ldg(a.len + rows.seq[i]), 0), a.max_pages * KV4_PAGE);
-            c[k] = tree_places(tree_plan(len, rows.row0[i + 1] - rows.row0[i], a.n_kv, a.n_rep, per_tile, a.wc));
+            c[k] = tree_places(tree_plan(len, rows.row0[i + 1] - rows.row0[i], a.n_kv, a.n_rep, a.group, unit));
         }
         sum += c[k];
     }
-    int run = sum;
+    if (tid < NT) {
+        run = sum;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, run, o);
-        if (lane >= o) run += v;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += v;
+        }
+        if (lane == 31) sums[warp] = run;
     }
-    if (lane == 31) sums[warp] = run;
     __syncthreads();
-    run -= sum;
-    for (int w = 0; w < warp; w++) run += sums[w];
+    if (tid < NT) {
+        run -= sum;
+        for (int w = 0; w < warp; w++) run += sums[w];
 #pragma unroll
-    for (int k = 0; k < PER; k++) {
-        const int i = tid * PER + k;
-        if (i < n) pre[i] = run;
-        run += c[k];
-        if (i == n - 1) pre[n] = run;
+        for (int k = 0; k < PER; k++) {
+            const int i = tid * PER + k;
+            if (i < n) pre[i] = run;
+            run += c[k];
+            if (i == n - 1) pre[n] = run;
+        }
     }
     __syncthreads();
 }
 
-// A row: sequence i, KV head r / n_cg, group of tiles r % n_cg; its first place,
-// and the units of it that fall to the CTA whose places are [cu0, cu1).
-struct TreeRow {
-    int i, r, nu, rows, n_cg, place, j0, j1;
+// A row: sequence i, KV head r / n_cg, group of columns r % n_cg; its first
+// place, and the units [j0, j1) of it that fall to the CTA with the places
+// [cu0, cu1).  first() and next() walk the rows that have units there: places
+// are TREE_OPEN and then one a unit.
+template <int N> struct TreeWalk {
+    const TreeArgs  &a;
+    const KvRows<N> &rows;
+    const int       *pre;
+    int              unit, total, cu0, cu1;
+    int              i, r, nu, n_rows, n_cg, place, j0, j1;
+
+    __device__ __forceinline__ TreeWalk(const TreeArgs &a_, const KvRows<N> &rows_, const int *pre_, int unit_, int cta, int ctas)
+        : a(a_), rows(rows_), pre(pre_), unit(unit_), total(pre_[rows_.n])
+    {
+        cu0 = (int)((long long)total * cta / ctas);
+        cu1 = (int)((long long)total * (cta + 1) / ctas);
+        int lo = 0, hi = rows.n;                          // the last sequence whose places begin at or before cu0
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (pre[mid] <= cu0) lo = mid;
+            else hi = mid;
+        }
+        i = lo;
+        enter();
+        r = (cu0 - place) / (nu + TREE_OPEN);
+        place += r * (nu + TREE_OPEN);
+        range();
+        while (place < cu1 && j1 <= j0) next();           // (its units end before the run, or begin behind it)
+    }
+    __device__ __forceinline__ int  len() const { return min(max(__ldg(a.len + rows.seq[i]), 0), a.max_pages * KV4_PAGE); }
+    __device__ __forceinline__ void range()
+    {
+        j0 = max(0, cu0 - place - TREE_OPEN);
+        j1 = min(nu, cu1 - place - TREE_OPEN);
+    }
+    __device__ __forceinline__ void enter()
+    {
+        const TreePlan p = tree_plan(len(), rows.row0[i + 1] - rows.row0[i], a.n_kv, a.n_rep, a.group, unit);
+        nu = p.nu;
+        n_rows = p.rows;
+        n_cg = p.n_cg;
+        r = 0;
+        place = pre[i];
+    }
+    __device__ __forceinline__ bool here() const { return place < cu1 && j1 > j0; }
+    __device__ __forceinline__ void next()
+    {
+        place += nu + TREE_OPEN;
+        if (++r == n_rows) {
+            do i++;
+            while (i < rows.n && pre[i + 1] == pre[i]);
+            if (i < rows.n) enter();
+            else place = total;
+        }
+        range();
+    }
+    __device__ __forceinline__ int page(int j) const { return __ldg(a.table + (size_t)rows.seq[i] * a.max_pages + j); }
 };
+
+// A sequence without positions: zeros.
+template <typename T, int N> __device__ __forceinline__ void tree_zeros(const TreeArgs &a, const KvRows<N> &rows, const int *pre, int hd)
+{
+    for (int i = blockIdx.x; i < rows.n; i += gridDim.x)
+        if (pre[i + 1] == pre[i])
+            for (int r = rows.row0[i]; r < rows.row0[i + 1]; r++)
+                for (int x = threadIdx.x; x < a.n_kv * a.n_rep * hd; x += blockDim.x) ((T *)a.out)[(size_t)r * a.out_stride + x] = kv4_from<T>(0.0f);
+}
 
 template <typename T, int NB, int N>
 __global__ void __launch_bounds__(TREE_WARPS * 32, 1) k_kv4_tree(const __grid_constant__ TreeArgs a, const __grid_constant__ KvRows<N> rows)
 {
     using S = TreeShape<T, NB>;
-    constexpr int HD = S::HD, P = S::P, C = S::C, STAGE = S::STAGE, LD = S::LD, ENTRY = S::ENTRY, RR = P == 2 ? 1 : 2;
+    constexpr int HD = S::HD, P = S::P, C = S::C, STAGE = S::STAGE, LD = S::LD, RR = P == 2 ? 1 : 2;
     extern __shared__ __align__(128) uint8_t smem[];
     float *parts = reinterpret_cast<float *>(smem + S::ring);
     int   *pre = reinterpret_cast<int *>(smem + S::ring + S::parts);
@@ -128,79 +198,32 @@ __global__ void __launch_bounds__(TREE_WARPS * 32, 1) k_kv4_tree(const __grid_co
     __shared__ int   sums[TREE_WARPS];
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-    const int n = rows.n, cap = a.max_pages * KV4_PAGE, WC = a.wc, WP = TREE_WARPS / WC, wc = warp % WC, wp = warp / WC;
+    const int WC = a.wc, WP = TREE_WARPS / WC, wc = warp % WC, wp = warp / WC;
     pdl_wait();
     pdl_trigger();
-    tree_scan<TREE_WARPS * 32>(a, rows, C, pre, sums);
-
-    auto len_of = [&](int i) { return min(max(__ldg(a.len + rows.seq[i]), 0), cap); };
-    // a sequence without positions: zeros
-    for (int i = blockIdx.x; i < n; i += gridDim.x)
-        if (pre[i + 1] == pre[i]) {
-            const int width = a.n_kv * a.n_rep * HD;
-            for (int r = rows.row0[i]; r < rows.row0[i + 1]; r++)
-                for (int x = tid; x < width; x += TREE_WARPS * 32) ((T *)a.out)[(size_t)r * a.out_stride + x] = kv4_from<T>(0.0f);
-        }
-    const int total = pre[n], ctas = min((int)gridDim.x, total);
+    tree_scan<TREE_WARPS * 32>(a, rows, KV4_UNIT, pre, sums);
+    tree_zeros<T>(a, rows, pre, HD);
+    const int ctas = min((int)gridDim.x, pre[rows.n]);
     if ((int)blockIdx.x >= ctas) return;
-    const int cu0 = (int)((long long)total * blockIdx.x / ctas), cu1 = (int)((long long)total * (blockIdx.x + 1) / ctas);
-
-    auto range = [&](TreeRow &w) {
-        w.j0 = max(0, cu0 - w.place - TREE_OPEN);
-        w.j1 = min(w.nu, cu1 - w.place - TREE_OPEN);
-    };
-    auto enter = [&](TreeRow &w) {                        // sequence w.i's plan; its first row
-        const TreePlan p = tree_plan(len_of(w.i), rows.row0[w.i + 1] - rows.row0[w.i], a.n_kv, a.n_rep, C, WC);
-        w.nu = p.nu;
-        w.rows = p.rows;
-        w.n_cg = p.n_cg;
-        w.r = 0;
-        w.place = pre[w.i];
-    };
-    // the next row; its units are none (j1 <= j0) behind the run's end
-    auto next = [&](TreeRow &w) {
-        w.place += w.nu + TREE_OPEN;
-        if (++w.r == w.rows) {
-            do w.i++;
-            while (w.i < n && pre[w.i + 1] == pre[w.i]);
-            if (w.i < n) enter(w);
-            else w.place = total;
-        }
-        range(w);
-    };
-    TreeRow first;
-    {
-        int lo = 0, hi = n;                               // the last sequence whose places begin at or before cu0
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (pre[mid] <= cu0) lo = mid;
-            else hi = mid;
-        }
-        first.i = lo;
-        enter(first);
-        first.r = (cu0 - first.place) / (first.nu + TREE_OPEN);
-        first.place += first.r * (first.nu + TREE_OPEN);
-        range(first);
-    }
-    while (first.place < cu1 && first.j1 <= first.j0) next(first);    // (its units end before the run)
+    TreeWalk<N> row(a, rows, pre, KV4_UNIT, blockIdx.x, ctas);
 
     // ---- the group's copies: cursor `ahead` runs before the products
     const int      gt = WC * 32, gtid = wc * 32 + lane, A = WC == 1 ? 2 : 3, ST = WC == 1 ? 2 : 4;
     uint8_t       *ring = smem + (size_t)wp * ST * STAGE;
     const uint32_t ring_at = smem_addr(ring);
-    TreeRow        ahead = first;
+    TreeWalk<N>    ahead = row;
     int            aj = ahead.j0 + wp;
     auto settle = [&] {                                   // ahead's unit, in whichever row it lies
-        while (ahead.place < cu1 && aj >= ahead.j1) {
-            next(ahead);
+        while (ahead.place < ahead.cu1 && aj >= ahead.j1) {
+            ahead.next();
             aj = ahead.j0 + wp;
         }
     };
-    auto page_at = [&] { return ahead.place < cu1 ? __ldg(a.table + (size_t)rows.seq[ahead.i] * a.max_pages + aj / (KV4_PAGE / KV4_UNIT)) : 0; };
+    auto page_at = [&] { return ahead.place < ahead.cu1 ? ahead.page(aj / (KV4_PAGE / KV4_UNIT)) : 0; };
     settle();
     int  page = page_at();
     auto issue = [&](int slot) {
-        if (ahead.place < cu1) {
+        if (ahead.place < ahead.cu1) {
             const size_t   at = (size_t)min(max(page, 0), a.n_pages - 1) * a.page_bytes + (size_t)(ahead.r / ahead.n_cg) * (72 * HD);
             const uint8_t *src = a.layer + at;
             const int      half = aj & 1;
@@ -345,9 +368,11 @@ __global__ void __launch_bounds__(TREE_WARPS * 32, 1) k_kv4_tree(const __grid_co
                     vrow[x] = fmaxf(vrow[x], __shfl_xor_sync(0xffffffffu, vrow[x], o));
                     top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], o));
                 }
-                const float m = fmaxf(M[x], top[x] + exponent(vrow[x]));
-                const float alpha = m == -INFINITY ? 1.0f : kv4_ex2(M[x] - m);      // (nothing seen yet: nothing to rescale)
-                M[x] = m;
+                // (of this row alone: no row's bits depend on what shares its tile)
+                const float m = top[x] + exponent(vrow[x]);
+                const bool  grow = m > M[x] + KV4_SLACK;
+                const float alpha = grow ? kv4_ex2(M[x] - m) : 1.0f;
+                if (grow) M[x] = m;
                 l[x] *= alpha;
 #pragma unroll
                 for (int b = 0; b < NB; b++)
@@ -430,9 +455,9 @@ __global__ void __launch_bounds__(TREE_WARPS * 32, 1) k_kv4_tree(const __grid_co
     };
 
     int which = 0;
-    for (TreeRow row = first; row.place < cu1 && row.j1 > row.j0; next(row), which ^= 1) {
+    for (; row.here(); row.next(), which ^= 1) {
         float(&ml)[2][TREE_WARPS][C] = ml_s[which];
-        const int len = len_of(row.i), r0 = rows.row0[row.i], n_new = rows.row0[row.i + 1] - r0, base = len - n_new;
+        const int len = row.len(), r0 = rows.row0[row.i], n_new = rows.row0[row.i + 1] - r0, base = len - n_new;
         const int kvh = row.r / row.n_cg, cg = row.r - kvh * row.n_cg, cols = n_new * a.n_rep;
         const int col0 = (cg * WC + wc) * C;              // this warp's first column
         const bool mine = col0 < cols;
@@ -536,7 +561,7 @@ __global__ void __launch_bounds__(TREE_WARPS * 32, 1) k_kv4_tree(const __grid_co
         }
         __syncthreads();
         const bool complete = row.j0 == 0 && row.j1 == row.nu;
-        float     *entry = a.part + ((size_t)blockIdx.x * 2 + (row.j0 == 0)) * ENTRY;
+        float     *entry = a.part + ((size_t)blockIdx.x * 2 + (row.j0 == 0)) * (S::EC * (HD + 2));
         for (int x = tid; x < WC * C * (HD / 4); x += TREE_WARPS * 32) {
             const int d4 = x % (HD / 4), cc = x / (HD / 4), w0 = cc / C, cw = cc - w0 * C, col = cg * WC * C + cc;
             if (col >= cols) continue;
@@ -565,8 +590,8 @@ __global__ void __launch_bounds__(TREE_WARPS * 32, 1) k_kv4_tree(const __grid_co
             } else {
                 reinterpret_cast<float4 *>(entry)[cc * (HD / 4) + d4] = s;
                 if (d4 == 0) {
-                    entry[TREE_MAX_WC * C * HD + cc] = m;
-                    entry[TREE_MAX_WC * C * (HD + 1) + cc] = L;
+                    entry[S::EC * HD + cc] = m;
+                    entry[S::EC * (HD + 1) + cc] = L;
                 }
             }
         }
@@ -578,16 +603,15 @@ __global__ void __launch_bounds__(TREE_WARPS * 32, 1) k_kv4_tree(const __grid_co
 // Rows that several CTAs share: a block per CTA and 8 columns, which has work
 // where a row begins in that CTA and goes on behind it; a warp per column.
 template <typename T, int NB, int N>
-__global__ void __launch_bounds__(256) k_kv4_tree_join(const __grid_constant__ TreeArgs a, const __grid_constant__ KvRows<N> rows, int grid)
+__global__ void __launch_bounds__(256) k_kv4_tree_join(const __grid_constant__ TreeArgs a, const __grid_constant__ KvRows<N> rows, int unit, int grid)
 {
-    using S = TreeShape<T, NB>;
-    constexpr int HD = S::HD, C = S::C, ENTRY = S::ENTRY;
+    constexpr int  HD = NB * 32;
     __shared__ int pre[N + 1], sums[8];
-    const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = rows.n;
+    const int      warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = rows.n, EC = a.entry;
     pdl_wait();
     pdl_trigger();
-    tree_scan<256>(a, rows, C, pre, sums);
-    const int total = pre[n], ctas = min(grid, total), slices = (a.wc * C + 7) / 8, cta = blockIdx.x / slices;
+    tree_scan<256>(a, rows, unit, pre, sums);
+    const int total = pre[n], ctas = min(grid, total), slices = (a.group + 7) / 8, cta = blockIdx.x / slices;
     if (cta >= ctas) return;
     auto begin_of = [&](int b) { return (int)((long long)total * b / ctas); };
     const int cu0 = begin_of(cta), cu1 = begin_of(cta + 1);
@@ -599,26 +623,26 @@ __global__ void __launch_bounds__(256) k_kv4_tree_join(const __grid_constant__ T
         else hi = mid;
     }
     const int      len = min(max(__ldg(a.len + rows.seq[lo]), 0), a.max_pages * KV4_PAGE), r0 = rows.row0[lo], n_new = rows.row0[lo + 1] - r0;
-    const TreePlan p = tree_plan(len, n_new, a.n_kv, a.n_rep, C, a.wc);
+    const TreePlan p = tree_plan(len, n_new, a.n_kv, a.n_rep, a.group, unit);
     const int      r = (cu1 - 1 - pre[lo]) / (p.nu + TREE_OPEN), begin = pre[lo] + r * (p.nu + TREE_OPEN) + TREE_OPEN, end = begin + p.nu;
     if (begin < cu0 || begin >= cu1 || end <= cu1) return;
     int last = (int)((long long)(end - 1) * ctas / total);          // the CTA of the row's last unit
     while (begin_of(last + 1) <= end - 1) last++;
     while (begin_of(last) > end - 1) last--;
     const int np = last - cta + 1, kvh = r / p.n_cg, cg = r - kvh * p.n_cg;
-    const int cc = (blockIdx.x % slices) * 8 + warp, col = cg * a.wc * C + cc;
-    if (cc >= a.wc * C || col >= n_new * a.n_rep) return;
-    auto  entry = [&](int b) { return a.part + ((size_t)(cta + b) * 2 + (b == 0)) * ENTRY; };
+    const int cc = (blockIdx.x % slices) * 8 + warp, col = cg * a.group + cc;
+    if (cc >= a.group || col >= n_new * a.n_rep) return;
+    auto  entry = [&](int b) { return a.part + ((size_t)(cta + b) * 2 + (b == 0)) * ((size_t)EC * (HD + 2)); };
     float m = -INFINITY, L = 0.0f;
-    for (int b = lane; b < np; b += 32) m = fmaxf(m, __ldcg(entry(b) + TREE_MAX_WC * C * HD + cc));
+    for (int b = lane; b < np; b += 32) m = fmaxf(m, __ldcg(entry(b) + EC * HD + cc));
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int b0 = 0; b0 < np; b0 += 32) {
         float w = 0.0f;
         if (b0 + lane < np) {
-            const float l = __ldcg(entry(b0 + lane) + TREE_MAX_WC * C * (HD + 1) + cc);
-            w = l == 0.0f ? 0.0f : kv4_ex2(__ldcg(entry(b0 + lane) + TREE_MAX_WC * C * HD + cc) - m);
+            const float l = __ldcg(entry(b0 + lane) + EC * (HD + 1) + cc);
+            w = l == 0.0f ? 0.0f : kv4_ex2(__ldcg(entry(b0 + lane) + EC * HD + cc) - m);
             L = fmaf(w, l, L);
         }
         const int k1 = min(32, np - b0);

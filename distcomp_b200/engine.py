@@ -128,6 +128,7 @@ SIGNATURES = [
     ("ecu_inject_wait_timeout", C.c_int, [C.c_void_p]),
     ("ecu_inject_late_warp", C.c_int, [C.c_void_p]),
     ("ecu_inject_prompt_timeout", C.c_int, [C.c_int]),
+    ("ecu_inject_tree_timeout", C.c_int, [C.c_int]),
     ("ecu_matvec_bench", C.c_int, [C.c_uint, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int,
                                    C.c_int, C.c_int, C.POINTER(C.c_double)]),
     ("ecu_matvec_stream_bench", C.c_int, [C.c_uint, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
@@ -602,6 +603,13 @@ def matvec_bench(gtype: int, raw: np.ndarray, n_in: int, n_out: int, x: np.ndarr
 def set_wait_ns(ns: int, device: int = 0) -> None:
     """The limit after which every bounded wait in the kernels gives up."""
     if lib().ecu_set_wait_ns(device, int(ns)) != 0:
+        raise EngineError(last_error())
+
+
+def inject_tree_timeout(device: int = 0) -> None:
+    """The next attention of drafted rows on the tensor cores waits for keys that never come
+    (ecu_inject_tree_timeout): failure-path testing."""
+    if lib().ecu_inject_tree_timeout(int(device)) != 0:
         raise EngineError(last_error())
 
 

@@ -477,7 +477,12 @@ int  ecu_kv_append_rope(ecu_kv *kv, int layer, const ecu_rope *rope, int dtype, 
  * that it does not see have no effect.  ws: ecu_kv_tree_ws_bytes() bytes of
  * device memory that no other call uses at the same time; NULL: the pool's own
  * for this stream, as in ecu_kv_attend.  The lengths are read on the device when
- * the call runs, so a captured call follows its sequences. */
+ * the call runs, so a captured call follows its sequences.  Sums and the softmax
+ * are fp32; of fp32 queries, and of their weights, 22 bits count; 16-bit queries
+ * of many columns (rows times query heads of a KV head, some 32 and more) see
+ * keys and values rounded to fp16's 11 bits, as the prompts of a batch do.
+ * Every wait in the kernel is bounded (ecu_set_wait_ns): where one gives up, the
+ * call's rows mean nothing, and ecu_attn_prompt_status reports it. */
 int    ecu_kv_attend_tree(ecu_kv *kv, int layer, int dtype, const void *q, void *out, int n_head, long q_stride,
                           long out_stride, const int *seq, const int *n_new, int n, const uint64_t *mask, float scale,
                           void *ws, void *stream);
@@ -535,10 +540,10 @@ int  ecu_kv_keep(ecu_kv *kv, const int *seq, const int *n_new, const int *kept, 
 int  ecu_attn_prompt(int dtype, const void *q, const void *k, const void *v, void *out, int n_head, int n_head_kv,
                      int head_dim, long q_stride, long k_stride, long v_stride, long out_stride, const int *cu_q,
                      const int *cu_k, int n_seq, float scale, int device, void *stream);
-/* Waits for the stream; -1 where a wait of an ecu_attn_prompt call on
- * `device` has given up since this was last asked (until then, waits of later
- * calls that take longer than a millisecond give up with it), or the status
- * cannot be read.  The calls inside ecu_batch_feed and ecu_prefill report
+/* Waits for the stream; -1 where a wait of an ecu_attn_prompt or
+ * ecu_kv_attend_tree call on `device` has given up since this was last asked
+ * (until then, waits of later calls that take longer than a millisecond give up
+ * with it), or the status cannot be read.  The calls inside ecu_batch_feed and ecu_prefill report
  * through those. */
 int  ecu_attn_prompt_status(int device, void *stream);
 
@@ -598,13 +603,15 @@ int  ecu_batch_feed(ecu_batch *b, const int *seq, const int *n_tok, int n, const
  * ecu_inject_prompt_timeout: the next prompt attention on `device`
  * (ecu_attn_prompt, or inside ecu_batch_feed or ecu_prefill) never copies its
  * first keys, so that its waits run out: ecu_attn_prompt_status, or the call
- * around it, returns -1.  ecu_kv_inject_failure: of the launches with which
+ * around it, returns -1.  ecu_inject_tree_timeout: the same of the next
+ * ecu_kv_attend_tree that runs on the tensor memory.  ecu_kv_inject_failure: of the launches with which
  * the next change of the pool updates the device (a pool without one counts
  * them alike), number `launch`, from 0, fails. */
 int  ecu_set_wait_ns(int device, unsigned long long ns);
 int  ecu_inject_wait_timeout(ecu_ctx *c);
 int  ecu_inject_late_warp(ecu_ctx *c);
 int  ecu_inject_prompt_timeout(int device);
+int  ecu_inject_tree_timeout(int device);
 int  ecu_kv_inject_failure(ecu_kv *kv, int launch);
 
 /* ---- measurement --------------------------------------------------------- */

@@ -8,7 +8,9 @@ Tolerances, from the arithmetic:
     rounded once: three roundings of at most 2^-24 of |a| + |b| (times the
     factor), then half a step of its type;
   * the attention as in test_gpu_kv4.py, whose scores, weights and sums it
-    shares;
+    shares; 16-bit queries of many columns have K and V themselves rounded to
+    fp16 (half a step, 2^-11, of each value): a score is off by |scale| A 2^-11
+    more, and V adds once more sum p |v|;
   * verification and kept rows are whole numbers, or bits that move: equal.
 """
 import math
@@ -213,7 +215,7 @@ def tree_check(pool, vals, q, seq, new, masks, out, scale=None):
     H, hd = q.shape[1], q.shape[2]
     half, wide = torch.finfo(q.dtype).eps / 2, q.dtype == torch.float32
     scale = hd ** -0.5 if scale is None else scale
-    hw, extra = (0.0, 0.0) if wide else (H16, 2.0 ** -24)
+    hw, extra, hk = (0.0, 0.0, 0.0) if wide else (2 * H16, 2.0 ** -24, H16)
     qn, r0 = q.double().cpu().numpy(), 0
     for s, m, mk in zip(seq, new, masks):
         k, v = vals[s]
@@ -235,7 +237,7 @@ def tree_check(pool, vals, q, seq, new, masks, out, scale=None):
                     if np.isnan(sc).any():
                         want[j, h] = np.nan
                         continue
-                    ds = abs(scale) * A * 2.0 ** -23 * (hd / 2 + 16) + 2.0 ** -20
+                    ds = abs(scale) * A * (2.0 ** -23 * (hd / 2 + 16) + hk) + 2.0 ** -20
                     p = np.exp(sc - sc.max())
                     p /= p.sum()
                     want[j, h] = p @ vv
@@ -297,6 +299,51 @@ def test_tree_long(dtype, n_kv, rep, lens, new):
     assert torch.equal(got, again) and torch.equal(got, third)
 
 
+@pytest.mark.parametrize("hd,rep", [(128, 4), (128, 7), (64, 8), (64, 4)])
+@pytest.mark.parametrize("dtype", TYPES[1:])
+def test_tree_of_many_columns(hd, rep, dtype):
+    """16-bit queries of up to 512 columns a KV head (the tensor-memory kernel): lengths around the borders of its units."""
+    n_kv, lens, new = 5, [1, 63, 64, 65, 127, 128, 129, 200, 256, 257, 383, 700], [1, 40, 64, 33, 17, 64, 2, 20, 64, 64, 0, 31]
+    pool, vals = filled(n_kv, hd, lens, hd + rep)
+    masks, mask = make(hd * rep, new)
+    q = rows(7, sum(new), n_kv * rep, hd, spread=1.5).to(dtype)
+    out = torch.full((sum(new) + 1, n_kv * rep, hd), 77.0, dtype=dtype, device="cuda")
+    got = pool.attend_tree(0, q, list(range(len(lens))), new, mask, out=out[:-1])
+    tree_check(pool, vals, q, range(len(lens)), new, masks, got)
+    assert (out[-1] == 77).all()
+
+
+@pytest.mark.parametrize("n_kv,rep,lens,new,dtype", [(8, 5, [1000] * 3, [7] * 3, torch.float16), (8, 8, [2000] * 8, [16] * 8, torch.bfloat16),
+                                                     (8, 4, [300] * 40, [24] * 40, torch.float16), (2, 4, [5000] * 5, [6] * 5, torch.float32)])
+def test_tree_gives_the_same_bits_again(n_kv, rep, lens, new, dtype):
+    """Many rows a CTA, rows shared by CTAs: no order of the warps shows."""
+    pool, _ = filled(n_kv, 128, lens, 11)
+    _, mask = make(5, new)
+    q = rows(9, sum(new), n_kv * rep, 128, spread=1.5).to(dtype)
+    seq = list(range(len(new)))
+    want = pool.attend_tree(0, q, seq, new, mask)
+    for _ in range(60):
+        assert torch.equal(pool.attend_tree(0, q, seq, new, mask), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("big", [2.0 ** 14, 60000.0, 500000.0])
+def test_tree_of_large_values(dtype, big):
+    """Keys and values past fp16's range (the cache holds up to 8 * 65504), from some unit on."""
+    hd, n_kv, rep, lens, new = 128, 6, 8, [700, 900, 130, 400], [20, 16, 9, 24]
+    pool, vals = filled(n_kv, hd, lens, 3)
+    masks, mask = make(8, new)
+    k, v = rows(1, 160, n_kv, hd), rows(2, 160, n_kv, hd)
+    v[3, 1, 40] = v[90, :, 7] = -big
+    k[30, 2, 5] = big
+    v[110, 3] = big
+    pool.append(0, k[:100], v[:100], [1], [100])
+    pool.append(0, k[100:], v[100:], [2], [60])
+    vals = [tuple(x.astype(np.float64) for x in pool.read(0, s)) for s in range(4)]
+    q = (rows(5, sum(new), n_kv * rep, hd) * 1e-3).to(dtype)
+    tree_check(pool, vals, q, range(4), new, masks, pool.attend_tree(0, q, [0, 1, 2, 3], new, mask))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_tree_without_masks_is_causal(dtype):
     hd, n_kv, rep, lens, new = 64, 2, 4, [500, 20, 64], [20, 20, 1]
@@ -313,9 +360,10 @@ def test_tree_without_masks_is_causal(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-def test_tree_masks_of_any_bits(dtype):
+@pytest.mark.parametrize("n_kv,rep", [(2, 2), (40, 3)])
+def test_tree_masks_of_any_bits(dtype, n_kv, rep):
     """Rows that see nothing, only others, every bit of the word; sequences of drafts alone."""
-    hd, n_kv, rep, lens, new = 128, 2, 2, [64, 64, 7, 100], [64, 64, 7, 4]
+    hd, lens, new = 128, [64, 64, 7, 100], [64, 64, 7, 4]
     pool, vals = filled(n_kv, hd, lens, 3)
     r = np.random.default_rng(4)
     masks = [[int(x) for x in r.integers(0, 2 ** 64, m, dtype=np.uint64)] for m in new]
@@ -331,10 +379,10 @@ def test_tree_masks_of_any_bits(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("hd,rep", [(64, 2), (128, 8)])
-def test_tree_values_that_are_not_finite(dtype, hd, rep):
+@pytest.mark.parametrize("hd,n_kv,rep", [(64, 2, 2), (128, 2, 8), (128, 9, 8), (64, 9, 8)])
+def test_tree_values_that_are_not_finite(dtype, hd, n_kv, rep):
     """NaN keys and values: without effect where they are not seen, NaN where they are, however little they weigh."""
-    n_kv, lens, new = 2, [150, 2000], [12, 20]
+    lens, new = [150, 2000], [12, 20]
     pool, vals = filled(n_kv, hd, lens, 3)
     masks, mask = make(8, new)
     vals = [list(v) for v in vals]
@@ -377,11 +425,12 @@ def test_tree_of_a_cached_nan():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-def test_tree_peaked_flat_and_scaled(dtype):
-    hd, n_kv, rep, lens, new = 128, 1, 4, [900, 700], [9, 8]
+@pytest.mark.parametrize("n_kv,rep", [(1, 4), (12, 6)])
+def test_tree_peaked_flat_and_scaled(dtype, n_kv, rep):
+    hd, lens, new = 128, [900, 700], [9, 8]
     pool, vals = filled(n_kv, hd, lens, 3)
     masks, mask = make(3, new)
-    q = rows(3, 17, rep, hd)
+    q = rows(3, 17, n_kv * rep, hd)
     q[0] *= 40.0
     q[1] *= 1e-6
     q[2] = 0.0
@@ -869,3 +918,25 @@ def test_wrappers_refuse():
     for call in (lambda: pool.attend_tree(0, q, [0, 1], [3, 2]), lambda: pool.append_rope(0, rope, q, k, k, [0, 1], [3, 2]), lambda: pool.keep([0], [1], [[0]])):
         with pytest.raises(E):
             call()
+
+
+def test_tree_wait_that_gives_up():
+    """Operands that never come: the kernel ends, the status says so, and the next call is right again."""
+    hd, n_kv, rep, lens, new = 128, 8, 8, [2000] * 4, [16] * 4
+    pool, vals = filled(n_kv, hd, lens, 3)
+    _, mask = make(8, new)
+    q = rows(5, sum(new), n_kv * rep, hd).half()
+    want = pool.attend_tree(0, q, [0, 1, 2, 3], new, mask)
+    kv4.prompt_status()
+    engine.set_wait_ns(50_000_000)
+    try:
+        engine.inject_tree_timeout()
+        pool.attend_tree(0, q, [0, 1, 2, 3], new, mask)
+        with pytest.raises(engine.EngineError, match="bounded wait"):
+            kv4.prompt_status()
+    finally:
+        engine.set_wait_ns(2_000_000_000)
+    kv4.prompt_status()
+    assert torch.equal(pool.attend_tree(0, q, [0, 1, 2, 3], new, mask), want)
+    with pytest.raises(engine.EngineError):
+        engine.inject_tree_timeout(99)
