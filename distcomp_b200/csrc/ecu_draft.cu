@@ -93,11 +93,11 @@ static int rope_launch(ecu_kv *kv, RopeArgs a, const int *seq, int first, const 
     const int total = r.row0[n], hd = kv->head_dim;
     if (total == 0) return 0;
     // a block takes whole rows, or, of few rows, a part of their heads: enough
-    // blocks for every SM first, then up to 8 KV heads and some 24 KB of keys
+    // blocks for every SM first, then up to 8 KV heads and some 40 KB of keys
     a.heads = std::min(a.kv.n_kv, 8);
     while (a.heads > 1 && (long long)total * ((a.kv.n_kv + a.heads - 1) / a.heads) < kv->sms) a.heads = (a.heads + 1) / 2;
-    const int chunks = (a.kv.n_kv + a.heads - 1) / a.heads, per_row = a.turns.rot * 8 + a.heads * hd * 8;
-    a.rows = std::max(1, std::min({64, 24576 / per_row, (int)((long long)total * chunks / (4 * kv->sms))}));
+    const int chunks = (a.kv.n_kv + a.heads - 1) / a.heads, per_row = (a.turns.rot / 2 + 7) / 8 * 128 + a.heads * hd * 8;
+    a.rows = std::max(1, std::min({64, 40960 / per_row, (int)((long long)total * chunks / (4 * kv->sms))}));
     const long long blocks = (long long)((total + a.rows - 1) / a.rows) * chunks;
     if (blocks > INT_MAX) return say("ecu_kv_append_rope", "too many rows");
     return launched("ecu_kv_append_rope",
@@ -198,6 +198,7 @@ extern "C" int ecu_kv_append_rope(ecu_kv *kv, int layer, const ecu_rope *rope, i
         a.kv.n_pages = kv->book.n_pages;
         a.kv.n_kv = kv->n_head_kv;
         a.kv.nb = kv->head_dim / 32;
+        a.kv.nb_inv = (65536 + a.kv.nb - 1) / a.kv.nb;    // exact below 32768: at most 8 heads of 4 blocks
         a.kv.wide = !(((uintptr_t)k | (uintptr_t)v | (uintptr_t)(k_stride * (long)es) | (uintptr_t)(v_stride * (long)es)) & 15);
         a.kv.wide_out = !(((uintptr_t)k_out | (uintptr_t)v_out) & 15);
         a.q = q;

@@ -7,9 +7,13 @@
 // w_i itself); no table, and no angle that grows.
 //
 // A 4-bit code changes by a whole step where the turned key crosses the border
-// between two codes, so a key is turned and quantised in 64 bits: its code is
-// that of the exact value but for one in about 10^14, and the same from every
-// implementation.  A query is turned in 32 bits and rounded once.
+// between two codes.  So a key is turned in pairs of floats (the products and
+// their sum with what they round off, cosine and sine of 48 bits): about 2^-46
+// of its pair's size, and its code is that of the exact value but for one in
+// some 10^12, the same from every implementation.  What such a pair of floats
+// cannot decide at a glance (a block whose largest values differ in sign alone,
+// a scale halfway between two fp16 numbers, subnormal scales) is decided in
+// 64-bit arithmetic.  A query is turned in 32 bits and rounded once.
 #pragma once
 #include "ecu_kv4.cuh"
 
@@ -101,25 +105,86 @@ __device__ __forceinline__ uint32_t kv4_quantise64(const double (&x)[8], unsigne
     return fine ? w : 0x88888888u;
 }
 
+// A key as it turned: h + l, |l| at most half a step of h.
+struct RopePair {
+    float h, l;
+};
+
+// x0 * c - x1 * s for c = t.x + t.y, s = t.z + t.w
+__device__ __forceinline__ RopePair rope_turn(float x0, float x1, float ch, float cl, float sh, float sl)
+{
+    const float p = __fmul_rn(x0, ch), pe = __fmaf_rn(x0, ch, -p), q = __fmul_rn(x1, sh), qe = __fmaf_rn(x1, sh, -q);
+    const float d = __fsub_rn(p, q), b = __fsub_rn(d, p), e = __fsub_rn(__fsub_rn(p, __fsub_rn(d, b)), __fadd_rn(q, b));
+    const float r = __fadd_rn(e, __fadd_rn(__fsub_rn(pe, qe), __fmaf_rn(x0, cl, -__fmul_rn(x1, sl))));
+    RopePair    y;
+    y.h = __fadd_rn(d, r);
+    y.l = __fsub_rn(r, __fsub_rn(y.h, d));
+    return y;
+}
+
+// kv4_quantise of pairs of floats: the same decisions, with l where it counts.
+__device__ __forceinline__ uint32_t kv4_quantise_pair(const float (&h)[8], const float (&l)[8], unsigned mask, int c, __half &dh, float (&y)[8])
+{
+    float p = h[0], q = -h[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) {
+        p = kv4_max(p, h[i]);
+        q = kv4_max(q, -h[i]);
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        p = kv4_max(p, __shfl_xor_sync(mask, p, o));
+        q = kv4_max(q, __shfl_xor_sync(mask, q, o));
+    }
+    const float m = p > q ? p : -q, size = fabsf(m);
+    // (the same in the group's four lanes) equal in size; a scale m / 8 whose 13 bits below fp16's are 1000..., or one
+    // below fp16's normal numbers, where those bits are others
+    if (p == q || (__float_as_uint(m) & 0x1FFFu) == 0x1000u || size < 0.00048828125f) {
+        double x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = (double)h[i] + (double)l[i];
+        return kv4_quantise64(x, mask, c, dh, y);
+    }
+    const bool fine = size < INFINITY;
+    dh = __float2half_rn(fminf(fmaxf(m * -0.125f, -65504.0f), 65504.0f));
+    if (!fine) dh = __ushort_as_half(0x7FFF);
+    const float d = __half2float(dh), sign = copysignf(1.0f, d), inv = __frcp_rn(d), half = 0.5f * fabsf(d);
+    uint32_t    w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        float k = __fsub_rn(__fadd_rn(__fmaf_rn(h[i], inv, -3.814697265625e-6f), 12582912.0f), 12582912.0f);
+        // near the border the difference is exact, and l decides
+        if (__fsub_rn(__fmul_rn(__fmaf_rn(-k, d, h[i]), sign), half) >= -l[i] * sign) k += 1.0f;
+        k = fminf(fmaxf(k, -8.0f), 7.0f);
+        w += __float_as_uint(k + 8388616.0f) << (4 * i);
+        y[i] = k * d;
+    }
+    return fine ? w - 0xFB000000u : 0x88888888u;
+}
+
 // A block takes a.rows rows and a.heads KV heads with their query heads: the
 // angles' cosines and sines into shared memory, then the queries turned, and
 // the keys, which wait in shared memory (a block of 32 dimensions and its
-// partners may lie in different threads), then codes for K and V, four lanes to
-// a block of 32 dimensions.
+// partners may lie in different threads), then codes for K and V.
 template <typename T, typename O, int N>
-__global__ void __launch_bounds__(256) k_kv4_append_rope(const __grid_constant__ RopeArgs a, const __grid_constant__ KvRows<N> rows)
+__global__ void __launch_bounds__(256, 4) k_kv4_append_rope(const __grid_constant__ RopeArgs a, const __grid_constant__ KvRows<N> rows)
 {
-    extern __shared__ __align__(16) double rope_sm[];
-    __shared__ int s_seq[64], s_pos[64];
-    pdl_wait();
-    pdl_trigger();
+    extern __shared__ __align__(16) uint8_t rope_sm[];
+    __shared__ int       s_seq[64], s_pos[64];
+    __shared__ long long s_turn[64];
     const int hd = a.kv.nb * 32, rot = a.turns.rot, half = rot / 2, tid = threadIdx.x;
     const int chunks = (a.kv.n_kv + a.heads - 1) / a.heads;
     const int r0 = (int)(blockIdx.x / chunks) * a.rows, h0 = (int)(blockIdx.x % chunks) * a.heads;
     const int nr = min(a.rows, rows.row0[rows.n] - r0), nh = min(a.heads, a.kv.n_kv - h0);
-    double2  *cs = reinterpret_cast<double2 *>(rope_sm);         // [rows][half]
-    double   *ks = rope_sm + 2 * a.rows * half;                  // [rows][heads][hd]
-    // where each row stands
+    // Slices: eight pairs each, then eight dimensions each of those that do not turn.
+    const int n_pair = (half + 7) / 8, n_rest = (hd - rot + 7) / 8;
+    // cosines and sines, and what they round off: pair i of slice x of row r at [r][i][x], so that lanes of consecutive
+    // slices meet different banks
+    float2   *cs = reinterpret_cast<float2 *>(rope_sm), *cs_rest = cs + a.rows * 8 * n_pair;
+    float    *kh = reinterpret_cast<float *>(cs_rest + a.rows * 8 * n_pair), *kl = kh + a.rows * a.heads * hd;      // [rows][heads][hd]
+    pdl_wait();
+    pdl_trigger();
+    // where each row stands, and how far it turns
     if (tid < nr) {
         const int r = r0 + tid;
         int       lo = 0, hi = rows.n;
@@ -128,125 +193,159 @@ __global__ void __launch_bounds__(256) k_kv4_append_rope(const __grid_constant__
             if (rows.row0[mid] <= r) lo = mid;
             else hi = mid;
         }
+        const int first = __ldg(a.kv.len + rows.seq[lo]) - (rows.row0[lo + 1] - rows.row0[lo]), at = r - rows.row0[lo];
         s_seq[tid] = rows.seq[lo];
-        s_pos[tid] = __ldg(a.kv.len + rows.seq[lo]) - (rows.row0[lo + 1] - r);
-    }
-    for (int x = tid; x < nr * half; x += 256) {
-        const int r = r0 + x / half, i = x % half;
-        int       lo = 0, hi = rows.n;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (rows.row0[mid] <= r) lo = mid;
-            else hi = mid;
-        }
-        const int       first = __ldg(a.kv.len + rows.seq[lo]) - (rows.row0[lo + 1] - rows.row0[lo]);
-        const long long pos = (long long)first + (a.depth ? __ldg(a.depth + r) : r - rows.row0[lo]);
-        const long long turn = (long long)((unsigned long long)pos * a.turns.turn[i]);
-        double          s, c;
-        sincospi((double)turn * 0x1p-63, &s, &c);
-        cs[x] = make_double2(c * a.turns.factor, s * a.turns.factor);
+        s_pos[tid] = first + at;
+        s_turn[tid] = (long long)first + (a.depth ? __ldg(a.depth + r) : at);
     }
     __syncthreads();
-    // slices: eight pairs each, then eight dimensions each of those that do not turn
-    const int  n_pair = (half + 7) / 8, n_rest = (hd - rot + 7) / 8, per_head = n_pair + n_rest;
-    const bool even = half % 8 == 0;                             // slices begin at multiples of eight elements
+    for (int x = tid; x < nr * half; x += 256) {
+        const int r = x / half, i = x - r * half;
+        double    s, c;
+        sincospi((double)(long long)((unsigned long long)s_turn[r] * a.turns.turn[i]) * 0x1p-63, &s, &c);
+        c *= a.turns.factor;
+        s *= a.turns.factor;
+        const float ch = (float)c, sh = (float)s;
+        const int   at = (r * 8 + (i & 7)) * n_pair + (i >> 3);
+        cs[at] = make_float2(ch, sh);
+        cs_rest[at] = make_float2((float)(c - (double)ch), (float)(s - (double)sh));
+    }
+    __syncthreads();
+    // Slices begin at multiples of eight elements, but for second halves of other lengths and what lies behind them.
+    const bool apart = !a.turns.interleaved, even = !apart || half % 8 == 0, even_rest = rot % 8 == 0;
     const int  q_heads = a.q ? nh * a.n_rep : 0, all = q_heads + nh;
-    for (int x = tid; x < nr * all * per_head; x += 256) {
-        const int  sl = x % per_head, hh = x / per_head % all, r = x / (per_head * all);
-        const bool is_q = hh < q_heads;
-        const T   *p = is_q ? (const T *)a.q + (size_t)(r0 + r) * a.q_stride + (size_t)(h0 * a.n_rep + hh) * hd
+    auto from = [&](int r, int hh) {                              // row r's head hh: the queries', then the keys'
+        return hh < q_heads ? (const T *)a.q + (size_t)(r0 + r) * a.q_stride + (size_t)(h0 * a.n_rep + hh) * hd
                             : (const T *)a.kv.k + (size_t)(r0 + r) * a.kv.k_stride + (size_t)(h0 + hh - q_heads) * hd;
-        T         *o = is_q ? (T *)a.q_out + (size_t)(r0 + r) * a.q_out_stride + (size_t)(h0 * a.n_rep + hh) * hd : nullptr;
-        double    *kd = ks + ((size_t)r * a.heads + (hh - q_heads)) * hd;
-        const bool wide = even && (is_q ? a.wide_q : a.kv.wide);
-        float      u[8], v[8];
-        if (sl >= n_pair) {
-            const int d = rot + 8 * (sl - n_pair), n = hd - d;
-            rope_load(p + d, n, wide, u);
-            if (is_q) rope_store(o + d, n, wide, u);
-            else
+    };
+    auto to = [&](int r, int hh) { return (T *)a.q_out + (size_t)(r0 + r) * a.q_out_stride + (size_t)(h0 * a.n_rep + hh) * hd; };
+    // The pairs' first and second values lie in slices u and v, or, interleaved, are every other one of both.
+    struct Slice { int i0, n, d0, d1, n0, n1; };
+    auto slice = [&](int sl) {
+        Slice x;
+        x.i0 = 8 * sl;
+        x.n = min(8, half - x.i0);
+        x.d0 = apart ? x.i0 : 2 * x.i0;
+        x.d1 = apart ? half + x.i0 : 2 * x.i0 + 8;
+        x.n0 = apart ? x.n : 2 * x.n;
+        x.n1 = apart ? x.n : 2 * x.n - 8;
+        return x;
+    };
+    // Queries: a thread keeps its slice of a row and takes heads in turn.
+    const int combos = nr * n_pair, lanes = combos >= 256 ? 1 : combos ? 256 / combos : 0;
+    for (int x = tid; x < combos * lanes && q_heads > 0; x += 256) {
+        const int     hl = x / combos, combo = x - hl * combos, r = combo / n_pair, sl = combo - r * n_pair;
+        const Slice   at = slice(sl);
+        const float2 *t = cs + r * 8 * n_pair + sl;
+        float2        e[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    if (i < n) kd[d + i] = (double)u[i];
-            continue;
-        }
-        const int      i0 = 8 * sl, n = min(8, half - i0);
-        const double2 *t = cs + r * half + i0;
-        if (a.turns.interleaved) {
-            rope_load(p + 2 * i0, 2 * n, wide, u);
-            rope_load(p + 2 * i0 + 8, 2 * n - 8, wide, v);
-            if (is_q) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const double2 e = t[min(i, n - 1)];
-                    const float   c = (float)e.x, s = (float)e.y;
-                    float        &p0 = i < 4 ? u[2 * (i & 3)] : v[2 * (i & 3)], &p1 = i < 4 ? u[2 * (i & 3) + 1] : v[2 * (i & 3) + 1];
-                    const float   y0 = fmaf(p0, c, -p1 * s), y1 = fmaf(p1, c, p0 * s);
-                    p0 = y0;
-                    p1 = y1;
-                }
-                rope_store(o + 2 * i0, 2 * n, wide, u);
-                rope_store(o + 2 * i0 + 8, 2 * n - 8, wide, v);
-            } else {
+        for (int i = 0; i < 8; i++) e[i] = t[min(i, at.n - 1) * n_pair];
+        for (int hh = hl; hh < q_heads; hh += lanes) {
+            const T *p = from(r, hh);
+            T       *o = to(r, hh);
+            float    u[8], v[8];
+            rope_load(p + at.d0, at.n0, a.wide_q, u);
+            rope_load(p + at.d1, at.n1, even && a.wide_q, v);
+            if (apart) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    if (i >= n) continue;
-                    const double2 e = t[i];
-                    const double  p0 = i < 4 ? u[2 * (i & 3)] : v[2 * (i & 3)], p1 = i < 4 ? u[2 * (i & 3) + 1] : v[2 * (i & 3) + 1];
-                    kd[2 * (i0 + i)] = fma(p0, e.x, -p1 * e.y);
-                    kd[2 * (i0 + i) + 1] = fma(p1, e.x, p0 * e.y);
-                }
-            }
-        } else {
-            rope_load(p + i0, n, wide, u);
-            rope_load(p + half + i0, n, wide, v);
-            if (is_q) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const double2 e = t[min(i, n - 1)];
-                    const float   c = (float)e.x, s = (float)e.y, y0 = fmaf(u[i], c, -v[i] * s), y1 = fmaf(v[i], c, u[i] * s);
+                    const float y0 = fmaf(u[i], e[i].x, -v[i] * e[i].y), y1 = fmaf(v[i], e[i].x, u[i] * e[i].y);
                     u[i] = y0;
                     v[i] = y1;
                 }
-                rope_store(o + i0, n, wide, u);
-                rope_store(o + half + i0, n, wide, v);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    if (i >= n) continue;
-                    const double2 e = t[i];
-                    kd[i0 + i] = fma((double)u[i], e.x, -(double)v[i] * e.y);
-                    kd[half + i0 + i] = fma((double)v[i], e.x, (double)u[i] * e.y);
+                    float      &p0 = i < 4 ? u[2 * (i & 3)] : v[2 * (i & 3)], &p1 = i < 4 ? u[2 * (i & 3) + 1] : v[2 * (i & 3) + 1];
+                    const float y0 = fmaf(p0, e[i].x, -p1 * e[i].y), y1 = fmaf(p1, e[i].x, p0 * e[i].y);
+                    p0 = y0;
+                    p1 = y1;
                 }
             }
+            rope_store(o + at.d0, at.n0, a.wide_q, u);
+            rope_store(o + at.d1, at.n1, even && a.wide_q, v);
         }
     }
+    // Keys
+    for (int x = tid; x < nr * nh * n_pair; x += 256) {
+        const int     r = x / (nh * n_pair), in_row = x - r * (nh * n_pair), h = in_row / n_pair, sl = in_row - h * n_pair;
+        const Slice   at = slice(sl);
+        const float2 *t = cs + r * 8 * n_pair + sl, *rest = cs_rest + r * 8 * n_pair + sl;
+        const T      *p = from(r, q_heads + h);
+        const int     kd = (r * a.heads + h) * hd;
+        float         u[8], v[8], ul[8], vl[8];
+        rope_load(p + at.d0, at.n0, a.kv.wide, u);
+        rope_load(p + at.d1, at.n1, even && a.kv.wide, v);
+        auto turn = [&](float &p0, float &p1, float &q0, float &q1, int i) {
+            const float2   e = t[min(i, at.n - 1) * n_pair], f = rest[min(i, at.n - 1) * n_pair];
+            const RopePair y0 = rope_turn(p0, p1, e.x, f.x, e.y, f.y), y1 = rope_turn(p1, -p0, e.x, f.x, e.y, f.y);
+            p0 = y0.h, q0 = y0.l;
+            p1 = y1.h, q1 = y1.l;
+        };
+        if (apart)
+#pragma unroll
+            for (int i = 0; i < 8; i++) turn(u[i], v[i], ul[i], vl[i], i);
+        else
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                turn(u[2 * i], u[2 * i + 1], ul[2 * i], ul[2 * i + 1], i);
+                turn(v[2 * i], v[2 * i + 1], vl[2 * i], vl[2 * i + 1], 4 + i);
+            }
+        rope_store(kh + kd + at.d0, at.n0, true, u);
+        rope_store(kl + kd + at.d0, at.n0, true, ul);
+        rope_store(kh + kd + at.d1, at.n1, even, v);
+        rope_store(kl + kd + at.d1, at.n1, even, vl);
+    }
+    for (int x = tid; x < nr * all * n_rest; x += 256) {
+        const int r = x / (all * n_rest), in_row = x - r * all * n_rest, hh = in_row / n_rest, d = rot + 8 * (in_row - hh * n_rest), n = hd - d;
+        const T  *p = from(r, hh);
+        float     u[8];
+        rope_load(p + d, n, even_rest && (hh < q_heads ? a.wide_q : a.kv.wide), u);
+        if (hh < q_heads) rope_store(to(r, hh) + d, n, even_rest && a.wide_q, u);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (i < n) {
+                    kh[(r * a.heads + hh - q_heads) * hd + d + i] = u[i];
+                    kl[(r * a.heads + hh - q_heads) * hd + d + i] = 0.0f;
+                }
+    }
     __syncthreads();
-    const int blocks = nh * a.kv.nb, groups = nr * blocks;       // of four lanes
-    for (int g0 = 0; g0 < groups; g0 += 64) {
-        const int      g = g0 + tid / 4, c = tid & 3;
+    // Codes, four lanes to a block of 32 dimensions: blocks hb of row r in turn.
+    const int blocks = nh * a.kv.nb, step_r = 64 / blocks, step_hb = 64 - step_r * blocks;
+    int       r = tid / 4 / blocks, hb = tid / 4 - r * blocks;
+    for (; r < nr; r += step_r, hb += step_hb) {
+        if (hb >= blocks) {
+            hb -= blocks;
+            if (++r >= nr) break;
+        }
+        const int      c = tid & 3, h = (int)((unsigned)hb * a.kv.nb_inv >> 16), b = hb - h * a.kv.nb;
         const unsigned mask = 0xFu << (tid & 28);
-        if (g >= groups) continue;                               // whole groups of four
-        const int  r = g / blocks, hb = g - r * blocks, h = hb / a.kv.nb, b = hb - h * a.kv.nb;
+        const size_t   at = (size_t)h0 * hd + 32 * hb + 8 * c, out = (size_t)(r0 + r) * a.kv.n_kv * hd + at;
+        float          y[8], x[8], l[8];
+        __half         d[2];
+        uint32_t       w[2];
+        kv4_load8((const T *)a.kv.v + (size_t)(r0 + r) * a.kv.v_stride + at, a.kv.wide, x);
         const int  pos = s_pos[r], t = pos & (KV4_PAGE - 1);
         const bool placed = pos >= 0 && pos < a.kv.max_pages * KV4_PAGE;
         const int  page = placed ? __ldg(a.kv.table + (size_t)s_seq[r] * a.kv.max_pages + pos / KV4_PAGE) : -1;
-        const bool wr = (unsigned)page < (unsigned)a.kv.n_pages; // no page: nothing to write to
-        uint8_t   *p = a.kv.layer + (size_t)(wr ? page : 0) * a.kv.page_bytes + (size_t)(h0 + h) * 72 * hd;
-        const size_t at = (size_t)(h0 + h) * hd + 32 * b + 8 * c, out = (size_t)(r0 + r) * a.kv.n_kv * hd + at;
-        float      y[8], xv[8];
-        __half     d;
-        kv4_load8((const T *)a.kv.v + (size_t)(r0 + r) * a.kv.v_stride + at, a.kv.wide, xv);
-        double     xk[8];
+        w[1] = kv4_quantise(x, mask, c, d[1], y);
+        if (a.kv.k_out) kv4_store8((O *)a.kv.v_out + out, a.kv.wide_out, y);
+        const int kd = r * a.heads * hd + 32 * hb + 8 * c;
 #pragma unroll
-        for (int i = 0; i < 8; i++) xk[i] = ks[((size_t)r * a.heads + h) * hd + 32 * b + 8 * c + i];
+        for (int i = 0; i < 8; i += 4) {
+            const float4 fh = *reinterpret_cast<const float4 *>(kh + kd + i), fl = *reinterpret_cast<const float4 *>(kl + kd + i);
+            x[i] = fh.x, x[i + 1] = fh.y, x[i + 2] = fh.z, x[i + 3] = fh.w;
+            l[i] = fl.x, l[i + 1] = fl.y, l[i + 2] = fl.z, l[i + 3] = fl.w;
+        }
+        w[0] = kv4_quantise_pair(x, l, mask, c, d[0], y);
+        if (a.kv.k_out) kv4_store8((O *)a.kv.k_out + out, a.kv.wide_out, y);
+        if ((unsigned)page >= (unsigned)a.kv.n_pages) continue;   // no page: nothing to write to
+        uint8_t *p = a.kv.layer + (size_t)page * a.kv.page_bytes + (size_t)(h0 + h) * 72 * hd;
 #pragma unroll
         for (int side = 0; side < 2; side++) {
-            const uint32_t w = side ? kv4_quantise(xv, mask, c, d, y) : kv4_quantise64(xk, mask, c, d, y);
-            if (a.kv.k_out) kv4_store8((O *)(side ? a.kv.v_out : a.kv.k_out) + out, a.kv.wide_out, y);
-            if (!wr) continue;
-            *reinterpret_cast<uint32_t *>(p + side * 32 * hd + t * (hd / 2) + kv4_place(t, b, a.kv.nb) * 16 + 4 * c) = w;
-            if (c == 0) *reinterpret_cast<__half *>(p + 64 * hd + side * 4 * hd + (t * a.kv.nb + b) * 2) = d;
+            *reinterpret_cast<uint32_t *>(p + side * 32 * hd + t * (hd / 2) + kv4_place(t, b, a.kv.nb) * 16 + 4 * c) = w[side];
+            if (c == 0) *reinterpret_cast<__half *>(p + 64 * hd + side * 4 * hd + (t * a.kv.nb + b) * 2) = d[side];
         }
     }
 }
