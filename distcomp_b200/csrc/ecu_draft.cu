@@ -232,8 +232,8 @@ static int verify_launch(VerifyArgs a, const int *n_row, int n, int sms, cudaStr
     for (int i = 0; i < n; i++) r.row0[i + 1] = r.row0[i] + n_row[i];
     // CTAs of a sequence: as many as keep all sequences in flight together, two
     // CTAs an SM, and find a few hundred tokens a warp
-    int cl = 8;
-    while (cl > 1 && ((long long)cl * n > 2 * sms || a.vocab < cl * VER_WARPS * 64)) cl /= 2;
+    const int most = std::max(1, std::min(8, std::min(2 * sms / n, a.vocab / (VER_WARPS * 64))));
+    const int cl = most;
     cudaLaunchConfig_t  cfg = {};
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

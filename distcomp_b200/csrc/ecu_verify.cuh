@@ -14,7 +14,12 @@
 // draw in a hundred of a vocabulary of 128256 fall to a neighbour.
 //
 // A cluster of CTAs walks one sequence's tree; its warps hold equal runs of the
-// vocabulary, and sums meet through distributed shared memory.
+// vocabulary, and sums meet through distributed shared memory.  A row is read
+// once: its largest logit, whether it is a distribution at all, and the sum of
+// 2^((l - c) / T log2 e) come out of one pass, c being the row's first logit (64
+// bits hold 2^+-1000 around it; where that is not enough, a second pass takes
+// the largest).  What bounds it is that pass, ten operations of 64 bits a logit;
+// the exponential is a table of 2^(k/256) and four terms of its series.
 #pragma once
 #include "ecu_kv4.cuh"
 
@@ -45,13 +50,53 @@ struct VerTop {
     float v;
     int   at;
 };
+__device__ __forceinline__ double warp_total(double v)
+{
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __hiloint2double(__shfl_xor_sync(0xffffffffu, __double2hiint(v), o), __shfl_xor_sync(0xffffffffu, __double2loint(v), o));
+    return v;
+}
+
 __device__ __forceinline__ VerTop ver_top(VerTop a, VerTop b)
 {
     return b.v > a.v || (b.v == a.v && b.at < a.at) ? b : a;
 }
 
+#define VER_TABLE 256
+
+// 2^t; t < -1000: 0, t > 1000: infinity.  t = k / 256 + f with |f| <= 1/512, and
+// 2^f by its series up to f^4 (the next term is below 2^-54).
+__device__ __forceinline__ double ver_ex2(double t, const double *table)
+{
+    const double magic = 26388279066624.0;                // 1.5 * 2^44: a sum's last bit is 1/256
+    const double m = t + magic, f = t - (m - magic);
+    const int    k = __double2loint(m);
+    double       p = fma(f, 0.009618129107628477, 0.05550410866482158);
+    p = fma(f, p, 0.2402265069591007);
+    p = fma(f, p, 0.6931471805599453);
+    const double w = table[k & (VER_TABLE - 1)];
+    p = fma(w, f * p, w);
+    p = __hiloint2double(__double2hiint(p) + ((k >> 8) << 20), __double2loint(p));
+    return t < -1000.0 ? 0.0 : t > 1000.0 ? INFINITY : p;
+}
+
+// f(x, logit) for this lane's elements of [x0, x1), x0 a multiple of eight.
+template <typename T, typename F> __device__ __forceinline__ void ver_each(const T *row, int x0, int x1, bool wide, int lane, F f)
+{
+    constexpr int V = 16 / (int)sizeof(T);                // elements of 16 bytes
+    int           x = x0;
+    if (wide)
+        for (; x + 32 * V <= x1; x += 32 * V) {
+            __align__(16) T v[V];
+            *reinterpret_cast<uint4 *>(v) = __ldg(reinterpret_cast<const uint4 *>(row + x + lane * V));
+#pragma unroll
+            for (int k = 0; k < V; k++) f(x + lane * V + k, kv4_float(v[k]));
+        }
+    for (x += lane; x < x1; x += 32) f(x, kv4_float(row[x]));
+}
+
 template <typename T, int N>
-__global__ void __launch_bounds__(VER_WARPS * 32) k_draft_verify(const VerifyArgs a, const __grid_constant__ VerifyRows<N> rows)
+__global__ void __launch_bounds__(VER_WARPS * 32, 2) k_draft_verify(const VerifyArgs a, const __grid_constant__ VerifyRows<N> rows)
 {
     namespace cg = cooperative_groups;
     cg::cluster_group cl = cg::this_cluster();
@@ -65,7 +110,9 @@ __global__ void __launch_bounds__(VER_WARPS * 32) k_draft_verify(const VerifyArg
     __shared__ double   F_s[VER_ROWS + 1];                // f's sums at the current row, before each rejection
     __shared__ int      gone_s[VER_ROWS], tok_s[VER_ROWS], par_s[VER_ROWS];
     __shared__ float    u_s[VER_ROWS];
+    __shared__ double   table[VER_TABLE];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid < VER_TABLE) table[tid] = exp2((double)tid / VER_TABLE);
     pdl_wait();
     pdl_trigger();
     const int i = (int)blockIdx.x / CL, r0 = rows.row0[i], n = rows.row0[i + 1] - r0, W = CL * VER_WARPS;
@@ -84,7 +131,7 @@ __global__ void __launch_bounds__(VER_WARPS * 32) k_draft_verify(const VerifyArg
     }
     const float  temp = a.temperature ? __ldg(a.temperature + seq) : 1.0f;
     const bool   greedy = !(temp > 0.0f);
-    const double inv = greedy ? 1.0 : 1.0 / (double)temp;
+    const double inv = greedy ? 1.0 : 1.4426950408889634 / (double)temp;
     // this warp's run of the vocabulary, a multiple of 8 but for the last
     const int per = ((a.vocab + W - 1) / W + 7) & ~7, me = rank * VER_WARPS + warp;
     const int x0 = min(a.vocab, me * per), x1 = min(a.vocab, x0 + per);
@@ -93,10 +140,11 @@ __global__ void __launch_bounds__(VER_WARPS * 32) k_draft_verify(const VerifyArg
     const T     *lg = nullptr;
     const float *dr = nullptr;
     VerTop       top{-INFINITY, 0x7FFFFFFF};
+    double       from = 0.0;                              // c
     bool         bad = false;
     int          n_gone = 0, n_res = 0;                   // tokens taken out, subtractions
 
-    // every warp's value, at every CTA
+    // every warp's sum, at every CTA, and their total, in the order of the warps by every thread alike
     auto exchange = [&](double sum) {
         if (lane == 0) x_sum[turn][warp] = sum;
         cl.sync();
@@ -104,43 +152,50 @@ __global__ void __launch_bounds__(VER_WARPS * 32) k_draft_verify(const VerifyArg
         __syncthreads();
         turn ^= 1;
     };
-    auto total = [&] {                                    // in the order of the warps, by every thread alike
+    auto total = [&] {
         double s = 0.0;
         for (int k = lane; k < W; k += 32) s += b_sum[k];
-#pragma unroll
-        for (int o = 16; o; o >>= 1) s += kv4_shfl_xor(0xffffffffu, s, o);
-        __syncthreads();                                  // b_sum may be written again
-        return s;
+        return warp_total(s);
     };
-    auto weight = [&](float l) { return l == -INFINITY ? 0.0 : exp(((double)l - (double)top.v) * inv); };
+    auto weight = [&](float l) { return l == -INFINITY ? 0.0 : ver_ex2(((double)l - from) * inv, table); };
     // f(x) as the rejections so far left it
-    auto f_of = [&](int x) {
+    auto f_at = [&](int x, float l) {
         for (int k = 0; k < n_gone; k++)
             if (gone_s[k] == x) return 0.0;
-        double f = weight(kv4_float(lg[x]));
+        double f = weight(l);
         if (n_res) {
             const double q = (double)__ldg(dr + x);
             for (int k = 0; k < n_res; k++) f = fmax(f / F_s[k] - q, 0.0);
         }
         return f;
     };
+    auto f_of = [&](int x) { return f_at(x, kv4_float(lg[x])); };
     auto sum_f = [&] {
         double s = 0.0;
-        for (int x = x0 + lane; x < x1; x += 32) s += f_of(x);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) s += kv4_shfl_xor(0xffffffffu, s, o);
-        exchange(s);
+        ver_each(lg, x0, x1, a.wide, lane, [&](int x, float l) { s += f_at(x, l); });
+        exchange(warp_total(s));
+        return total();
     };
-    auto open_row = [&](int j) {                          // row j becomes the current one: its largest value
+    // Row j becomes the current one: its largest logit, whether it is a distribution, f's sum.
+    auto open_row = [&](int j) {
         lg = (const T *)a.logits + (size_t)(r0 + j) * a.stride;
         dr = a.draft ? a.draft + (size_t)(r0 + j) * a.draft_stride : nullptr;
+        const float first = kv4_float(lg[0]);
+        from = fabsf(first) < INFINITY ? (double)first : 0.0;
+        n_gone = n_res = 0;
         top = VerTop{-INFINITY, 0x7FFFFFFF};
-        int b = 0;
-        for (int x = x0 + lane; x < x1; x += 32) {
-            const float v = kv4_float(lg[x]);
-            b |= !(v < INFINITY);                         // NaN or an infinity
-            if (v > top.v) top = VerTop{v, x};
-        }
+        int    b = 0;
+        double s0 = 0.0, s1 = 0.0;
+        ver_each(lg, x0, x1, a.wide, lane, [&](int x, float l) {
+            b |= !(l < INFINITY);                         // NaN or an infinity
+            if (l > top.v || (l == top.v && x < top.at)) top = VerTop{l, x};
+            if (!greedy) {
+                const double w = weight(l);
+                if (x & 1) s1 += w;
+                else s0 += w;
+            }
+        });
+        const double s = warp_total(s0 + s1);
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
             top = ver_top(top, VerTop{__shfl_xor_sync(0xffffffffu, top.v, o), __shfl_xor_sync(0xffffffffu, top.at, o)});
@@ -151,11 +206,16 @@ __global__ void __launch_bounds__(VER_WARPS * 32) k_draft_verify(const VerifyArg
             x_at[turn][warp] = top.at;
             x_bad[turn][warp] = b;
         }
+        const int was = turn;
+        __syncthreads();                                  // (b_sum and the others are read no more)
+        if (lane == 0) x_sum[turn][warp] = s;
         cl.sync();
         for (int k = tid; k < W; k += VER_WARPS * 32) {
-            b_top[k] = cl.map_shared_rank(&x_top[turn][0], k / VER_WARPS)[k % VER_WARPS];
-            b_at[k] = cl.map_shared_rank(&x_at[turn][0], k / VER_WARPS)[k % VER_WARPS];
-            b_bad[k] = cl.map_shared_rank(&x_bad[turn][0], k / VER_WARPS)[k % VER_WARPS];
+            const unsigned from_rank = k / VER_WARPS, w = k % VER_WARPS;
+            b_sum[k] = cl.map_shared_rank(&x_sum[was][0], from_rank)[w];
+            b_top[k] = cl.map_shared_rank(&x_top[was][0], from_rank)[w];
+            b_at[k] = cl.map_shared_rank(&x_at[was][0], from_rank)[w];
+            b_bad[k] = cl.map_shared_rank(&x_bad[was][0], from_rank)[w];
         }
         __syncthreads();
         turn ^= 1;
@@ -170,15 +230,18 @@ __global__ void __launch_bounds__(VER_WARPS * 32) k_draft_verify(const VerifyArg
             top = ver_top(top, VerTop{__shfl_xor_sync(0xffffffffu, top.v, o), __shfl_xor_sync(0xffffffffu, top.at, o)});
             b |= __shfl_xor_sync(0xffffffffu, b, o);
         }
-        __syncthreads();
         bad = b || top.v == -INFINITY;
-        n_gone = n_res = 0;
+        double F = total();
+        if (!bad && !greedy && !(F >= 0x1p-100 && F < INFINITY)) {        // the first logit lies too far from the largest
+            from = (double)top.v;
+            __syncthreads();
+            F = sum_f();
+        }
+        return F;
     };
 
     int    cur = 0, held = 1;
-    double F = 0.0;
-    open_row(0);
-    bool have = false;                                    // F is f's sum
+    double F = open_row(0), whole = F;                    // f's sum; that of the row as it was
     if (rank == 0 && tid < n) a.kept[r0 + tid] = tid == 0 ? 0 : -1;
     __syncthreads();
     for (int j = 1; j < n && !bad; j++) {
@@ -188,31 +251,33 @@ __global__ void __launch_bounds__(VER_WARPS * 32) k_draft_verify(const VerifyArg
         bool take;
         if (greedy) take = x == top.at;
         else {
-            if (!have) {
-                sum_f();
-                F = total();
-                have = true;
-            }
             const double f = f_of(x), q = dr ? (double)__ldg(dr + x) : 1.0;
             take = (double)u_s[j] * q * F < f;
             if (!take) {
+                // a difference that has lost digits (little is left, in all or of its warp's run) is summed anew
+                const double run = dr ? 0.0 : b_sum[x / per];
+                const bool   anew = dr || !(F - f > whole * 0x1p-10) || !(run - f > run * 0x1p-20);
+                __syncthreads();                          // b_sum, F_s and gone_s are read no more
                 if (dr) {
                     if (tid == 0) F_s[n_res] = F;
                     n_res++;
                 } else {
-                    if (tid == 0) gone_s[n_gone] = x;
+                    if (tid == 0) {
+                        gone_s[n_gone] = x;
+                        b_sum[x / per] -= f;
+                    }
                     n_gone++;
+                    F -= f;
                 }
                 __syncthreads();
-                have = false;
+                if (anew) F = whole = sum_f();
             }
         }
         if (!take) continue;
         cur = j;
         if (rank == 0 && tid == 0) a.kept[r0 + held] = j;
         held++;
-        open_row(j);
-        have = false;
+        F = whole = open_row(j);
     }
     if (rank == 0 && tid == 0) a.n_kept[seq] = held;
     if (bad || greedy) {
@@ -220,12 +285,10 @@ __global__ void __launch_bounds__(VER_WARPS * 32) k_draft_verify(const VerifyArg
         cl.sync();                                        // no CTA leaves while others read its shared memory
         return;
     }
-    sum_f();
-    F = total();
     if (!(F > 0.0)) {                                     // a rejection of all there was: the target's own distribution
         n_gone = n_res = 0;
-        sum_f();
-        F = total();
+        __syncthreads();
+        F = sum_f();
     }
     // the warp whose run holds the draw
     const double mark = (double)__ldg(a.u_next + seq) * F;
@@ -243,23 +306,39 @@ __global__ void __launch_bounds__(VER_WARPS * 32) k_draft_verify(const VerifyArg
     const bool past = owner < 0;                          // rounding: the last token that has any weight
     if (past) owner = last;
     if (owner == me) {
+        // four tokens a lane in turn: their sum, the sums before them, and the first that passes the mark
         int    pick = -1;
         double run = before;
-        for (int b = x0; b < x1; b += 32) {
-            const int    x = b + lane;
-            const double f = x < x1 ? f_of(x) : 0.0;
-            double       in = f;
+        for (int b = x0; b < x1; b += 128) {
+            double f[4], in = 0.0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int x = b + 4 * lane + k;
+                f[k] = x < x1 ? f_of(x) : 0.0;
+                in += f[k];
+            }
+            const double mine = in;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const double v = __hiloint2double(__shfl_up_sync(0xffffffffu, __double2hiint(in), o), __shfl_up_sync(0xffffffffu, __double2loint(in), o));
                 if (lane >= o) in += v;
             }
-            const unsigned hit = __ballot_sync(0xffffffffu, f > 0.0 && run + in > mark && !past), any = __ballot_sync(0xffffffffu, f > 0.0);
-            if (hit) {
-                pick = b + __ffs(hit) - 1;
+            double at = run + (in - mine);
+            int    hit = -1, any = -1;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                at += f[k];
+                if (f[k] > 0.0) {
+                    any = b + 4 * lane + k;
+                    if (hit < 0 && !past && at > mark) hit = any;
+                }
+            }
+            const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), some = __ballot_sync(0xffffffffu, any >= 0);
+            if (hits) {
+                pick = __shfl_sync(0xffffffffu, hit, __ffs(hits) - 1);
                 break;
             }
-            if (any) pick = b + 31 - __clz(any);          // where none passes: the last
+            if (some) pick = __shfl_sync(0xffffffffu, any, 31 - __clz(some));      // where none passes: the last
             run += __hiloint2double(__shfl_sync(0xffffffffu, __double2hiint(in), 31), __shfl_sync(0xffffffffu, __double2loint(in), 31));
         }
         if (lane == 0) a.next[seq] = pick;
