@@ -249,14 +249,16 @@ int ecu_kv_compact(ecu_kv *kv, void *stream)
 
 struct KvMove { int from, to; uint16_t at; };
 
+// What is left of the moves and of the last operation's device words, as much
+// as a launch carries: a sequence's moves that do not fit go on in the next.
 template <int N>
-static int move_launch(ecu_kv *kv, const std::vector<KvMove> &moves, const std::vector<int> &first, size_t &i, size_t &j, cudaStream_t s)
+static int keep_launch(ecu_kv *kv, const std::vector<KvMove> &moves, const std::vector<int> &first, size_t &i, size_t &j, size_t &w, cudaStream_t s)
 {
     KvMoves<N> m;
-    m.n = 0;
+    m.n = m.n_set = 0;
     m.first[0] = 0;
     int k = 0;
-    while (k < N && j < moves.size()) {                   // a sequence that does not fit goes on in the next launch
+    while (k < N && j < moves.size()) {
         const int take = std::min<int>(N - k, first[i + 1] - (int)j);
         for (int x = 0; x < take; x++, k++, j++) {
             m.from[k] = moves[j].from;
@@ -266,8 +268,14 @@ static int move_launch(ecu_kv *kv, const std::vector<KvMove> &moves, const std::
         m.first[++m.n] = k;
         if ((int)j == first[i + 1]) i++;
     }
-    return launched("ecu_kv_keep", ecu_launch_early(k_kv4_move<N>, (unsigned)m.n * kv->n_layer, 256, 0, s, kv->data, kv->page_bytes,
-                                                    kv->page_bytes * kv->book.n_pages, kv->n_layer, kv->n_head_kv, kv->head_dim / 32, m));
+    for (; m.n_set < 2 * N && w < kv->book.sets.size(); m.n_set++, w++) {
+        m.word[m.n_set] = kv->book.sets[w].at;
+        m.value[m.n_set] = kv->book.sets[w].value;
+    }
+    if (kv->device < 0) return 0;
+    const long long blocks = (long long)m.n * kv->n_layer + (m.n_set + 255) / 256;
+    return launched("ecu_kv_keep", ecu_launch_early(k_kv4_move<N>, (unsigned)blocks, 256, 0, s, kv->data, kv->page_bytes,
+                                                    kv->page_bytes * kv->book.n_pages, kv->n_layer, kv->n_head_kv, kv->head_dim / 32, kv->meta, m));
 }
 
 extern "C" int ecu_kv_keep(ecu_kv *kv, const int *seq, const int *n_new, const int *kept, const int *n_kept, int n, void *stream)
@@ -312,17 +320,24 @@ extern "C" int ecu_kv_keep(ecu_kv *kv, const int *seq, const int *n_new, const i
         std::optional<DeviceScope> d;
         if (kv->device >= 0) d.emplace(kv->device);
         if (d && !d->ok) return say(what, "the pool's device cannot be used");
-        // The tables first: a launch that fails there is taken back.  The moves
-        // name their pages themselves, and those given back are taken only by
-        // later calls.
+        // (The moves name their pages themselves, and those given back are taken
+        // only by later calls.)
         changing = true;
-        if (kv->book.truncate(seq, len.data(), n) != 0 || update(kv, (cudaStream_t)stream) != 0) return -1;
-        for (size_t i = 0, j = 0; kv->device >= 0 && j < moves.size();)
-            if ((moves.size() - j <= 64 ? move_launch<64>(kv, moves, first, i, j, (cudaStream_t)stream)
-                                        : move_launch<512>(kv, moves, first, i, j, (cudaStream_t)stream)) != 0) {
-                kv->broken = true;
-                return -1;
-            }
+        if (kv->book.truncate(seq, len.data(), n) != 0) return -1;
+        changing = false;
+        const int fail_at = kv->inject;
+        kv->inject = -1;
+        size_t i = 0, j = 0, w = 0;
+        for (int k = 0; j < moves.size() || w < kv->book.sets.size(); k++) {
+            const bool small = moves.size() - j <= 64 && kv->book.sets.size() - w <= 128;
+            const int  rc = k == fail_at ? say(what, "launch failed: injected")
+                            : small      ? keep_launch<64>(kv, moves, first, i, j, w, (cudaStream_t)stream)
+                                         : keep_launch<512>(kv, moves, first, i, j, w, (cudaStream_t)stream);
+            if (rc == 0) continue;
+            if (k == 0) kv->book.fail();
+            else kv->broken = true;
+            return -1;
+        }
         return 0;
     } catch (const std::exception &e) {
         if (changing) kv->book.fail();

@@ -227,25 +227,31 @@ __global__ void __launch_bounds__(256) k_kv4_update(uint8_t *data, size_t page_b
 // Rows moved within their sequences, by value: group i (a sequence) has moves
 // first[i] .. first[i + 1] - 1, in the order of its positions, towards lower ones.
 template <int N> struct KvMoves {
-    int      n;
+    int      n, n_set;
     int      first[N + 1];
     int      from[N], to[N];          // pages
     uint16_t at[N];                   // positions in them: from, and to << 8
+    int      word[2 * N], value[2 * N];       // device words besides
 };
 
 #define KV4_MOVE_ITEMS 4          // blocks of 32 dimensions that a thread holds
 
-// A CTA per sequence and layer.  A row may be another's place, so a round of
+// A CTA per sequence and layer, and behind them those that set words.  A row may be another's place, so a round of
 // moves is read whole before any of it is written; a later round reads only
 // positions behind all that were written.  A move of a KV head of 128
 // dimensions reads and writes 144 bytes.
 template <int N>
-__global__ void __launch_bounds__(256) k_kv4_move(uint8_t *data, size_t page_bytes, size_t layer_bytes, int n_layer, int n_kv, int nb,
+__global__ void __launch_bounds__(256) k_kv4_move(uint8_t *data, size_t page_bytes, size_t layer_bytes, int n_layer, int n_kv, int nb, int *meta,
                                                   const __grid_constant__ KvMoves<N> m)
 {
     pdl_wait();
     pdl_trigger();
-    const int  i = blockIdx.x / n_layer, hd = nb * 32;
+    const int i = blockIdx.x / n_layer, hd = nb * 32;
+    if (i >= m.n) {
+        const int x = (int)(blockIdx.x - m.n * n_layer) * 256 + (int)threadIdx.x;
+        if (x < m.n_set) meta[m.word[x]] = m.value[x];
+        return;
+    }
     uint8_t   *layer = data + (size_t)(blockIdx.x - i * n_layer) * layer_bytes;
     const int  heads = min(n_kv, 256 * KV4_MOVE_ITEMS / (2 * nb)), end = m.first[i + 1];
     for (int h0 = 0; h0 < n_kv; h0 += heads) {

@@ -95,7 +95,7 @@ static int tree_start(ecu_kv *kv, const TreeArgs &a, const KvRows<N> &r, const T
     const bool shared = captured || !t.even || t.rows % grid != 0;
     if (launch(grid) != 0) return -1;
     if (!shared) return 0;
-    return launched("ecu_kv_attend_tree", ecu_launch_early(k_kv4_tree_join<T, NB, N>, (unsigned)grid * ((a.group + 7) / 8), 256, 0, s, a, r, unit, grid));
+    return launched("ecu_kv_attend_tree", ecu_launch_early(k_kv4_tree_join<T, NB, N>, (unsigned)grid * ((a.group + TREE_JOIN - 1) / TREE_JOIN), 256, 0, s, a, r, unit, grid));
 }
 
 template <typename T, int NB, int N>

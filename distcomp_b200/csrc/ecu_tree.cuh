@@ -600,8 +600,10 @@ __global__ void __launch_bounds__(TREE_WARPS * 32, 1) k_kv4_tree(const __grid_co
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Rows that several CTAs share: a block per CTA and 8 columns, which has work
-// where a row begins in that CTA and goes on behind it; a warp per column.
+// Rows that several CTAs share: a block per CTA and TREE_JOIN columns, which has
+// work where a row begins in that CTA and goes on behind it; a warp takes columns
+// in turn.
+#define TREE_JOIN 32
 template <typename T, int NB, int N>
 __global__ void __launch_bounds__(256) k_kv4_tree_join(const __grid_constant__ TreeArgs a, const __grid_constant__ KvRows<N> rows, int unit, int grid)
 {
@@ -611,7 +613,7 @@ __global__ void __launch_bounds__(256) k_kv4_tree_join(const __grid_constant__ T
     pdl_wait();
     pdl_trigger();
     tree_scan<256>(a, rows, unit, pre, sums);
-    const int total = pre[n], ctas = min(grid, total), slices = (a.group + 7) / 8, cta = blockIdx.x / slices;
+    const int total = pre[n], ctas = min(grid, total), slices = (a.group + TREE_JOIN - 1) / TREE_JOIN, cta = blockIdx.x / slices;
     if (cta >= ctas) return;
     auto begin_of = [&](int b) { return (int)((long long)total * b / ctas); };
     const int cu0 = begin_of(cta), cu1 = begin_of(cta + 1);
@@ -630,42 +632,45 @@ __global__ void __launch_bounds__(256) k_kv4_tree_join(const __grid_constant__ T
     while (begin_of(last + 1) <= end - 1) last++;
     while (begin_of(last) > end - 1) last--;
     const int np = last - cta + 1, kvh = r / p.n_cg, cg = r - kvh * p.n_cg;
-    const int cc = (blockIdx.x % slices) * 8 + warp, col = cg * a.group + cc;
-    if (cc >= a.group || col >= n_new * a.n_rep) return;
-    auto  entry = [&](int b) { return a.part + ((size_t)(cta + b) * 2 + (b == 0)) * ((size_t)EC * (HD + 2)); };
-    float m = -INFINITY, L = 0.0f;
-    for (int b = lane; b < np; b += 32) m = fmaxf(m, __ldcg(entry(b) + EC * HD + cc));
+    auto      entry = [&](int b) { return a.part + ((size_t)(cta + b) * 2 + (b == 0)) * ((size_t)EC * (HD + 2)); };
+    const int cc0 = (blockIdx.x % slices) * TREE_JOIN;
+    for (int cc = cc0 + warp; cc < min(cc0 + TREE_JOIN, a.group); cc += 8) {
+        const int col = cg * a.group + cc;
+        if (col >= n_new * a.n_rep) return;
+        float m = -INFINITY, L = 0.0f;
+        for (int b = lane; b < np; b += 32) m = fmaxf(m, __ldcg(entry(b) + EC * HD + cc));
 #pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int b0 = 0; b0 < np; b0 += 32) {
-        float w = 0.0f;
-        if (b0 + lane < np) {
-            const float l = __ldcg(entry(b0 + lane) + EC * (HD + 1) + cc);
-            w = l == 0.0f ? 0.0f : kv4_ex2(__ldcg(entry(b0 + lane) + EC * HD + cc) - m);
-            L = fmaf(w, l, L);
-        }
-        const int k1 = min(32, np - b0);
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int b0 = 0; b0 < np; b0 += 32) {
+            float w = 0.0f;
+            if (b0 + lane < np) {
+                const float l = __ldcg(entry(b0 + lane) + EC * (HD + 1) + cc);
+                w = l == 0.0f ? 0.0f : kv4_ex2(__ldcg(entry(b0 + lane) + EC * HD + cc) - m);
+                L = fmaf(w, l, L);
+            }
+            const int k1 = min(32, np - b0);
 #pragma unroll 4
-        for (int k = 0; k < k1; k++) {
-            const float f = __shfl_sync(0xffffffffu, w, k);
-            if (lane < HD / 4) {
-                const float4 v = __ldcg(reinterpret_cast<const float4 *>(entry(b0 + k)) + cc * (HD / 4) + lane);
-                s.x = fmaf(f, v.x, s.x);
-                s.y = fmaf(f, v.y, s.y);
-                s.z = fmaf(f, v.z, s.z);
-                s.w = fmaf(f, v.w, s.w);
+            for (int k = 0; k < k1; k++) {
+                const float f = __shfl_sync(0xffffffffu, w, k);
+                if (lane < HD / 4) {
+                    const float4 v = __ldcg(reinterpret_cast<const float4 *>(entry(b0 + k)) + cc * (HD / 4) + lane);
+                    s.x = fmaf(f, v.x, s.x);
+                    s.y = fmaf(f, v.y, s.y);
+                    s.z = fmaf(f, v.z, s.z);
+                    s.w = fmaf(f, v.w, s.w);
+                }
             }
         }
-    }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    if (lane >= HD / 4) return;
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    const int   t = col / a.n_rep, h = col - t * a.n_rep;
-    T          *o = (T *)a.out + (size_t)(r0 + t) * a.out_stride + (size_t)(kvh * a.n_rep + h) * HD + 4 * lane;
-    o[0] = kv4_from<T>(s.x * inv);
-    o[1] = kv4_from<T>(s.y * inv);
-    o[2] = kv4_from<T>(s.z * inv);
-    o[3] = kv4_from<T>(s.w * inv);
+        for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        if (lane >= HD / 4) continue;
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        const int   t = col / a.n_rep, h = col - t * a.n_rep;
+        T          *o = (T *)a.out + (size_t)(r0 + t) * a.out_stride + (size_t)(kvh * a.n_rep + h) * HD + 4 * lane;
+        o[0] = kv4_from<T>(s.x * inv);
+        o[1] = kv4_from<T>(s.y * inv);
+        o[2] = kv4_from<T>(s.z * inv);
+        o[3] = kv4_from<T>(s.w * inv);
+    }
 }

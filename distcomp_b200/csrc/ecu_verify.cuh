@@ -26,7 +26,7 @@
 #include <cooperative_groups.h>
 
 #define VER_WARPS 16
-#define VER_MAX_CTAS 16           // of a cluster
+#define VER_MAX_CTAS 8            // of a cluster
 #define VER_ROWS 64               // rows of a tree
 
 struct VerifyArgs {
@@ -62,6 +62,49 @@ __device__ __forceinline__ VerTop ver_top(VerTop a, VerTop b)
     return b.v > a.v || (b.v == a.v && b.at < a.at) ? b : a;
 }
 
+// Of n sums (at most 128) that begin at `before`, the first positive one that the
+// running sum passes the mark in, and the sum before it; where none does
+// (rounding), or `end` says so already, the last positive one.  By a warp.
+struct VerDraw {
+    int    at;
+    double before;
+    bool   end;
+};
+__device__ __forceinline__ VerDraw ver_find(const double *sums, int n, double before, double mark, bool end, int lane)
+{
+    double w[4], in = 0.0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        w[k] = 4 * lane + k < n ? sums[4 * lane + k] : 0.0;
+        in += w[k];
+    }
+    const double mine = in;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double v = __hiloint2double(__shfl_up_sync(0xffffffffu, __double2hiint(in), o), __shfl_up_sync(0xffffffffu, __double2loint(in), o));
+        if (lane >= o) in += v;
+    }
+    double run = before + (in - mine), at = run;
+    int    hit = -1, any = -1;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        if (w[k] > 0.0) {
+            any = 4 * lane + k;
+            if (hit < 0 && !end && run + w[k] > mark) {
+                hit = any;
+                at = run;
+            }
+        }
+        run += w[k];
+    }
+    const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), some = __ballot_sync(0xffffffffu, any >= 0);
+    VerDraw        d{-1, 0.0, hits == 0};
+    const int      from = hits ? __ffs(hits) - 1 : some ? 31 - __clz(some) : 0;
+    d.at = __shfl_sync(0xffffffffu, hits ? hit : any, from);
+    d.before = __hiloint2double(__shfl_sync(0xffffffffu, __double2hiint(at), from), __shfl_sync(0xffffffffu, __double2loint(at), from));
+    return d;
+}
+
 #define VER_TABLE 256
 
 // 2^t; t < -1000: 0, t > 1000: infinity.  t = k / 256 + f with |f| <= 1/512, and
@@ -83,15 +126,27 @@ __device__ __forceinline__ double ver_ex2(double t, const double *table)
 // f(x, logit) for this lane's elements of [x0, x1), x0 a multiple of eight.
 template <typename T, typename F> __device__ __forceinline__ void ver_each(const T *row, int x0, int x1, bool wide, int lane, F f)
 {
-    constexpr int V = 16 / (int)sizeof(T);                // elements of 16 bytes
+    constexpr int V = 16 / (int)sizeof(T), U = 16 / V;    // elements of 16 bytes; loads in flight together
     int           x = x0;
-    if (wide)
-        for (; x + 32 * V <= x1; x += 32 * V) {
-            __align__(16) T v[V];
-            *reinterpret_cast<uint4 *>(v) = __ldg(reinterpret_cast<const uint4 *>(row + x + lane * V));
+    if (wide) {
+        for (; x + V <= x1; x += 32 * V * U) {
+            uint4 w[U];
 #pragma unroll
-            for (int k = 0; k < V; k++) f(x + lane * V + k, kv4_float(v[k]));
+            for (int i = 0; i < U; i++) {
+                const int at = x + (32 * i + lane) * V;
+                w[i] = at + V <= x1 ? __ldg(reinterpret_cast<const uint4 *>(row + at)) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+                const int at = x + (32 * i + lane) * V;
+                const T  *v = reinterpret_cast<const T *>(&w[i]);
+                if (at + V <= x1)
+#pragma unroll
+                    for (int k = 0; k < V; k++) f(at + k, kv4_float(v[k]));
+            }
         }
+        x = x1 - (x1 - x0) % V;                           // (fewer than V are left)
+    }
     for (x += lane; x < x1; x += 32) f(x, kv4_float(row[x]));
 }
 
@@ -254,9 +309,8 @@ __global__ void __launch_bounds__(VER_WARPS * 32, 2) k_draft_verify(const Verify
             const double f = f_of(x), q = dr ? (double)__ldg(dr + x) : 1.0;
             take = (double)u_s[j] * q * F < f;
             if (!take) {
-                // a difference that has lost digits (little is left, in all or of its warp's run) is summed anew
-                const double run = dr ? 0.0 : b_sum[x / per];
-                const bool   anew = dr || !(F - f > whole * 0x1p-10) || !(run - f > run * 0x1p-20);
+                // a difference that has lost digits (little is left, in all or, next to all, of its warp's run) is summed anew
+                const bool anew = dr || !(F - f > whole * 0x1p-10) || !(b_sum[x / per] - f > whole * 0x1p-40);
                 __syncthreads();                          // b_sum, F_s and gone_s are read no more
                 if (dr) {
                     if (tid == 0) F_s[n_res] = F;
@@ -292,56 +346,58 @@ __global__ void __launch_bounds__(VER_WARPS * 32, 2) k_draft_verify(const Verify
     }
     // the warp whose run holds the draw
     const double mark = (double)__ldg(a.u_next + seq) * F;
-    double       before = 0.0, s = 0.0;
-    int          owner = -1, last = -1;
-    for (int k = 0; k < W; k++) {                         // the same at every thread
-        const double w = b_sum[k];
-        if (w > 0.0) last = k;
-        if (owner < 0 && w > 0.0 && s + w > mark) {
-            owner = k;
-            before = s;
-        }
-        s += w;
-    }
-    const bool past = owner < 0;                          // rounding: the last token that has any weight
-    if (past) owner = last;
-    if (owner == me) {
-        // four tokens a lane in turn: their sum, the sums before them, and the first that passes the mark
-        int    pick = -1;
-        double run = before;
-        for (int b = x0; b < x1; b += 128) {
-            double f[4], in = 0.0;
+    const VerDraw draw = ver_find(b_sum, W, 0.0, mark, false, lane);
+    const int     owner = draw.at;
+    // its CTA's warps share the run once more: their sums, and the one that holds the draw (or the last weight)
+    if (owner >= 0 && owner / VER_WARPS == rank) {
+        const int o0 = min(a.vocab, owner * per), o1 = min(a.vocab, o0 + per), part = ((o1 - o0 + VER_WARPS - 1) / VER_WARPS + 3) & ~3;
+        const int p0 = min(o1, o0 + warp * part), p1 = min(o1, p0 + part);
+        double    mine = 0.0;
+        for (int x = p0 + lane; x < p1; x += 32) mine += f_of(x);
+        mine = warp_total(mine);
+        if (lane == 0) x_sum[turn][warp] = mine;          // (no CTA reads it any more)
+        __syncthreads();
+        const VerDraw part_draw = ver_find(x_sum[turn], VER_WARPS, draw.before, mark, draw.end, lane);
+        const bool    end = part_draw.end;
+        if (part_draw.at < 0 && tid == 0) a.next[seq] = top.at;
+        if (part_draw.at == warp) {
+            // four tokens a lane in turn: their sum, the sums before them, and the first that passes the mark
+            int    pick = -1;
+            double run = part_draw.before;
+            for (int b = p0; b < p1; b += 128) {
+                double f[4], in = 0.0;
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const int x = b + 4 * lane + k;
-                f[k] = x < x1 ? f_of(x) : 0.0;
-                in += f[k];
-            }
-            const double mine = in;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double v = __hiloint2double(__shfl_up_sync(0xffffffffu, __double2hiint(in), o), __shfl_up_sync(0xffffffffu, __double2loint(in), o));
-                if (lane >= o) in += v;
-            }
-            double at = run + (in - mine);
-            int    hit = -1, any = -1;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                at += f[k];
-                if (f[k] > 0.0) {
-                    any = b + 4 * lane + k;
-                    if (hit < 0 && !past && at > mark) hit = any;
+                for (int k = 0; k < 4; k++) {
+                    const int x = b + 4 * lane + k;
+                    f[k] = x < p1 ? f_of(x) : 0.0;
+                    in += f[k];
                 }
+                const double mine = in;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double v = __hiloint2double(__shfl_up_sync(0xffffffffu, __double2hiint(in), o), __shfl_up_sync(0xffffffffu, __double2loint(in), o));
+                    if (lane >= o) in += v;
+                }
+                double at = run + (in - mine);
+                int    hit = -1, any = -1;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    at += f[k];
+                    if (f[k] > 0.0) {
+                        any = b + 4 * lane + k;
+                        if (hit < 0 && !end && at > mark) hit = any;
+                    }
+                }
+                const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), some = __ballot_sync(0xffffffffu, any >= 0);
+                if (hits) {
+                    pick = __shfl_sync(0xffffffffu, hit, __ffs(hits) - 1);
+                    break;
+                }
+                if (some) pick = __shfl_sync(0xffffffffu, any, 31 - __clz(some));      // where none passes: the last
+                run += __hiloint2double(__shfl_sync(0xffffffffu, __double2hiint(in), 31), __shfl_sync(0xffffffffu, __double2loint(in), 31));
             }
-            const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), some = __ballot_sync(0xffffffffu, any >= 0);
-            if (hits) {
-                pick = __shfl_sync(0xffffffffu, hit, __ffs(hits) - 1);
-                break;
-            }
-            if (some) pick = __shfl_sync(0xffffffffu, any, 31 - __clz(some));      // where none passes: the last
-            run += __hiloint2double(__shfl_sync(0xffffffffu, __double2hiint(in), 31), __shfl_sync(0xffffffffu, __double2loint(in), 31));
+            if (lane == 0) a.next[seq] = pick;
         }
-        if (lane == 0) a.next[seq] = pick;
     }
     cl.sync();
 }

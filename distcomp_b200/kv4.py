@@ -19,6 +19,7 @@ EngineError.
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 
 import numpy as np
 import torch
@@ -310,9 +311,14 @@ class KvPool:
         s, n_new = _ints(seq), _ints(n_new)
         if len(s) != len(n_new) or len(s) != len(kept):
             raise EngineError(f"{len(s)} sequences, {len(n_new)} counts and {len(kept)} lists of rows")
-        count = _ints([len(r) for r in kept])
-        flat = _ints([j for r in kept for j in r])
-        if lib().ecu_kv_keep(self.h, _at(s), _at(n_new), _at(flat), _at(count), len(s), self._stream(stream)) != 0:
+        flat, count = array("i"), array("i", map(len, kept))
+        try:
+            for rows in kept:
+                flat.extend(rows)
+        except (TypeError, OverflowError):
+            raise EngineError("kept: lists of rows are wanted") from None
+        if lib().ecu_kv_keep(self.h, _at(s), _at(n_new), flat.buffer_info()[0], count.buffer_info()[0], len(s),
+                             self._stream(stream)) != 0:
             raise EngineError(last_error())
 
     def attend(self, layer: int, q: torch.Tensor, seq=None, out: torch.Tensor | None = None, scale: float | None = None,
