@@ -121,12 +121,13 @@ static int tree_launch(ecu_kv *kv, TreeArgs a, const int *seq, int first, const 
     }
     if constexpr (sizeof(T) == 2 && NB % 2 == 0) {
         const TreeTotal x = tree_total(kv, a, r, TT_COLS, TT_UNIT, 1);
-        // A unit of 128 positions and 128 columns takes 2.0 us, whatever columns it has, one of 32 positions and 16
-        // columns 0.22 to 0.29: even at 32 columns (32768 positions of 4 sequences 120 against 128 us; 16 columns 119
-        // against 82, 64: 123 against 220).  With less than a unit an SM the finer units are ahead (900 positions, 256
-        // columns: 35 against 31 us).
-        if (x.units >= kv->sms && x.units * 7.5 < best) {
+        // A unit of 128 positions and 128 columns takes 1.9 us whatever columns it has, one of 32 positions and 16 columns
+        // 0.22 to 0.29 (of 64-wide heads 1.8 and 0.13 to 0.15), and the former has some two units more to begin and end.
+        // 4 sequences of 16384 positions, 4 query heads a KV head, 32 / 64 columns: 79 against 83 / 82 against 130 us (64-wide
+        // 70 against 57 / 71 against 85); 2 of 2000: 38 against 33 / 40 against 43.
+        if ((x.units + 2.0 * kv->sms) * (NB == 4 ? 7.0 : 11.0) < best) {
             a.group = a.entry = TT_COLS;
+            a.open = TT_OPEN;
             auto kern = k_kv4_tree_tc<T, NB * 32, N>;
             int *status = ecu_prompt_status_word(kv->device);
             if (!status) return say("ecu_kv_attend_tree", "the status word cannot be had");
@@ -146,6 +147,7 @@ static int tree_launch(ecu_kv *kv, TreeArgs a, const int *seq, int first, const 
     }
     a.group = S::C * a.wc;
     a.entry = S::EC;
+    a.open = TREE_OPEN;
     auto kern = k_kv4_tree<T, NB, N>;
     return tree_start<T, NB>(kv, a, r, t, KV4_UNIT, captured, s, [&](int grid) {
         static std::atomic<unsigned> done{0};
@@ -158,7 +160,7 @@ template <typename T, int NB> static int tree_list(ecu_kv *kv, TreeArgs a, const
 {
     // at most 2^31 - 1 places in a launch, however the sequences may grow
     const TreePlan  p = tree_plan(kv->book.max_pages * KV4_PAGE, TREE_ROWS, a.n_kv, a.n_rep, TreeShape<T, NB>::C, KV4_UNIT);
-    const long long places = (long long)p.rows * (p.nu + TREE_OPEN);
+    const long long places = (long long)p.rows * (p.nu + std::max(TREE_OPEN, TT_OPEN));
     if (places > INT_MAX) return say("ecu_kv_attend_tree", "too many positions and heads a sequence");
     const int most = (int)std::min<long long>(KV4_LIST, INT_MAX / places);
     for (int i = 0; i < n; i += most) {

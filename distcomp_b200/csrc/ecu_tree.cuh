@@ -33,7 +33,7 @@
 
 #define TREE_ROWS 64              // drafted rows of a sequence: bits of a mask
 #define TREE_WARPS 12
-#define TREE_OPEN 6               // places of a row beside its units
+#define TREE_OPEN 12              // places of a row beside its units
 #define TREE_MAX_WC 4
 
 struct TreeArgs {
@@ -46,6 +46,7 @@ struct TreeArgs {
     const long long *mask;        // nullptr: each row sees those before it
     int            max_pages, n_pages, n_kv, n_rep, wc;
     int            group;         // columns of a row: wc tiles of them
+    int            open;          // places of a row beside its units
     int            entry;         // columns of a partial
     float          scale;
     bool           wide_q, wide_out;
@@ -74,7 +75,7 @@ __host__ __device__ inline TreePlan tree_plan(int len, int n_new, int n_kv, int 
     p.rows = p.nu ? n_kv * p.n_cg : 0;
     return p;
 }
-__host__ __device__ inline int tree_places(const TreePlan &p) { return p.rows * (p.nu + TREE_OPEN); }
+__host__ __device__ inline int tree_places(const TreePlan &p, int open) { return p.rows * (p.nu + open); }
 
 // pre[i]: places before sequence i, by the first NT threads of a block that
 // meets as a whole.
@@ -90,7 +91,7 @@ __device__ __forceinline__ void tree_scan(const TreeArgs &a, const KvRows<N> &ro
         c[k] = 0;
         if (i < n && tid < NT) {
             const int len = min(max(__ldg(a.len + rows.seq[i]), 0), a.max_pages * KV4_PAGE);
-            c[k] = tree_places(tree_plan(len, rows.row0[i + 1] - rows.row0[i], a.n_kv, a.n_rep, a.group, unit));
+            c[k] = tree_places(tree_plan(len, rows.row0[i + 1] - rows.row0[i], a.n_kv, a.n_rep, a.group, unit), a.open);
         }
         sum += c[k];
     }
@@ -121,7 +122,7 @@ __device__ __forceinline__ void tree_scan(const TreeArgs &a, const KvRows<N> &ro
 // A row: sequence i, KV head r / n_cg, group of columns r % n_cg; its first
 // place, and the units [j0, j1) of it that fall to the CTA with the places
 // [cu0, cu1).  first() and next() walk the rows that have units there: places
-// are TREE_OPEN and then one a unit.
+// are a.open (what its beginning and end cost) and then one a unit.
 template <int N> struct TreeWalk {
     const TreeArgs  &a;
     const KvRows<N> &rows;
@@ -142,16 +143,16 @@ template <int N> struct TreeWalk {
         }
         i = lo;
         enter();
-        r = (cu0 - place) / (nu + TREE_OPEN);
-        place += r * (nu + TREE_OPEN);
+        r = (cu0 - place) / (nu + a.open);
+        place += r * (nu + a.open);
         range();
         while (place < cu1 && j1 <= j0) next();           // (its units end before the run, or begin behind it)
     }
     __device__ __forceinline__ int  len() const { return min(max(__ldg(a.len + rows.seq[i]), 0), a.max_pages * KV4_PAGE); }
     __device__ __forceinline__ void range()
     {
-        j0 = max(0, cu0 - place - TREE_OPEN);
-        j1 = min(nu, cu1 - place - TREE_OPEN);
+        j0 = max(0, cu0 - place - a.open);
+        j1 = min(nu, cu1 - place - a.open);
     }
     __device__ __forceinline__ void enter()
     {
@@ -165,7 +166,7 @@ template <int N> struct TreeWalk {
     __device__ __forceinline__ bool here() const { return place < cu1 && j1 > j0; }
     __device__ __forceinline__ void next()
     {
-        place += nu + TREE_OPEN;
+        place += nu + a.open;
         if (++r == n_rows) {
             do i++;
             while (i < rows.n && pre[i + 1] == pre[i]);
@@ -626,7 +627,7 @@ __global__ void __launch_bounds__(256) k_kv4_tree_join(const __grid_constant__ T
     }
     const int      len = min(max(__ldg(a.len + rows.seq[lo]), 0), a.max_pages * KV4_PAGE), r0 = rows.row0[lo], n_new = rows.row0[lo + 1] - r0;
     const TreePlan p = tree_plan(len, n_new, a.n_kv, a.n_rep, a.group, unit);
-    const int      r = (cu1 - 1 - pre[lo]) / (p.nu + TREE_OPEN), begin = pre[lo] + r * (p.nu + TREE_OPEN) + TREE_OPEN, end = begin + p.nu;
+    const int      r = (cu1 - 1 - pre[lo]) / (p.nu + a.open), begin = pre[lo] + r * (p.nu + a.open) + a.open, end = begin + p.nu;
     if (begin < cu0 || begin >= cu1 || end <= cu1) return;
     int last = (int)((long long)(end - 1) * ctas / total);          // the CTA of the row's last unit
     while (begin_of(last + 1) <= end - 1) last++;

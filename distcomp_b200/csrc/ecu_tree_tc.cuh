@@ -43,6 +43,7 @@
 static_assert(4 * 80 + 2 * 64 + 48 <= 7 * TT_REGS, "the groups' registers are those of the launch");
 #define TT_UNIT 128
 #define TT_COLS 128
+#define TT_OPEN 6                 // places of a row beside its units
 #define TT_BASE 9.0f              // weights are 2^(t - M + TT_BASE) ...
 #define TT_SLACK 6.0f             // ... and M follows when t has passed it by so much: below 2^15, and fp16 down to 2^-33
 #define TT_SHIFT 4
