@@ -87,13 +87,19 @@ template <int N> static TreeTotal tree_total(const ecu_kv *kv, const TreeArgs &a
 }
 
 template <typename T, int NB, int N, typename F>
-static int tree_start(ecu_kv *kv, const TreeArgs &a, const KvRows<N> &r, const TreeTotal &t, int unit, bool captured, cudaStream_t s, F launch)
+static int tree_start(ecu_kv *kv, TreeArgs a, const KvRows<N> &r, const TreeTotal &t, int unit, bool captured, cudaStream_t s, F launch)
 {
-    // One CTA an SM; fewer where a CTA would find less than two units.  Rows of
-    // one length that fill whole CTAs are not shared, and need no join.
-    const int  grid = captured ? kv->sms : (int)std::max(1ll, std::min<long long>(kv->sms, t.want));
+    // One CTA an SM; fewer where a CTA would find less than two units.  Few rows
+    // of one length get as many CTAs each, whose parts are equal when a row's
+    // beginning takes no place; and rows of one length that fill whole CTAs are
+    // not shared, and need no join.
+    int grid = captured ? kv->sms : (int)std::max(1ll, std::min<long long>(kv->sms, t.want));
+    if (!captured && t.even && t.rows <= grid) {
+        grid -= (int)(grid % t.rows);
+        a.open = 0;
+    }
     const bool shared = captured || !t.even || t.rows % grid != 0;
-    if (launch(grid) != 0) return -1;
+    if (launch(a, grid) != 0) return -1;
     if (!shared) return 0;
     return launched("ecu_kv_attend_tree", ecu_launch_early(k_kv4_tree_join<T, NB, N>, (unsigned)grid * ((a.group + TREE_JOIN - 1) / TREE_JOIN), 256, 0, s, a, r, unit, grid));
 }
@@ -133,7 +139,7 @@ static int tree_launch(ecu_kv *kv, TreeArgs a, const int *seq, int first, const 
             if (!status) return say("ecu_kv_attend_tree", "the status word cannot be had");
             int stall = 0;
             if (kv->device < 32 && g_stall.load(std::memory_order_relaxed)) stall = (int)(g_stall.fetch_and(~(1u << kv->device)) >> kv->device & 1u);
-            return tree_start<T, NB>(kv, a, r, x, TT_UNIT, captured, s, [&](int grid) {
+            return tree_start<T, NB>(kv, a, r, x, TT_UNIT, captured, s, [&](const TreeArgs &a, int grid) {
                 static std::atomic<unsigned> done{0};
                 CK(ecu_allow_smem(kern, TreeTc<NB * 32>::smem(N), kv->device, done));
                 static const int regs = [&] {
@@ -149,7 +155,7 @@ static int tree_launch(ecu_kv *kv, TreeArgs a, const int *seq, int first, const 
     a.entry = S::EC;
     a.open = TREE_OPEN;
     auto kern = k_kv4_tree<T, NB, N>;
-    return tree_start<T, NB>(kv, a, r, t, KV4_UNIT, captured, s, [&](int grid) {
+    return tree_start<T, NB>(kv, a, r, t, KV4_UNIT, captured, s, [&](const TreeArgs &a, int grid) {
         static std::atomic<unsigned> done{0};
         CK(ecu_allow_smem(kern, S::smem(N), kv->device, done));
         return launched("ecu_kv_attend_tree", ecu_launch_early(kern, (unsigned)grid, TREE_WARPS * 32, S::smem(n), s, a, r));

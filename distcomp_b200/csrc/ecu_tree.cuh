@@ -62,6 +62,27 @@ template <typename T, int NB> struct TreeShape {
     static constexpr size_t smem(int n) { return ring + parts + (size_t)(n + 1) * 4; }
 };
 
+// Two fp32 values in one register pair, for the packed fp32 units.
+__device__ __forceinline__ uint64_t tree_two(float a, float b)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void     tree_untwo(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t tree_fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t tree_add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // Places of one sequence's rows (KV heads times groups of columns).
 struct TreePlan {
     int nu, rows, n_cg;           // units of a row, rows, groups of columns
@@ -286,7 +307,7 @@ __global__ void __launch_bounds__(TREE_WARPS * 32, 1) k_kv4_tree(const __grid_co
                 }
 #pragma unroll
         for (int kt = 0; kt < 2; kt++) {
-            float    acc[2][4];
+            uint64_t acc[2][2];                           // pairs of positions 2c, 2c + 1
             uint32_t ks[2][NB];
 #pragma unroll
             for (int y = 0; y < 2; y++) {
@@ -297,8 +318,7 @@ __global__ void __launch_bounds__(TREE_WARPS * 32, 1) k_kv4_tree(const __grid_co
                     ks[y][k] = kp[k];
                     vs[2 * kt + y][k] = vp[k];
                 }
-#pragma unroll
-                for (int k = 0; k < 4; k++) acc[y][k] = 0.0f;
+                acc[y][0] = acc[y][1] = 0ull;
             }
             const int t2 = kt * 16 + mt_row;
 #pragma unroll
@@ -318,21 +338,23 @@ __global__ void __launch_bounds__(TREE_WARPS * 32, 1) k_kv4_tree(const __grid_co
                         kv4_mma0(e, q0[0], q0[1], q0[2], q0[3], x[0], x[1]);
                         kv4_mma(e, q1[0], q1[1], q1[2], q1[3], x[2], x[3]);
                         const float s0 = half_of(ks[y][(b + d) / 2], (b + d) & 1), s1 = half_of(ks[y][(NB + b + d) / 2], (NB + b + d) & 1);
-                        acc[y][0] = fmaf(s0, e[0], acc[y][0]);
-                        acc[y][1] = fmaf(s1, e[1], acc[y][1]);
-                        acc[y][2] = fmaf(s0, e[2], acc[y][2]);
-                        acc[y][3] = fmaf(s1, e[3], acc[y][3]);
+                        const uint64_t s2 = tree_two(s0, s1);
+                        acc[y][0] = tree_fma2(s2, tree_two(e[0], e[1]), acc[y][0]);
+                        acc[y][1] = tree_fma2(s2, tree_two(e[2], e[3]), acc[y][1]);
                     }
                 }
             }
 #pragma unroll
             for (int y = 0; y < 2; y++) {
                 const int nt = 2 * kt + y;
+                float     row[2][2];
+                tree_untwo(acc[y][0], row[0][0], row[0][1]);
+                tree_untwo(acc[y][1], row[1][0], row[1][1]);
 #pragma unroll
                 for (int e = 0; e < 2; e++)
 #pragma unroll
                     for (int x = 0; x < RR; x++) {
-                        const float s = P == 2 ? acc[y][e] + acc[y][2 + e] : acc[y][2 * x + e];
+                        const float s = P == 2 ? row[0][e] + row[1][e] : row[x][e];
                         sc[nt][2 * x + e] = s;
                         if (!CUT || (live[x] >> (2 * nt + e) & 1u)) top[x] = fmaxf(top[x], s);
                     }
@@ -450,7 +472,8 @@ __global__ void __launch_bounds__(TREE_WARPS * 32, 1) k_kv4_tree(const __grid_co
 #pragma unroll
                     for (int j = 0; j < 4; j++)
 #pragma unroll
-                        for (int k = 0; k < 4; k++) O[b + d][j][k] += e[j][k];
+                        for (int k = 0; k < 4; k += 2)
+                            tree_untwo(tree_add2(tree_two(O[b + d][j][k], O[b + d][j][k + 1]), tree_two(e[j][k], e[j][k + 1])), O[b + d][j][k], O[b + d][j][k + 1]);
             }
         }
     };
