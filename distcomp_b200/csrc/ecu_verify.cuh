@@ -45,10 +45,14 @@ template <int N> struct VerifyRows {
     int row0[N + 1];
 };
 
-// The largest value so far and its first place; a NaN or an infinity shows in `bad`.
+// The largest value so far and its first place; -1 where a NaN or an infinity was among them.
 struct VerTop {
     float v;
     int   at;
+};
+struct __align__(16) VerWord {
+    double sum;
+    VerTop top;
 };
 __device__ __forceinline__ double warp_total(double v)
 {
@@ -59,6 +63,7 @@ __device__ __forceinline__ double warp_total(double v)
 
 __device__ __forceinline__ VerTop ver_top(VerTop a, VerTop b)
 {
+    if (a.at < 0 || b.at < 0) return VerTop{0.0f, -1};
     return b.v > a.v || (b.v == a.v && b.at < a.at) ? b : a;
 }
 
@@ -156,12 +161,9 @@ __global__ void __launch_bounds__(VER_WARPS * 32, 2) k_draft_verify(const Verify
     namespace cg = cooperative_groups;
     cg::cluster_group cl = cg::this_cluster();
     const int CL = (int)cl.num_blocks(), rank = (int)cl.block_rank();
-    __shared__ double   x_sum[2][VER_WARPS];              // what this CTA's warps tell the cluster, two exchanges in turn
-    __shared__ float    x_top[2][VER_WARPS];
-    __shared__ int      x_at[2][VER_WARPS], x_bad[2][VER_WARPS];
-    __shared__ double   b_sum[VER_MAX_CTAS * VER_WARPS];
-    __shared__ float    b_top[VER_MAX_CTAS * VER_WARPS];
-    __shared__ int      b_at[VER_MAX_CTAS * VER_WARPS], b_bad[VER_MAX_CTAS * VER_WARPS];
+    __shared__ VerWord  x_word[2][VER_WARPS];             // what this CTA's warps tell the cluster, two exchanges in turn
+    __shared__ VerTop   b_top[VER_MAX_CTAS * VER_WARPS];  // what all warps said
+    __shared__ double   b_sum[VER_MAX_CTAS * VER_WARPS], p_sum[VER_WARPS];
     __shared__ double   F_s[VER_ROWS + 1];                // f's sums at the current row, before each rejection
     __shared__ int      gone_s[VER_ROWS], tok_s[VER_ROWS], par_s[VER_ROWS];
     __shared__ float    u_s[VER_ROWS];
@@ -201,9 +203,9 @@ __global__ void __launch_bounds__(VER_WARPS * 32, 2) k_draft_verify(const Verify
 
     // every warp's sum, at every CTA, and their total, in the order of the warps by every thread alike
     auto exchange = [&](double sum) {
-        if (lane == 0) x_sum[turn][warp] = sum;
+        if (lane == 0) x_word[turn][warp].sum = sum;
         cl.sync();
-        for (int k = tid; k < W; k += VER_WARPS * 32) b_sum[k] = cl.map_shared_rank(&x_sum[turn][0], k / VER_WARPS)[k % VER_WARPS];
+        for (int k = tid; k < W; k += VER_WARPS * 32) b_sum[k] = cl.map_shared_rank(&x_word[turn][0], k / VER_WARPS)[k % VER_WARPS].sum;
         __syncthreads();
         turn ^= 1;
     };
@@ -251,41 +253,25 @@ __global__ void __launch_bounds__(VER_WARPS * 32, 2) k_draft_verify(const Verify
             }
         });
         const double s = warp_total(s0 + s1);
+        auto reduce = [&] {
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            top = ver_top(top, VerTop{__shfl_xor_sync(0xffffffffu, top.v, o), __shfl_xor_sync(0xffffffffu, top.at, o)});
-            b |= __shfl_xor_sync(0xffffffffu, b, o);
-        }
-        if (lane == 0) {
-            x_top[turn][warp] = top.v;
-            x_at[turn][warp] = top.at;
-            x_bad[turn][warp] = b;
-        }
-        const int was = turn;
-        __syncthreads();                                  // (b_sum and the others are read no more)
-        if (lane == 0) x_sum[turn][warp] = s;
-        cl.sync();
+            for (int o = 16; o; o >>= 1) top = ver_top(top, VerTop{__shfl_xor_sync(0xffffffffu, top.v, o), __shfl_xor_sync(0xffffffffu, top.at, o)});
+        };
+        if (b) top.at = -1;
+        reduce();
+        if (lane == 0) x_word[turn][warp] = VerWord{s, top};
+        cl.sync();                                        // (b_sum and b_top are read no more)
         for (int k = tid; k < W; k += VER_WARPS * 32) {
-            const unsigned from_rank = k / VER_WARPS, w = k % VER_WARPS;
-            b_sum[k] = cl.map_shared_rank(&x_sum[was][0], from_rank)[w];
-            b_top[k] = cl.map_shared_rank(&x_top[was][0], from_rank)[w];
-            b_at[k] = cl.map_shared_rank(&x_at[was][0], from_rank)[w];
-            b_bad[k] = cl.map_shared_rank(&x_bad[was][0], from_rank)[w];
+            const VerWord w = cl.map_shared_rank(&x_word[turn][0], k / VER_WARPS)[k % VER_WARPS];
+            b_sum[k] = w.sum;
+            b_top[k] = w.top;
         }
         __syncthreads();
         turn ^= 1;
         top = VerTop{-INFINITY, 0x7FFFFFFF};
-        b = 0;
-        for (int k = lane; k < W; k += 32) {
-            top = ver_top(top, VerTop{b_top[k], b_at[k]});
-            b |= b_bad[k];
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            top = ver_top(top, VerTop{__shfl_xor_sync(0xffffffffu, top.v, o), __shfl_xor_sync(0xffffffffu, top.at, o)});
-            b |= __shfl_xor_sync(0xffffffffu, b, o);
-        }
-        bad = b || top.v == -INFINITY;
+        for (int k = lane; k < W; k += 32) top = ver_top(top, b_top[k]);
+        reduce();
+        bad = top.at < 0 || top.v == -INFINITY;
         double F = total();
         if (!bad && !greedy && !(F >= 0x1p-100 && F < INFINITY)) {        // the first logit lies too far from the largest
             from = (double)top.v;
@@ -355,9 +341,9 @@ __global__ void __launch_bounds__(VER_WARPS * 32, 2) k_draft_verify(const Verify
         double    mine = 0.0;
         for (int x = p0 + lane; x < p1; x += 32) mine += f_of(x);
         mine = warp_total(mine);
-        if (lane == 0) x_sum[turn][warp] = mine;          // (no CTA reads it any more)
+        if (lane == 0) p_sum[warp] = mine;
         __syncthreads();
-        const VerDraw part_draw = ver_find(x_sum[turn], VER_WARPS, draw.before, mark, draw.end, lane);
+        const VerDraw part_draw = ver_find(p_sum, VER_WARPS, draw.before, mark, draw.end, lane);
         const bool    end = part_draw.end;
         if (part_draw.at < 0 && tid == 0) a.next[seq] = top.at;
         if (part_draw.at == warp) {
