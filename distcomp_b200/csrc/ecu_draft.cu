@@ -232,8 +232,7 @@ static int verify_launch(VerifyArgs a, const int *n_row, int n, int sms, cudaStr
     for (int i = 0; i < n; i++) r.row0[i + 1] = r.row0[i] + n_row[i];
     // CTAs of a sequence: as many as keep all sequences in flight together, two
     // CTAs an SM, and find a few hundred tokens a warp
-    const int most = std::max(1, std::min(8, std::min(2 * sms / n, a.vocab / (VER_WARPS * 64))));
-    const int cl = most;
+    const int cl = std::max(1, std::min(VER_MAX_CTAS, std::min(2 * sms / n, a.vocab / (VER_WARPS * 64))));
     cudaLaunchConfig_t  cfg = {};
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -275,6 +274,7 @@ extern "C" int ecu_draft_verify(int dtype, const void *logits, long stride, int 
     const size_t es = dtype_bytes(dtype);
     if (!es) return say(what, "unknown element type");
     if (n < 0 || (n > 0 && (!n_row || !u_next || !n_kept || !next)) || n_vocab < 1) return say(what, "null argument, negative count or no vocabulary");
+    if (n_vocab > 1 << 30) return say(what, "a vocabulary of more than 2^30 tokens");       // (tokens are counted in an int, past the end too)
     long long rows = 0;
     for (int i = 0; i < n; i++) {
         if (n_row[i] < 0 || n_row[i] > VER_ROWS) {

@@ -18,8 +18,15 @@
 // once: its largest logit, whether it is a distribution at all, and the sum of
 // 2^((l - c) / T log2 e) come out of one pass, c being the row's first logit (64
 // bits hold 2^+-1000 around it; where that is not enough, a second pass takes
-// the largest).  What bounds it is that pass, ten operations of 64 bits a logit;
-// the exponential is a table of 2^(k/256) and four terms of its series.
+// the largest).  The exponential is a table of 2^(k/256) and four terms of its
+// series: ten operations of 64 bits a logit.
+//
+// Latency bounds it: the rows of a path come one behind the other, each a pass
+// and an exchange between the cluster's CTAs.  A chain of 5 drafts over 128256
+// fp32 logits takes 14 us (of a row's 0.5 MB on 8 CTAs), 48 trees of 4 to 16
+// rows (bf16) 47 us: 51 MB through L2, 57 % of the issue slots and 22 % of the
+// fp64 units' time.  Two passes over a row, the maximum first and then exp()'s
+// sums, took 44 and 191.
 #pragma once
 #include "ecu_kv4.cuh"
 

@@ -457,10 +457,12 @@ int  ecu_rope_set(ecu_rope *r, int rot, int interleaved, const double *freq, dou
  * Row r of a sequence that gets n_new[i] rows is written at position len -
  * n_new[i] + r and turned by the position len - n_new[i] + depth[r] (depth:
  * device, one number for each row of the call; NULL: r), len read on the device
- * when the call runs.  A key is turned and quantised in 64-bit arithmetic, its
- * code that of the exact value; a query is turned in 32 bits and rounded once
- * to `dtype`.  q_out may be q with its stride; else it is apart from the rows
- * read.  Everything else as in ecu_kv_append. */
+ * when the call runs.  A key is turned to some 46 bits and quantised from
+ * them, so that its code is that of the exact value (but for about one in
+ * 10^12); one that passes fp32's range on the way (values near 2^127) reads as
+ * NaN.  A query is turned in 32 bits and rounded once to `dtype`.  q_out may be
+ * q with its stride; else it is apart from the rows read.  Everything else as
+ * in ecu_kv_append. */
 int  ecu_kv_append_rope(ecu_kv *kv, int layer, const ecu_rope *rope, int dtype, const void *q, const void *k,
                         const void *v, int n_head, long q_stride, long k_stride, long v_stride, const int *seq,
                         const int *n_new, int n, const int *depth, void *q_out, long q_out_stride, int out_dtype,
@@ -490,7 +492,7 @@ size_t ecu_kv_tree_ws_bytes(const ecu_kv *kv);
 
 /* Drafted tokens held against the target's probabilities with given random
  * numbers.  Sequence i has n_row[i] (at most ECU_DRAFT_ROWS) consecutive rows:
- * logits [n_vocab] (`dtype`, rows `stride` elements apart), the token of each
+ * logits [n_vocab] (at most 2^30; `dtype`, rows `stride` elements apart), the token of each
  * row and its parent, an earlier row of the sequence (row 0's are not looked
  * at).  From row 0 on, rows are tried in order: one that hangs on the current
  * row, with token x, is accepted where u[row] q(x) F < f(x), and becomes the

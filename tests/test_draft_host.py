@@ -184,6 +184,10 @@ def test_verify_refuses(over, why):
     assert verify_args(**over) == -1 and why in error()
 
 
+def test_verify_refuses_a_vocabulary_past_counting():
+    assert verify_args(vocab=2 ** 30 + 1, stride=2 ** 30 + 1) == -1 and "2^30" in error()
+
+
 def test_verify_of_nothing():
     assert verify_args(n=0) == 0
 
