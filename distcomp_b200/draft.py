@@ -23,7 +23,7 @@ import numpy as np
 import torch
 
 from .engine import EngineError, int_list as _ints, last_error, lib
-from .kv4 import _DTYPES, _at, _current
+from .kv4 import _DTYPES, _at, _current, _total
 
 ROWS = 64                      # drafted rows of a sequence, at most
 _SCALING = {None: 0, "linear": 1, "bands": 2, "yarn": 3}
@@ -105,7 +105,7 @@ def tree(parents, device: int | None = 0):
 def _vector(t: torch.Tensor | None, what: str, dtype: torch.dtype, n: int, dev: int) -> int | None:
     if t is None:
         return None
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous() or not t.is_cuda or t.get_device() != dev:
+    if t.dtype is not dtype or t.dim() != 1 or t.numel() != n or not t.is_contiguous() or t.get_device() != dev:
         raise EngineError(f"{what}: {n} contiguous {str(dtype)[6:]} numbers on CUDA device {dev} are wanted")
     return t.data_ptr()
 
@@ -125,7 +125,7 @@ def verify(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, n_
     (float32; 0: greedy), one a sequence; draft [rows, n_vocab] (float32), the distributions that a row's children were
     drawn from.  kept (one a row), n_kept and next (one a sequence) are int32."""
     cnt = _ints(n_row)
-    n, rows = len(cnt), int(cnt.sum(dtype=np.int64))
+    n, rows = len(cnt), _total(cnt)
     ls = _matrix(logits, "logits", rows)
     dev, vocab = logits.get_device(), logits.shape[1]
     if logits.dtype not in _DTYPES:

@@ -23,6 +23,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+from array import array
 from pathlib import Path
 
 import numpy as np
@@ -54,6 +55,11 @@ def int_list(a) -> np.ndarray:
     """A list or array as C ints; one of other values, or of more dimensions, is refused."""
     if type(a) is np.ndarray and a.dtype == np.int32 and a.ndim == 1 and a.flags.c_contiguous:
         return a
+    try:
+        if type(a) is list:
+            return np.frombuffer(array("i", a), dtype=np.int32) if a else np.zeros(0, np.int32)
+    except (OverflowError, TypeError):                    # (floats that are whole pass below)
+        pass
     try:
         b = np.ascontiguousarray(a, dtype=np.int32)
         if b.ndim == 1 and np.array_equal(b, a):

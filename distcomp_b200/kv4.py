@@ -47,8 +47,8 @@ def _at(a: np.ndarray) -> int:
         return a.ctypes.data
 
 
-def _row(t: torch.Tensor, what: str, heads: int | None, hd: int, device: int) -> tuple[int, int]:
-    """(heads, row stride) of rows [n, heads, hd] or [n, heads * hd]."""
+def _rows(t: torch.Tensor, what: str, heads: int | None, hd: int, device: int) -> tuple:
+    """(heads, row stride, shape, strides) of rows [n, heads, hd] or [n, heads * hd]."""
     if t.dtype not in _DTYPES or not t.is_cuda or t.get_device() != device:
         raise EngineError(f"{what}: rows of float32, float16 or bfloat16 on CUDA device {device} are wanted")
     shape, st = t.shape, t.stride()
@@ -61,7 +61,21 @@ def _row(t: torch.Tensor, what: str, heads: int | None, hd: int, device: int) ->
     if not good or h < 1 or (heads is not None and h != heads):
         raise EngineError(f"{what}: rows {tuple(shape)} with strides {st} are not [n, "
                           f"{'heads' if heads is None else heads}, {hd}] with their heads one after the other")
-    return h, st[0] if shape[0] > 1 else h * hd
+    return h, st[0] if shape[0] > 1 else h * hd, shape, st
+
+
+def _row(t: torch.Tensor, what: str, heads: int | None, hd: int, device: int) -> tuple[int, int]:
+    """(heads, row stride) of rows [n, heads, hd] or [n, heads * hd]."""
+    return _rows(t, what, heads, hd, device)[:2]
+
+
+def _total(counts: np.ndarray) -> int:
+    return sum(counts.tolist()) if len(counts) <= 256 else int(counts.sum(dtype=np.int64))
+
+
+def _same(t: torch.Tensor, dtype: torch.dtype, shape: tuple, strides: tuple, device: int) -> bool:
+    """Laid out as another on that device, which has been checked (each attribute that is asked of a tensor counts here)."""
+    return t.dtype is dtype and t.shape == shape and t.stride() == strides and t.get_device() == device
 
 
 def _current(device: int) -> int:
@@ -229,22 +243,25 @@ class KvPool:
         q_out (which may be q; ecu_kv_append_rope).  depth: int32, one a row, how far behind the positions held before
         the row stands; by default its number in its sequence."""
         heads, hd, dev = self.n_head_kv, self.head_dim, self.device
-        _, ks = _row(k, "k", heads, hd, dev)
-        vs = ks if _like(v, k) else _row(v, "v", heads, hd, dev)[1]
         n_new = _ints(n_new)
         s = None if seq is None else _ints(seq)
-        n = len(n_new)
-        rows = sum(n_new.tolist()) if n <= 256 else int(n_new.sum(dtype=np.int64))
-        if (s is not None and len(s) != n) or k.shape[0] != rows or v.shape[0] != rows or k.dtype != v.dtype:
+        n, rows = len(n_new), _total(n_new)
+        _, ks, shape, strides = _rows(k, "k", heads, hd, dev)
+        vs, vn, dt = ks, shape[0], k.dtype
+        if not _same(v, dt, shape, strides, dev):
+            _, vs, (vn, *_), _ = _rows(v, "v", heads, hd, dev)
+        if (s is not None and len(s) != n) or shape[0] != rows or vn != rows or v.dtype is not dt:
             raise EngineError(f"k and v: {rows} rows of one type are wanted, and a count for each sequence")
         qp = qo = None
         nh = qs = qos = 0
         if q is not None:
-            nh, qs = _row(q, "q", None, hd, dev)
+            nh, qs, shape, strides = _rows(q, "q", None, hd, dev)
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            qos = qs if _like(q_out, q) else _row(q_out, "q_out", nh, hd, dev)[1]
-            if q.dtype != k.dtype or q_out.dtype != q.dtype or q.shape[0] != rows or q_out.shape[0] != rows:
+                q_out = torch.empty(shape, dtype=q.dtype, device=q.device)
+            qos, on = qs, shape[0]
+            if not _same(q_out, dt, shape, strides, dev):
+                _, qos, (on, *_), _ = _rows(q_out, "q_out", nh, hd, dev)
+            if q.dtype is not dt or q_out.dtype is not dt or shape[0] != rows or on != rows:
                 raise EngineError(f"q and q_out: {rows} rows of k's type are wanted")
             qp, qo = q.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
@@ -255,16 +272,16 @@ class KvPool:
         if (k_out is None) != (v_out is None):
             raise EngineError("k_out and v_out come together")
         ko = vo = None
-        od = k.dtype
+        od = dt
         if k_out is not None:
-            _row(k_out, "k_out", heads, hd, dev)
-            if not _like(v_out, k_out):
-                _row(v_out, "v_out", heads, hd, dev)
-            if k_out.shape[0] != rows or v_out.shape[0] != rows or k_out.dtype != v_out.dtype or \
-                    not k_out.is_contiguous() or not v_out.is_contiguous():
+            _, _, shape, strides = _rows(k_out, "k_out", heads, hd, dev)
+            vn, od = shape[0], k_out.dtype
+            if not _same(v_out, od, shape, strides, dev):
+                _, _, (vn, *_), _ = _rows(v_out, "v_out", heads, hd, dev)
+            if shape[0] != rows or vn != rows or v_out.dtype is not od or not k_out.is_contiguous() or not v_out.is_contiguous():
                 raise EngineError(f"k_out and v_out: {rows} contiguous rows of one type are wanted")
-            ko, vo, od = k_out.data_ptr(), v_out.data_ptr(), k_out.dtype
-        if lib().ecu_kv_append_rope(self.h, self._layer(layer), rope.at, _DTYPES[k.dtype], qp, k.data_ptr(), v.data_ptr(), nh, qs, ks,
+            ko, vo = k_out.data_ptr(), v_out.data_ptr()
+        if lib().ecu_kv_append_rope(self.h, self._layer(layer), rope.at, _DTYPES[dt], qp, k.data_ptr(), v.data_ptr(), nh, qs, ks,
                                     vs, None if s is None else _at(s), _at(n_new), n, None if depth is None else depth.data_ptr(),
                                     qo, qos, _DTYPES[od], ko, vo, self._stream(stream)) != 0:
             raise EngineError(last_error())
@@ -276,14 +293,16 @@ class KvPool:
         """The newest n_new[i] positions of each sequence over those before them and, of themselves, those whose bit is
         set in their mask (int64, one a row; draft.tree makes them; by default each row sees those before it;
         ecu_kv_attend_tree).  ws: tree_workspace() for calls that are captured or may overlap."""
-        heads, qs = _row(q, "q", None, self.head_dim, self.device)
+        heads, qs, shape, strides = _rows(q, "q", None, self.head_dim, self.device)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        os_ = qs if _like(out, q) else _row(out, "out", heads, self.head_dim, self.device)[1]
+            out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        os_, on = qs, shape[0]
+        if not _same(out, q.dtype, shape, strides, self.device):
+            _, os_, (on, *_), _ = _rows(out, "out", heads, self.head_dim, self.device)
         n_new = _ints(n_new)
         s = None if seq is None else _ints(seq)
-        n, rows = len(n_new), int(n_new.sum(dtype=np.int64))
-        if out.dtype != q.dtype or out.shape[0] != rows or q.shape[0] != rows or (s is not None and len(s) != n):
+        n, rows = len(n_new), _total(n_new)
+        if out.dtype is not q.dtype or on != rows or shape[0] != rows or (s is not None and len(s) != n):
             raise EngineError(f"q and out: {rows} rows of one type are wanted, and a count for each sequence")
         if mask is not None and (mask.dtype != torch.int64 or mask.dim() != 1 or mask.shape[0] != rows or
                                  not mask.is_contiguous() or not mask.is_cuda or mask.get_device() != self.device):
@@ -311,10 +330,11 @@ class KvPool:
         s, n_new = _ints(seq), _ints(n_new)
         if len(s) != len(n_new) or len(s) != len(kept):
             raise EngineError(f"{len(s)} sequences, {len(n_new)} counts and {len(kept)} lists of rows")
-        flat, count = array("i"), array("i", map(len, kept))
+        numbers, count = [], array("i", list(map(len, kept)))
         try:
             for rows in kept:
-                flat.extend(rows)
+                numbers.extend(rows)
+            flat = array("i", numbers)
         except (TypeError, OverflowError):
             raise EngineError("kept: lists of rows are wanted") from None
         if lib().ecu_kv_keep(self.h, _at(s), _at(n_new), flat.buffer_info()[0], count.buffer_info()[0], len(s),

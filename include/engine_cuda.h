@@ -478,8 +478,9 @@ int  ecu_kv_append_rope(ecu_kv *kv, int layer, const ecu_rope *rope, int dtype, 
  * finite in K makes the row NaN, one in V its block of 32 dimensions; positions
  * that it does not see have no effect.  ws: ecu_kv_tree_ws_bytes() bytes of
  * device memory that no other call uses at the same time; NULL: the pool's own
- * for this stream, as in ecu_kv_attend.  The lengths are read on the device when
- * the call runs, so a captured call follows its sequences.  Sums and the softmax
+ * for this stream, as in ecu_kv_attend.  out and q do not overlap.  The lengths
+ * are read on the device when the call runs, so a captured call follows its
+ * sequences.  Sums and the softmax
  * are fp32; of fp32 queries, and of their weights, 22 bits count; 16-bit queries
  * of many columns (rows times query heads of a KV head, some 32 and more) see
  * keys and values rounded to fp16's 11 bits, as the prompts of a batch do.
