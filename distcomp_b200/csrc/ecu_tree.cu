@@ -86,22 +86,40 @@ template <int N> static TreeTotal tree_total(const ecu_kv *kv, const TreeArgs &a
     return t;
 }
 
-template <typename T, int NB, int N, typename F>
-static int tree_start(ecu_kv *kv, TreeArgs a, const KvRows<N> &r, const TreeTotal &t, int unit, bool captured, cudaStream_t s, F launch)
+// How a launch cuts its rows: its CTAs, whether rows are shared and so joined,
+// and how long that takes: `start`, `step` for each of a CTA's units, `row` for
+// each of its rows, `join` where there is a second launch (us, measured).
+struct TreeWay { int grid; bool shared, even; double us; };
+static TreeWay tree_way(const TreeTotal &t, int sms, bool captured, double start, double step, double row, double join)
 {
-    // One CTA an SM; fewer where a CTA would find less than two units.  Few rows
-    // of one length get as many CTAs each, whose parts are equal when a row's
-    // beginning takes no place; and rows of one length that fill whole CTAs are
-    // not shared, and need no join.
-    int grid = captured ? kv->sms : (int)std::max(1ll, std::min<long long>(kv->sms, t.want));
-    if (!captured && t.even && t.rows <= grid) {
-        grid -= (int)(grid % t.rows);
-        a.open = 0;
-    }
-    const bool shared = captured || !t.even || t.rows % grid != 0;
-    if (launch(a, grid) != 0) return -1;
-    if (!shared) return 0;
-    return launched("ecu_kv_attend_tree", ecu_launch_early(k_kv4_tree_join<T, NB, N>, (unsigned)grid * ((a.group + TREE_JOIN - 1) / TREE_JOIN), 256, 0, s, a, r, unit, grid));
+    auto us = [&](int grid, bool shared, double fewest) {
+        return start + std::max(fewest, t.units / grid) * step + (double)t.rows / grid * row + (shared ? join : 0.0);
+    };
+    // One CTA an SM; fewer where a CTA would find less than two units a group.
+    // (A captured launch's sequences grow: nothing of its plan may depend on them.)
+    TreeWay w;
+    w.grid = captured ? sms : (int)std::max(1ll, std::min<long long>(sms, t.want));
+    w.even = !captured && t.even;
+    // Few rows of one length get as many CTAs each, whose parts are equal when a row's beginning takes no place.
+    if (w.even && t.rows <= w.grid) w.grid -= (int)(w.grid % t.rows);
+    w.shared = !w.even || t.rows % w.grid != 0;
+    w.us = us(w.grid, w.shared, 1.0);
+    if (!w.even || !w.shared) return w;
+    // Or whole rows of one length, as many a CTA, and no join.
+    int whole = (int)std::min<long long>(sms, t.rows);
+    while (t.rows % whole) whole--;
+    const double alone = us(whole, false, 1.0);
+    if (alone < w.us) w = {whole, false, true, alone};
+    return w;
+}
+
+template <typename T, int NB, int N, typename F>
+static int tree_start(TreeArgs a, const KvRows<N> &r, const TreeWay &w, long long rows, int unit, cudaStream_t s, F launch)
+{
+    if (w.even && rows <= w.grid) a.open = 0;
+    if (launch(a, w.grid) != 0) return -1;
+    if (!w.shared) return 0;
+    return launched("ecu_kv_attend_tree", ecu_launch_early(k_kv4_tree_join<T, NB, N>, (unsigned)w.grid * ((a.group + TREE_JOIN - 1) / TREE_JOIN), 256, 0, s, a, r, unit, w.grid));
 }
 
 template <typename T, int NB, int N>
@@ -111,27 +129,34 @@ static int tree_launch(ecu_kv *kv, TreeArgs a, const int *seq, int first, const 
     KvRows<N> r;
     fill_rows(r, seq, first, n_new, n);
     if (r.row0[n] == 0) return 0;
-    // Tiles of a group: the width at which the sequences' units cost least (a
-    // unit of a group of wc warps occupies them all, whether a warp has a tile
-    // or not, and no unit passes faster than its bytes arrive)
-    double    best = 0.0;
-    TreeTotal t;
+    // Tiles of a group: the width that is estimated to take least.  (A step of the groups, 32 positions each, takes 3.0 us
+    // at 128-wide heads and 1.7 at 64, a row's queries, merge and output 5 to 8.5, a join 12 to 18.  Narrow groups spread few
+    // rows over more CTAs, wide ones read the cache less often: one sequence of 2000 positions with 16 drafts of 4 query
+    // heads, bf16, 26, 32, 35 and 40 us with 1 to 4 tiles; 32 of 1 to 4096 positions of 8 query heads, fp32, 545, 468, 440
+    // and 437.)
+    const double size = S::C * S::HD / 1024.0;
+    TreeWay      best{};
+    long long    best_rows = 0;
     for (int wc = TREE_MAX_WC; wc >= 1; wc--) {
-        const TreeTotal x = tree_total(kv, a, r, S::C * wc, KV4_UNIT, 2 * (TREE_WARPS / wc));
-        const double    cost = x.units * wc * (wc == 1 ? 1.2 : 1.0);
-        if (wc == TREE_MAX_WC || cost < best) {
-            best = cost;
+        const int       groups = TREE_WARPS / wc;
+        const TreeTotal t = tree_total(kv, a, r, S::C * wc, KV4_UNIT, 2 * groups);
+        TreeTotal       steps = t;                        // the groups take a row's units in turn
+        steps.units /= groups;
+        const TreeWay w = tree_way(steps, kv->sms, captured, 3.0, 0.4 + 0.65 * NB, 2.3 + 3.1 * size, 8.0 + 3.0 * size + 1.5 * wc);
+        if (!best.grid || w.us < best.us) {
+            best = w;
+            best_rows = t.rows;
             a.wc = wc;
-            t = x;
         }
     }
     if constexpr (sizeof(T) == 2 && NB % 2 == 0) {
-        const TreeTotal x = tree_total(kv, a, r, TT_COLS, TT_UNIT, 1);
-        // A unit of 128 positions and 128 columns takes 1.9 us whatever columns it has, one of 32 positions and 16 columns
-        // 0.22 to 0.29 (of 64-wide heads 1.8 and 0.13 to 0.15), and the former has some two units more to begin and end.
-        // 4 sequences of 16384 positions, 4 query heads a KV head, 32 / 64 columns: 79 against 83 / 82 against 130 us (64-wide
-        // 70 against 57 / 71 against 85); 2 of 2000: 38 against 33 / 40 against 43.
-        if ((x.units + 2.0 * kv->sms) * (NB == 4 ? 7.0 : 11.0) < best) {
+        // A unit of 128 positions and up to 128 columns, however many it has, takes 1.85 us (of 64-wide heads 1.6), the first
+        // and the last some 14 more.  (4 sequences of 16384 positions, 4 query heads a KV head, 32 / 64 columns: 79 against 83 /
+        // 82 against 130 us, 64-wide 70 against 57 / 71 against 85.  Over 570 calls of 1 to 32 sequences of up to 4096
+        // positions, these estimates take 1 to 3 % longer than the best of all choices, counts of units alone 14 to 17.)
+        const TreeTotal t = tree_total(kv, a, r, TT_COLS, TT_UNIT, 1);
+        const TreeWay   w = tree_way(t, kv->sms, captured, 17.0, NB == 4 ? 1.85 : 1.6, 0.0, 13.0);
+        if (w.us < best.us) {
             a.group = a.entry = TT_COLS;
             a.open = TT_OPEN;
             auto kern = k_kv4_tree_tc<T, NB * 32, N>;
@@ -139,7 +164,7 @@ static int tree_launch(ecu_kv *kv, TreeArgs a, const int *seq, int first, const 
             if (!status) return say("ecu_kv_attend_tree", "the status word cannot be had");
             int stall = 0;
             if (kv->device < 32 && g_stall.load(std::memory_order_relaxed)) stall = (int)(g_stall.fetch_and(~(1u << kv->device)) >> kv->device & 1u);
-            return tree_start<T, NB>(kv, a, r, x, TT_UNIT, captured, s, [&](const TreeArgs &a, int grid) {
+            return tree_start<T, NB>(a, r, w, t.rows, TT_UNIT, s, [&](const TreeArgs &a, int grid) {
                 static std::atomic<unsigned> done{0};
                 CK(ecu_allow_smem(kern, TreeTc<NB * 32>::smem(N), kv->device, done));
                 static const int regs = [&] {
@@ -155,7 +180,7 @@ static int tree_launch(ecu_kv *kv, TreeArgs a, const int *seq, int first, const 
     a.entry = S::EC;
     a.open = TREE_OPEN;
     auto kern = k_kv4_tree<T, NB, N>;
-    return tree_start<T, NB>(kv, a, r, t, KV4_UNIT, captured, s, [&](const TreeArgs &a, int grid) {
+    return tree_start<T, NB>(a, r, best, best_rows, KV4_UNIT, s, [&](const TreeArgs &a, int grid) {
         static std::atomic<unsigned> done{0};
         CK(ecu_allow_smem(kern, S::smem(N), kv->device, done));
         return launched("ecu_kv_attend_tree", ecu_launch_early(kern, (unsigned)grid, TREE_WARPS * 32, S::smem(n), s, a, r));
