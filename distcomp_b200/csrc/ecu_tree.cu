@@ -92,8 +92,8 @@ template <int N> static TreeTotal tree_total(const ecu_kv *kv, const TreeArgs &a
 struct TreeWay { int grid; bool shared, even; double us; };
 static TreeWay tree_way(const TreeTotal &t, int sms, bool captured, double start, double step, double row, double join)
 {
-    auto us = [&](int grid, bool shared, double fewest) {
-        return start + std::max(fewest, t.units / grid) * step + (double)t.rows / grid * row + (shared ? join : 0.0);
+    auto us = [&](int grid, bool shared) {
+        return start + std::max(1.0, t.units / grid) * step + (double)t.rows / grid * row + (shared ? join : 0.0);
     };
     // One CTA an SM; fewer where a CTA would find less than two units a group.
     // (A captured launch's sequences grow: nothing of its plan may depend on them.)
@@ -103,12 +103,12 @@ static TreeWay tree_way(const TreeTotal &t, int sms, bool captured, double start
     // Few rows of one length get as many CTAs each, whose parts are equal when a row's beginning takes no place.
     if (w.even && t.rows <= w.grid) w.grid -= (int)(w.grid % t.rows);
     w.shared = !w.even || t.rows % w.grid != 0;
-    w.us = us(w.grid, w.shared, 1.0);
+    w.us = us(w.grid, w.shared);
     if (!w.even || !w.shared) return w;
     // Or whole rows of one length, as many a CTA, and no join.
     int whole = (int)std::min<long long>(sms, t.rows);
     while (t.rows % whole) whole--;
-    const double alone = us(whole, false, 1.0);
+    const double alone = us(whole, false);
     if (alone < w.us) w = {whole, false, true, alone};
     return w;
 }
@@ -119,7 +119,10 @@ static int tree_start(TreeArgs a, const KvRows<N> &r, const TreeWay &w, long lon
     if (w.even && rows <= w.grid) a.open = 0;
     if (launch(a, w.grid) != 0) return -1;
     if (!w.shared) return 0;
-    return launched("ecu_kv_attend_tree", ecu_launch_early(k_kv4_tree_join<T, NB, N>, (unsigned)w.grid * ((a.group + TREE_JOIN - 1) / TREE_JOIN), 256, 0, s, a, r, unit, w.grid));
+    // Columns of a block of the join: one a warp where rows have many parts (1 sequence of 4000 positions, 128 columns a KV
+    // head: 39, 47 and 57 us with 8, 16 and 32), else two (17 of 2000: 104, 102 and 108).
+    const int slice = rows * 4 <= w.grid ? 8 : 16;
+    return launched("ecu_kv_attend_tree", ecu_launch_early(k_kv4_tree_join<T, NB, N>, (unsigned)w.grid * ((a.group + slice - 1) / slice), 256, 0, s, a, r, unit, w.grid, slice));
 }
 
 template <typename T, int NB, int N>

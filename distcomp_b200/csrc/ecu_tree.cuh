@@ -30,12 +30,14 @@
 // the order of the CTAs.
 //
 // Short calls are bound by latency: 6 drafts of one sequence of 900 positions
-// (32 query and 8 KV heads of 128, fp32) take 24 us with the host's call, 17
-// sequences of up to 3000 positions (16 and 4 heads of 64, fp16) 34.  Many
-// columns are bound by the scales between the products, which the tensor cores
-// do not apply: 32 sequences of 1 to 4096 positions (64 and 8 heads of 128) take
-// 437 us in fp32, 545 before the fp32 sums were packed and rows' own places
-// counted.  In 16 bits such calls run on ecu_tree_tc.cuh's kernel instead.
+// (32 query and 8 KV heads of 128, fp32) take 16 us (the host's call alone 12),
+// 17 sequences of up to 3000 positions (16 and 4 heads of 64, fp16) 34: a step of
+// the groups takes about 3 us (64-wide heads 1.7), a row's queries, merge and
+// output 5 to 8, a join 12.  Many columns are bound by the scales between the
+// products, which the tensor cores do not apply: 32 sequences of 1 to 4096
+// positions (64 and 8 heads of 128) take 437 us in fp32, 545 before the fp32 sums
+// were packed and rows' own places counted.  In 16 bits such calls run on
+// ecu_tree_tc.cuh's kernel instead.
 #pragma once
 #include "ecu_kv4.cuh"
 
@@ -384,24 +386,26 @@ __global__ void __launch_bounds__(TREE_WARPS * 32, 1) k_kv4_tree(const __grid_co
         if (!CUT)
 #pragma unroll
             for (int x = 0; x < RR; x++) vrow[x] = fmaxf(__low2float(vm), __high2float(vm));
+        auto still = [&](int x) { return top[x] + exponent(vrow[x]) <= M[x] + KV4_SLACK || (CUT && live[x] == 0u); };
         bool calm = true;
 #pragma unroll
         for (int x = 0; x < RR; x++) {
             top[x] *= fac[x];
-            calm = calm && (top[x] + exponent(vrow[x]) <= M[x] + KV4_SLACK || (CUT && live[x] == 0u));
+            calm = calm && still(x);
         }
         if (!__all_sync(0xffffffffu, calm)) {
             // M follows the largest score + log2 of the largest V scale
 #pragma unroll
             for (int x = 0; x < RR; x++) {
+                const unsigned asked = __ballot_sync(0xffffffffu, !still(x)) >> (lane & 28) & 15u;
 #pragma unroll
                 for (int o = 1; o < 4; o <<= 1) {
                     vrow[x] = fmaxf(vrow[x], __shfl_xor_sync(0xffffffffu, vrow[x], o));
                     top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], o));
                 }
-                // (of this row alone: no row's bits depend on what shares its tile)
+                // (of this row alone, and where one of its own lanes asked for it: no row's bits depend on what shares its tile)
                 const float m = top[x] + exponent(vrow[x]);
-                const bool  grow = m > M[x] + KV4_SLACK;
+                const bool  grow = asked && m > M[x] + KV4_SLACK;
                 const float alpha = grow ? kv4_ex2(M[x] - m) : 1.0f;
                 if (grow) M[x] = m;
                 l[x] *= alpha;
@@ -632,12 +636,11 @@ __global__ void __launch_bounds__(TREE_WARPS * 32, 1) k_kv4_tree(const __grid_co
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Rows that several CTAs share: a block per CTA and TREE_JOIN columns, which has
+// Rows that several CTAs share: a block per CTA and `slice` columns, which has
 // work where a row begins in that CTA and goes on behind it; a warp takes columns
 // in turn.
-#define TREE_JOIN 32
 template <typename T, int NB, int N>
-__global__ void __launch_bounds__(256) k_kv4_tree_join(const __grid_constant__ TreeArgs a, const __grid_constant__ KvRows<N> rows, int unit, int grid)
+__global__ void __launch_bounds__(256) k_kv4_tree_join(const __grid_constant__ TreeArgs a, const __grid_constant__ KvRows<N> rows, int unit, int grid, int slice)
 {
     constexpr int  HD = NB * 32;
     __shared__ int pre[N + 1], sums[8];
@@ -645,7 +648,7 @@ __global__ void __launch_bounds__(256) k_kv4_tree_join(const __grid_constant__ T
     pdl_wait();
     pdl_trigger();
     tree_scan<256>(a, rows, unit, pre, sums);
-    const int total = pre[n], ctas = min(grid, total), slices = (a.group + TREE_JOIN - 1) / TREE_JOIN, cta = blockIdx.x / slices;
+    const int total = pre[n], ctas = min(grid, total), slices = (a.group + slice - 1) / slice, cta = blockIdx.x / slices;
     if (cta >= ctas) return;
     auto begin_of = [&](int b) { return (int)((long long)total * b / ctas); };
     const int cu0 = begin_of(cta), cu1 = begin_of(cta + 1);
@@ -665,8 +668,8 @@ __global__ void __launch_bounds__(256) k_kv4_tree_join(const __grid_constant__ T
     while (begin_of(last) > end - 1) last--;
     const int np = last - cta + 1, kvh = r / p.n_cg, cg = r - kvh * p.n_cg;
     auto      entry = [&](int b) { return a.part + ((size_t)(cta + b) * 2 + (b == 0)) * ((size_t)EC * (HD + 2)); };
-    const int cc0 = (blockIdx.x % slices) * TREE_JOIN;
-    for (int cc = cc0 + warp; cc < min(cc0 + TREE_JOIN, a.group); cc += 8) {
+    const int cc0 = (blockIdx.x % slices) * slice;
+    for (int cc = cc0 + warp; cc < min(cc0 + slice, a.group); cc += 8) {
         const int col = cg * a.group + cc;
         if (col >= n_new * a.n_rep) return;
         float m = -INFINITY, L = 0.0f;

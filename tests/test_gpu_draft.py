@@ -210,8 +210,8 @@ def random_tree(r, n):
     return [-1 if j == 0 or r.random() < 0.1 else int(r.integers(max(0, j - 6), j)) for j in range(n)]
 
 
-def tree_check(pool, vals, q, seq, new, masks, out, scale=None):
-    """masks: per sequence a list of Python ints."""
+def tree_check(pool, vals, q, seq, new, masks, out, scale=None, every=1):
+    """masks: per sequence a list of Python ints.  every: one in so many heads is looked at."""
     H, hd = q.shape[1], q.shape[2]
     half, wide = torch.finfo(q.dtype).eps / 2, q.dtype == torch.float32
     scale = hd ** -0.5 if scale is None else scale
@@ -224,7 +224,7 @@ def tree_check(pool, vals, q, seq, new, masks, out, scale=None):
         for j in range(m):
             seen[j, base:] = [mk[j] >> t & 1 for t in range(m)]
         want, tol = np.zeros((m, H, hd)), np.zeros((m, H, hd))
-        for h in range(H):
+        for h in range(0, H, every):
             kh, vh = k[:, h // (H // k.shape[1])], v[:, h // (H // k.shape[1])]
             for j in range(m):
                 see = seen[j]
@@ -244,7 +244,7 @@ def tree_check(pool, vals, q, seq, new, masks, out, scale=None):
                     fin = np.nan_to_num(np.abs(vv))
                     vmax = fin.max()
                     tol[j, h] = vmax * (2 * ds + 2.0 ** -23 * (n / 16 + 64) + extra) + hw * (p @ fin) + half * np.nan_to_num(np.abs(want[j, h]))
-        check(out[r0:r0 + m], want, tol)
+        check(out[r0:r0 + m, ::every], want[:, ::every], tol[:, ::every])
         r0 += m
     assert r0 == q.shape[0]
 
@@ -440,6 +440,80 @@ def test_tree_peaked_flat_and_scaled(dtype, n_kv, rep):
     for scale in (None, 0.0, -0.3, 1e-3):
         out = pool.attend_tree(0, q, [0, 1], new, mask, scale=scale)
         tree_check(pool, vals, q, range(2), new, masks, out, scale=scale)
+
+
+# Calls of many columns, whose 16-bit queries the kernel on tensor memory takes.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_tree_values_that_are_not_finite_among_many(dtype, hd):
+    n_kv, rep, lens, new = 8, 8, [150, 2000, 1500, 700, 900], [12, 20, 64, 33, 16]
+    pool, vals = filled(n_kv, hd, lens, 3)
+    masks, mask = make(8, new)
+    k, v = (torch.from_numpy(np.concatenate([x[j][-m:] for x, m in zip(vals, new)])).float().cuda() for j in (0, 1))
+    k[3, 0, 1] = v[5, 7, 40] = k[12 + 7, 1, 0] = v[12 + 7, 1, hd - 1] = v[32 + 50, 6, 3] = math.nan
+    v[12 + 9, 0, 33] = math.inf
+    v[4, 1] = v[32 + 9, 3] = 60000.0
+    pool.append(0, k, v, range(5), new)
+    vals = [tuple(x.astype(np.float64) for x in pool.read(0, s)) for s in range(5)]
+    q = rows(5, sum(new), n_kv * rep, hd, spread=1.5).to(dtype)
+    out = pool.attend_tree(0, q, range(5), new, mask)
+    tree_check(pool, vals, q, range(5), new, masks, out, every=13)
+    q[2, 1, 5] = math.nan
+    q[100, 0, 3] = math.inf
+    two = pool.attend_tree(0, q, range(5), new, mask)
+    assert torch.isnan(two[2, 1]).all() and torch.isnan(two[100, 0]).all()
+    keep = torch.ones_like(out, dtype=torch.bool)
+    keep[2, 1] = keep[100, 0] = False
+    assert torch.equal(torch.nan_to_num(out[keep]), torch.nan_to_num(two[keep]))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_tree_masks_of_any_bits_among_many(dtype, hd):
+    n_kv, rep, lens, new = 8, 8, [64, 64, 7, 100, 1500, 2000], [64, 64, 7, 4, 64, 33]
+    pool, vals = filled(n_kv, hd, lens, 3)
+    r = np.random.default_rng(4)
+    masks = [[int(x) for x in r.integers(0, 2 ** 64, m, dtype=np.uint64)] for m in new]
+    masks[0][0] = masks[0][9] = masks[2][6] = masks[4][63] = 0
+    masks[0][63] = 1 << 63
+    masks[1][1] = 2 ** 64 - 1
+    masks[3] = [0, 1 << 63, 0xF0, 8]                  # bits behind the last row have no effect
+    mask = torch.from_numpy(np.array([x for m in masks for x in m], dtype=np.uint64).view(np.int64)).cuda()
+    q = rows(2, sum(new), n_kv * rep, hd).to(dtype)
+    out = pool.attend_tree(0, q, range(6), new, mask)
+    tree_check(pool, vals, q, range(6), new, masks, out, every=13)
+    assert not out[0].any() and not out[9].any() and not out[64 + 64 + 6].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_tree_peaked_flat_and_scaled_among_many(dtype, hd):
+    n_kv, rep, lens, new = 9, 8, [900, 2100, 1300], [64, 40, 33]
+    pool, vals = filled(n_kv, hd, lens, 3)
+    masks, mask = make(3, new)
+    q = rows(3, sum(new), n_kv * rep, hd)
+    q[0] *= 40.0
+    q[1] *= 1e-6
+    q[2] = 0.0
+    q[3] *= 1e-20 if dtype == torch.float32 else 1e-4
+    q[70] *= 300.0
+    q = q.to(dtype)
+    for scale in (None, 0.0, -0.3, 1e-3):
+        out = pool.attend_tree(0, q, range(3), new, mask, scale=scale)
+        tree_check(pool, vals, q, range(3), new, masks, out, scale=scale, every=23)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n_kv,rep,n,len_,new", [(8, 4, 17, 300, 64), (8, 8, 17, 100, 16), (8, 8, 1, 4000, 16), (8, 4, 8, 100, 64), (8, 4, 1, 900, 6), (7, 3, 11, 500, 20)])
+def test_tree_rows_of_one_length(dtype, hd, n_kv, rep, n, len_, new):
+    """Whole rows, as many a CTA, and few rows in many parts, joined in blocks of fewer columns."""
+    pool, vals = filled(n_kv, hd, [len_] * n, 7)
+    masks, mask = make(9, [new] * n)
+    q = rows(6, new * n, n_kv * rep, hd, spread=1.5).to(dtype)
+    out = torch.full((new * n + 1, n_kv * rep, hd), 77.0, dtype=dtype, device="cuda")
+    tree_check(pool, vals, q, range(n), [new] * n, masks, pool.attend_tree(0, q, range(n), [new] * n, mask, out=out[:-1]), every=11)
+    assert (out[-1] == 77).all()
 
 
 def test_tree_strided_misaligned_and_many():
