@@ -193,6 +193,7 @@ __global__ void __launch_bounds__(VER_WARPS * 32, 2) k_draft_verify(const Verify
         par_s[tid] = __ldg(a.parent + r0 + tid);
         u_s[tid] = __ldg(a.u + r0 + tid);
     }
+    __syncthreads();                                      // the table's warps are not its only readers
     const float  temp = a.temperature ? __ldg(a.temperature + seq) : 1.0f;
     const bool   greedy = !(temp > 0.0f);
     const double inv = greedy ? 1.0 : 1.4426950408889634 / (double)temp;

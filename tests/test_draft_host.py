@@ -2,6 +2,7 @@
 the calls refuse, and the pool's bookkeeping of kept rows."""
 import ctypes as C
 import math
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -190,6 +191,28 @@ def test_verify_refuses_a_vocabulary_past_counting():
 
 def test_verify_of_nothing():
     assert verify_args(n=0) == 0
+
+
+# ------------------------------------------------------------------ verify ---
+
+def statements(text):
+    """What stands outside of all braces."""
+    depth, out = 0, []
+    for c in text:
+        depth += c == "{"
+        if depth == 0:
+            out.append(c)
+        depth -= c == "}"
+    return "".join(out)
+
+
+def test_verify_meets_between_the_table_and_its_readers():
+    """Eight of a block's sixteen warps write the exponential's table, all read it from the first row on: the block meets in
+    between (the missing barrier cannot be made to show: the logits' loads hide it)."""
+    source = (Path(engine.__file__).parent / "csrc" / "ecu_verify.cuh").read_text()
+    kernel = source[source.index("k_draft_verify("):]
+    written, read = kernel.index("table[tid] ="), kernel.index("open_row(0)")
+    assert written < read and "__syncthreads();" in statements(kernel[written:read])
 
 
 # ------------------------------------------------------------------- keep ---

@@ -822,6 +822,20 @@ def test_verify_strided_given_and_captured():
     verify_check(case, n_row, got)
 
 
+@pytest.mark.parametrize("vocab", [128, 1024, 2048])
+@pytest.mark.parametrize("n", [1, 300, 700])
+def test_verify_short_rows_at_once(n, vocab):
+    """Rows so short that a warp reads them in one step, soon after its block began: the exponential's table is whole by
+    then, in every block and in launches one behind the other."""
+    g = np.random.default_rng(n + vocab)
+    n_row = [int(x) for x in g.integers(1, 4, n)]
+    case = verify_case(n, n_row, vocab, torch.float32, False, False)
+    want = verify_check(case, n_row)
+    dev = [None if x is None else torch.as_tensor(x).cuda() for x in case]
+    outs = [draft.verify(dev[0], dev[2], dev[3], n_row, dev[4], dev[5], temperature=dev[6]) for _ in range(50)]
+    assert all(torch.equal(a, b) for got in outs for a, b in zip(got, want))
+
+
 # ------------------------------------------------------------------ keep ---
 
 @pytest.mark.parametrize("hd,n_kv,layers", [(128, 8, 3), (64, 1, 2), (32, 5, 1), (96, 3, 2), (64, 300, 1)])
