@@ -327,16 +327,18 @@ class KvPool:
     def keep(self, seq, n_new, kept, stream: int | None = None) -> None:
         """Of the newest n_new[i] positions of each sequence the rows kept[i] (rising) stay, moved together; the others
         are given back (ecu_kv_keep)."""
-        s, n_new = _ints(seq), _ints(n_new)
-        if len(s) != len(n_new) or len(s) != len(kept):
-            raise EngineError(f"{len(s)} sequences, {len(n_new)} counts and {len(kept)} lists of rows")
-        numbers, count = [], array("i", list(map(len, kept)))
+        s, n_new, numbers = _ints(seq), _ints(n_new), []
         try:
+            count = array("i", list(map(len, kept)))
             for rows in kept:
                 numbers.extend(rows)
             flat = array("i", numbers)
         except (TypeError, OverflowError):
             raise EngineError("kept: lists of rows are wanted") from None
+        if len(s) != len(n_new) or len(s) != len(count):
+            raise EngineError(f"{len(s)} sequences, {len(n_new)} counts and {len(count)} lists of rows")
+        if len(flat) != sum(count):
+            raise EngineError("kept: lists of rows are wanted")
         if lib().ecu_kv_keep(self.h, _at(s), _at(n_new), flat.buffer_info()[0], count.buffer_info()[0], len(s),
                              self._stream(stream)) != 0:
             raise EngineError(last_error())

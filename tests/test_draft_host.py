@@ -284,3 +284,13 @@ def test_keep_refuses_lists():
     assert L.ecu_kv_keep(p.h, None, ptr(one), ptr(one), ptr(one), 1, None) == -1
     assert L.ecu_kv_keep(None, ptr(ints(0)), ptr(one), ptr(ints(0)), ptr(one), 1, None) == -1
     p.keep([0], [1], [[0]])
+
+
+def test_keep_refuses_what_are_no_lists_of_rows():
+    p = pool()
+    p.extend([0], [10])
+    for kept in ([0], [None], [iter([0])], [np.array(0)], [[[0]]], [["0"]], None, 7, iter([[0]])):
+        with pytest.raises(engine.EngineError):
+            p.keep([0], [1], kept)
+    assert p.length(0) == 10
+    p.keep([0], [1], [(0,)])
