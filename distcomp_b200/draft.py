@@ -81,12 +81,16 @@ class Rope:
 def tree(parents, device: int | None = 0):
     """(depth, mask) of drafted rows, for append_rope and attend_tree: parents is one list, or a list of lists (one a
     sequence), of each row's parent, -1 for none.  int32 and int64 tensors on the device (None: numpy arrays)."""
-    lists = [parents] if len(parents) and np.ndim(parents[0]) == 0 else parents
+    try:
+        lists = [parents] if len(parents) and np.ndim(parents[0]) == 0 else parents
+        lists = [(p, len(p)) for p in lists]
+    except TypeError:
+        raise EngineError("parents: a list of whole numbers, or a list of such lists, is wanted") from None
     depth, mask = [], []
-    for p in lists:
-        p = _ints(p) if len(p) else np.zeros(0, np.int32)
-        if len(p) > ROWS:
-            raise EngineError(f"{len(p)} drafted rows of a sequence ({ROWS} at most)")
+    for p, n in lists:
+        p = _ints(p) if n else np.zeros(0, np.int32)
+        if n > ROWS:
+            raise EngineError(f"{n} drafted rows of a sequence ({ROWS} at most)")
         d, m = [], []
         for j, up in enumerate(p.tolist()):
             if not -1 <= up < j:

@@ -193,6 +193,12 @@ def test_verify_of_nothing():
     assert verify_args(n=0) == 0
 
 
+@pytest.mark.parametrize("parents", [None, 5, iter([-1]), [None], [[-1], None], [[-1], 3], [-1, [0]], [[[-1]]], "ab"])
+def test_tree_refuses_what_are_no_lists(parents):
+    with pytest.raises(engine.EngineError):
+        draft.tree(parents, device=None)
+
+
 # ------------------------------------------------------------------ verify ---
 
 def statements(text):
