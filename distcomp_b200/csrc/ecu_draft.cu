@@ -236,7 +236,7 @@ static int verify_launch(VerifyArgs a, const int *n_row, int n, int sms, cudaStr
     cudaLaunchConfig_t  cfg = {};
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[0].val.programmaticStreamSerializationAllowed = early_on(s);
     at[1].id = cudaLaunchAttributeClusterDimension;
     at[1].val.clusterDim.x = (unsigned)cl;
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;

@@ -907,3 +907,47 @@ def test_pool_over_given_memory_and_its_end():
     for f in (lambda: pool.table, lambda: pool.lengths, lambda: pool.read(0, 1)):
         with pytest.raises(engine.EngineError):
             f()
+
+
+THREADS = '''
+import sys, threading
+sys.path[:0] = sys.argv[1:]
+import torch
+from distcomp_b200 import draft, kv4
+hd, n_kv, n = 64, 2, 3000
+pool = kv4.KvPool(1, n_kv, hd, 120, 2, 60)
+pool.extend([0, 1], [n, 100])
+k, q = torch.randn(n, n_kv, hd, device="cuda"), torch.randn(16, n_kv, hd, device="cuda")
+pool.append(0, k, k, [0], [n])
+logits, zero = torch.randn(16, 5000, device="cuda"), torch.zeros(16, device="cuda")
+rope, ints = draft.Rope(hd), torch.zeros(16, dtype=torch.int32, device="cuda")
+calls = [lambda: pool.attend(0, q[:1], [0], stream=2),
+         lambda: pool.append(0, k[:16], k[:16], [1], [16], stream=2),
+         lambda: pool.append_rope(0, rope, q, k[:16], k[:16], [1], [16], stream=2),
+         lambda: pool.attend_tree(0, q, [0], [16], stream=2),
+         lambda: draft.verify(logits, ints, ints, [16], zero, zero[:1], stream=2),
+         lambda: kv4.prompt_attention(k, k, k, [0, n], stream=2)]
+torch.cuda.synchronize()
+
+def work(call):
+    for _ in range(20):
+        call()
+for call in calls * 3:                                # one after the other on the host, each ended with work under way
+    t = threading.Thread(target=work, args=(call,))
+    t.start()
+    t.join()
+torch.cuda.synchronize()
+print("all through")
+'''
+
+
+def test_threads_that_end_with_work_under_way():
+    """Calls on the default streams of threads that end at once, while the next thread calls: in a process of its own,
+    which a limit ends where the threads would wait for one another."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    root = Path(kv4.__file__).resolve().parents[1]
+    for _ in range(4):
+        r = subprocess.run([sys.executable, "-c", THREADS, str(root)], capture_output=True, text=True, timeout=120)
+        assert r.returncode == 0 and "all through" in r.stdout, r.stderr[-2000:]
