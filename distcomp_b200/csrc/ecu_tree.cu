@@ -20,6 +20,14 @@
     } while (0)
 
 static std::atomic<unsigned> g_stall{0};        // devices (bits) whose next call's waits run out
+static std::atomic<unsigned> g_regs{0};         // ... whose next call finds the kernel on tensor memory compiled to other registers
+
+// The device's bit of a mask, taken out of it.
+static int injected(std::atomic<unsigned> &mask, int device)
+{
+    if (device >= 32 || !mask.load(std::memory_order_relaxed)) return 0;
+    return (int)(mask.fetch_and(~(1u << device)) >> device & 1u);
+}
 
 // Two partials a CTA, of up to 128 columns
 extern "C" size_t ecu_kv_tree_ws_bytes(const ecu_kv *kv)
@@ -33,6 +41,13 @@ extern "C" int ecu_inject_tree_timeout(int device)
 {
     if (device < 0 || device >= 32) return say("ecu_inject_tree_timeout", "no such device to stall");
     g_stall.fetch_or(1u << device);
+    return 0;
+}
+
+extern "C" int ecu_inject_tree_registers(int device)
+{
+    if (device < 0 || device >= 32) return say("ecu_inject_tree_registers", "no such device");
+    g_regs.fetch_or(1u << device);
     return 0;
 }
 
@@ -113,6 +128,19 @@ static TreeWay tree_way(const TreeTotal &t, int sms, bool captured, double start
     return w;
 }
 
+// Is the kernel on tensor memory compiled to the registers that its roles share (more than the launch has would wait
+// forever)?  If not, the other kernel takes its calls.
+template <typename T, int HD, int N> static bool tree_tc_fits(int device)
+{
+    static std::atomic<int> regs{0};
+    cudaFuncAttributes      f;
+    if (!regs.load(std::memory_order_relaxed)) {
+        if (cudaFuncGetAttributes(&f, k_kv4_tree_tc<T, HD, N>) == cudaSuccess) regs.store(f.numRegs, std::memory_order_relaxed);
+        else cudaGetLastError();
+    }
+    return regs.load(std::memory_order_relaxed) == TT_REGS && !injected(g_regs, device);
+}
+
 template <typename T, int NB, int N, typename F>
 static int tree_start(TreeArgs a, const KvRows<N> &r, const TreeWay &w, long long rows, int unit, cudaStream_t s, F launch)
 {
@@ -159,22 +187,16 @@ static int tree_launch(ecu_kv *kv, TreeArgs a, const int *seq, int first, const 
         // positions, these estimates take 1 to 3 % longer than the best of all choices, counts of units alone 14 to 17.)
         const TreeTotal t = tree_total(kv, a, r, TT_COLS, TT_UNIT, 1);
         const TreeWay   w = tree_way(t, kv->sms, captured, 17.0, NB == 4 ? 1.85 : 1.6, 0.0, 13.0);
-        if (w.us < best.us) {
+        if (w.us < best.us && tree_tc_fits<T, NB * 32, N>(kv->device)) {
             a.group = a.entry = TT_COLS;
             a.open = TT_OPEN;
             auto kern = k_kv4_tree_tc<T, NB * 32, N>;
             int *status = ecu_prompt_status_word(kv->device);
             if (!status) return say("ecu_kv_attend_tree", "the status word cannot be had");
-            int stall = 0;
-            if (kv->device < 32 && g_stall.load(std::memory_order_relaxed)) stall = (int)(g_stall.fetch_and(~(1u << kv->device)) >> kv->device & 1u);
+            const int stall = injected(g_stall, kv->device);
             return tree_start<T, NB>(a, r, w, t.rows, TT_UNIT, s, [&](const TreeArgs &a, int grid) {
                 static std::atomic<unsigned> done{0};
                 CK(ecu_allow_smem(kern, TreeTc<NB * 32>::smem(N), kv->device, done));
-                static const int regs = [&] {
-                    cudaFuncAttributes f;
-                    return cudaFuncGetAttributes(&f, kern) == cudaSuccess ? f.numRegs : 0;
-                }();
-                if (regs != TT_REGS) return say("ecu_kv_attend_tree", "the kernel was compiled to other registers than its roles share");
                 return launched("ecu_kv_attend_tree", ecu_launch_early(kern, (unsigned)grid, TT_THREADS, TreeTc<NB * 32>::smem(n), s, a, r, status, stall));
             });
         }

@@ -43,7 +43,8 @@
 #define TT_THREADS 896
 // Registers a thread at launch (7 groups of four warps: 504 between them), and
 // then 4 * 80 for the softmax, 2 * 64, 48.  More than there are would wait
-// forever, so the launch looks at what the kernel was compiled to.
+// forever, so the launch looks at what the kernel was compiled to
+// (tree_tc_fits).
 #define TT_REGS 72
 static_assert(4 * 80 + 2 * 64 + 48 <= 7 * TT_REGS, "the groups' registers are those of the launch");
 #define TT_UNIT 128

@@ -135,6 +135,7 @@ SIGNATURES = [
     ("ecu_inject_late_warp", C.c_int, [C.c_void_p]),
     ("ecu_inject_prompt_timeout", C.c_int, [C.c_int]),
     ("ecu_inject_tree_timeout", C.c_int, [C.c_int]),
+    ("ecu_inject_tree_registers", C.c_int, [C.c_int]),
     ("ecu_matvec_bench", C.c_int, [C.c_uint, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_int,
                                    C.c_int, C.c_int, C.POINTER(C.c_double)]),
     ("ecu_matvec_stream_bench", C.c_int, [C.c_uint, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_void_p,
@@ -616,6 +617,13 @@ def inject_tree_timeout(device: int = 0) -> None:
     """The next attention of drafted rows on the tensor cores waits for keys that never come
     (ecu_inject_tree_timeout): failure-path testing."""
     if lib().ecu_inject_tree_timeout(int(device)) != 0:
+        raise EngineError(last_error())
+
+
+def inject_tree_registers(device: int = 0) -> None:
+    """The next attention of drafted rows that would run on the tensor memory finds its kernel compiled to other registers
+    than its roles share (ecu_inject_tree_registers): failure-path testing."""
+    if lib().ecu_inject_tree_registers(int(device)) != 0:
         raise EngineError(last_error())
 
 

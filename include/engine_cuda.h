@@ -607,14 +607,17 @@ int  ecu_batch_feed(ecu_batch *b, const int *seq, const int *n_tok, int n, const
  * (ecu_attn_prompt, or inside ecu_batch_feed or ecu_prefill) never copies its
  * first keys, so that its waits run out: ecu_attn_prompt_status, or the call
  * around it, returns -1.  ecu_inject_tree_timeout: the same of the next
- * ecu_kv_attend_tree that runs on the tensor memory.  ecu_kv_inject_failure: of the launches with which
- * the next change of the pool updates the device (a pool without one counts
- * them alike), number `launch`, from 0, fails. */
+ * ecu_kv_attend_tree that runs on the tensor memory.  ecu_inject_tree_registers:
+ * the next one that would finds its kernel compiled to other registers than
+ * its roles share, and runs on the other.  ecu_kv_inject_failure: of the
+ * launches with which the next change of the pool updates the device (a pool
+ * without one counts them alike), number `launch`, from 0, fails. */
 int  ecu_set_wait_ns(int device, unsigned long long ns);
 int  ecu_inject_wait_timeout(ecu_ctx *c);
 int  ecu_inject_late_warp(ecu_ctx *c);
 int  ecu_inject_prompt_timeout(int device);
 int  ecu_inject_tree_timeout(int device);
+int  ecu_inject_tree_registers(int device);
 int  ecu_kv_inject_failure(ecu_kv *kv, int launch);
 
 /* ---- measurement --------------------------------------------------------- */
