@@ -375,6 +375,14 @@ struct KvAttendArgs {
 // and multiply (about 800 a unit and warp); 64 sequences of 1 to 4096: 50 us.
 #define KV4_BASE 8.0f
 #define KV4_SLACK 6.0f
+// Where M passes 2^20, a float near it has no room for the base beside it (its
+// step is 1/8 there; at 2^27 it is 16, and a weight that is off by 2^16 passes
+// fp16's range or vanishes).  There a unit's scores are rounded to floats before
+// M is taken off, which is then exact, and weights are 2^(score - M): relative to
+// M + KV4_BASE all the same (kv4_rel) where they meet others.
+#define KV4_FAR 1048576.0f
+__device__ __forceinline__ bool  kv4_far(float M) { return !(fabsf(M) < KV4_FAR); }
+__device__ __forceinline__ float kv4_rel(float M) { return kv4_far(M) ? M + KV4_BASE : M; }
 #define KV4_UNIT 32
 #define KV4_STAGES 2
 #define KV4_MAX_CTAS 192

@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(TREE_WARPS * 32, 1) k_kv4_tree(const __grid_co
                 // (of this row alone, and where one of its own lanes asked for it: no row's bits depend on what shares its tile)
                 const float m = top[x] + exponent(vrow[x]);
                 const bool  grow = asked && m > M[x] + KV4_SLACK;
-                const float alpha = grow ? kv4_ex2(M[x] - m) : 1.0f;
+                const float alpha = grow ? kv4_ex2(kv4_rel(M[x]) - kv4_rel(m)) : 1.0f;
                 if (grow) M[x] = m;
                 l[x] *= alpha;
 #pragma unroll
@@ -424,12 +424,21 @@ __global__ void __launch_bounds__(TREE_WARPS * 32, 1) k_kv4_tree(const __grid_co
         }
 #pragma unroll
         for (int x = 0; x < RR; x++) {
-            const float off = KV4_BASE - M[x];
+            // (17 short sequences take 35.8 us for 35.3 with scores as they may be, past KV4_FAR, 32 in fp32 444 for 434)
+            float off = KV4_BASE - M[x], times = fac[x];
+            if (kv4_far(M[x])) {
+                off = -M[x];
+                times = 1.0f;
+#pragma unroll
+                for (int nt = 0; nt < 4; nt++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) sc[nt][2 * x + e] *= fac[x];
+            }
 #pragma unroll
             for (int nt = 0; nt < 4; nt++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    float p = kv4_ex2(fmaf(sc[nt][2 * x + e], fac[x], off));
+                    float p = kv4_ex2(fmaf(sc[nt][2 * x + e], times, off));
                     if (CUT && !(live[x] >> (2 * nt + e) & 1u)) p = 0.0f;
                     sc[nt][2 * x + e] = p;
                     l[x] += p;
@@ -565,6 +574,7 @@ __global__ void __launch_bounds__(TREE_WARPS * 32, 1) k_kv4_tree(const __grid_co
         // ---- the row's end: the groups' partials, each relative to the largest M
 #pragma unroll
         for (int x = 0; x < RR; x++) {
+            M[x] = kv4_rel(M[x]);
             l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
             l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
             if (c == 0) {

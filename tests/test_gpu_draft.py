@@ -634,6 +634,53 @@ def test_tree_on_two_streams():
     pool.close()
 
 
+def clear_check(q, kn, vn, seen, scale, out, hk):
+    """Rows whose largest score is clear of all rounding show its value: weights are off by 2^-11, values by as much
+    where they are rounded to fp16, and the output is rounded once.  All rows are finite.  seen [rows, positions]."""
+    R, H, hd = q.shape
+    rep = H // kn.shape[1]
+    k, v = (torch.from_numpy(np.ascontiguousarray(x)).cuda().repeat_interleave(rep, 1) for x in (kn, vn))
+    assert torch.isfinite(out).all()
+    sc = torch.einsum("rhd,thd->rht", q.double(), k) * scale
+    size = (torch.einsum("rhd,thd->rht", q.double().abs(), k.abs()) * abs(scale)).masked_fill(~seen[:, None], 0.0).amax(-1)
+    two = sc.masked_fill(~seen[:, None], -math.inf).topk(2, -1)
+    clear = two.values[..., 0] - two.values[..., 1] > 2 * size * (2.0 ** -23 * (hd / 2 + 16) + hk) + 64
+    want = v[two.indices[..., 0], torch.arange(H, device="cuda")[None]]
+    half, wide = torch.finfo(q.dtype).eps / 2, q.dtype == torch.float32
+    tol = (half + (2.0 ** -20 if wide else 2 * H16)) * want.abs() + 2.0 ** -20
+    err = ((out.double() - want).abs() / tol).amax(-1)[clear]
+    assert clear.sum() > 0.2 * clear.numel() and err.max() <= 1.0, (clear.sum(), err.max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd,count", [(64, 8), (128, 8), (32, 2), (96, 2), (128, 1)])
+@pytest.mark.parametrize("top", [18, 20, 24, 27, 30])
+def test_tree_of_large_scores(dtype, hd, count, top):
+    """Scores around 2^top and beyond, past which a float has no room for anything beside them."""
+    n, m, n_kv, rep = 150 if count > 1 else 6000, 64, 8, 8
+    pool = kv4.KvPool(1, n_kv, hd, (n // PAGE + 1) * count, count, n // PAGE + 1)
+    pool.extend(range(count), [n] * count)
+    k, v, q = rows(1, n, n_kv, hd), rows(2, n, n_kv, hd), rows(5, m * count, n_kv * rep, hd).to(dtype)
+    k[70] *= 2.0 ** 12
+    k[-30] *= 2.0 ** 12                               # of the drafts too
+    for s in range(count):
+        pool.append(0, k, v, [s], [n])
+    kn, vn = stored(k), stored(v)
+    masks, mask = make(3, [m] * count)
+    seen = torch.ones(m * count, n, dtype=torch.bool)
+    for i, x in enumerate(np.array(masks, dtype=np.uint64).reshape(-1)):
+        seen[i, n - m:] = torch.tensor([bool(int(x) >> t & 1) for t in range(m)])
+    size = torch.einsum("rhd,hd->rh", q.double(), torch.from_numpy(kn[70]).cuda().repeat_interleave(rep, 0)).abs().median()
+    scale = 2.0 ** top / float(size)
+    got = pool.attend_tree(0, q, range(count), [m] * count, mask, scale=scale)
+    clear_check(q, kn, vn, seen.cuda(), scale, got, 0.0 if dtype == torch.float32 else H16)
+    if dtype != torch.float32 and count == 8:         # the other kernel, on the codes themselves
+        engine.inject_tree_registers()
+        other = pool.attend_tree(0, q, range(count), [m] * count, mask, scale=scale)
+        assert not torch.equal(got, other)
+        clear_check(q, kn, vn, seen.cuda(), scale, other, 0.0)
+
+
 # ---------------------------------------------------------------- verify ---
 
 def verify_plain(logits, tokens, parents, n_row, u, u_next, temp, q):
