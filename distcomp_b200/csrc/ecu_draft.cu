@@ -236,7 +236,7 @@ static int verify_launch(VerifyArgs a, const int *n_row, int n, int sms, cudaStr
     cudaLaunchConfig_t  cfg = {};
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = early_on(s);
+    at[0].val.programmaticStreamSerializationAllowed = 1;
     at[1].id = cudaLaunchAttributeClusterDimension;
     at[1].val.clusterDim.x = (unsigned)cl;
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
@@ -245,6 +245,7 @@ static int verify_launch(VerifyArgs a, const int *n_row, int n, int sms, cudaStr
     cfg.stream = s;
     cfg.attrs = at;
     cfg.numAttrs = 2;
+    if (s == cudaStreamPerThread) ecu_on_thread_stream();
     return launched("ecu_draft_verify", cudaLaunchKernelEx(&cfg, k_draft_verify<T, N>, a, r));
 }
 

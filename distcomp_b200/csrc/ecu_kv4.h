@@ -93,12 +93,9 @@ template <typename F> cudaError_t ecu_allow_smem(F kern, size_t bytes, int dev, 
     return e;
 }
 
-// May a launch on this stream begin while what comes before it ends?  Not on the
-// default stream of a thread: where a thread ended with such launches under way
-// and another one called meanwhile, both have spun in the driver for good, one
-// while its stream was being taken down, one in its call, and the GPU idle (one
-// run in two of test_attend_keeps_a_workspace_a_stream).
-inline int early_on(cudaStream_t s) { return s != cudaStreamPerThread; }
+// Work is enqueued on the calling thread's own default stream of the current
+// device: the thread waits for it where it ends.
+void ecu_on_thread_stream();
 
 // A launch that may begin while what comes before it in the stream ends (the
 // kernel waits for that itself, pdl_wait, before it touches global memory).
@@ -108,13 +105,14 @@ cudaError_t ecu_launch_early(void (*kern)(P...), unsigned grid, unsigned block, 
     cudaLaunchConfig_t  cfg = {};
     cudaLaunchAttribute early;
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = early_on(s);
+    early.val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(block);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = &early;
     cfg.numAttrs = 1;
+    if (s == cudaStreamPerThread) ecu_on_thread_stream();
     return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 

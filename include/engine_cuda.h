@@ -339,7 +339,8 @@ size_t ecu_kv4_page_bytes(int n_head_kv, int head_dim);
  * sequence holds which page, how many hold a page) is on the host, its table
  * and lengths are mirrored in device memory at fixed addresses.  device -1:
  * the bookkeeping alone, without a GPU (to plan capacity).  A pool is
- * single-threaded, like a context. */
+ * single-threaded, like a context.  A thread that has calls enqueued on its own
+ * default stream (cudaStreamPerThread) waits for them where it ends. */
 int  ecu_kv_open(ecu_kv **out, int n_layer, int n_head_kv, int head_dim, int n_pages, int n_seq, int max_pages,
                  int device, void *data, char *err, size_t errlen);
 void ecu_kv_close(ecu_kv *kv);
