@@ -813,7 +813,7 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
 #pragma unroll
             for (int h = 0; h < HL; h++) {
                 const float m = fmaxf(M[h], top[h] + vw);
-                alpha[h] = kv4_ex2(M[h] - m);
+                alpha[h] = kv4_ex2(kv4_rel(M[h]) - kv4_rel(m));
                 M[h] = m;
                 l[h] *= alpha[h];
             }
@@ -829,12 +829,20 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
         }
 #pragma unroll
         for (int h = 0; h < HL; h++) {
-            const float base = KV4_BASE - M[h];
+            float base = KV4_BASE - M[h], times = fac[h];
+            if (kv4_far(M[h])) {
+                base = -M[h];
+                times = 1.0f;
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int x = 0; x < 2; x++) sc[mt][x][h] *= fac[h];
+            }
 #pragma unroll
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
-                    sc[mt][x][h] = kv4_ex2(fmaf(sc[mt][x][h], fac[h], base));
+                    sc[mt][x][h] = kv4_ex2(fmaf(sc[mt][x][h], times, base));
                     if (CUT && mt * 16 + g + 8 * x >= left) sc[mt][x][h] = 0.0f;
                     l[h] += sc[mt][x][h];
                 }
@@ -925,7 +933,7 @@ __global__ void __launch_bounds__(KvWarps<NT>::N * 32, 1) k_kv4_attend(const KvA
 #pragma unroll
             for (int h = 0; h < HL; h++) {
                 const int hh = P == 2 ? h * 4 + c : (h >> 1) * 8 + 2 * c + (h & 1);
-                e[hh * (HD + 2) + HD] = M[h];
+                e[hh * (HD + 2) + HD] = kv4_rel(M[h]);
                 e[hh * (HD + 2) + HD + 1] = l[h];
             }
     };

@@ -16,6 +16,8 @@ Tolerances, from the arithmetic (h = half a step of a type, relative):
     prompt) times sum p |v|, plus fp16's smallest step at the top of its
     range; and every output by h of its type.
 """
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -951,3 +953,33 @@ def test_threads_that_end_with_work_under_way():
     for _ in range(4):
         r = subprocess.run([sys.executable, "-c", THREADS, str(root)], capture_output=True, text=True, timeout=120)
         assert r.returncode == 0 and "all through" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hd,lens", [(64, [150] * 8), (128, [6000]), (96, [700, 1, 90])])
+@pytest.mark.parametrize("top", [18, 20, 24, 27, 30])
+def test_attend_scores_past_what_a_float_steps_over(dtype, hd, lens, top):
+    """Scores around 2^top and beyond: rows stay finite, and one whose largest score is clear of all rounding shows its
+    value (its weight and the output are rounded once each, the weights' sum is not)."""
+    n_kv, rep = 2, 8
+    pool = kv4.KvPool(1, n_kv, hd, sum(-(-n // PAGE) for n in lens), len(lens), -(-max(lens) // PAGE))
+    n, half = max(lens), torch.finfo(dtype).eps / 2
+    k, v, q = rows(1, n, n_kv, hd), rows(2, n, n_kv, hd), rows(5, len(lens), n_kv * rep, hd).to(dtype)
+    k[70] *= 2.0 ** 12
+    pool.extend(range(len(lens)), lens)
+    for s, m in enumerate(lens):
+        pool.append(0, k[:m], v[:m], [s], [m])
+    kn, vn = (torch.from_numpy(stored(x)).cuda().repeat_interleave(rep, 1) for x in (k, v))
+    scale = 2.0 ** top / float(torch.einsum("rhd,hd->rh", q.double(), kn[70]).abs().median())
+    got, clear_rows = pool.attend(0, q, list(range(len(lens))), scale=scale), 0
+    assert torch.isfinite(got).all()
+    for s, m in enumerate(lens):
+        sc = torch.einsum("hd,thd->ht", q[s].double(), kn[:m]) * scale
+        size = (torch.einsum("hd,thd->ht", q[s].double().abs(), kn[:m].abs()) * scale).amax(-1)
+        two = torch.cat((sc, torch.full_like(sc[:, :1], -math.inf)), 1).topk(2, -1)
+        clear = two.values[:, 0] - two.values[:, 1] > 2 * size * 2.0 ** -23 * (hd / 2 + 16) + 64
+        want = vn[two.indices[:, 0], torch.arange(n_kv * rep, device="cuda")]
+        tol = (half + (2.0 ** -20 if dtype == torch.float32 else H16)) * want.abs() + 2.0 ** -20
+        assert ((got[s].double() - want).abs() <= tol)[clear].all()
+        clear_rows += int(clear.sum())
+    assert clear_rows > 0.2 * q.shape[0] * q.shape[1]
