@@ -214,6 +214,17 @@ __device__ __forceinline__ float pa_max3(float a, float b, float c)
     return r;
 }
 
+// The power of two that brings a maximum of 2^23 or more below that, else 1: a
+// float's step is 1/2 up to there.  Beyond, a weight could not tell its place
+// beside the maximum (at 2^27 it would be off by 2^16, past fp16's range or
+// nothing), so a row goes on in smaller units of its scores, which are off by
+// more than such a unit already.
+__device__ __forceinline__ float pa_near(float m)
+{
+    const int e = (int)(__float_as_uint(m) >> 23 & 255u) - 127;
+    return e >= 23 && e < 128 ? __uint_as_float((uint32_t)(127 + 22 - e) << 23) : 1.0f;
+}
+
 // 2^t on the FMA units: t = n + f with |f| <= 1/2, n added to the polynomial's
 // exponent.  Below -126 it is zero, as ex2's: what a row does not see has
 // t = -inf, and 2^-126 times a large bf16 value would count.  So the result is
@@ -459,7 +470,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lanes + 128 * t, to = tmem + lanes + 256 + HD * t;
         if (t < n_tile) {
             const int   row = tile_of(t) * 128 + r, vis = seen(row);
-            const float sl = a.scale * 1.4426950408889634f;
+            float       sl = a.scale * 1.4426950408889634f;
             float       m = -INFINITY, l = 0.0f;          // the maximum that P is relative to; this half's weights' sum
             for (int j = 0; j < n; j++) {
                 wait(s_full + t, (uint32_t)j & 1u);
@@ -495,6 +506,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                     named_bar(pair, 64);
                     mx = pa_max(mx, half_s[t][hf ^ 1][r]);
                     const bool  grow = grows();
+                    if (grow) sl *= pa_near(mx * sl);
                     const float f = grow && j > 0 ? kv4_ex2((m - mx) * sl) : 1.0f;
                     if (grow) m = mx;
                     l *= f;

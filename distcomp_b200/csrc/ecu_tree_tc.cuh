@@ -53,17 +53,6 @@ static_assert(4 * 80 + 2 * 64 + 48 <= 7 * TT_REGS, "the groups' registers are th
 #define TT_BASE 9.0f              // weights are 2^(t - M + TT_BASE) ...
 #define TT_SLACK 6.0f             // ... and M follows when t has passed it by so much: below 2^15, and fp16 down to 2^-33
 #define TT_SHIFT 4
-// The power of two that brings a maximum of 2^23 or more below that, else 1: a
-// float's step is 1/2 up to there.  Beyond, a weight could not tell its place
-// beside M (at 2^27 it would be off by 2^16, past fp16's range or nothing), so
-// the column goes on in smaller units of its scores, which are off by more than
-// such a unit already.  (Rounding the scores first, as ecu_tree.cuh's kernel does
-// there, took 233 us for 223 at 131025 positions; this takes 227.)
-__device__ __forceinline__ float tt_near(float M)
-{
-    const int e = (int)(__float_as_uint(M) >> 23 & 255u) - 127;
-    return e >= 23 && e < 128 ? __uint_as_float((uint32_t)(127 + 22 - e) << 23) : 1.0f;
-}
 #define TT_RING 4
 
 template <int HD> struct TreeTc {
@@ -409,7 +398,9 @@ __global__ void __launch_bounds__(TT_THREADS, 1) k_kv4_tree_tc(const __grid_cons
                 if (tt_any(team, gone())) return false;
                 mx = pa_max(pa_max3(part_s[0][cw], part_s[1][cw], part_s[2][cw]), part_s[3][cw]);
                 const bool grow = grows(), first = flags & TT_FIRST;
-                const float less = grow ? tt_near(mx) : 1.0f;
+                // (past 2^23, rounding the scores first, as ecu_tree.cuh's kernel does there, took 233 us for 223 at 131025
+                // positions; this takes 227)
+                const float less = grow ? pa_near(mx) : 1.0f;
                 float       f = grow && !first ? kv4_ex2((m - mx) * less) : 1.0f;
                 if (grow) m = mx * less;
                 fac *= less;

@@ -983,3 +983,26 @@ def test_attend_scores_past_what_a_float_steps_over(dtype, hd, lens, top):
         assert ((got[s].double() - want).abs() <= tol)[clear].all()
         clear_rows += int(clear.sum())
     assert clear_rows > 0.2 * q.shape[0] * q.shape[1]
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("top", [18, 20, 24, 27, 30])
+def test_prompt_scores_past_what_a_float_steps_over(dtype, hd, top):
+    """As test_attend_scores_past_what_a_float_steps_over, of a prompt: rows stay finite, and one whose largest score is
+    clear of all rounding shows its value."""
+    n, n_kv, rep, half = 600, 2, 4, torch.finfo(dtype).eps / 2
+    k, v, q = rows(1, n, n_kv, hd).to(dtype), rows(2, n, n_kv, hd).to(dtype), rows(3, n, n_kv * rep, hd).to(dtype)
+    k[70] *= 2.0 ** 10
+    kk, vv = k.double().repeat_interleave(rep, 1), v.double().repeat_interleave(rep, 1)
+    sc = torch.einsum("rhd,thd->rht", q.double(), kk)
+    scale = 2.0 ** top / float(sc[100:].abs().amax(-1).median())
+    unseen = torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1)[:, None]
+    size = (torch.einsum("rhd,thd->rht", q.double().abs(), kk.abs()) * scale).masked_fill(unseen, 0.0).amax(-1)
+    two = (sc * scale).masked_fill(unseen, -math.inf).topk(2, -1)
+    clear = two.values[..., 0] - two.values[..., 1] > 2 * size * 2.0 ** -23 * (hd / 2 + 16) + 64
+    want = vv[two.indices[..., 0], torch.arange(n_kv * rep, device="cuda")[None]]
+    got = kv4.prompt_attention(q, k, v, [0, n], scale=scale)
+    assert torch.isfinite(got).all()
+    assert clear.sum() > 0.2 * clear.numel()
+    assert ((got.double() - want).abs() <= 2 * half * want.abs() + 2.0 ** -20)[clear].all()
