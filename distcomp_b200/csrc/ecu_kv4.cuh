@@ -241,8 +241,8 @@ template <int N> struct KvMoves {
 // written; a later round reads only positions behind all that were written.  A
 // move of a KV head of 128 dimensions reads and writes 144 bytes, in chunks of
 // 16 and 2 bytes.  64 trees over 32 layers of 8 heads take 9 us, 8 sequences over
-// two layers 3.5, bound by latency (two dependent copies); the call around them
-// takes 42 and 25 us, most of it the host's bookkeeping.  (Moves and words in two
+// two layers 3.5, bound by latency (two dependent copies); the calls around them
+// take 36 and 25 us, most of it the host's bookkeeping.  (Moves and words in two
 // launches: 64 us.)
 template <int N>
 __global__ void __launch_bounds__(256) k_kv4_move(uint8_t *data, size_t page_bytes, size_t layer_bytes, int n_layer, int n_kv, int nb, int *meta,

@@ -15,11 +15,13 @@
 // a scale halfway between two fp16 numbers, subnormal scales) is decided in
 // 64-bit arithmetic.  A query is turned in 32 bits and rounded once.
 //
-// Instruction issue bounds long calls: 8310 rows of 7 prompts (32 query and 8 KV
-// heads of 128, bf16, the stored values handed back) take 73 us, where their 214
-// MB take 33 at the rate of a copy: 44 million warp instructions in 56 % of the
-// issue slots.  Keys in 64-bit arithmetic throughout took 149.  One row of each
-// of 64 sequences takes 15 us, the host's call.
+// The latency of a block's phases bounds long calls (angles, turned pairs, codes:
+// three barriers for four rows, with 44 % of the warps there could be): 8310 rows
+// of 7 prompts (32 query and 8 KV heads of 128, bf16, the stored values handed
+// back) take 73 us, where their 214 MB take 33 at the rate of a copy; 44 million
+// warp instructions use 56 % of the issue slots.  Keys in 64-bit arithmetic
+// throughout took 149.  One row of each of 64 sequences takes 13 us, the host's
+// call.
 #pragma once
 #include "ecu_kv4.cuh"
 
@@ -116,7 +118,7 @@ struct RopePair {
     float h, l;
 };
 
-// x0 * c - x1 * s for c = t.x + t.y, s = t.z + t.w
+// x0 * c - x1 * s for c = ch + cl, s = sh + sl
 __device__ __forceinline__ RopePair rope_turn(float x0, float x1, float ch, float cl, float sh, float sl)
 {
     const float p = __fmul_rn(x0, ch), pe = __fmaf_rn(x0, ch, -p), q = __fmul_rn(x1, sh), qe = __fmaf_rn(x1, sh, -q);

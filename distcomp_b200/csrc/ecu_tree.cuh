@@ -12,7 +12,11 @@
 // The columns are the products' rows, 16 to a tile: then the scores lie in the
 // registers as the second product wants its weights.  An fp32 query is two rows
 // of a tile, g its fp16 part and g + 8 the fp16 part of the rest (22 bits), and
-// so are its weights; they add up in one thread.  Ranges, the power of two that
+// so are its weights; they add up in one thread.  The weights of 16-bit queries
+// are one fp16 number each (off by 2^-11 of a weight at most, as their outputs are
+// rounded by 2^-11, and of bf16 by 2^-8): a second part would double the second
+// product's rows, and with them the tiles of a call.  The weights' sum is
+// of the unrounded ones.  Ranges, the power of two that
 // a query is scaled by and the maximum that is followed lazily are those of
 // ecu_kv4.cuh's attention.
 //
@@ -31,13 +35,15 @@
 //
 // Short calls are bound by latency: 6 drafts of one sequence of 900 positions
 // (32 query and 8 KV heads of 128, fp32) take 16 us (the host's call alone 12),
-// 17 sequences of up to 3000 positions (16 and 4 heads of 64, fp16) 34: a step of
+// 17 sequences of up to 3000 positions (16 and 4 heads of 64, fp16) 35: a step of
 // the groups takes about 3 us (64-wide heads 1.7), a row's queries, merge and
 // output 5 to 8, a join 12.  Many columns are bound by the scales between the
 // products, which the tensor cores do not apply: 32 sequences of 1 to 4096
-// positions (64 and 8 heads of 128) take 437 us in fp32, 545 before the fp32 sums
+// positions (64 and 8 heads of 128) take 444 us in fp32, 545 before the fp32 sums
 // were packed and rows' own places counted.  In 16 bits such calls run on
-// ecu_tree_tc.cuh's kernel instead.
+// ecu_tree_tc.cuh's kernel instead.  At 128-wide heads the 168 registers that 12
+// warps leave spill 144 bytes a thread in 16 bits, 92 in fp32, at 96-wide ones 12
+// and none.
 #pragma once
 #include "ecu_kv4.cuh"
 

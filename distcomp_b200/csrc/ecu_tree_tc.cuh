@@ -16,13 +16,13 @@
 // A chain of short steps bounds it (a unit's scores, their softmax, their
 // product with V), not any one unit of the SM: so the roles are many and run
 // apart, on two units' operands.  64 drafts behind 131025 positions (32 query
-// and 8 KV heads of 128, bf16) take 230 us: 600 TFLOP/s, the tensor pipe 32 % and
+// and 8 KV heads of 128, bf16) take 228 us: 603 TFLOP/s, the tensor pipe 31 % and
 // the issue slots 67 % in use, 152 MB read once at 0.65 TB/s; 32 sequences of 1 to
 // 4096 positions with 1 to 24 drafts (64 and 8 heads) 137 us, of which the
-// products take 23 % of the tensor pipe (columns that no row fills among them).
+// products take 22 % of the tensor pipe (columns that no row fills among them).
 // The kernel on mma.sync takes 769 and 381.
 // K and V are (code - 8) * scale rounded to fp16, as the batch's prompts take
-// them (a score is off by 2^-12 of its products' size at most, an eighth of what
+// them (a score is off by 2^-11 of its products' size at most, an eighth of what
 // the rounding of bf16 queries leaves; exact keys, with a second operand for
 // their rest, took 1.4 times as long), the weights are rounded to fp16.
 // Where a scale passes 2^12 (values past 2^15), the row's K and V are taken 2^-4

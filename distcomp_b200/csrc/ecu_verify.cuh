@@ -24,9 +24,10 @@
 // Latency bounds it: the rows of a path come one behind the other, each a pass
 // and an exchange between the cluster's CTAs.  A chain of 5 drafts over 128256
 // fp32 logits takes 14 us (of a row's 0.5 MB on 8 CTAs), 48 trees of 4 to 16
-// rows (bf16) 47 us: 51 MB through L2, 57 % of the issue slots and 22 % of the
-// fp64 units' time.  Two passes over a row, the maximum first and then exp()'s
-// sums, took 44 and 191.
+// rows (bf16) 48 to 54 us: 51 MB through L2, 57 % of the issue slots and 22 % of
+// the fp64 units' time.  The 64 registers that two CTAs an SM leave spill 80 to
+// 124 bytes a thread, and the table is read at a random place a lane.  Two passes
+// over a row, the maximum first and then exp()'s sums, took 44 and 191.
 #pragma once
 #include "ecu_kv4.cuh"
 

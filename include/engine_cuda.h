@@ -425,7 +425,9 @@ int    ecu_kv_read(ecu_kv *kv, int layer, int seq, int pos, int n, float *k, flo
  * sequence by them, write their rows (ecu_kv_append_rope), attend to the cache
  * and to each other along a tree (ecu_kv_attend_tree), hold them against the
  * target's probabilities (ecu_draft_verify), and keep what was accepted
- * (ecu_kv_keep).  The drafted rows are a sequence's newest positions; row 0 is
+ * (ecu_kv_keep).  These calls are for programs that run a model's layers
+ * themselves: ecu_batch_feed takes no trees and hands back a sequence's last row
+ * alone.  The drafted rows are a sequence's newest positions; row 0 is
  * the token that was picked last, every other row hangs on an earlier one.  No
  * counterpart in the reference, which feeds one token a step
  * (src/shard.c:911-917). */
@@ -477,14 +479,28 @@ int  ecu_kv_append_rope(ecu_kv *kv, int layer, const ecu_rope *rope, int dtype, 
  * consecutive sequences one after the other, as in ecu_kv_attend.  A row that
  * sees nothing becomes zeros.  A position that a row sees and that is not
  * finite in K makes the row NaN, one in V its block of 32 dimensions; positions
- * that it does not see have no effect.  ws: ecu_kv_tree_ws_bytes() bytes of
+ * that it does not see have no effect (but for values past 2^15, see below).
+ * ws: ecu_kv_tree_ws_bytes() bytes of
  * device memory that no other call uses at the same time; NULL: the pool's own
- * for this stream, as in ecu_kv_attend.  out and q do not overlap.  The lengths
+ * for this stream, as in ecu_kv_attend, but of the first stream too made on its
+ * first call (some 20 MB).  out and q do not overlap.  The lengths
  * are read on the device when the call runs, so a captured call follows its
  * sequences.  Sums and the softmax
- * are fp32; of fp32 queries, and of their weights, 22 bits count; 16-bit queries
- * of many columns (rows times query heads of a KV head, some 32 and more) see
- * keys and values rounded to fp16's 11 bits, as the prompts of a batch do.
+ * are fp32; of fp32 queries, and of their weights, 22 bits count; the weights of
+ * 16-bit queries are rounded to fp16's 11.  Calls of many columns (rows times
+ * query heads of a KV head, some 32 and more) of 16-bit queries and 64- or
+ * 128-wide heads see keys and values rounded to 11 bits too, as the prompts of
+ * a batch do.  Whether a call does goes by an estimate of its time over all of
+ * its sequences, as does how they are cut among the SMs: so a sequence's last
+ * bits are the same in every call of the same lists and lengths, but may differ
+ * beside other sequences, and in a captured call.  Where a call of many columns
+ * meets a position whose values pass 2^15, a drafted one that a row does not see
+ * too, all rows of the sequence take keys and values from that unit of 128
+ * positions on with scales rounded to multiples of 2^-20 (a value is off by
+ * 2^-18 more at most).  Rows of large scores stay finite; where a row's largest
+ * passes some 2^22 in size, in a call of many columns, its scores count as if
+ * divided by the power of two that brings it below (their own rounding is of that
+ * size).
  * Every wait in the kernel is bounded (ecu_set_wait_ns): where one gives up, the
  * call's rows mean nothing, and ecu_attn_prompt_status reports it. */
 int    ecu_kv_attend_tree(ecu_kv *kv, int layer, int dtype, const void *q, void *out, int n_head, long q_stride,
@@ -501,10 +517,10 @@ size_t ecu_kv_tree_ws_bytes(const ecu_kv *kv);
  * current one.  f is softmax(logits / temperature) of the current row, F its
  * sum, q the distribution that its children were drawn from: row `current` of
  * draft (fp32, rows draft_stride apart), or 1 where draft is NULL (the drafter
- * does not draw).  A rejected row leaves f <- max(f / F - q, 0), or f(x) <- 0;
- * where nothing is left of f it is softmax(logits / temperature) again.  At the
- * end next[i] is the first x with f(x) > 0 whose running sum passes
- * u_next[i] F.  A temperature (one a sequence; NULL: 1) that is not above 0
+ * does not draw).  A rejected row leaves f <- max(f / F - q, 0), or f(x) <- 0.
+ * At the end next[i] is the first x with f(x) > 0 whose running sum passes
+ * u_next[i] F; where nothing is left of f (so that no later row was accepted
+ * either) f is softmax(logits / temperature) again for that.  A temperature (one a sequence; NULL: 1) that is not above 0
  * takes the first of the largest logits instead, and accepts it alone.
  * Everything compared is 64-bit.  A token outside the vocabulary is not tried.
  * A row whose logits hold a NaN or +infinity, or -infinity alone, ends the walk
@@ -537,7 +553,8 @@ int  ecu_kv_keep(ecu_kv *kv, const int *seq, const int *n_new, const int *kept, 
  * behind the last row, or in keys that a row does not see (NaN and infinities
  * too), has no effect.  Sums and the softmax are fp32, relative to weights of
  * up to 2^8 (bf16 values near 2^127 / 2^8 / keys can pass fp32's range); the
- * weights are rounded to `dtype` before their product with V.  out overlaps
+ * weights are rounded to `dtype` before their product with V; scores past some
+ * 2^22 count as in ecu_kv_attend_tree's calls of many columns.  out overlaps
  * none of the others.
  * Every wait in the kernel is bounded (ecu_set_wait_ns): one that gives up
  * leaves rows of NaN, which ecu_attn_prompt_status reports. */

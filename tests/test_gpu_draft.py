@@ -2,7 +2,7 @@
 definitions.
 
 Tolerances, from the arithmetic:
-  * a turned key is quantised exactly (but for one value in about 10^14): the
+  * a turned key is quantised exactly (but for one value in some 10^12): the
     stored values are equal bit for bit;
   * a turned query is two products and a sum in fp32, of cosines and sines
     rounded once: three roundings of at most 2^-24 of |a| + |b| (times the
